@@ -17,7 +17,9 @@ typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16_t;
 typedef int int4_t __attribute__((ext_vector_type(4)));
+typedef int int8_t_v __attribute__((ext_vector_type(8)));
 typedef int int16_t_v __attribute__((ext_vector_type(16)));
 
 // ---- host-side error reporting (thread-local, read through ff_last_error) ----
@@ -57,6 +59,13 @@ __device__ __forceinline__ float dpp(float v) {
 __device__ __forceinline__ float swz_xor16(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F));
 }
+
+// Eight consecutive 16-bit values from 16 aligned bytes, and one value of either type to and from fp32 (to nearest, ties to
+// even).
+template <typename T>
+using vec8_t = T __attribute__((ext_vector_type(8)));
+template <typename T>
+using vec4_t = T __attribute__((ext_vector_type(4)));
 
 // Sum over the 64 lanes, in every lane: within each 32-lane half by one swizzle and four DPP steps (partners l ^ 16,
 // ^ 15, ^ 7, ^ 3, ^ 1 cover all 32), then across the halves by one permute.

@@ -24,6 +24,9 @@ ENV = "FOIDFINDER_ROCM_KERNELS"  # path to a prebuilt library (the reference's $
 # Epilogue codes (include/foidfinder_rocm.h); 0-2 as foidfinder/backends/cuda/engine.py:24.
 EPI_QKV_ROPE, EPI_RESIDUAL, EPI_GELU_F16, EPI_SWIGLU, EPI_BIAS_F16, EPI_I32 = 0, 1, 2, 3, 4, 5
 
+# Norm codes of quant_mx4 and qk_norm_rope (include/foidfinder_rocm.h).
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+
 _vp, _i64, _f32, _int = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_int
 SIGNATURES = {
     "ff_abi_version": ([], _int),
@@ -48,9 +51,15 @@ SIGNATURES = {
     "ff_pool_tree": ([*[_vp] * 5, _i64, _f32, *[_i64] * 5, _vp, _vp], _int),
     "ff_pool_leaf": ([_vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp], _int),
     "ff_patch_embed": ([_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp], _int),
+    "ff_quant_mx4": ([_vp, _int, *[_i64] * 3, _int, _int, _i64, _vp, _vp, _f32, _vp, _vp, _vp], _int),
+    "ff_dequant_mx4": ([_vp, _vp, _i64, _i64, _vp, _int, _vp], _int),
+    "ff_gemm_mx4": ([*[_vp] * 4, *[_i64] * 3, *[_vp] * 3, _int, _int, _int, _vp], _int),
+    "ff_gemm_mx4_variants": ([], _int),
+    "ff_qk_norm_rope": ([*[_vp, _i64, _i64] * 4, _int, *[_i64] * 4, _int, *[_vp] * 4, _f32, _vp, _vp, _i64, _i64, _int, _vp,
+                         _int, _f32, _vp], _int),
     "ff_head": ([_vp, _i64, _vp, _vp, _f32, _vp, _vp, _i64, _i64, _i64, _vp, _vp], _int),
 }
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 
 @cache
@@ -462,6 +471,117 @@ def head(x: torch.Tensor, W: torch.Tensor, bias: torch.Tensor, out: torch.Tensor
          _ptr(out))
 
 
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _mx4(codes: torch.Tensor, scale: torch.Tensor, name: str) -> tuple[int, int]:
+    """Rows and columns of an MX4 tensor: codes uint8 [T, C / 2], scale int32 [C / 128, T]."""
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.size(1) % 64 != 0:
+        raise RuntimeError(f"{name} codes must be uint8 [T, C / 2] with C a multiple of 128")
+    T, C = codes.size(0), codes.size(1) * 2
+    if scale.dtype != torch.int32 or tuple(scale.shape) != (C // 128, T):
+        raise RuntimeError(f"{name} scale must be int32 {(C // 128, T)}")
+    return T, C
+
+
+def _no_grad(*ts: torch.Tensor | None) -> None:
+    """Refuses tensors that autograd would follow: these ops write into given tensors and have no backward."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError("this op has no backward: call it under torch.no_grad() or detach its tensors")
+
+
+def quant_mx4(x: torch.Tensor, out: torch.Tensor, scale: torch.Tensor, rotate: bool = True, norm: int = NORM_NONE,
+              gamma: torch.Tensor | None = None, beta: torch.Tensor | None = None, c_real: int = 0,
+              eps: float = 1e-6) -> None:
+    """x fp16 or bf16 [T, C] (C % 128 == 0; any row stride from C up that is a multiple of 8) -> MX4: out uint8 [T, C / 2],
+    scale int32 [C / 128, T] (include/foidfinder_rocm.h, ff_quant_mx4). First the norm over the first c_real columns
+    (default: all) with gamma, and beta for NORM_LAYER, fp32 [C] with zeros past c_real (`pad_norm` builds them); then with
+    `rotate` the rotation by blockdiag(H128). Weights are prepared by the same call: rows [N, K], no norm."""
+    _no_grad(x, gamma, beta)
+    dev = _on_gpu(out, scale, gamma, beta)
+    _require(x.dim() == 2 and x.dtype in (torch.float16, torch.bfloat16), "x must be fp16 or bf16 [T, C]")
+    _require(x.is_cuda and x.get_device() == dev, "x must be on the outputs' GPU")
+    T, C = _mx4(out, scale, "out")
+    _require(tuple(x.shape) == (T, C) and x.stride(1) == 1, f"x must be [{T}, {C}] with contiguous rows")
+    for t in (gamma, beta):
+        if t is not None:
+            _float(C, t)
+    stride = x.stride(0) if T > 1 else C  # a single row's stride says nothing
+    _run("ff_quant_mx4", dev, _ptr(x), _DTYPES[x.dtype], T, C, stride, int(rotate), norm, c_real or C, _ptr(gamma),
+         _ptr(beta), eps, _ptr(out), _ptr(scale))
+
+
+def dequant_mx4(codes: torch.Tensor, scale: torch.Tensor, out: torch.Tensor) -> None:
+    """The values of MX4 codes into out [T, C], fp16, bf16 or fp32 (ff_dequant_mx4)."""
+    dev = _on_gpu(codes, scale, out)
+    T, C = _mx4(codes, scale, "the")
+    _require(out.dtype in _DTYPES and tuple(out.shape) == (T, C), f"out must be fp16, bf16 or fp32 [{T}, {C}]")
+    _run("ff_dequant_mx4", dev, _ptr(codes), _ptr(scale), T, C, _ptr(out), _DTYPES[out.dtype])
+
+
+def gemm_mx4(A: torch.Tensor, a_scale: torch.Tensor, W: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None,
+             out: torch.Tensor, epi: int, stages: int = 0, residual: torch.Tensor | None = None) -> None:
+    """MX4 A [M, K] x MX4 W [N, K] + bias fp32 [N] (or None) -> epilogue into out: EPI_BIAS_F16 (out fp16, bf16 or fp32),
+    EPI_GELU_F16, EPI_SWIGLU (out [M, N / 2]) or EPI_RESIDUAL (out = y + residual of out's type; None: out itself).
+    `stages` selects the tile variant (0 = by the sizes) (ff_gemm_mx4)."""
+    _no_grad(bias, residual)
+    dev = _on_gpu(A, a_scale, W, w_scale, bias, out, residual)
+    M, K = _mx4(A, a_scale, "A's")
+    N, KW = _mx4(W, w_scale, "W's")
+    _require(KW == K, "A and W must share K")
+    shape = out_shape(M, N, epi)
+    if out.dtype not in _DTYPES or tuple(out.shape) != shape:
+        raise RuntimeError(f"out must be fp16, bf16 or fp32 {shape}")
+    if bias is not None:
+        _float(N, bias)
+    if epi == EPI_RESIDUAL:
+        residual = out if residual is None else residual
+        _require(residual.dtype == out.dtype and residual.shape == out.shape, "residual must be like out")
+    else:
+        _require(residual is None, "a residual goes with EPI_RESIDUAL")
+    _run("ff_gemm_mx4", dev, _ptr(A), _ptr(a_scale), _ptr(W), _ptr(w_scale), M, N, K, _ptr(bias), _ptr(residual), _ptr(out),
+         _DTYPES[out.dtype], epi, stages)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: torch.Tensor, norm: int,
+                 q_gamma: torch.Tensor | None, k_gamma: torch.Tensor | None, q_beta: torch.Tensor | None,
+                 k_beta: torch.Tensor | None, rope_cos: torch.Tensor, rope_sin: torch.Tensor,
+                 positions: torch.Tensor | None = None, pairs: bool = True, eps: float = 1e-6,
+                 q_scale: float = 1.0) -> None:
+    """Norm of each head's query and key and their rotation by position in one pass (include/foidfinder_rocm.h,
+    ff_qk_norm_rope): q fp16 or bf16 [T, heads, D], k [T, kv_heads, D], views with any token and head strides (of a packed
+    [T, 3 C] row, say: `qkv.view(T, 3, heads, D)[:, 0]`) -> q_out, k_out of the same shapes; an output may be its input
+    itself and shares no other memory with q or k. gamma (with a norm) and beta (NORM_LAYER) fp32 [D]; tables fp32 [L, R / 2];
+    positions int32 or int64 [T], or None: t % L. `pairs`: columns (2 i, 2 i + 1) turn together, else (i, i + R / 2)."""
+    _no_grad(q, k, q_gamma, k_gamma, q_beta, k_beta, rope_cos, rope_sin)
+    dev = _on_gpu(q_gamma, k_gamma, q_beta, k_beta, rope_cos, rope_sin, positions)
+    _require(q.dim() == 3 and k.dim() == 3, "q and k must be [T, heads, D]")
+    (T, H, D), KV = q.shape, k.size(1)
+    dt = q.dtype
+    _require(dt in (torch.float16, torch.bfloat16), "q and k must be fp16 or bf16")
+    _require(k.size(0) == T and k.size(2) == D, "q and k must share T and D")
+    for t, shape in ((q, (T, H, D)), (k, (T, KV, D)), (q_out, (T, H, D)), (k_out, (T, KV, D))):
+        _require(t.is_cuda and t.get_device() == dev and t.dtype == dt and tuple(t.shape) == shape and
+                 (t.stride(2) == 1 or D == 1), f"need {dt} {shape} on the tables' GPU with contiguous columns")
+    _require(rope_cos.dtype == rope_sin.dtype == torch.float32 and rope_cos.dim() == 2 and rope_cos.shape == rope_sin.shape,
+             "RoPE tables must be fp32 [L, R / 2]")
+    for t in (q_gamma, k_gamma, q_beta, k_beta):
+        if t is not None:
+            _float(D, t)
+    pos64 = False
+    if positions is not None:
+        _require(positions.dtype in (torch.int32, torch.int64) and tuple(positions.shape) == (T,),
+                 f"positions must be int32 or int64 [{T}]")
+        pos64 = positions.dtype == torch.int64
+    L, half = rope_cos.shape
+    strides = [(t.stride(0) if T > 1 else 0, t.stride(1) if t.size(1) > 1 else 0) for t in (q, k, q_out, k_out)]
+    for (a, b), x, y in ((strides[::2], q, q_out), (strides[1::2], k, k_out)):
+        _require(a == b or x.data_ptr() != y.data_ptr(), "an output in its input's place must have its strides")
+    _run("ff_qk_norm_rope", dev, _ptr(q), *strides[0], _ptr(k), *strides[1], _ptr(q_out), *strides[2], _ptr(k_out),
+         *strides[3], _DTYPES[dt], T, H, KV, D, norm, _ptr(q_gamma), _ptr(k_gamma), _ptr(q_beta), _ptr(k_beta), eps,
+         _ptr(rope_cos), _ptr(rope_sin), L, 2 * half, int(pairs), _ptr(positions), int(pos64), q_scale)
+
+
 # ---- torch.ops.foidfinder_rocm registration (schemas as kernels.cu:268-273, plus eps / the fused norm) ----
 
 _LIB = torch.library.Library("foidfinder_rocm", "DEF")
@@ -497,6 +617,17 @@ _LIB.define("head(Tensor x, Tensor W, Tensor bias, Tensor(a!) out, Tensor? gamma
 for _fn in (pool_weights, pool_sum, pool_values, pool_queries, pool_keys, pool_tree, pool_leaf, patch_embed, head):
     _LIB.impl(_fn.__name__, _fn, "CUDA")
 _LIB.impl("layer_norm2", layer_norm2, "CUDA")
+# the MX4 linear and the norm of queries and keys (no reference counterpart; out-param ops in the same style)
+_LIB.define("quant_mx4(Tensor x, Tensor(a!) out, Tensor(b!) scale, bool rotate=True, int norm=0, Tensor? gamma=None, "
+            "Tensor? beta=None, int c_real=0, float eps=1e-06) -> ()")
+_LIB.define("dequant_mx4(Tensor codes, Tensor scale, Tensor(a!) out) -> ()")
+_LIB.define("gemm_mx4(Tensor A, Tensor a_scale, Tensor W, Tensor w_scale, Tensor? bias, Tensor(a!) out, int epi, "
+            "int stages=0, Tensor? residual=None) -> ()")
+_LIB.define("qk_norm_rope(Tensor q, Tensor k, Tensor(a!) q_out, Tensor(b!) k_out, int norm, Tensor? q_gamma, "
+            "Tensor? k_gamma, Tensor? q_beta, Tensor? k_beta, Tensor rope_cos, Tensor rope_sin, Tensor? positions=None, "
+            "bool pairs=True, float eps=1e-06, float q_scale=1.0) -> ()")
+for _fn in (quant_mx4, dequant_mx4, gemm_mx4, qk_norm_rope):
+    _LIB.impl(_fn.__name__, _fn, "CUDA")
 _LIB.impl("slot_weights", slot_weights, "CUDA")
 
 

@@ -16,6 +16,8 @@ Modules:
              the int8-semantics and float forwards
   haruka     Haruka Tagger (EVA02-B + slot-sigmoid tree pool): weight conversion, stem, tree-pool head, the
              int8-semantics and float forwards
+  mx4        MX4 quantization with the fused norm and rotation, the codes' values and the product (no reference path)
+  qk_norm    norm of each head's query and key with the rotation by position, float64 (no reference path)
 
 Pinning (what checks each function beyond restating it) is listed per function in `PINNED`; tests/test_oracle.py
 runs those checks.
@@ -53,4 +55,10 @@ PINNED = {
     "haruka.pool_head": "equals the model card's MHAttnPool (unfolded key scale, child queries broadcast per coarse "
     "query, einsum leaves) in float64 torch",
     "haruka.forward_int8": "agrees with the float forward (no quantization) within the int8 error budget",
+    "mx4.encode": "nearest value of the 15 by brute force, ties to the even code, saturation; the exponent of the largest "
+    "value; blocks of zeros and of values that are not finite (tests/test_mx4.py)",
+    "mx4.quant_mx4": "norm and rotation against float64 formulas to fp32 rounding; sums independent of the padding",
+    "mx4.gemm_mx4": "equals the product of the values by exact rational arithmetic on small shapes",
+    "qk_norm.qk_norm_rope": "complex multiplication by e^(i angle) per pair; unit mean square after the RMS norm; position 0 "
+    "leaves the normed head",
 }

@@ -1,0 +1,262 @@
+"""MX4 and the head norm without a GPU: the oracles pinned against definitions, and every refusal of the entry points (they
+come before any HIP call)."""
+
+from __future__ import annotations
+
+from fractions import Fraction
+
+import numpy as np
+import pytest
+import torch
+
+from foidfinder_amd import kernels as K
+from oracle import mx4 as OX
+from oracle import qk_norm as OQ
+
+FF_OK, FF_EINVAL = 0, 1
+ALL_VALUES = [s * g for g in OX.GRID for s in (1, -1)]
+
+
+def err(status):
+    return status, K.lib().ff_last_error().decode()
+
+
+def test_encode_picks_the_nearest_value_and_the_even_code_on_ties():
+    rng = np.random.default_rng(0)
+    v = rng.standard_normal((64, 32)).astype(np.float32) * np.exp2(rng.integers(-20, 20, (64, 1))).astype(np.float32)
+    v[0] = np.arange(32) * 0.25  # every midpoint of the grid at exponent 0 (the largest value, 7.75, in [4, 8))
+    v[1] = -v[0]
+    code, e = OX.encode(v)
+    for r in range(64):
+        top = float(np.abs(v[r]).max())
+        unit = 2.0 ** (int(e[r, 0]) - 127)
+        assert 4 * unit <= top < 8 * unit
+        for x, c in zip(v[r].tolist(), code[r].tolist()):
+            m = abs(x) / unit
+            d = [abs(m - g) for g in OX.GRID]
+            best = [i for i, t in enumerate(d) if t == min(d)]
+            want = best[0] if len(best) == 1 else next(i for i in best if i % 2 == 0)
+            if m > 6:
+                want = 7
+            assert c & 7 == want and (c >> 3 == 1) == (np.signbit(x)), (x, c, want)
+
+
+def test_encode_of_zeros_subnormals_and_values_that_are_not_finite():
+    v = np.zeros((1, 160), np.float32)
+    v[0, 32] = 2.0**-130
+    v[0, 64] = np.inf
+    v[0, 96] = np.nan
+    v[0, 128] = np.finfo(np.float32).max
+    code, e = OX.encode(v)
+    assert e[0].tolist() == [0, 0, 255, 255, 252]
+    assert not code[0, :32].any() and code[0, 32] == 0  # 2^-130 / 2^-127 = 1/8 rounds to 0
+    vals = OX.values(*OX.pack(np.pad(code, ((0, 0), (0, 96))), np.pad(e, ((0, 0), (0, 3)))))
+    assert np.isnan(vals[0, 64:128]).all() and vals[0, 128] == 6 * 2.0**125 and not vals[0, :64].any()
+
+
+def test_pack_puts_even_columns_low_and_four_exponents_in_a_word():
+    code = np.arange(256, dtype=np.uint8).reshape(1, 256) % 16
+    codes, scale = OX.pack(code, np.arange(8, dtype=np.uint8).reshape(1, 8) + 100)
+    assert codes[0, 0] == 0x10 and codes[0, 1] == 0x32 and scale.shape == (2, 1)
+    assert scale[1, 0] == 104 | 105 << 8 | 106 << 16 | 107 << 24
+    back = OX.unpack(codes, scale)
+    assert np.array_equal(back[0], code) and back[1][0].tolist() == list(range(100, 108))
+
+
+@pytest.mark.parametrize("norm", [OX.RMS, OX.LAYER])
+@pytest.mark.parametrize(("C", "c_real"), [(128, 1), (640, 640), (1024, 1000), (2816, 2730)])
+def test_norm_rows_against_float64(norm, C, c_real):
+    """A sum of n terms in 64 partial sums is off by at most (n / 64 + 6) 2^-24 of the sum of magnitudes: with the mean's
+    and the variance's quotient, root and products (1/2 ulp each, under ten of them) a value is off by (C / 32 + 32) 2^-24
+    of the row's largest normed value at most."""
+    rng = np.random.default_rng(C + norm)
+    x = rng.standard_normal((5, C)).astype(np.float32)
+    g = np.where(np.arange(C) < c_real, 1 + 0.1 * rng.standard_normal(C), 0).astype(np.float32)
+    b = np.where(np.arange(C) < c_real, 0.1 * rng.standard_normal(C), 0).astype(np.float32) if norm == OX.LAYER else None
+    got = OX.norm_rows(x, norm, c_real, g, b, 1e-6)
+    want = np.zeros((5, C))
+    want[:, :c_real] = OQ.head_norm(x[:, :c_real], norm, g[:c_real], None if b is None else b[:c_real], 1e-6)
+    assert not got[:, c_real:].any()
+    assert np.abs(got - want).max() <= (C / 32 + 32) * 2.0**-24 * max(1.0, np.abs(want).max())
+
+
+def test_rotation_equals_the_hadamard_product():
+    """Seven stages, one rounding of at most half an ulp each, and the factor's: 8 * 2^-24 of the sum of magnitudes."""
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((4, 256)).astype(np.float32)
+    i = np.arange(128)
+    h = np.array([[(-1.0) ** bin(a & b).count("1") for b in i] for a in i]) / np.sqrt(128.0)
+    v = OX.fwht_rows(x.reshape(-1, 128), tuple(range(7))) * OX.INV_SQRT_128
+    want = x.reshape(-1, 128).astype(np.float64) @ h
+    assert np.abs(v - want).max() <= 9 * 2.0**-24 * np.abs(x).reshape(-1, 128).sum(1).max() / np.sqrt(128.0)
+    codes, scale = OX.quant_mx4(x)
+    back = OX.values(codes, scale)
+    # a value is off by half a spacing: 1/2 under 4, 1 up to 6, and saturation (6 for values under 8): 2 units of 2^e
+    unit = np.repeat(np.ldexp(1.0, OX.unpack(codes, scale)[1].astype(int) - 127), 32, axis=1)
+    assert (np.abs(back - v.reshape(4, 256)) <= 2 * unit).all()
+
+
+def test_gemm_oracle_against_rationals():
+    rng = np.random.default_rng(5)
+    a, w = (OX.pack(rng.integers(0, 16, (n, 128)).astype(np.uint8), rng.integers(60, 190, (n, 4)).astype(np.uint8))
+            for n in (2, 3))
+    bias = rng.standard_normal(3).astype(np.float32)
+    y, size = OX.gemm_mx4(a, w, bias)
+    (ac, ae), (wc, we) = OX.unpack(*a), OX.unpack(*w)
+
+    def val(c, e):
+        return Fraction(float(OX.GRID[c & 7])) * (-1 if c & 8 else 1) * Fraction(2) ** (int(e) - 127)
+
+    for m in range(2):
+        for n in range(3):
+            s = sum(val(ac[m, k], ae[m, k // 32]) * val(wc[n, k], we[n, k // 32]) for k in range(128))
+            assert abs(float(s + Fraction(float(bias[n]))) - y[m, n]) <= 1e-13 * size[m, n]
+
+
+@pytest.mark.parametrize("pairs", [True, False])
+def test_rotation_oracle_is_a_complex_product(pairs):
+    rng = np.random.default_rng(7)
+    x = rng.standard_normal((3, 2, 24))
+    ang = rng.uniform(-4, 4, (5, 8))
+    pos = np.array([0, 4, 2])
+    ang[0] = 0
+    y, _ = OQ.qk_norm_rope(x, OQ.NONE, None, None, 1e-6, np.cos(ang), np.sin(ang), pos, pairs, 3.0)
+    for t in range(3):
+        for i in range(8):
+            a, b = (2 * i, 2 * i + 1) if pairs else (i, i + 8)
+            z = (x[t, :, a] + 1j * x[t, :, b]) * np.exp(1j * ang[pos[t], i]) * 3
+            assert np.allclose(y[t, :, a], z.real, atol=1e-14) and np.allclose(y[t, :, b], z.imag, atol=1e-14)
+    assert np.array_equal(y[..., 16:], x[..., 16:] * 3) and np.allclose(y[0], x[0] * 3)
+    n, _ = OQ.qk_norm_rope(x, OQ.RMS, np.ones(24), None, 1e-12, np.cos(ang), np.sin(ang), np.array([0, 5, -1]), pairs)
+    assert np.allclose((n[0] ** 2).mean(-1), 1) and np.isnan(n[1:]).all()
+
+
+# ---- refusals of the C entries ----
+
+
+def test_quant_mx4_rejects_bad_arguments():
+    def call(x=256, dtype=0, T=4, C=1024, xs=1024, rotate=1, norm=0, c_real=1024, g=None, b=None, eps=1e-6, out=256, s=256):
+        return err(K.lib().ff_quant_mx4(x, dtype, T, C, xs, rotate, norm, c_real, g, b, eps, out, s, None))
+
+    assert call(T=0, x=None) == (FF_OK, "")
+    for kw, what in ((dict(dtype=2), "fp16 or bf16"), (dict(T=-1), "T"), (dict(T=1 << 31), "T"), (dict(C=0, xs=0), "C"),
+                     (dict(C=1000), "C"), (dict(C=6272, xs=6272), "C"), (dict(xs=1016), "x_stride"),
+                     (dict(xs=1028), "x_stride"), (dict(rotate=2), "rotate"), (dict(norm=3), "norm"),
+                     (dict(norm=1), "gamma"), (dict(g=256), "gamma"), (dict(norm=2, g=256), "beta"),
+                     (dict(norm=1, g=256, b=256), "beta"), (dict(norm=1, g=256, c_real=0), "c_real"),
+                     (dict(norm=1, g=256, c_real=1025), "c_real"), (dict(norm=1, g=256, eps=0.0), "eps"),
+                     (dict(norm=1, g=256, eps=float("nan")), "eps"), (dict(x=None), "null"), (dict(out=None), "null"),
+                     (dict(s=None), "null"), (dict(x=264), "misaligned"), (dict(out=258), "misaligned"),
+                     (dict(s=257), "misaligned"), (dict(norm=1, g=260), "misaligned")):
+        status, msg = call(**kw)
+        assert status == FF_EINVAL and what in msg, (kw, msg)
+
+
+def test_dequant_mx4_rejects_bad_arguments():
+    def call(c=256, s=256, T=4, C=1024, out=256, dtype=0):
+        return err(K.lib().ff_dequant_mx4(c, s, T, C, out, dtype, None))
+
+    assert call(T=0, c=None) == (FF_OK, "")
+    for kw, what in ((dict(dtype=3), "fp32"), (dict(T=-1), "T"), (dict(C=64), "C"), (dict(c=None), "null"),
+                     (dict(s=None), "null"), (dict(out=None), "null"), (dict(out=264), "misaligned"),
+                     (dict(c=258), "misaligned"), (dict(s=258), "misaligned")):
+        status, msg = call(**kw)
+        assert status == FF_EINVAL and what in msg, (kw, msg)
+
+
+def test_gemm_mx4_rejects_bad_arguments():
+    def call(A=256, As=256, W=256, Ws=256, M=8, N=16, Kd=128, bias=256, res=None, out=256, dtype=0, epi=4, variant=0):
+        return err(K.lib().ff_gemm_mx4(A, As, W, Ws, M, N, Kd, bias, res, out, dtype, epi, variant, None))
+
+    assert call(M=0, A=None) == (FF_OK, "")
+    for kw, what in ((dict(epi=0), "epilogue"), (dict(epi=5), "epilogue"), (dict(dtype=3), "out must"),
+                     (dict(dtype=2, epi=2), "out must"), (dict(variant=-1), "variant"), (dict(variant=99), "variant"),
+                     (dict(Kd=64), "K must"), (dict(Kd=0), "K must"), (dict(N=0), "N must"), (dict(N=15, epi=3), "even"),
+                     (dict(M=-1), "not supported"), (dict(N=(1 << 21) + 1), "not supported"),
+                     (dict(Kd=(1 << 22) + 128), "not supported"), (dict(epi=1), "null"), (dict(A=None), "null"),
+                     (dict(Ws=None), "null"), (dict(out=None), "null"), (dict(A=264), "misaligned"),
+                     (dict(bias=260), "misaligned"), (dict(out=264), "misaligned"), (dict(As=258), "misaligned"),
+                     (dict(epi=1, res=264), "misaligned")):
+        status, msg = call(**kw)
+        assert status == FF_EINVAL and what in msg, (kw, msg)
+
+
+def test_qk_norm_rope_rejects_bad_arguments():
+    def call(q=256, k=256, qo=256, ko=256, st=((1024, 64),) * 4, dtype=0, T=4, H=16, KV=16, D=64, norm=1, g=256, b=None,
+             eps=1e-6, cos=256, L=8, R=64, pairs=1, pos=None, pos64=0):
+        return err(K.lib().ff_qk_norm_rope(q, *st[0], k, *st[1], qo, *st[2], ko, *st[3], dtype, T, H, KV, D, norm, g, g, b,
+                                           b, eps, cos, cos, L, R, pairs, pos, pos64, 1.0, None))
+
+    ok = (1024, 64)
+    assert call(T=0, q=None) == (FF_OK, "")
+    for kw, what in ((dict(dtype=2), "fp16 or bf16"), (dict(D=60), "heads must"), (dict(D=264), "heads must"),
+                     (dict(R=0), "rotated"), (dict(R=60), "rotated"), (dict(R=72), "rotated"), (dict(H=0), "heads"),
+                     (dict(KV=65536), "heads"), (dict(T=-1), "T"), (dict(T=1 << 27), "2^31"), (dict(L=0), "rope_len"),
+                     (dict(norm=3), "norm"), (dict(norm=0), "gamma"), (dict(g=None), "gamma"), (dict(b=256), "beta"),
+                     (dict(norm=2), "beta"), (dict(eps=0.0), "eps"), (dict(q=None), "null"), (dict(ko=None), "null"),
+                     (dict(cos=None), "null"), (dict(q=260), "misaligned"), (dict(cos=264), "misaligned"),
+                     (dict(pos=258), "misaligned"), (dict(pos=260, pos64=1), "misaligned"),
+                     (dict(st=((1022, 64), ok, ok, ok)), "misaligned"), (dict(st=((-1024, 64), ok, ok, ok)), "negative"),
+                     (dict(st=(ok, ok, (960, 64), ok)), "overlap"), (dict(st=(ok, ok, ok, (1024, 56))), "overlap"),
+                     (dict(st=(ok, ok, (0, 64), ok)), "overlap"), (dict(st=(ok, ok, (64, 192), ok)), "overlap")):
+        status, msg = call(**kw)
+        assert status == FF_EINVAL and what in msg, (kw, msg)
+
+
+def test_python_layer_refuses_wrong_tensors(monkeypatch):
+    """The checks of the wrappers, with the device check taken as passed (it comes first and needs a GPU)."""
+    monkeypatch.setattr(K, "_on_gpu", lambda *ts: -1)
+    monkeypatch.setattr(K, "_run", lambda *a: None)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+
+    def mx(T, C):
+        return torch.zeros(T, C // 2, dtype=torch.uint8), torch.zeros(C // 128, T, dtype=torch.int32)
+
+    x = torch.zeros(3, 256, dtype=torch.half)
+    K.quant_mx4(x, *mx(3, 256))
+    K.quant_mx4(torch.zeros(3, 512, dtype=torch.half)[:, :256], *mx(3, 256))
+    for bad, out in ((x.float(), mx(3, 256)), (x, mx(3, 128)), (x, mx(4, 256)), (x.t(), mx(256, 128)),
+                     (x, (mx(3, 256)[0].int(), mx(3, 256)[1])), (x, (mx(3, 256)[0], mx(3, 256)[1].long()))):
+        with pytest.raises(RuntimeError):
+            K.quant_mx4(bad, *out)
+    with pytest.raises(RuntimeError, match="fp32"):
+        K.quant_mx4(x, *mx(3, 256), True, K.NORM_RMS, torch.zeros(128))
+    with pytest.raises(RuntimeError, match="backward"):
+        K.quant_mx4(x.clone().requires_grad_(), *mx(3, 256))
+    with torch.no_grad():
+        K.quant_mx4(x.clone().requires_grad_(), *mx(3, 256))
+    a, w, o = mx(3, 256), mx(6, 256), torch.zeros(3, 6)
+    K.gemm_mx4(*a, *w, None, o, K.EPI_BIAS_F16)
+    for call in (lambda: K.gemm_mx4(*a, *mx(6, 128), None, o, K.EPI_BIAS_F16),
+                 lambda: K.gemm_mx4(*a, *w, torch.zeros(5), o, K.EPI_BIAS_F16),
+                 lambda: K.gemm_mx4(*a, *w, None, o[:, :3], K.EPI_BIAS_F16),
+                 lambda: K.gemm_mx4(*a, *w, None, o, K.EPI_SWIGLU),
+                 lambda: K.gemm_mx4(*a, *w, None, o, K.EPI_BIAS_F16, 0, o),
+                 lambda: K.gemm_mx4(*a, *w, None, o, K.EPI_RESIDUAL, 0, o.half()),
+                 lambda: K.dequant_mx4(*a, torch.zeros(3, 128)),
+                 lambda: K.dequant_mx4(*a, torch.zeros(3, 256, dtype=torch.double))):
+        with pytest.raises(RuntimeError):
+            call()
+    q, t, g = torch.zeros(5, 4, 64, dtype=torch.half), torch.zeros(7, 32), torch.ones(64)
+
+    def qk(q=q, k=q[:, :2], qo=q.clone(), ko=q[:, :2].clone(), gq=g, gk=g, cos=t, sin=t, pos=None):
+        K.qk_norm_rope(q, k, qo, ko, K.NORM_RMS, gq, gk, None, None, cos, sin, pos)
+
+    qk()
+    qk(pos=torch.zeros(5, dtype=torch.int32))
+    for kw in (dict(k=q[:4]), dict(q=q.float()), dict(qo=q.bfloat16()), dict(ko=q), dict(gq=g[:32]), dict(sin=t[:, :16]),
+               dict(cos=t.half(), sin=t.half()), dict(pos=torch.zeros(4, dtype=torch.int64)), dict(pos=torch.zeros(5)),
+               dict(qo=q.as_strided((5, 4, 64), (64, 320, 1)))):
+        with pytest.raises(RuntimeError):
+            qk(**kw)
+    with pytest.raises(RuntimeError, match="GPU tensors"):
+        monkeypatch.undo()
+        K.dequant_mx4(*a, torch.zeros(3, 256))
+
+
+def test_op_schemas():
+    ops = K.kernels()
+    assert "Tensor(a!) out, Tensor(b!) scale, bool rotate=True" in str(ops.quant_mx4.default._schema)
+    assert "Tensor(a!) out, int epi, int stages=0, Tensor? residual=None" in str(ops.gemm_mx4.default._schema)
+    assert "Tensor(a!) q_out, Tensor(b!) k_out, int norm" in str(ops.qk_norm_rope.default._schema)
+    assert "Tensor(a!) out" in str(ops.dequant_mx4.default._schema)

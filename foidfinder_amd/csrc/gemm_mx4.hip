@@ -12,6 +12,7 @@
 // The product is computed transposed (W is the row operand), so that a lane holds one output row m and runs of four
 // consecutive columns n: column pairs (SwiGLU) are in-lane and stores are whole runs.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "gemm_common.h"
@@ -162,8 +163,243 @@ __global__ __launch_bounds__(256) void gemm_mx4_split_kernel(const Mx4Args args)
   finish4<EPI, T>(args, m0 + r, n0 + c, y);
 }
 
+// ---------------- tiles from an LDS ring ----------------
+//
+// BM x BN tiles, WAVES_M x WAVES_N waves, a ring of S slots that hold one unit (128 columns of K) of the tile's rows: 64
+// bytes of codes a row, in 16-byte chunks swizzled against bank conflicts, and the rows' exponent words behind them. Buffer
+// loads fill the slots without passing through registers; rows past the matrix read as zeros.
+template <int BM, int BN>
+constexpr int slot_bytes() {
+  return (BM + BN) * 68;
+}
+
+// Physical 16-byte chunk of a row's chunk c: the 16 rows that one read pass touches land in 16 distinct slots of 256 bytes.
+__device__ __forceinline__ int mx4_swz(int row, int c) { return row * 64 + ((c ^ ((row >> 2) & 3)) << 4); }
+
+__device__ __forceinline__ void word_to_lds(const void* base, int nbytes, uint8_t* lds_dst, uint32_t voff) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, nbytes, RSRC_WORD3);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)lds_dst, 4, voff, 0, 0, 0);
+}
+
+// The epilogue of one wave's rows m_base .. and columns n_base ..: acc[i][j][4 q + t] is row m_base + 32 j + lane % 32, column
+// n_base + 32 i + 8 q + 4 (lane / 32) + t. 32 rows at a time the results go through the wave's own LDS (`stage`), so that
+// global accesses are runs of a row, 16 bytes a lane.
+template <int EPI, typename T, int NI>
+constexpr int mx4_stage_row() {
+  return (EPI == FF_EPI_SWIGLU ? NI * 16 : NI * 32) * static_cast<int>(sizeof(T)) + 16;
+}
+
+template <int EPI, typename T, int NI, int MI>
+__device__ __forceinline__ void store_tile(const float16_t (&acc)[NI][MI], int m_base, int n_base, int lane,
+                                           const Mx4Args& args, uint8_t* stage, const float* bias) {
+  constexpr bool SWI = EPI == FF_EPI_SWIGLU;
+  constexpr int RB = mx4_stage_row<EPI, T, NI>(), COLS = SWI ? NI * 16 : NI * 32;
+  constexpr int E = 16 / static_cast<int>(sizeof(T));  // values of a 16-byte run
+  constexpr int LPR = COLS / E, RPP = 64 / LPR;        // lanes a row, rows a pass
+  typedef T run_t __attribute__((ext_vector_type(E)));
+  const int fr = lane & 31, fh = lane >> 5;
+  const int ld = SWI ? args.N >> 1 : args.N, n0 = SWI ? n_base >> 1 : n_base;
+  const int n = n0 + (lane % LPR) * E, r0 = lane / LPR;
+  const bool runs = (ld & (4 / sizeof(T) - 1)) == 0 && n + E <= ld;  // 4-byte aligned rows, the run inside them
+  float4_t b[NI][4];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) b[i][q] = *reinterpret_cast<const float4_t*>(bias + 32 * i + 8 * q + 4 * fh);
+#pragma unroll
+  for (int j = 0; j < MI; ++j) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float y[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          y[t] = acc[i][j][4 * q + t] + b[i][q][t];
+          if constexpr (EPI == FF_EPI_GELU_F16) y[t] = gelu_tanh(y[t]);
+        }
+        const int c = 32 * i + 8 * q + 4 * fh;
+        if constexpr (SWI) {
+          typedef T two_t __attribute__((ext_vector_type(2)));
+          *reinterpret_cast<two_t*>(stage + fr * RB + c) =
+              two_t{static_cast<T>(silu(y[0]) * y[1]), static_cast<T>(silu(y[2]) * y[3])};
+        } else if constexpr (EPI == FF_EPI_RESIDUAL) {
+          // y itself: the sum with the residual is rounded once
+          *reinterpret_cast<float4_t*>(stage + fr * (NI * 128 + 16) + 4 * c) = float4_t{y[0], y[1], y[2], y[3]};
+        } else {
+          *reinterpret_cast<vec4_t<T>*>(stage + fr * RB + c * static_cast<int>(sizeof(T))) =
+              vec4_t<T>{static_cast<T>(y[0]), static_cast<T>(y[1]), static_cast<T>(y[2]), static_cast<T>(y[3])};
+        }
+      }
+#pragma unroll
+    for (int p = 0; p < 32 / RPP; ++p) {
+      const int r = p * RPP + r0, m = m_base + 32 * j + r;
+      run_t h;
+      if (m < args.M && n < ld) {
+        const int64_t at = static_cast<int64_t>(m) * ld + n;
+        T* o = static_cast<T*>(args.out) + at;
+        if constexpr (EPI == FF_EPI_RESIDUAL) {
+          const float* y = reinterpret_cast<const float*>(stage + r * (NI * 128 + 16)) + (lane % LPR) * E;
+          const T* x = static_cast<const T*>(args.residual) + at;
+          if (runs) {
+            run_t xv;
+            __builtin_memcpy(&xv, x, 16);
+#pragma unroll
+            for (int e = 0; e < E; ++e) h[e] = static_cast<T>(y[e] + static_cast<float>(xv[e]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) h[e] = static_cast<T>(y[e] + (n + e < ld ? static_cast<float>(x[e]) : 0.f));
+          }
+        } else {
+          h = *reinterpret_cast<const run_t*>(stage + r * RB + (lane % LPR) * 16);
+        }
+        if (runs) {
+          __builtin_memcpy(o, &h, 16);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (n + e < ld) o[e] = h[e];
+        }
+      }
+    }
+  }
+}
+
+template <int EPI, typename T, int BM, int BN, int WAVES_M, int WAVES_N, int S>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gemm_mx4_ring_kernel(const Mx4Args args) {
+  constexpr int WAVES = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 32, NI = WN / 32;
+  constexpr int SLOT = slot_bytes<BM, BN>(), CODES = (BM + BN) * 64;
+  constexpr int BLOCKS = CODES / 1024, A_BLOCKS = BM * 64 / 1024;  // 1 KB blocks (16 rows) of a slot; A's come first
+  constexpr int LOADS = BLOCKS / WAVES;                            // of them a wave loads
+  constexpr int WORDS = (BM + BN) / 64, WLOADS = (WORDS + WAVES - 1) / WAVES;  // 64-row runs of exponent words
+  static_assert(BLOCKS % WAVES == 0 && BM % 64 == 0 && BN % 64 == 0, "even shares");
+  constexpr int STAGE = 32 * (EPI == FF_EPI_RESIDUAL ? NI * 128 + 16 : mx4_stage_row<EPI, T, NI>());
+  static_assert(WAVES * STAGE + BN * 4 <= S * SLOT, "staging must fit in the ring");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S * SLOT];
+  const int tid = threadIdx.x, lane = tid & 63, fr = lane & 31, fh = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+  const int M = args.M, N = args.N;
+  // tiles in groups of 8 row tiles by all column tiles, so that what runs at once on an XCD shares rows and columns
+  const int tiles_m = (M + BM - 1) / BM, tiles_n = (N + BN - 1) / BN;
+  const int t = xcd_remap(blockIdx.x, gridDim.x);
+  const int g = t / (8 * tiles_n), in_g = t % (8 * tiles_n), gm = min(8, tiles_m - 8 * g);
+  const int m0 = (8 * g + in_g % gm) * BM, n0 = in_g / gm * BN;
+  const int kb = args.K >> 1, units = args.K >> 7;
+
+  uint32_t voff[LOADS];
+#pragma unroll
+  for (int p = 0; p < LOADS; ++p) {
+    const int blk = wave * LOADS + p, row = (blk < A_BLOCKS ? blk : blk - A_BLOCKS) * 16 + (lane >> 2);
+    voff[p] = static_cast<uint32_t>(row * kb + mx4_swz(row, lane & 3) - row * 64);
+  }
+  const int64_t a_rows = static_cast<int64_t>(M - m0) * kb, w_rows = static_cast<int64_t>(N - n0) * kb;
+  const int a_words = buf_bytes(4ll * (M - m0)), w_words = buf_bytes(4ll * (N - n0));
+  auto issue = [&](int u) __attribute__((always_inline)) {
+    uint8_t* st = smem + (u % S) * SLOT;
+    const uint8_t* ab = args.A + static_cast<int64_t>(m0) * kb + 64 * u;
+    const uint8_t* wb = args.W + static_cast<int64_t>(n0) * kb + 64 * u;
+    const int an = buf_bytes(a_rows - 64 * u), wn_ = buf_bytes(w_rows - 64 * u);
+#pragma unroll
+    for (int p = 0; p < LOADS; ++p) {
+      const int blk = wave * LOADS + p;
+      buffer_to_lds(blk < A_BLOCKS ? ab : wb, blk < A_BLOCKS ? an : wn_, st + blk * 1024, voff[p]);
+    }
+    const uint32_t* as = args.a_scale + static_cast<int64_t>(u) * M + m0;
+    const uint32_t* ws = args.w_scale + static_cast<int64_t>(u) * N + n0;
+#pragma unroll
+    for (int p = 0; p < WLOADS; ++p) {
+      const int i = min(wave * WLOADS + p, WORDS - 1);  // a run past the last loads the last one once more
+      const bool a = i < BM / 64;
+      word_to_lds(a ? as : ws, a ? a_words : w_words, st + CODES + i * 256, 4u * ((a ? i : i - BM / 64) * 64 + lane));
+    }
+  };
+
+  float16_t acc[NI][MI] = {};
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s)
+    if (s < units) issue(s);
+
+  int4_t xw[2][NI], ya[2][MI];
+  uint32_t sw[NI], sa[MI];
+  auto read_frags = [&](const uint8_t* st, int step, int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      xw[b][i] = *reinterpret_cast<const int4_t*>(st + BM * 64 + mx4_swz(wn * WN + 32 * i + fr, 2 * fh + step));
+#pragma unroll
+    for (int j = 0; j < MI; ++j)
+      ya[b][j] = *reinterpret_cast<const int4_t*>(st + mx4_swz(wm * WM + 32 * j + fr, 2 * fh + step));
+  };
+  auto read_words = [&](const uint8_t* slot) __attribute__((always_inline)) {  // the two exponents of the lane's half
+    const uint8_t* st = slot + CODES + 2 * fh;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) sw[i] = *reinterpret_cast<const uint16_t*>(st + 4 * (BM + wn * WN + 32 * i + fr));
+#pragma unroll
+    for (int j = 0; j < MI; ++j) sa[j] = *reinterpret_cast<const uint16_t*>(st + 4 * (wm * WM + 32 * j + fr));
+  };
+  auto mfmas = [&](auto step) __attribute__((always_inline)) {
+    constexpr int b = decltype(step)::value;
+#pragma unroll
+    for (int j = 0; j < MI; ++j)
+#pragma unroll
+      for (int i = 0; i < NI; ++i) acc[i][j] = mfma_mx4<b>(xw[b][i], ya[b][j], acc[i][j], sw[i], sa[j]);
+  };
+  auto interleave = [] __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < NI + MI; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // 1 MFMA
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // 1 DS read
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, NI * MI - (NI + MI), 0);
+  };
+  if (units >= S - 1)
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * (LOADS + WLOADS)) : "memory");
+  else
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  read_frags(smem, 0, 0);
+  read_words(smem);
+  // One unit: the second half's fragments are read under the first half's products, the next unit's first half (after its
+  // barrier) under the second half's. On the last unit that reads a stale slot and is not used.
+  auto unit = [&](int u, auto steady) __attribute__((always_inline)) {
+    if constexpr (decltype(steady)::value) issue(u + S - 1);
+    read_frags(smem + u % S * SLOT, 1, 1);
+    mfmas(std::integral_constant<int, 0>{});
+    interleave();
+    // Slot u + 1 has landed once at most the loads of the newer slots are outstanding; lgkmcnt(0): this wave's reads of older
+    // slots are complete, so that after the barrier any of them may be refilled.
+    if constexpr (decltype(steady)::value)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * (LOADS + WLOADS)) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    read_frags(smem + (u + 1) % S * SLOT, 0, 0);
+    mfmas(std::integral_constant<int, 1>{});
+    interleave();
+    read_words(smem + (u + 1) % S * SLOT);
+  };
+  int u = 0;
+  for (; u + S - 1 < units; ++u) unit(u, std::true_type{});
+  for (; u < units; ++u) unit(u, std::false_type{});
+  __syncthreads();  // every wave is done with the ring: it becomes the staging area, with the tile's bias behind it
+  float* bias = reinterpret_cast<float*>(smem + WAVES * STAGE);
+  for (int i = tid; i < BN; i += 64 * WAVES) bias[i] = args.bias && n0 + i < N ? args.bias[n0 + i] : 0.f;
+  __syncthreads();
+  store_tile<EPI, T, NI, MI>(acc, m0 + wm * WM, n0 + wn * WN, lane, args, smem + wave * STAGE, bias + wn * WN);
+}
+
+template <int EPI, typename T, int BM, int BN, int WAVES_M, int WAVES_N, int S>
+static int launch_ring(const Mx4Args& a, hipStream_t st) {
+  const int64_t tiles = static_cast<int64_t>((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
+  if (tiles > 0x7fffffff) return fail(FF_EINVAL, "gemm_mx4: too many tiles");
+  gemm_mx4_ring_kernel<EPI, T, BM, BN, WAVES_M, WAVES_N, S>
+      <<<dim3(static_cast<unsigned>(tiles)), 64 * WAVES_M * WAVES_N, 0, st>>>(a);
+  return check_launch("gemm_mx4");
+}
+
 template <int EPI, typename T>
-static int launch_mx4(const Mx4Args& a, hipStream_t st) {
+static int launch_mx4(const Mx4Args& a, int variant, hipStream_t st) {
+  if (variant == 2 || (variant == 0 && a.M > 256)) return launch_ring<EPI, T, 256, 128, 2, 2, 3>(a, st);
   const int64_t blocks = static_cast<int64_t>((a.M + 31) / 32) * ((a.N + 31) / 32);
   if (blocks > 0x7fffffff) return fail(FF_EINVAL, "gemm_mx4: too many tiles");
   gemm_mx4_split_kernel<EPI, T><<<dim3(static_cast<unsigned>(blocks)), 256, 0, st>>>(a);
@@ -171,12 +407,12 @@ static int launch_mx4(const Mx4Args& a, hipStream_t st) {
 }
 
 template <typename T>
-static int launch_mx4_epi(const Mx4Args& a, int epi, hipStream_t st) {
+static int launch_mx4_epi(const Mx4Args& a, int epi, int variant, hipStream_t st) {
   switch (epi) {
-    case FF_EPI_RESIDUAL: return launch_mx4<FF_EPI_RESIDUAL, T>(a, st);
-    case FF_EPI_GELU_F16: return launch_mx4<FF_EPI_GELU_F16, T>(a, st);
-    case FF_EPI_SWIGLU: return launch_mx4<FF_EPI_SWIGLU, T>(a, st);
-    default: return launch_mx4<FF_EPI_BIAS_F16, T>(a, st);
+    case FF_EPI_RESIDUAL: return launch_mx4<FF_EPI_RESIDUAL, T>(a, variant, st);
+    case FF_EPI_GELU_F16: return launch_mx4<FF_EPI_GELU_F16, T>(a, variant, st);
+    case FF_EPI_SWIGLU: return launch_mx4<FF_EPI_SWIGLU, T>(a, variant, st);
+    default: return launch_mx4<FF_EPI_BIAS_F16, T>(a, variant, st);
   }
 }
 
@@ -208,9 +444,9 @@ extern "C" int ff_gemm_mx4(const uint8_t* A, const uint32_t* a_scale, const uint
   const Mx4Args a{A, a_scale, W, w_scale, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), bias, residual,
                   out};
   const hipStream_t st = as_stream(stream);
-  if (dtype == FF_F16) return launch_mx4_epi<half_t>(a, epi, st);
-  if (dtype == FF_BF16) return launch_mx4_epi<bf16_t>(a, epi, st);
-  return launch_mx4<FF_EPI_BIAS_F16, float>(a, st);
+  if (dtype == FF_F16) return launch_mx4_epi<half_t>(a, epi, variant, st);
+  if (dtype == FF_BF16) return launch_mx4_epi<bf16_t>(a, epi, variant, st);
+  return launch_mx4<FF_EPI_BIAS_F16, float>(a, variant, st);
 }
 
-extern "C" int ff_gemm_mx4_variants(void) { return 1; }
+extern "C" int ff_gemm_mx4_variants(void) { return 2; }

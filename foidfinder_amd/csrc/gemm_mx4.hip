@@ -165,17 +165,27 @@ __global__ __launch_bounds__(256) void gemm_mx4_split_kernel(const Mx4Args args)
 
 // ---------------- tiles from an LDS ring ----------------
 //
-// BM x BN tiles, WAVES_M x WAVES_N waves, a ring of S slots that hold one unit (128 columns of K) of the tile's rows: 64
-// bytes of codes a row, in 16-byte chunks swizzled against bank conflicts, and the rows' exponent words behind them. Buffer
-// loads fill the slots without passing through registers; rows past the matrix read as zeros.
-template <int BM, int BN>
+// BM x BN tiles, WAVES_M x WAVES_N waves, a ring of S slots that hold U units of the tile's rows: 64 U bytes of codes a row,
+// in 16-byte chunks swizzled against bank conflicts, and the units' exponent words behind them. Buffer loads fill the slots
+// without passing through registers; rows past the matrix read as zeros.
+template <int BM, int BN, int U>
 constexpr int slot_bytes() {
-  return (BM + BN) * 68;
+  return (BM + BN) * 68 * U;
 }
 
 // Physical 16-byte chunk of a row's chunk c: the 16 rows that one read pass touches land in 16 distinct slots of 256 bytes.
-__device__ __forceinline__ int mx4_swz(int row, int c) { return row * 64 + ((c ^ ((row >> 2) & 3)) << 4); }
+template <int U>
+__device__ __forceinline__ int mx4_swz(int row, int c) {
+  if constexpr (U == 1)
+    return row * 64 + ((c ^ ((row >> 2) & 3)) << 4);
+  else
+    return row * 128 + ((c ^ ((row >> 1) & 7)) << 4);
+}
 
+__device__ __forceinline__ void buffer_to_lds_at(const void* base, int nbytes, uint8_t* lds_dst, uint32_t voff, int soff) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, nbytes, RSRC_WORD3);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)lds_dst, 16, voff, soff, 0, 0);
+}
 __device__ __forceinline__ void word_to_lds(const void* base, int nbytes, uint8_t* lds_dst, uint32_t voff) {
   const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, nbytes, RSRC_WORD3);
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)lds_dst, 4, voff, 0, 0, 0);
@@ -189,9 +199,11 @@ constexpr int mx4_stage_row() {
   return (EPI == FF_EPI_SWIGLU ? NI * 16 : NI * 32) * static_cast<int>(sizeof(T)) + 16;
 }
 
-template <int EPI, typename T, int NI, int MI>
+// Rows past M are dropped by the descriptor's range. WHOLE: every run lies inside the rows and is 4-byte aligned (no masks);
+// otherwise runs that do not are taken value by value.
+template <int EPI, typename T, int NI, int MI, bool WHOLE>
 __device__ __forceinline__ void store_tile(const float16_t (&acc)[NI][MI], int m_base, int n_base, int lane,
-                                           const Mx4Args& args, uint8_t* stage, const float* bias) {
+                                           const Mx4Args& args, uint8_t* stage) {
   constexpr bool SWI = EPI == FF_EPI_SWIGLU;
   constexpr int RB = mx4_stage_row<EPI, T, NI>(), COLS = SWI ? NI * 16 : NI * 32;
   constexpr int E = 16 / static_cast<int>(sizeof(T));  // values of a 16-byte run
@@ -200,81 +212,92 @@ __device__ __forceinline__ void store_tile(const float16_t (&acc)[NI][MI], int m
   const int fr = lane & 31, fh = lane >> 5;
   const int ld = SWI ? args.N >> 1 : args.N, n0 = SWI ? n_base >> 1 : n_base;
   const int n = n0 + (lane % LPR) * E, r0 = lane / LPR;
-  const bool runs = (ld & (4 / sizeof(T) - 1)) == 0 && n + E <= ld;  // 4-byte aligned rows, the run inside them
-  float4_t b[NI][4];
+  const bool run = WHOLE || ((ld & (4 / static_cast<int>(sizeof(T)) - 1)) == 0 && n + E <= ld);
+  const int64_t first = static_cast<int64_t>(m_base) * ld;
+  const int bytes = buf_bytes((static_cast<int64_t>(args.M) * ld - first) * static_cast<int64_t>(sizeof(T)));
+  T* out = static_cast<T*>(args.out) + first;
+  const T* res = static_cast<const T*>(args.residual) + first;
+  const uint32_t pitch = static_cast<uint32_t>(ld) * sizeof(T);  // at most 2^23: a wave's rows stay below 2^31 bytes
+  const uint32_t off = r0 * pitch + n * static_cast<uint32_t>(sizeof(T));
+  // The residual's rows of block j, as the store phase walks them; they go through the staging area into the lanes that hold
+  // the sums, so that sum and residual are rounded once.
+  run_t x[32 / RPP];
+  auto load_residual = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+    for (int p = 0; p < 32 / RPP; ++p) {
+      const uint32_t at = off + (32 * j + p * RPP) * pitch;
+      if (run) {
+        x[p] = __builtin_bit_cast(run_t, buf_load_f4(res, bytes, at));
+      } else {
+        x[p] = run_t{};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) b[i][q] = *reinterpret_cast<const float4_t*>(bias + 32 * i + 8 * q + 4 * fh);
+        for (int e = 0; e < E; ++e)
+          if (m_base + 32 * j + p * RPP + r0 < args.M && n + e < ld)
+            x[p][e] = res[static_cast<int64_t>(32 * j + p * RPP + r0) * ld + n + e];
+      }
+    }
+  };
+  if constexpr (EPI == FF_EPI_RESIDUAL) load_residual(0);
 #pragma unroll
   for (int j = 0; j < MI; ++j) {
+    if constexpr (EPI == FF_EPI_RESIDUAL) {
+#pragma unroll
+      for (int p = 0; p < 32 / RPP; ++p)
+        *reinterpret_cast<run_t*>(stage + (p * RPP + r0) * RB + (lane % LPR) * 16) = x[p];
+      if (j + 1 < MI) load_residual(j + 1);
+    }
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
+        const int c = 32 * i + 8 * q + 4 * fh;
         float y[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          y[t] = acc[i][j][4 * q + t] + b[i][q][t];
+          y[t] = acc[i][j][4 * q + t];
           if constexpr (EPI == FF_EPI_GELU_F16) y[t] = gelu_tanh(y[t]);
         }
-        const int c = 32 * i + 8 * q + 4 * fh;
         if constexpr (SWI) {
           typedef T two_t __attribute__((ext_vector_type(2)));
           *reinterpret_cast<two_t*>(stage + fr * RB + c) =
               two_t{static_cast<T>(silu(y[0]) * y[1]), static_cast<T>(silu(y[2]) * y[3])};
-        } else if constexpr (EPI == FF_EPI_RESIDUAL) {
-          // y itself: the sum with the residual is rounded once
-          *reinterpret_cast<float4_t*>(stage + fr * (NI * 128 + 16) + 4 * c) = float4_t{y[0], y[1], y[2], y[3]};
         } else {
-          *reinterpret_cast<vec4_t<T>*>(stage + fr * RB + c * static_cast<int>(sizeof(T))) =
-              vec4_t<T>{static_cast<T>(y[0]), static_cast<T>(y[1]), static_cast<T>(y[2]), static_cast<T>(y[3])};
+          vec4_t<T>* at = reinterpret_cast<vec4_t<T>*>(stage + fr * RB + c * static_cast<int>(sizeof(T)));
+          if constexpr (EPI == FF_EPI_RESIDUAL) {
+            const vec4_t<T> r = *at;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) y[t] = y[t] + static_cast<float>(r[t]);
+          }
+          *at = vec4_t<T>{static_cast<T>(y[0]), static_cast<T>(y[1]), static_cast<T>(y[2]), static_cast<T>(y[3])};
         }
       }
 #pragma unroll
     for (int p = 0; p < 32 / RPP; ++p) {
-      const int r = p * RPP + r0, m = m_base + 32 * j + r;
-      run_t h;
-      if (m < args.M && n < ld) {
-        const int64_t at = static_cast<int64_t>(m) * ld + n;
-        T* o = static_cast<T*>(args.out) + at;
-        if constexpr (EPI == FF_EPI_RESIDUAL) {
-          const float* y = reinterpret_cast<const float*>(stage + r * (NI * 128 + 16)) + (lane % LPR) * E;
-          const T* x = static_cast<const T*>(args.residual) + at;
-          if (runs) {
-            run_t xv;
-            __builtin_memcpy(&xv, x, 16);
+      const run_t h = *reinterpret_cast<const run_t*>(stage + (p * RPP + r0) * RB + (lane % LPR) * 16);
+      if (run) {
+        buf_store_h8(__builtin_bit_cast(half8_t, h), out, bytes, off + (32 * j + p * RPP) * pitch);
+      } else if (m_base + 32 * j + p * RPP + r0 < args.M) {
+        T* o = out + static_cast<int64_t>(32 * j + p * RPP + r0) * ld + n;
 #pragma unroll
-            for (int e = 0; e < E; ++e) h[e] = static_cast<T>(y[e] + static_cast<float>(xv[e]));
-          } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) h[e] = static_cast<T>(y[e] + (n + e < ld ? static_cast<float>(x[e]) : 0.f));
-          }
-        } else {
-          h = *reinterpret_cast<const run_t*>(stage + r * RB + (lane % LPR) * 16);
-        }
-        if (runs) {
-          __builtin_memcpy(o, &h, 16);
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (n + e < ld) o[e] = h[e];
-        }
+        for (int e = 0; e < E; ++e)
+          if (n + e < ld) o[e] = h[e];
       }
     }
   }
 }
 
-template <int EPI, typename T, int BM, int BN, int WAVES_M, int WAVES_N, int S>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gemm_mx4_ring_kernel(const Mx4Args args) {
+template <int EPI, typename T, int BM, int BN, int WAVES_M, int WAVES_N, int U, int S, int OCC>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, OCC) void gemm_mx4_ring_kernel(const Mx4Args args) {
   constexpr int WAVES = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, MI = WM / 32, NI = WN / 32;
-  constexpr int SLOT = slot_bytes<BM, BN>(), CODES = (BM + BN) * 64;
-  constexpr int BLOCKS = CODES / 1024, A_BLOCKS = BM * 64 / 1024;  // 1 KB blocks (16 rows) of a slot; A's come first
+  constexpr int ROW = 64 * U, SLOT = slot_bytes<BM, BN, U>(), CODES = (BM + BN) * ROW;
+  constexpr int CPR = ROW / 16;                                    // 16-byte chunks of a row
+  constexpr int BLOCKS = CODES / 1024, A_BLOCKS = BM * ROW / 1024;  // 1 KB blocks of a slot; A's come first
   constexpr int LOADS = BLOCKS / WAVES;                            // of them a wave loads
-  constexpr int WORDS = (BM + BN) / 64, WLOADS = (WORDS + WAVES - 1) / WAVES;  // 64-row runs of exponent words
+  constexpr int RUNS = (BM + BN) / 64, WORDS = U * RUNS;           // 64-row runs of exponent words, plane by plane
+  constexpr int WLOADS = (WORDS + WAVES - 1) / WAVES;
   static_assert(BLOCKS % WAVES == 0 && BM % 64 == 0 && BN % 64 == 0, "even shares");
-  constexpr int STAGE = 32 * (EPI == FF_EPI_RESIDUAL ? NI * 128 + 16 : mx4_stage_row<EPI, T, NI>());
-  static_assert(WAVES * STAGE + BN * 4 <= S * SLOT, "staging must fit in the ring");
+  constexpr int STAGE = 32 * mx4_stage_row<EPI, T, NI>();
+  static_assert(WAVES * STAGE <= S * SLOT, "staging must fit in the ring");
   __shared__ __attribute__((aligned(1024))) uint8_t smem[S * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, fr = lane & 31, fh = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -285,57 +308,91 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gemm_mx4_ring_kerne
   const int t = xcd_remap(blockIdx.x, gridDim.x);
   const int g = t / (8 * tiles_n), in_g = t % (8 * tiles_n), gm = min(8, tiles_m - 8 * g);
   const int m0 = (8 * g + in_g % gm) * BM, n0 = in_g / gm * BN;
-  const int kb = args.K >> 1, units = args.K >> 7;
+  const int kb = args.K >> 1, units = args.K >> 7, slots = (units + U - 1) / U;
 
   uint32_t voff[LOADS];
 #pragma unroll
   for (int p = 0; p < LOADS; ++p) {
-    const int blk = wave * LOADS + p, row = (blk < A_BLOCKS ? blk : blk - A_BLOCKS) * 16 + (lane >> 2);
-    voff[p] = static_cast<uint32_t>(row * kb + mx4_swz(row, lane & 3) - row * 64);
+    const int blk = wave * LOADS + p, row = (blk < A_BLOCKS ? blk : blk - A_BLOCKS) * (1024 / ROW) + lane / CPR;
+    voff[p] = static_cast<uint32_t>(row * kb + mx4_swz<U>(row, lane % CPR) - row * ROW);
   }
-  const int64_t a_rows = static_cast<int64_t>(M - m0) * kb, w_rows = static_cast<int64_t>(N - n0) * kb;
-  const int a_words = buf_bytes(4ll * (M - m0)), w_words = buf_bytes(4ll * (N - n0));
-  auto issue = [&](int u) __attribute__((always_inline)) {
-    uint8_t* st = smem + (u % S) * SLOT;
-    const uint8_t* ab = args.A + static_cast<int64_t>(m0) * kb + 64 * u;
-    const uint8_t* wb = args.W + static_cast<int64_t>(n0) * kb + 64 * u;
-    const int an = buf_bytes(a_rows - 64 * u), wn_ = buf_bytes(w_rows - 64 * u);
+  // The tile's rows through one descriptor an operand (at most 256 rows of 2^21 bytes), a slot by the scalar offset: rows past
+  // the matrix lie past the descriptor's end. (Behind the last unit of an odd count a slot holds what follows the row, which
+  // is never used.) The exponent words' plane of a unit has a base of its own.
+  const uint8_t* a_base = args.A + static_cast<int64_t>(m0) * kb;
+  const uint8_t* w_base = args.W + static_cast<int64_t>(n0) * kb;
+  const int a_bytes = min(BM, M - m0) * kb, w_bytes = min(BN, N - n0) * kb;
+  const int a_words = min(BM, M - m0) * 4, w_words = min(BN, N - n0) * 4;
+  const uint32_t* a_plane = args.a_scale + m0;
+  const uint32_t* w_plane = args.w_scale + n0;
+  int next = 0, next_slot = 0;  // the slot to be loaded next, and its LDS offset
+  auto issue = [&]() __attribute__((always_inline)) {
+    uint8_t* st = smem + next_slot;
 #pragma unroll
     for (int p = 0; p < LOADS; ++p) {
       const int blk = wave * LOADS + p;
-      buffer_to_lds(blk < A_BLOCKS ? ab : wb, blk < A_BLOCKS ? an : wn_, st + blk * 1024, voff[p]);
+      buffer_to_lds_at(blk < A_BLOCKS ? a_base : w_base, blk < A_BLOCKS ? a_bytes : w_bytes, st + blk * 1024, voff[p],
+                       ROW * next);
     }
-    const uint32_t* as = args.a_scale + static_cast<int64_t>(u) * M + m0;
-    const uint32_t* ws = args.w_scale + static_cast<int64_t>(u) * N + n0;
 #pragma unroll
     for (int p = 0; p < WLOADS; ++p) {
       const int i = min(wave * WLOADS + p, WORDS - 1);  // a run past the last loads the last one once more
-      const bool a = i < BM / 64;
-      word_to_lds(a ? as : ws, a ? a_words : w_words, st + CODES + i * 256, 4u * ((a ? i : i - BM / 64) * 64 + lane));
+      const int plane = i / RUNS, run = i % RUNS;
+      const bool a = run < BM / 64, in = U * next + plane < units;  // planes past the last are empty
+      word_to_lds((a ? a_plane : w_plane) + (in ? static_cast<int64_t>(plane) * (a ? M : N) : 0),
+                  in ? (a ? a_words : w_words) : 0, st + CODES + i * 256, 4u * ((a ? run : run - BM / 64) * 64 + lane));
     }
+    a_plane += static_cast<int64_t>(U) * M;
+    w_plane += static_cast<int64_t>(U) * N;
+    ++next;
+    next_slot = next_slot == (S - 1) * SLOT ? 0 : next_slot + SLOT;
   };
 
-  float16_t acc[NI][MI] = {};
+  // The sums start from the bias: acc[i][j][4 q + t] is row 32 j + fr, column 32 i + 8 q + 4 fh + t of the wave's tile.
+  float16_t acc[NI][MI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = n0 + wn * WN + 32 * i + 8 * q + 4 * fh;
+      float4_t b = {};
+      if (args.bias) {
+        if ((N & 3) == 0) {
+          b = buf_load_f4(args.bias, 4 * N, 4u * n);
+        } else {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) b[t] = buf_load_f1(args.bias, 4 * N, 4u * (n + t));
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int j = 0; j < MI; ++j) acc[i][j][4 * q + t] = b[t];
+    }
 #pragma unroll
   for (int s = 0; s < S - 1; ++s)
-    if (s < units) issue(s);
+    if (s < slots) issue();
 
   int4_t xw[2][NI], ya[2][MI];
   uint32_t sw[NI], sa[MI];
-  auto read_frags = [&](const uint8_t* st, int step, int b) __attribute__((always_inline)) {
+  // the fragments of half unit k of a slot
+  auto read_frags = [&](const uint8_t* st, int k) __attribute__((always_inline)) {
+    const int c = 4 * (k >> 1) + 2 * fh + (k & 1);
 #pragma unroll
     for (int i = 0; i < NI; ++i)
-      xw[b][i] = *reinterpret_cast<const int4_t*>(st + BM * 64 + mx4_swz(wn * WN + 32 * i + fr, 2 * fh + step));
+      xw[k & 1][i] = *reinterpret_cast<const int4_t*>(st + BM * ROW + mx4_swz<U>(wn * WN + 32 * i + fr, c));
 #pragma unroll
     for (int j = 0; j < MI; ++j)
-      ya[b][j] = *reinterpret_cast<const int4_t*>(st + mx4_swz(wm * WM + 32 * j + fr, 2 * fh + step));
+      ya[k & 1][j] = *reinterpret_cast<const int4_t*>(st + mx4_swz<U>(wm * WM + 32 * j + fr, c));
   };
-  auto read_words = [&](const uint8_t* slot) __attribute__((always_inline)) {  // the two exponents of the lane's half
-    const uint8_t* st = slot + CODES + 2 * fh;
+  // the two exponents of the lane's half in a unit of a slot
+  auto read_words = [&](const uint8_t* slot, int unit, uint32_t (&w)[NI],
+                        uint32_t (&a)[MI]) __attribute__((always_inline)) {
+    const uint8_t* st = slot + CODES + unit * RUNS * 256 + 2 * fh;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) sw[i] = *reinterpret_cast<const uint16_t*>(st + 4 * (BM + wn * WN + 32 * i + fr));
+    for (int i = 0; i < NI; ++i) w[i] = *reinterpret_cast<const uint16_t*>(st + 4 * (BM + wn * WN + 32 * i + fr));
 #pragma unroll
-    for (int j = 0; j < MI; ++j) sa[j] = *reinterpret_cast<const uint16_t*>(st + 4 * (wm * WM + 32 * j + fr));
+    for (int j = 0; j < MI; ++j) a[j] = *reinterpret_cast<const uint16_t*>(st + 4 * (wm * WM + 32 * j + fr));
   };
   auto mfmas = [&](auto step) __attribute__((always_inline)) {
     constexpr int b = decltype(step)::value;
@@ -344,62 +401,97 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 2) void gemm_mx4_ring_kerne
 #pragma unroll
       for (int i = 0; i < NI; ++i) acc[i][j] = mfma_mx4<b>(xw[b][i], ya[b][j], acc[i][j], sw[i], sa[j]);
   };
-  auto interleave = [] __attribute__((always_inline)) {
+  auto interleave = [](auto per) __attribute__((always_inline)) {  // `per` LDS reads after each product
+    constexpr int n = NI + MI < NI * MI ? NI + MI : NI * MI;
 #pragma unroll
-    for (int x = 0; x < NI + MI; ++x) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // 1 MFMA
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // 1 DS read
+    for (int x = 0; x < n; ++x) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                    // 1 MFMA
+      __builtin_amdgcn_sched_group_barrier(0x100, decltype(per)::value, 0);  // DS reads
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, NI * MI - (NI + MI), 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, NI * MI - n, 0);
   };
-  if (units >= S - 1)
+  if (slots >= S - 1)
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * (LOADS + WLOADS)) : "memory");
   else
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
-  read_frags(smem, 0, 0);
-  read_words(smem);
-  // One unit: the second half's fragments are read under the first half's products, the next unit's first half (after its
-  // barrier) under the second half's. On the last unit that reads a stale slot and is not used.
-  auto unit = [&](int u, auto steady) __attribute__((always_inline)) {
-    if constexpr (decltype(steady)::value) issue(u + S - 1);
-    read_frags(smem + u % S * SLOT, 1, 1);
-    mfmas(std::integral_constant<int, 0>{});
-    interleave();
-    // Slot u + 1 has landed once at most the loads of the newer slots are outstanding; lgkmcnt(0): this wave's reads of older
-    // slots are complete, so that after the barrier any of them may be refilled.
-    if constexpr (decltype(steady)::value)
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * (LOADS + WLOADS)) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    read_frags(smem + (u + 1) % S * SLOT, 0, 0);
-    mfmas(std::integral_constant<int, 1>{});
-    interleave();
-    read_words(smem + (u + 1) % S * SLOT);
+  read_frags(smem, 0);
+  read_words(smem, 0, sw, sa);
+  // One slot: each half unit's fragments are read under the products of the half before it, a unit's exponents under the
+  // unit before it, and the next slot's first ones (after its barrier) under this slot's last products. On the last slot
+  // that reads a stale slot and is not used.
+  int slot = 0;
+  auto step = [&](auto kc, auto steady) __attribute__((always_inline)) {
+    constexpr int k = decltype(kc)::value;
+    uint32_t nw[NI], na[MI];
+    if constexpr (k + 1 < 2 * U) {
+      if constexpr (k & 1) read_words(smem + slot, (k + 1) / 2, nw, na);
+      read_frags(smem + slot, k + 1);
+    } else {
+      // The next slot has landed once at most the loads of the newer slots are outstanding; lgkmcnt(0): this wave's reads of
+      // older slots are complete, so that after the barrier any of them may be refilled.
+      if constexpr (decltype(steady)::value)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * (LOADS + WLOADS)) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      slot = slot == (S - 1) * SLOT ? 0 : slot + SLOT;
+      read_words(smem + slot, 0, nw, na);
+      read_frags(smem + slot, 0);
+    }
+    mfmas(std::integral_constant<int, k & 1>{});
+    interleave(std::integral_constant<int, (k & 1) + 1>{});
+    if constexpr (k & 1) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) sw[i] = nw[i];
+#pragma unroll
+      for (int j = 0; j < MI; ++j) sa[j] = na[j];
+    }
+  };
+  auto whole = [&](auto steady) __attribute__((always_inline)) {
+    if constexpr (decltype(steady)::value) issue();
+    step(std::integral_constant<int, 0>{}, steady);
+    step(std::integral_constant<int, 1>{}, steady);
+    if constexpr (U == 2) {
+      step(std::integral_constant<int, 2>{}, steady);
+      step(std::integral_constant<int, 3>{}, steady);
+    }
   };
   int u = 0;
-  for (; u + S - 1 < units; ++u) unit(u, std::true_type{});
-  for (; u < units; ++u) unit(u, std::false_type{});
-  __syncthreads();  // every wave is done with the ring: it becomes the staging area, with the tile's bias behind it
-  float* bias = reinterpret_cast<float*>(smem + WAVES * STAGE);
-  for (int i = tid; i < BN; i += 64 * WAVES) bias[i] = args.bias && n0 + i < N ? args.bias[n0 + i] : 0.f;
-  __syncthreads();
-  store_tile<EPI, T, NI, MI>(acc, m0 + wm * WM, n0 + wn * WN, lane, args, smem + wave * STAGE, bias + wn * WN);
+  for (; u + S - 1 < slots; ++u) whole(std::true_type{});
+  for (; u < units / U; ++u) whole(std::false_type{});
+  if constexpr (U == 2) {
+    if (u < slots) {  // an odd unit
+      step(std::integral_constant<int, 0>{}, std::false_type{});
+      step(std::integral_constant<int, 1>{}, std::false_type{});
+    }
+  }
+  __syncthreads();  // every wave is done with the ring: it becomes the staging area
+  const int ld = EPI == FF_EPI_SWIGLU ? N >> 1 : N;
+  if (n0 + BN <= N && (ld & (4 / static_cast<int>(sizeof(T)) - 1)) == 0)
+    store_tile<EPI, T, NI, MI, true>(acc, m0 + wm * WM, n0 + wn * WN, lane, args, smem + wave * STAGE);
+  else
+    store_tile<EPI, T, NI, MI, false>(acc, m0 + wm * WM, n0 + wn * WN, lane, args, smem + wave * STAGE);
 }
 
-template <int EPI, typename T, int BM, int BN, int WAVES_M, int WAVES_N, int S>
+template <int EPI, typename T, int BM, int BN, int WAVES_M, int WAVES_N, int U, int S, int OCC>
 static int launch_ring(const Mx4Args& a, hipStream_t st) {
   const int64_t tiles = static_cast<int64_t>((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
   if (tiles > 0x7fffffff) return fail(FF_EINVAL, "gemm_mx4: too many tiles");
-  gemm_mx4_ring_kernel<EPI, T, BM, BN, WAVES_M, WAVES_N, S>
+  gemm_mx4_ring_kernel<EPI, T, BM, BN, WAVES_M, WAVES_N, U, S, OCC>
       <<<dim3(static_cast<unsigned>(tiles)), 64 * WAVES_M * WAVES_N, 0, st>>>(a);
   return check_launch("gemm_mx4");
 }
 
 template <int EPI, typename T>
 static int launch_mx4(const Mx4Args& a, int variant, hipStream_t st) {
-  if (variant == 2 || (variant == 0 && a.M > 256)) return launch_ring<EPI, T, 256, 128, 2, 2, 3>(a, st);
+  switch (variant ? variant : (a.M > 256 ? 4 : 1)) {
+    case 2: return launch_ring<EPI, T, 64, 64, 2, 2, 2, 3, 3>(a, st);
+    case 3: return launch_ring<EPI, T, 128, 128, 2, 2, 1, 3, 3>(a, st);
+    case 4: return launch_ring<EPI, T, 256, 128, 2, 2, 1, 3, 2>(a, st);
+    case 5: return launch_ring<EPI, T, 256, 256, 2, 4, 1, 3, 2>(a, st);
+    default: break;
+  }
   const int64_t blocks = static_cast<int64_t>((a.M + 31) / 32) * ((a.N + 31) / 32);
   if (blocks > 0x7fffffff) return fail(FF_EINVAL, "gemm_mx4: too many tiles");
   gemm_mx4_split_kernel<EPI, T><<<dim3(static_cast<unsigned>(blocks)), 256, 0, st>>>(a);
@@ -449,4 +541,4 @@ extern "C" int ff_gemm_mx4(const uint8_t* A, const uint32_t* a_scale, const uint
   return launch_mx4<FF_EPI_BIAS_F16, float>(a, variant, st);
 }
 
-extern "C" int ff_gemm_mx4_variants(void) { return 2; }
+extern "C" int ff_gemm_mx4_variants(void) { return 5; }

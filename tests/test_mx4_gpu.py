@@ -158,7 +158,7 @@ def test_dequant_mx4_exact(dev, rng, kind):
 
 # ---- product ----
 
-VARIANTS = [0, 1, 2]
+VARIANTS = [0, 1, 2, 3, 4, 5]
 SHAPES = [(1, 1, 128), (1, 2304, 768), (3, 17, 256), (16, 1000, 1152), (33, 31, 384), (64, 66, 128), (130, 257, 640),
           (300, 1024, 2816), (257, 514, 1024), (1025, 768, 1024)]
 

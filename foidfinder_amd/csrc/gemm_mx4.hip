@@ -37,6 +37,39 @@ __device__ __forceinline__ uint32_t buf_load_u32(const void* base, int nbytes, u
   return __builtin_bit_cast(uint32_t, buf_load_f1(base, nbytes, voff));
 }
 
+__device__ __forceinline__ uint16_t buf_load_u16(const void* base, int nbytes, uint32_t voff) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, nbytes, RSRC_WORD3);
+  return __builtin_amdgcn_raw_buffer_load_b16(r, voff, 0, 0);
+}
+__device__ __forceinline__ void buf_store_u32(uint32_t v, void* base, int nbytes, uint32_t voff) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(base, 0, nbytes, RSRC_WORD3);
+  __builtin_amdgcn_raw_buffer_store_b32(v, r, voff, 0, 0);
+}
+__device__ __forceinline__ void buf_store_u16(uint16_t v, void* base, int nbytes, uint32_t voff) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(base, 0, nbytes, RSRC_WORD3);
+  __builtin_amdgcn_raw_buffer_store_b16(v, r, voff, 0, 0);
+}
+
+// One lane's run (16, 4 or 2 bytes) through a descriptor.
+template <typename R>
+__device__ __forceinline__ R buf_load_run(const void* base, int nbytes, uint32_t voff) {
+  if constexpr (sizeof(R) == 16)
+    return __builtin_bit_cast(R, buf_load_f4(base, nbytes, voff));
+  else if constexpr (sizeof(R) == 4)
+    return __builtin_bit_cast(R, buf_load_f1(base, nbytes, voff));
+  else
+    return __builtin_bit_cast(R, buf_load_u16(base, nbytes, voff));
+}
+template <typename R>
+__device__ __forceinline__ void buf_store_run(R v, void* base, int nbytes, uint32_t voff) {
+  if constexpr (sizeof(R) == 16)
+    buf_store_h8(__builtin_bit_cast(half8_t, v), base, nbytes, voff);
+  else if constexpr (sizeof(R) == 4)
+    buf_store_u32(__builtin_bit_cast(uint32_t, v), base, nbytes, voff);
+  else
+    buf_store_u16(__builtin_bit_cast(uint16_t, v), base, nbytes, voff);
+}
+
 // D += W-fragment x A-fragment over 64 columns; S: the byte of the exponent words that holds this step's block.
 template <int S>
 __device__ __forceinline__ float16_t mfma_mx4(int4_t w, int4_t a, float16_t c, uint32_t ws, uint32_t as) {
@@ -199,51 +232,43 @@ constexpr int mx4_stage_row() {
   return (EPI == FF_EPI_SWIGLU ? NI * 16 : NI * 32) * static_cast<int>(sizeof(T)) + 16;
 }
 
-// Rows past M are dropped by the descriptor's range. WHOLE: every run lies inside the rows and is 4-byte aligned (no masks);
-// otherwise runs that do not are taken value by value.
+// Rows past M are dropped by the descriptor's range. WHOLE: the tile's columns lie inside the rows and these are 4-byte
+// aligned; otherwise the columns are taken one a lane.
 template <int EPI, typename T, int NI, int MI, bool WHOLE>
 __device__ __forceinline__ void store_tile(const float16_t (&acc)[NI][MI], int m_base, int n_base, int lane,
                                            const Mx4Args& args, uint8_t* stage) {
   constexpr bool SWI = EPI == FF_EPI_SWIGLU;
   constexpr int RB = mx4_stage_row<EPI, T, NI>(), COLS = SWI ? NI * 16 : NI * 32;
-  constexpr int E = 16 / static_cast<int>(sizeof(T));  // values of a 16-byte run
-  constexpr int LPR = COLS / E, RPP = 64 / LPR;        // lanes a row, rows a pass
+  constexpr int E = WHOLE ? 16 / static_cast<int>(sizeof(T)) : 1;  // values of a lane's run
+  constexpr int LPR = COLS / E < 64 ? COLS / E : 64;               // lanes a row
+  constexpr int RPP = 64 / LPR, PASSES = 32 / RPP;                 // rows a pass
+  static_assert(COLS / E <= 64, "a row fits a pass");
   typedef T run_t __attribute__((ext_vector_type(E)));
   const int fr = lane & 31, fh = lane >> 5;
   const int ld = SWI ? args.N >> 1 : args.N, n0 = SWI ? n_base >> 1 : n_base;
-  const int n = n0 + (lane % LPR) * E, r0 = lane / LPR;
-  const bool run = WHOLE || ((ld & (4 / static_cast<int>(sizeof(T)) - 1)) == 0 && n + E <= ld);
+  const int c0 = (lane % LPR) * E, r0 = lane / LPR;
   const int64_t first = static_cast<int64_t>(m_base) * ld;
   const int bytes = buf_bytes((static_cast<int64_t>(args.M) * ld - first) * static_cast<int64_t>(sizeof(T)));
   T* out = static_cast<T*>(args.out) + first;
   const T* res = static_cast<const T*>(args.residual) + first;
   const uint32_t pitch = static_cast<uint32_t>(ld) * sizeof(T);  // at most 2^23: a wave's rows stay below 2^31 bytes
-  const uint32_t off = r0 * pitch + n * static_cast<uint32_t>(sizeof(T));
+  const uint32_t off = WHOLE || n0 + c0 < ld ? r0 * pitch + (n0 + c0) * static_cast<uint32_t>(sizeof(T)) : OOB_OFFSET;
+  auto at = [&](int j, int p) __attribute__((always_inline)) { return off + (32 * j + p * RPP) * pitch; };
+  T* const own = reinterpret_cast<T*>(stage + r0 * RB) + c0;  // the lane's run of a pass, RPP rows apart
   // The residual's rows of block j, as the store phase walks them; they go through the staging area into the lanes that hold
   // the sums, so that sum and residual are rounded once.
-  run_t x[32 / RPP];
+  run_t x[PASSES];
   auto load_residual = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-    for (int p = 0; p < 32 / RPP; ++p) {
-      const uint32_t at = off + (32 * j + p * RPP) * pitch;
-      if (run) {
-        x[p] = __builtin_bit_cast(run_t, buf_load_f4(res, bytes, at));
-      } else {
-        x[p] = run_t{};
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (m_base + 32 * j + p * RPP + r0 < args.M && n + e < ld)
-            x[p][e] = res[static_cast<int64_t>(32 * j + p * RPP + r0) * ld + n + e];
-      }
-    }
+    for (int p = 0; p < PASSES; ++p) x[p] = buf_load_run<run_t>(res, bytes, at(j, p));
   };
   if constexpr (EPI == FF_EPI_RESIDUAL) load_residual(0);
 #pragma unroll
   for (int j = 0; j < MI; ++j) {
     if constexpr (EPI == FF_EPI_RESIDUAL) {
 #pragma unroll
-      for (int p = 0; p < 32 / RPP; ++p)
-        *reinterpret_cast<run_t*>(stage + (p * RPP + r0) * RB + (lane % LPR) * 16) = x[p];
+      for (int p = 0; p < PASSES; ++p)
+        *reinterpret_cast<run_t*>(reinterpret_cast<uint8_t*>(own) + p * RPP * RB) = x[p];
       if (j + 1 < MI) load_residual(j + 1);
     }
 #pragma unroll
@@ -262,27 +287,19 @@ __device__ __forceinline__ void store_tile(const float16_t (&acc)[NI][MI], int m
           *reinterpret_cast<two_t*>(stage + fr * RB + c) =
               two_t{static_cast<T>(silu(y[0]) * y[1]), static_cast<T>(silu(y[2]) * y[3])};
         } else {
-          vec4_t<T>* at = reinterpret_cast<vec4_t<T>*>(stage + fr * RB + c * static_cast<int>(sizeof(T)));
+          vec4_t<T>* to = reinterpret_cast<vec4_t<T>*>(stage + fr * RB + c * static_cast<int>(sizeof(T)));
           if constexpr (EPI == FF_EPI_RESIDUAL) {
-            const vec4_t<T> r = *at;
+            const vec4_t<T> r = *to;
 #pragma unroll
             for (int t = 0; t < 4; ++t) y[t] = y[t] + static_cast<float>(r[t]);
           }
-          *at = vec4_t<T>{static_cast<T>(y[0]), static_cast<T>(y[1]), static_cast<T>(y[2]), static_cast<T>(y[3])};
+          *to = vec4_t<T>{static_cast<T>(y[0]), static_cast<T>(y[1]), static_cast<T>(y[2]), static_cast<T>(y[3])};
         }
       }
 #pragma unroll
-    for (int p = 0; p < 32 / RPP; ++p) {
-      const run_t h = *reinterpret_cast<const run_t*>(stage + (p * RPP + r0) * RB + (lane % LPR) * 16);
-      if (run) {
-        buf_store_h8(__builtin_bit_cast(half8_t, h), out, bytes, off + (32 * j + p * RPP) * pitch);
-      } else if (m_base + 32 * j + p * RPP + r0 < args.M) {
-        T* o = out + static_cast<int64_t>(32 * j + p * RPP + r0) * ld + n;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (n + e < ld) o[e] = h[e];
-      }
-    }
+    for (int p = 0; p < PASSES; ++p)
+      buf_store_run(*reinterpret_cast<const run_t*>(reinterpret_cast<const uint8_t*>(own) + p * RPP * RB), out, bytes,
+                    at(j, p));
   }
 }
 

@@ -5,8 +5,11 @@
 // p = positions[t] (or t mod L): the pair (x0, x1) becomes (x0 cos - x1 sin, x0 sin + x1 cos), pairs being neighbours
 // (2 i, 2 i + 1) or halves (i, i + R / 2); q is then multiplied by q_scale. All of it in fp32 with one rounding at the store.
 //
-// HBM-bound: 4 bytes a column (read and written once). A head is VEC columns a lane in a group of 2^k lanes of one wave: its
-// sums are lane permutes, its neighbour pairs in-lane and its halves one permute away.
+// HBM-bound: 4 bytes a column (read and written once). A lane holds 8 columns of a head in two pieces of 4 that rotate in
+// the lane: neighbour pairs lie in 8 columns in a row, halves in columns 4 c .. and R / 2 + 4 c .., so either way there is no
+// exchange between lanes but the sums' (DPP), and lane c takes the table entries 4 c .. 4 c + 3. A group of 8, 16 or 32 lanes
+// holds a head; it keeps its head and strides over the tokens, so gamma and beta stay in registers and nothing is divided in
+// the loop. The next token's columns and entries load under this one's arithmetic, its position one token earlier still.
 #include <algorithm>
 
 #include "common.h"
@@ -14,119 +17,177 @@
 namespace ff {
 
 struct QkArgs {
-  const void* x[2];       // q, k
+  const void* x[2];  // q, k
   void* out[2];
-  int64_t xt[2], xh[2];   // strides in elements: token, head
+  int64_t xt[2], xh[2];  // strides in elements: token, head
   int64_t ot[2], oh[2];
   const float* gamma[2];
   const float* beta[2];
   const float* cos;  // [L, R / 2]
   const float* sin;
-  const void* pos;   // int32 or int64 [T], or null: t mod L
-  int pos64, tokens, heads, kv, D, R, L, norm;
-  int lanes;  // lanes a head: the power of two from D / VEC up
-  float eps, q_scale;
+  const void* pos;  // int32 or int64 [T], or null: t mod L
+  int pos64, tokens, heads[2], D, R, L, norm, wide;
+  float eps, scale[2];
 };
 
-template <typename T, int VEC>
-using vec_t = T __attribute__((ext_vector_type(VEC)));
+// Sum over groups of LANES lanes, in each of them.
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v) {
+  v = v + dpp<DPP_XOR1>(v);
+  v = v + dpp<DPP_XOR3>(v);
+  v = v + dpp<DPP_XOR7>(v);
+  if constexpr (LANES > 8) v = v + dpp<DPP_XOR15>(v);
+  if constexpr (LANES > 16) v = v + swz_xor16(v);
+  return v;
+}
 
-template <typename T, int VEC, bool PAIRS>
+template <typename T, int LANES, bool PAIRS, int NORM>
 __global__ __launch_bounds__(256) void qk_norm_kernel(const QkArgs a) {
-  const int lanes = a.lanes, c = threadIdx.x & (lanes - 1);
-  const int all = a.heads + a.kv, per = 256 / lanes;
-  const bool in = c * VEC < a.D;  // lanes past the head hold zeros and take part in the permutes
-  const int half = a.R / 2, hc = half / VEC;
-  const uint32_t n = static_cast<uint32_t>(a.tokens) * all;
-  for (uint32_t i0 = blockIdx.x * per; i0 < n; i0 += gridDim.x * per) {
-    const uint32_t i = i0 + threadIdx.x / lanes;
-    const bool live = i < n;
-    const uint32_t t = live ? i / all : 0;
-    const int h = live ? i - t * all : 0;
-    const int which = h >= a.heads, hh = which ? h - a.heads : h;
-    float v[VEC] = {};
-    if (live && in) {
-      const T* p = static_cast<const T*>(a.x[which]) + t * a.xt[which] + hh * a.xh[which] + c * VEC;
-      const vec_t<T, VEC> raw = *reinterpret_cast<const vec_t<T, VEC>*>(p);
+  constexpr int GROUPS = 256 / LANES;
+  const int c = threadIdx.x % LANES, half = a.R >> 1;
+  const int chunks = a.heads[0] + a.heads[1];
+  const int id = static_cast<int>(blockIdx.x) * GROUPS + threadIdx.x / LANES;
+  const int stride = static_cast<int>(gridDim.x) * GROUPS / chunks;  // groups that share a head
+  int t = id / chunks;
+  const int head = id - t * chunks, which = head >= a.heads[0], h = which ? head - a.heads[0] : head;
+  if (t >= stride || t >= a.tokens) return;  // the groups left over
+  // the lane's pieces: turned ones below R, plain ones from there on; lanes past the head load its first columns as zeros
+  const bool in = 8 * c < a.D, turned = 8 * c < a.R;
+  const int pa = !in ? 0 : PAIRS || !turned ? 8 * c : 4 * c;
+  const int pb = !in ? 4 : PAIRS || !turned ? 8 * c + 4 : half + 4 * c;
+  const bool whole = PAIRS && a.wide;  // both pieces in one aligned 16-byte access
+  float g[8], b[8];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = static_cast<float>(raw[e]);
+  for (int e = 0; e < 8; ++e) {
+    const int col = e < 4 ? pa + e : pb + e - 4;
+    if constexpr (NORM != FF_NORM_NONE) g[e] = a.gamma[which][col];
+    if constexpr (NORM == FF_NORM_LAYER) b[e] = a.beta[which][col];
+  }
+  const float q = a.scale[which], inv_d = 1.f / static_cast<float>(a.D);
+  const T* x = static_cast<const T*>(a.x[which]) + h * a.xh[which] + t * a.xt[which] + pa;
+  T* out = static_cast<T*>(a.out[which]) + h * a.oh[which] + t * a.ot[which] + pa;
+  const int64_t xstep = stride * a.xt[which], ostep = stride * a.ot[which];
+  const int apart = pb - pa;
+  const float* cos = a.cos + (turned ? 4 * c : 0);
+  const float* sin = a.sin + (turned ? 4 * c : 0);
+
+  // The table row of a token, -1 if there is none.
+  auto position = [&](int at) __attribute__((always_inline)) {
+    if (!a.pos64) {
+      const int p = static_cast<const int32_t*>(a.pos)[at];
+      return p < a.L ? p : -1;
     }
-    int64_t row = t % a.L;
-    if (a.pos && live)
-      row = a.pos64 ? static_cast<const int64_t*>(a.pos)[t] : static_cast<const int32_t*>(a.pos)[t];
-    const bool known = row >= 0 && row < a.L;
-    if (a.norm != FF_NORM_NONE) {
-      const float d = static_cast<float>(a.D);
-      if (a.norm == FF_NORM_LAYER) {
-        float s = 0.f;
+    const int64_t p = static_cast<const int64_t*>(a.pos)[at];
+    return p >= 0 && p < a.L ? static_cast<int>(p) : -1;
+  };
+  const int wrap = stride % a.L;  // the step of t mod L
+  const int last = a.tokens - 1;
+  int row = a.pos ? position(t) : t % a.L, after = a.pos ? position(min(t + stride, last)) : 0;
+  vec4_t<T> nx[2];
+  float4_t nc, ns;
+  auto load = [&]() __attribute__((always_inline)) {
+    if (whole) {
+      const vec8_t<T> w = *reinterpret_cast<const vec8_t<T>*>(x);
+      nx[0] = vec4_t<T>{w[0], w[1], w[2], w[3]};
+      nx[1] = vec4_t<T>{w[4], w[5], w[6], w[7]};
+    } else {
+      nx[0] = *reinterpret_cast<const vec4_t<T>*>(x);
+      nx[1] = *reinterpret_cast<const vec4_t<T>*>(x + apart);
+    }
+    const int64_t entry = static_cast<int64_t>(max(row, 0)) * half;
+    nc = *reinterpret_cast<const float4_t*>(cos + entry);
+    ns = *reinterpret_cast<const float4_t*>(sin + entry);
+  };
+  load();
+  for (;;) {
+    float v[8];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) s = s + v[e];
-        for (int m = lanes >> 1; m; m >>= 1) s = s + xor_shuffle(s, m);
-        const float mean = s / d;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = in ? v[e] - mean : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = in ? static_cast<float>(nx[e >> 2][e & 3]) : 0.f;
+    const float4_t co = nc, si = ns;
+    const float f = row >= 0 ? q : __builtin_nanf("");  // no such row in the table
+    const bool more = t < a.tokens - stride;
+    if (more) {  // the next token's columns and entries, and the position of the one after it
+      t += stride;
+      x += xstep;
+      if (a.pos) {
+        row = after;
+        after = position(t < a.tokens - stride ? t + stride : last);
+      } else {
+        row += wrap;
+        row = row >= a.L ? row - a.L : row;
       }
+      load();
+    }
+    if constexpr (NORM == FF_NORM_LAYER) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = s + v[e];
+      const float mean = group_sum<LANES>(s) * inv_d;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = in ? v[e] - mean : 0.f;
+    }
+    if constexpr (NORM != FF_NORM_NONE) {
       float sq = 0.f;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sq = __builtin_fmaf(v[e], v[e], sq);
-      for (int m = lanes >> 1; m; m >>= 1) sq = sq + xor_shuffle(sq, m);
-      const float rstd = 1.f / sqrtf(sq / d + a.eps);
-      const float* g = a.gamma[which];
-      const float* b = a.beta[which];
+      for (int e = 0; e < 8; ++e) sq = __builtin_fmaf(v[e], v[e], sq);
+      const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(group_sum<LANES>(sq), inv_d, a.eps));  // about 1 ulp
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        v[e] = in ? __builtin_fmaf(v[e] * rstd, g[c * VEC + e], b ? b[c * VEC + e] : 0.f) : 0.f;
+      for (int e = 0; e < 8; ++e)
+        v[e] = NORM == FF_NORM_LAYER ? __builtin_fmaf(v[e] * r, g[e], b[e]) : v[e] * r * g[e];
     }
-    if constexpr (PAIRS) {
-      if (known && c * VEC < a.R) {
-        const float* co = a.cos + row * half + c * (VEC / 2);
-        const float* si = a.sin + row * half + c * (VEC / 2);
+    if (turned) {
 #pragma unroll
-        for (int e = 0; e < VEC / 2; ++e) {
-          const float x0 = v[2 * e], x1 = v[2 * e + 1];
-          v[2 * e] = x0 * co[e] - x1 * si[e];
-          v[2 * e + 1] = x0 * si[e] + x1 * co[e];
-        }
-      }
-    } else {
-      const bool lo = c < hc, turned = c < 2 * hc;
-      const int lane = threadIdx.x & 63, from = turned ? (lo ? lane + hc : lane - hc) : lane;
-      float w[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) w[e] = __shfl(v[e], from, 64);
-      if (known && turned) {
-        const float* co = a.cos + row * half + (lo ? c : c - hc) * VEC;
-        const float* si = a.sin + row * half + (lo ? c : c - hc) * VEC;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = lo ? v[e] * co[e] - w[e] * si[e] : w[e] * si[e] + v[e] * co[e];
+      for (int i = 0; i < 4; ++i) {
+        float &x0 = v[PAIRS ? 2 * i : i], &x1 = v[PAIRS ? 2 * i + 1 : i + 4];
+        const float y0 = __builtin_fmaf(x0, co[i], -(x1 * si[i])), y1 = __builtin_fmaf(x0, si[i], x1 * co[i]);
+        x0 = y0;
+        x1 = y1;
       }
     }
-    if (live && in) {
-      vec_t<T, VEC> o;
+    if (in) {
+      vec8_t<T> w;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float y = which ? v[e] : v[e] * a.q_scale;
-        if (!known) y = __builtin_nanf("");  // no such row in the table
-        o[e] = static_cast<T>(y);
+      for (int e = 0; e < 8; ++e) w[e] = static_cast<T>(v[e] * f);
+      if (whole) {
+        *reinterpret_cast<vec8_t<T>*>(out) = w;
+      } else {
+        *reinterpret_cast<vec4_t<T>*>(out) = vec4_t<T>{w[0], w[1], w[2], w[3]};
+        *reinterpret_cast<vec4_t<T>*>(out + apart) = vec4_t<T>{w[4], w[5], w[6], w[7]};
       }
-      T* p = static_cast<T*>(a.out[which]) + t * a.ot[which] + hh * a.oh[which] + c * VEC;
-      *reinterpret_cast<vec_t<T, VEC>*>(p) = o;
     }
+    if (!more) break;
+    out += ostep;
   }
 }
 
-template <typename T, int VEC>
-static void launch_qk(const QkArgs& a, bool pairs, hipStream_t st) {
-  const int64_t groups = (static_cast<int64_t>(a.tokens) * (a.heads + a.kv) * a.lanes + 255) / 256;
-  const void* k = pairs ? reinterpret_cast<const void*>(&qk_norm_kernel<T, VEC, true>)
-                        : reinterpret_cast<const void*>(&qk_norm_kernel<T, VEC, false>);
-  int64_t cap = resident_blocks(k, 256, 0);
+template <typename T, int LANES, bool PAIRS, int NORM>
+static void launch_qk(const QkArgs& a, hipStream_t st) {
+  constexpr int GROUPS = 256 / LANES;
+  const int64_t chunks = a.heads[0] + a.heads[1];
+  int64_t cap = resident_blocks(reinterpret_cast<const void*>(&qk_norm_kernel<T, LANES, PAIRS, NORM>), 256, 0);
   if (cap <= 0) cap = 1024;
-  const dim3 grid(static_cast<unsigned>(std::min(groups, cap)));
-  if (pairs)
-    qk_norm_kernel<T, VEC, true><<<grid, 256, 0, st>>>(a);
+  const int64_t need = (a.tokens * chunks + GROUPS - 1) / GROUPS;
+  const int64_t grid = std::max(std::min(need, cap), (chunks + GROUPS - 1) / GROUPS);  // at least a group a head
+  qk_norm_kernel<T, LANES, PAIRS, NORM><<<dim3(static_cast<unsigned>(grid)), 256, 0, st>>>(a);
+}
+
+template <typename T, int LANES, bool PAIRS>
+static void launch_qk_norm(const QkArgs& a, hipStream_t st) {
+  switch (a.norm) {
+    case FF_NORM_RMS: return launch_qk<T, LANES, PAIRS, FF_NORM_RMS>(a, st);
+    case FF_NORM_LAYER: return launch_qk<T, LANES, PAIRS, FF_NORM_LAYER>(a, st);
+    default: return launch_qk<T, LANES, PAIRS, FF_NORM_NONE>(a, st);
+  }
+}
+
+template <typename T>
+static void launch_qk_shape(const QkArgs& a, bool pairs, hipStream_t st) {
+  if (a.D <= 64)
+    pairs ? launch_qk_norm<T, 8, true>(a, st) : launch_qk_norm<T, 8, false>(a, st);
+  else if (a.D <= 128)
+    pairs ? launch_qk_norm<T, 16, true>(a, st) : launch_qk_norm<T, 16, false>(a, st);
   else
-    qk_norm_kernel<T, VEC, false><<<grid, 256, 0, st>>>(a);
+    pairs ? launch_qk_norm<T, 32, true>(a, st) : launch_qk_norm<T, 32, false>(a, st);
 }
 
 }  // namespace ff
@@ -181,17 +242,13 @@ extern "C" int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, c
   };
   if (overlaps(qo_token, qo_head, heads) || overlaps(ko_token, ko_head, kv_heads))
     return fail(FF_EINVAL, "qk_norm_rope: the rows of an output overlap");
-  QkArgs a{{q, k}, {q_out, k_out}, {q_token, k_token}, {q_head, k_head}, {qo_token, ko_token}, {qo_head, ko_head},
-           {q_gamma, k_gamma}, {q_beta, k_beta}, rope_cos, rope_sin, positions, pos64, static_cast<int>(T),
-           static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(D), static_cast<int>(R),
-           static_cast<int>(rope_len), norm, 0, eps, q_scale};
-  const bool wide = (low & 15) == 0 && (pairs || R % 16 == 0);
-  a.lanes = 1;
-  while (a.lanes * (wide ? 8 : 4) < D) a.lanes *= 2;
-  const hipStream_t st = as_stream(stream);
+  const QkArgs a{{q, k}, {q_out, k_out}, {q_token, k_token}, {q_head, k_head}, {qo_token, ko_token}, {qo_head, ko_head},
+                 {q_gamma, k_gamma}, {q_beta, k_beta}, rope_cos, rope_sin, positions, pos64, static_cast<int>(T),
+                 {static_cast<int>(heads), static_cast<int>(kv_heads)}, static_cast<int>(D), static_cast<int>(R),
+                 static_cast<int>(rope_len), norm, (low & 15) == 0, eps, {q_scale, 1.f}};
   if (dtype == FF_F16)
-    wide ? launch_qk<half_t, 8>(a, pairs != 0, st) : launch_qk<half_t, 4>(a, pairs != 0, st);
+    launch_qk_shape<half_t>(a, pairs != 0, as_stream(stream));
   else
-    wide ? launch_qk<bf16_t, 8>(a, pairs != 0, st) : launch_qk<bf16_t, 4>(a, pairs != 0, st);
+    launch_qk_shape<bf16_t>(a, pairs != 0, as_stream(stream));
   return check_launch("qk_norm_rope");
 }

@@ -18,6 +18,7 @@
 //  * the norm ((x - mean) rstd) gamma + beta with a fused last step; for the RMS norm mean = beta = 0;
 //  * the rotation's stages over column bits 0..6 ascending, then one multiplication by fp32(1 / sqrt(128)).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "rotate.h"
@@ -92,11 +93,11 @@ __global__ __launch_bounds__(256) void quant_mx4_kernel(const T* __restrict__ x,
   const int nb = C >> 7, per = (nb + 3) >> 2;  // steps of four blocks a row
   const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15, gl = l16 ^ (l16 >> 1);
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int64_t waves = static_cast<int64_t>(gridDim.x) * 4, first = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  const int64_t row_step = waves / per;
-  const int step = static_cast<int>(waves % per);
+  // the wave's first step and its stride in whole rows and steps: one 32-bit division each, none in the loop
+  const int waves = static_cast<int>(gridDim.x) * 4, first = static_cast<int>(blockIdx.x) * 4 + wave;
+  const int row_step = waves / per, step = waves - row_step * per;
   int64_t row = first / per;
-  int i = static_cast<int>(first % per);
+  int i = first - static_cast<int>(row) * per;
   while (row < rows) {
     const int b = 4 * i + g;
     float v[8] = {};
@@ -120,81 +121,160 @@ __global__ __launch_bounds__(256) void quant_mx4_kernel(const T* __restrict__ x,
   }
 }
 
-// With a norm: one row a wave, all of it in registers. gamma and beta (zeros without one) sit in LDS for the workgroup's
-// rows, zero past c_real.
-template <typename T, int NI>
+// a / n for a whole number n > 0, inv = 1 / n rounded: the quotient corrected by its exact remainder is the rounded one
+// (Markstein), in three operations instead of a division's ten.
+__device__ __forceinline__ float divide_by(float a, float n, float inv) {
+  const float q = a * inv;
+  const float c = __builtin_fmaf(__builtin_fmaf(-q, n, a), inv, q);
+  return __builtin_isfinite(q) ? c : q;
+}
+
+// Column e of the lane's eight (packed in pairs, two bytes each) plus s, in fp32 with one rounding.
+template <typename T, int E>
+__device__ __forceinline__ float plus(const uint32_t (&w)[4], float s) {
+  if constexpr (std::is_same_v<T, half_t>)
+    return add_h<E & 1>(w[E >> 1], s);
+  else
+    return __builtin_bit_cast(float, E & 1 ? w[E >> 1] & 0xffff0000u : w[E >> 1] << 16) + s;
+}
+
+// With a norm: a row on G groups of 16 lanes, 4 / G rows a wave; lane group g takes blocks G i + g. The row stays in registers
+// as it was loaded, two columns a register, and wide rows form their fp32 values anew in each pass (the sum, the squares, the
+// norm's last step): that costs one operation a column, an addition that also converts, where held values spilled (4736
+// columns of bf16: 31 us, held 46; 2816 columns: 32.6, held 33.5). gamma and beta (zeros without one) sit in LDS for the
+// workgroup's rows, zero past c_real; the first rows load ahead of them. The arithmetic bounds it: 386 vector operations a
+// row of 1024 (24 a column: 10 for the norm, 7 for the butterflies) keep the SIMDs 75 % busy, 28.5 us at 32 800 rows where
+// the rows' bytes take 16.
+template <typename T, int NI, int G>
 __global__ __launch_bounds__(256) void quant_mx4_norm_kernel(const T* __restrict__ x, int64_t x_stride, int64_t rows, int C,
                                                              int c_real, const float* __restrict__ gamma,
                                                              const float* __restrict__ beta, bool centre, float eps,
                                                              bool rotate, uint8_t* __restrict__ out,
                                                              uint32_t* __restrict__ scale) {
-  extern __shared__ float4_t gb[];  // gamma as C / 4 float4, then beta
-  const int n4 = C >> 2, nb = C >> 7;
-  for (int i = threadIdx.x; i < 2 * n4; i += 256)
-    gb[i] = i < n4 ? reinterpret_cast<const float4_t*>(gamma)[i]
-                   : (beta ? reinterpret_cast<const float4_t*>(beta)[i - n4] : float4_t{});
+  constexpr int RPW = 4 / G, ACCS = 4 / G;  // rows a wave; partial sums a lane
+  // gamma as C / 4 float4, the even ones first, then the odd ones (a lane's two lie apart and 16 lanes read 256 bytes in a
+  // row, free of bank conflicts), then beta
+  extern __shared__ float4_t gb[];
+  const int n4 = C >> 2, n8 = C >> 3, nb = C >> 7;
+  const int lane = threadIdx.x & 63, g = (lane >> 4) & (G - 1), l16 = lane & 15, gl = l16 ^ (l16 >> 1);
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 4 * RPW;
+  int64_t row = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * RPW + lane / (16 * G);
+  uint32_t w[NI][4];
+  auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int b = G * i + g;  // lanes past the row hold zeros
+      const int4_t h = G == 1 || b < nb ? *reinterpret_cast<const int4_t*>(x + row * x_stride + b * 128 + 8 * gl) : int4_t{};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[i][k] = static_cast<uint32_t>(h[k]);
+    }
+  };
+  if (row < rows) load();
+  for (int i = threadIdx.x; i < n4; i += 256) {
+    gb[(i & 1) * n8 + (i >> 1)] = reinterpret_cast<const float4_t*>(gamma)[i];
+    gb[n4 + (i & 1) * n8 + (i >> 1)] = beta ? reinterpret_cast<const float4_t*>(beta)[i] : float4_t{};
+  }
   __syncthreads();
-  const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15, gl = l16 ^ (l16 >> 1);
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * 4;
-  const float n = static_cast<float>(c_real);
-  auto tree = [](float t) __attribute__((always_inline)) {
-    t = t + xor_shuffle(t, 32);
-    t = t + swz_xor16(t);
+  const float n = static_cast<float>(c_real), inv_n = 1.f / n;
+  const int real = c_real - g * 128 - 8 * gl;  // the lane's columns of block G i + g below c_real: real - 128 G i, 0 .. 8
+  // x + s for the lane's columns of block group i into d, zero past c_real; only groups that reach past it mask (uniform)
+  auto shifted = [&](int i, float s, float (&d)[8]) __attribute__((always_inline)) {
+    d[0] = plus<T, 0>(w[i], s), d[1] = plus<T, 1>(w[i], s), d[2] = plus<T, 2>(w[i], s), d[3] = plus<T, 3>(w[i], s);
+    d[4] = plus<T, 4>(w[i], s), d[5] = plus<T, 5>(w[i], s), d[6] = plus<T, 6>(w[i], s), d[7] = plus<T, 7>(w[i], s);
+    if ((G * i + G) * 128 > c_real) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = e < real - 128 * G * i ? d[e] : 0.f;
+    }
+  };
+  // Hides that the words are the previous pass's: without it the compiler keeps that pass's fp32 values in registers.
+  auto anew = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) asm("" : "+v"(w[i][k]));
+  };
+  // the 64 partial sums of a row folded in halves
+  auto fold = [](const float (&a)[ACCS]) __attribute__((always_inline)) {
+    float t;
+    if constexpr (G == 1) {
+      t = (a[0] + a[2]) + (a[1] + a[3]);
+    } else if constexpr (G == 2) {
+      t = a[0] + a[1];
+      t = t + swz_xor16(t);
+    } else {
+      t = a[0] + xor_shuffle(a[0], 32);
+      t = t + swz_xor16(t);
+    }
     t = t + dpp<DPP_XOR15>(t);
     t = t + dpp<DPP_XOR7>(t);
     t = t + dpp<DPP_XOR3>(t);
     return t + dpp<DPP_XOR1>(t);
   };
-  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); row < rows; row += stride) {
-    float v[8 * NI];
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int b = 4 * i + g;
-      const vec8_t<T> h =
-          b < nb ? *reinterpret_cast<const vec8_t<T>*>(x + row * x_stride + b * 128 + 8 * gl) : vec8_t<T>{};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[8 * i + e] = b * 128 + 8 * gl + e < c_real ? static_cast<float>(h[e]) : 0.f;
-    }
-    float mean = 0.f;
+  while (row < rows) {
+    float minus = 0.f;  // minus the mean
     if (centre) {
-      float s = 0.f;
+      float s[ACCS] = {};
 #pragma unroll
-      for (int i = 0; i < 8 * NI; ++i) s = s + v[i];
-      mean = tree(s) / n;
-    }
-    float sq = 0.f;
+      for (int i = 0; i < NI; ++i) {
+        float& a = s[i % ACCS];
+        if ((G * i + G) * 128 > c_real) {
+          float d[8];
+          shifted(i, 0.f, d);
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float d = (4 * i + g) * 128 + 8 * gl + e < c_real ? v[8 * i + e] - mean : 0.f;
-        v[8 * i + e] = d;
-        sq = __builtin_fmaf(d, d, sq);
-      }
-    const float rstd = 1.f / sqrtf(tree(sq) / n + eps);
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int b = 4 * i + g;
-      if (b < nb) {  // lanes past the row keep zeros
-        const int c4 = (b * 128 + 8 * gl) >> 2;
-        const float4_t g0 = gb[c4], g1 = gb[c4 + 1], b0 = gb[n4 + c4], b1 = gb[n4 + c4 + 1];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[8 * i + e] = __builtin_fmaf(v[8 * i + e] * rstd, g0[e], b0[e]);
-          v[8 * i + 4 + e] = __builtin_fmaf(v[8 * i + 4 + e] * rstd, g1[e], b1[e]);
+          for (int e = 0; e < 8; ++e) a = a + d[e];
+        } else {
+          a = plus<T, 0>(w[i], a), a = plus<T, 1>(w[i], a), a = plus<T, 2>(w[i], a), a = plus<T, 3>(w[i], a);
+          a = plus<T, 4>(w[i], a), a = plus<T, 5>(w[i], a), a = plus<T, 6>(w[i], a), a = plus<T, 7>(w[i], a);
         }
       }
+      minus = -divide_by(fold(s), n, inv_n);
+      anew();
     }
-    uint32_t q[NI], w[NI];
-    encode_blocks<NI>(v, rotate, gl, q, w);
+    float sq[ACCS] = {};
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int b = 4 * i + g;
-      if (b < nb) {
-        *reinterpret_cast<uint32_t*>(out + row * (C >> 1) + b * 64 + 4 * gl) = q[i];
-        if (l16 == 0) scale[b * rows + row] = w[i];
-      }
+      float d[8];
+      shifted(i, minus, d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sq[i % ACCS] = __builtin_fmaf(d[e], d[e], sq[i % ACCS]);
     }
+    const float rstd = 1.f / sqrtf(divide_by(fold(sq), n, inv_n) + eps);
+    if constexpr (NI > 4) anew();  // up to 32 columns a lane stay in fp32: no gain from more waves there
+    int first = g * 16 + gl;  // the lane's even float4 of its first block; opaque: else gamma and beta stay in registers
+    asm volatile("" : "+v"(first));
+    // two block groups at a time (one at the end of an odd count): the butterflies' wait states are shared
+    auto finish = [&](auto count, int i0) __attribute__((always_inline)) {
+      constexpr int N = decltype(count)::value;
+      float v[8 * N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int b = G * (i0 + j) + g;
+        float d[8];
+        shifted(i0 + j, minus, d);
+        const int c = G == 1 || b < nb ? first + 16 * G * (i0 + j) : 0;
+        const float4_t g0 = gb[c], g1 = gb[n8 + c], b0 = gb[n4 + c], b1 = gb[n4 + n8 + c];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[8 * j + e] = __builtin_fmaf(d[e] * rstd, g0[e], b0[e]);
+          v[8 * j + 4 + e] = __builtin_fmaf(d[4 + e] * rstd, g1[e], b1[e]);
+        }
+      }
+      uint32_t q[N], word[N];
+      encode_blocks<N>(v, rotate, gl, q, word);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int b = G * (i0 + j) + g;
+        if (G == 1 || b < nb) {
+          *reinterpret_cast<uint32_t*>(out + row * (C >> 1) + b * 64 + 4 * gl) = q[j];
+          if (l16 == 0) scale[b * rows + row] = word[j];
+        }
+      }
+    };
+#pragma unroll
+    for (int i = 0; i + 1 < NI; i += 2) finish(std::integral_constant<int, 2>{}, i);
+    if constexpr (NI & 1) finish(std::integral_constant<int, 1>{}, NI - 1);
+    row += stride;
+    if (row < rows) load();
   }
 }
 
@@ -208,11 +288,12 @@ template <typename T>
 __global__ __launch_bounds__(256) void dequant_mx4_kernel(const uint8_t* __restrict__ codes,
                                                           const uint32_t* __restrict__ scale, int64_t rows, int C,
                                                           T* __restrict__ out) {
-  const int per = C >> 3;
-  const int64_t n = rows * per, stride = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += stride) {
-    const int64_t row = i / per;
-    const int c = static_cast<int>(i - row * per);
+  const int per = C >> 3, threads = static_cast<int>(gridDim.x) * 256;
+  const int row_step = threads / per, step = threads - row_step * per;
+  int64_t row = (static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x)) / per;
+  int c = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x) - static_cast<int>(row) * per;
+  while (row < rows) {
+    const int64_t i = row * per + c;
     const uint32_t q = *reinterpret_cast<const uint32_t*>(codes + 4 * i);
     const float f = e8m0((scale[(c >> 4) * rows + row] >> (8 * ((c >> 2) & 3))) & 0xff);
     vec8_t<T> o;
@@ -224,6 +305,12 @@ __global__ __launch_bounds__(256) void dequant_mx4_kernel(const uint8_t* __restr
       o[e] = static_cast<T>((s ? -mag : mag) * f);
     }
     *reinterpret_cast<vec8_t<T>*>(out + 8 * i) = o;
+    row += row_step;
+    c += step;
+    if (c >= per) {
+      c -= per;
+      ++row;
+    }
   }
 }
 
@@ -233,31 +320,43 @@ static unsigned mx4_grid(const void* kernel, size_t smem, int64_t blocks) {
   return static_cast<unsigned>(std::min(blocks, cap));
 }
 
-template <typename T, int NI>
+template <typename T, int NI, int G>
 static void launch_quant_norm(hipStream_t st, const void* x, int64_t xs, int64_t rows, int C, int c_real, const float* g,
                               const float* b, bool centre, float eps, bool rotate, uint8_t* out, uint32_t* scale) {
   const size_t smem = 2 * C * sizeof(float);
-  const void* k = reinterpret_cast<const void*>(&quant_mx4_norm_kernel<T, NI>);
-  quant_mx4_norm_kernel<T, NI><<<mx4_grid(k, smem, (rows + 3) / 4), 256, smem, st>>>(
+  constexpr int ROWS = 4 * (4 / G);  // of a workgroup at once
+  const void* k = reinterpret_cast<const void*>(&quant_mx4_norm_kernel<T, NI, G>);
+  quant_mx4_norm_kernel<T, NI, G><<<mx4_grid(k, smem, (rows + ROWS - 1) / ROWS), 256, smem, st>>>(
       static_cast<const T*>(x), xs, rows, C, c_real, g, b, centre, eps, rotate, out, scale);
+}
+
+// Lane groups a row: four (a wave a row) where the rows are few or wide, or four divides the blocks; in narrow rows two or one
+// leave no group idle (768 columns of 32 800 rows: 21.2 us on two groups, 28.1 on four; 640: 16.9 on one, 23.7 on four; 2816
+// columns of 12 000 rows: 32.6 on four, 34.1 on two).
+static int quant_groups(int64_t rows, int nb) {
+  if (rows < 4096 || nb % 4 == 0 || nb > 11) return 4;
+  return nb % 2 == 0 ? 2 : 1;
 }
 
 template <typename T>
 static void launch_quant(hipStream_t st, const void* x, int64_t xs, int64_t rows, int C, int c_real, int norm,
                          const float* g, const float* b, float eps, bool rotate, uint8_t* out, uint32_t* scale) {
+  const int nb = C / 128;
   if (norm == FF_NORM_NONE) {
-    const int64_t items = rows * ((C / 128 + 3) / 4);
+    const int64_t items = rows * ((nb + 3) / 4);
     const void* k = reinterpret_cast<const void*>(&quant_mx4_kernel<T>);
     quant_mx4_kernel<T><<<mx4_grid(k, 0, (items + 3) / 4), 256, 0, st>>>(static_cast<const T*>(x), xs, rows, C, rotate, out,
                                                                         scale);
     return;
   }
   const bool centre = norm == FF_NORM_LAYER;
-  switch ((C / 128 + 3) / 4) {
-#define FF_MX4_CASE(N) \
-  case N: launch_quant_norm<T, N>(st, x, xs, rows, C, c_real, g, b, centre, eps, rotate, out, scale); break;
-    FF_MX4_CASE(1) FF_MX4_CASE(2) FF_MX4_CASE(3) FF_MX4_CASE(4) FF_MX4_CASE(5) FF_MX4_CASE(6)
-    FF_MX4_CASE(7) FF_MX4_CASE(8) FF_MX4_CASE(9) FF_MX4_CASE(10) FF_MX4_CASE(11) FF_MX4_CASE(12)
+  const int G = quant_groups(rows, nb);
+  switch (100 * G + (nb + G - 1) / G) {
+#define FF_MX4_CASE(GG, N)   case 100 * GG + N: launch_quant_norm<T, N, GG>(st, x, xs, rows, C, c_real, g, b, centre, eps, rotate, out, scale); break;
+    FF_MX4_CASE(1, 1) FF_MX4_CASE(1, 3) FF_MX4_CASE(1, 5) FF_MX4_CASE(1, 7) FF_MX4_CASE(1, 9) FF_MX4_CASE(1, 11)
+    FF_MX4_CASE(2, 1) FF_MX4_CASE(2, 3) FF_MX4_CASE(2, 5)
+    FF_MX4_CASE(4, 1) FF_MX4_CASE(4, 2) FF_MX4_CASE(4, 3) FF_MX4_CASE(4, 4) FF_MX4_CASE(4, 5) FF_MX4_CASE(4, 6)
+    FF_MX4_CASE(4, 7) FF_MX4_CASE(4, 8) FF_MX4_CASE(4, 9) FF_MX4_CASE(4, 10) FF_MX4_CASE(4, 11) FF_MX4_CASE(4, 12)
 #undef FF_MX4_CASE
     default: break;
   }

@@ -1,4 +1,4 @@
-// The cross-lane butterflies of the Walsh-Hadamard rotations (rotq8.hip, quant_mx4.hip): lane l of a 16-lane DPP row owns
+// What the Walsh-Hadamard rotations share (rotq8.hip, quant_mx4.hip). The cross-lane butterflies: lane l of a 16-lane DPP row owns
 // column chunk gray(l) = l ^ (l >> 1), so the partners for chunk bits 0..3 are lanes l ^ 1, ^ 3, ^ 7, ^ 15.
 #pragma once
 
@@ -30,5 +30,17 @@ __device__ __forceinline__ void bfly_stage(float (&v)[N], float s) {
 }
 
 __device__ __forceinline__ float gray_sign(int bit) { return bit ? -1.f : 1.f; }
+
+// An fp16 value folded into its first fp32 operation with v_fma_mix_f32, whose f16 source converts exactly and whose result
+// rounds once, so it equals the fp32 addition of the converted value: half HI of h2 plus s.
+template <int HI>
+__device__ __forceinline__ float add_h(uint32_t h2, float s) {
+  float r;
+  if constexpr (HI)
+    asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h2), "v"(s));
+  else
+    asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h2), "v"(s));
+  return r;
+}
 
 }  // namespace ff

@@ -39,18 +39,7 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
   return __builtin_amdgcn_perm(cd, ab, 0x05040100u);
 }
 
-// fp16 inputs folded into their first fp32 operation with v_fma_mix_f32, whose f16 sources convert exactly and whose
-// result rounds once, so each equals the fp32 operation on the converted value: half HI of h2 plus s; and the first
-// butterfly of an (even, odd) column pair held in one register: (lo + hi, lo - hi).
-template <int HI>
-__device__ __forceinline__ float add_h(uint32_t h2, float s) {
-  float r;
-  if constexpr (HI)
-    asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h2), "v"(s));
-  else
-    asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h2), "v"(s));
-  return r;
-}
+// fp16 inputs folded into their first fp32 operation (add_h, rotate.h).
 // 0 + the low half of h2 (a sum's first term, as the reference's sum starting from 0), with 0 an inline constant: a
 // register operand holding 0 would be hoisted out of the row loop and hold a register through it.
 __device__ __forceinline__ float add_h_zero(uint32_t h2) {
@@ -58,6 +47,7 @@ __device__ __forceinline__ float add_h_zero(uint32_t h2) {
   asm("v_fma_mix_f32 %0, %1, 1.0, 0 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h2));
   return r;
 }
+// The first butterfly of an (even, odd) column pair held in one register: (lo + hi, lo - hi).
 __device__ __forceinline__ void bfly0_h(uint32_t h2, float& lo_plus_hi, float& lo_minus_hi) {
   asm("v_fma_mix_f32 %0, %1, 1.0, %1 op_sel:[0,0,1] op_sel_hi:[1,0,1]" : "=v"(lo_plus_hi) : "v"(h2));
   asm("v_fma_mix_f32 %0, %1, -1.0, %1 op_sel:[1,0,0] op_sel_hi:[1,0,1]" : "=v"(lo_minus_hi) : "v"(h2));

@@ -472,6 +472,7 @@ def head(x: torch.Tensor, W: torch.Tensor, bias: torch.Tensor, out: torch.Tensor
 
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_HALVES = (torch.float16, torch.bfloat16)
 
 
 def _mx4(codes: torch.Tensor, scale: torch.Tensor, name: str) -> tuple[int, int]:
@@ -479,15 +480,17 @@ def _mx4(codes: torch.Tensor, scale: torch.Tensor, name: str) -> tuple[int, int]
     if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.size(1) % 64 != 0:
         raise RuntimeError(f"{name} codes must be uint8 [T, C / 2] with C a multiple of 128")
     T, C = codes.size(0), codes.size(1) * 2
-    if scale.dtype != torch.int32 or tuple(scale.shape) != (C // 128, T):
+    if scale.dtype != torch.int32 or scale.shape != (C // 128, T):
         raise RuntimeError(f"{name} scale must be int32 {(C // 128, T)}")
     return T, C
 
 
 def _no_grad(*ts: torch.Tensor | None) -> None:
     """Refuses tensors that autograd would follow: these ops write into given tensors and have no backward."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError("this op has no backward: call it under torch.no_grad() or detach its tensors")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("this op has no backward: call it under torch.no_grad() or detach its tensors")
 
 
 def quant_mx4(x: torch.Tensor, out: torch.Tensor, scale: torch.Tensor, rotate: bool = True, norm: int = NORM_NONE,
@@ -499,24 +502,28 @@ def quant_mx4(x: torch.Tensor, out: torch.Tensor, scale: torch.Tensor, rotate: b
     `rotate` the rotation by blockdiag(H128). Weights are prepared by the same call: rows [N, K], no norm."""
     _no_grad(x, gamma, beta)
     dev = _on_gpu(out, scale, gamma, beta)
-    _require(x.dim() == 2 and x.dtype in (torch.float16, torch.bfloat16), "x must be fp16 or bf16 [T, C]")
-    _require(x.is_cuda and x.get_device() == dev, "x must be on the outputs' GPU")
     T, C = _mx4(out, scale, "out")
-    _require(tuple(x.shape) == (T, C) and x.stride(1) == 1, f"x must be [{T}, {C}] with contiguous rows")
-    for t in (gamma, beta):
-        if t is not None:
-            _float(C, t)
-    stride = x.stride(0) if T > 1 else C  # a single row's stride says nothing
-    _run("ff_quant_mx4", dev, _ptr(x), _DTYPES[x.dtype], T, C, stride, int(rotate), norm, c_real or C, _ptr(gamma),
-         _ptr(beta), eps, _ptr(out), _ptr(scale))
+    if x.get_device() != dev or x.shape != (T, C) or x.dtype not in _HALVES:
+        raise RuntimeError(f"x must be fp16 or bf16 {(T, C)} on the outputs' GPU")
+    stride, one = x.stride()
+    _require(one == 1, "x must have contiguous rows")
+    if gamma is not None:
+        _float(C, gamma)
+    if beta is not None:
+        _float(C, beta)
+    if T <= 1:
+        stride = C  # a single row's stride says nothing
+    _run("ff_quant_mx4", dev, x.data_ptr(), _DTYPES[x.dtype], T, C, stride, rotate, norm, c_real or C, _ptr(gamma),
+         _ptr(beta), eps, out.data_ptr(), scale.data_ptr())
 
 
 def dequant_mx4(codes: torch.Tensor, scale: torch.Tensor, out: torch.Tensor) -> None:
     """The values of MX4 codes into out [T, C], fp16, bf16 or fp32 (ff_dequant_mx4)."""
     dev = _on_gpu(codes, scale, out)
     T, C = _mx4(codes, scale, "the")
-    _require(out.dtype in _DTYPES and tuple(out.shape) == (T, C), f"out must be fp16, bf16 or fp32 [{T}, {C}]")
-    _run("ff_dequant_mx4", dev, _ptr(codes), _ptr(scale), T, C, _ptr(out), _DTYPES[out.dtype])
+    if out.dtype not in _DTYPES or out.shape != (T, C):
+        raise RuntimeError(f"out must be fp16, bf16 or fp32 {(T, C)}")
+    _run("ff_dequant_mx4", dev, codes.data_ptr(), scale.data_ptr(), T, C, out.data_ptr(), _DTYPES[out.dtype])
 
 
 def gemm_mx4(A: torch.Tensor, a_scale: torch.Tensor, W: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None,
@@ -530,7 +537,7 @@ def gemm_mx4(A: torch.Tensor, a_scale: torch.Tensor, W: torch.Tensor, w_scale: t
     N, KW = _mx4(W, w_scale, "W's")
     _require(KW == K, "A and W must share K")
     shape = out_shape(M, N, epi)
-    if out.dtype not in _DTYPES or tuple(out.shape) != shape:
+    if out.dtype not in _DTYPES or out.shape != shape:
         raise RuntimeError(f"out must be fp16, bf16 or fp32 {shape}")
     if bias is not None:
         _float(N, bias)
@@ -539,8 +546,8 @@ def gemm_mx4(A: torch.Tensor, a_scale: torch.Tensor, W: torch.Tensor, w_scale: t
         _require(residual.dtype == out.dtype and residual.shape == out.shape, "residual must be like out")
     else:
         _require(residual is None, "a residual goes with EPI_RESIDUAL")
-    _run("ff_gemm_mx4", dev, _ptr(A), _ptr(a_scale), _ptr(W), _ptr(w_scale), M, N, K, _ptr(bias), _ptr(residual), _ptr(out),
-         _DTYPES[out.dtype], epi, stages)
+    _run("ff_gemm_mx4", dev, A.data_ptr(), a_scale.data_ptr(), W.data_ptr(), w_scale.data_ptr(), M, N, K, _ptr(bias),
+         _ptr(residual), out.data_ptr(), _DTYPES[out.dtype], epi, stages)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: torch.Tensor, norm: int,
@@ -556,30 +563,39 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: t
     _no_grad(q, k, q_gamma, k_gamma, q_beta, k_beta, rope_cos, rope_sin)
     dev = _on_gpu(q_gamma, k_gamma, q_beta, k_beta, rope_cos, rope_sin, positions)
     _require(q.dim() == 3 and k.dim() == 3, "q and k must be [T, heads, D]")
-    (T, H, D), KV = q.shape, k.size(1)
-    dt = q.dtype
-    _require(dt in (torch.float16, torch.bfloat16), "q and k must be fp16 or bf16")
-    _require(k.size(0) == T and k.size(2) == D, "q and k must share T and D")
-    for t, shape in ((q, (T, H, D)), (k, (T, KV, D)), (q_out, (T, H, D)), (k_out, (T, KV, D))):
-        _require(t.is_cuda and t.get_device() == dev and t.dtype == dt and tuple(t.shape) == shape and
-                 (t.stride(2) == 1 or D == 1), f"need {dt} {shape} on the tables' GPU with contiguous columns")
-    _require(rope_cos.dtype == rope_sin.dtype == torch.float32 and rope_cos.dim() == 2 and rope_cos.shape == rope_sin.shape,
-             "RoPE tables must be fp32 [L, R / 2]")
+    (T, H, D), (TK, KV, DK), dt = q.shape, k.shape, q.dtype
+    _require(TK == T and DK == D, "q and k must share T and D")
+    if not (dt in _HALVES and k.dtype == q_out.dtype == k_out.dtype == dt):
+        raise RuntimeError("q, k, q_out and k_out must be fp16 or bf16, of one type")
+    if q_out.shape != q.shape or k_out.shape != k.shape:
+        raise RuntimeError("q_out and k_out must have the shapes of q and k")
+    if not (q.get_device() == k.get_device() == q_out.get_device() == k_out.get_device() == dev):
+        raise RuntimeError("all tensors must be on one device")
+    (qt, qh, q1), (kt, kh, k1), (ot, oh, o1), (pt, ph, p1) = q.stride(), k.stride(), q_out.stride(), k_out.stride()
+    _require(q1 == k1 == o1 == p1 == 1, "q, k, q_out and k_out must have contiguous columns")
+    if T <= 1:  # a dimension of one has no stride
+        qt = kt = ot = pt = 0
+    if H == 1:
+        qh = oh = 0
+    if KV == 1:
+        kh = ph = 0
+    qp, kp, op, pp = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
+    if (qp == op and (qt, qh) != (ot, oh)) or (kp == pp and (kt, kh) != (pt, ph)):
+        raise RuntimeError("an output in its input's place must have its strides")
+    if not (rope_cos.dtype == rope_sin.dtype == torch.float32 and rope_cos.dim() == 2 and rope_cos.shape == rope_sin.shape):
+        raise RuntimeError("RoPE tables must be fp32 [L, R / 2]")
     for t in (q_gamma, k_gamma, q_beta, k_beta):
         if t is not None:
             _float(D, t)
     pos64 = False
     if positions is not None:
-        _require(positions.dtype in (torch.int32, torch.int64) and tuple(positions.shape) == (T,),
-                 f"positions must be int32 or int64 [{T}]")
         pos64 = positions.dtype == torch.int64
+        if not (pos64 or positions.dtype == torch.int32) or positions.shape != (T,):
+            raise RuntimeError(f"positions must be int32 or int64 [{T}]")
     L, half = rope_cos.shape
-    strides = [(t.stride(0) if T > 1 else 0, t.stride(1) if t.size(1) > 1 else 0) for t in (q, k, q_out, k_out)]
-    for (a, b), x, y in ((strides[::2], q, q_out), (strides[1::2], k, k_out)):
-        _require(a == b or x.data_ptr() != y.data_ptr(), "an output in its input's place must have its strides")
-    _run("ff_qk_norm_rope", dev, _ptr(q), *strides[0], _ptr(k), *strides[1], _ptr(q_out), *strides[2], _ptr(k_out),
-         *strides[3], _DTYPES[dt], T, H, KV, D, norm, _ptr(q_gamma), _ptr(k_gamma), _ptr(q_beta), _ptr(k_beta), eps,
-         _ptr(rope_cos), _ptr(rope_sin), L, 2 * half, int(pairs), _ptr(positions), int(pos64), q_scale)
+    _run("ff_qk_norm_rope", dev, qp, qt, qh, kp, kt, kh, op, ot, oh, pp, pt, ph, _DTYPES[dt], T, H, KV, D, norm,
+         _ptr(q_gamma), _ptr(k_gamma), _ptr(q_beta), _ptr(k_beta), eps, rope_cos.data_ptr(), rope_sin.data_ptr(), L,
+         2 * half, pairs, _ptr(positions), pos64, q_scale)
 
 
 # ---- torch.ops.foidfinder_rocm registration (schemas as kernels.cu:268-273, plus eps / the fused norm) ----

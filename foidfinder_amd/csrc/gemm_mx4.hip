@@ -12,6 +12,7 @@
 // The product is computed transposed (W is the row operand), so that a lane holds one output row m and runs of four
 // consecutive columns n: column pairs (SwiGLU) are in-lane and stores are whole runs.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -79,13 +80,13 @@ __device__ __forceinline__ float16_t mfma_mx4(int4_t w, int4_t a, float16_t c, u
 }
 
 // The epilogue of four consecutive columns n .. n + 3 of row m (n % 4 == 0, n < N): y holds the sums. One rounding, at the
-// store. Columns past N are not touched; whole runs are stored at once when N % 4 == 0 keeps them aligned.
+// store. Columns past N are not touched; runs inside the row go at once where its start is 4-byte aligned.
 template <int EPI, typename T>
 __device__ __forceinline__ void finish4(const Mx4Args& args, int m, int n, float4_t y) {
   const int N = args.N;
-  const bool whole = (N & 3) == 0;
+  const bool inside = n + 4 <= N;
   if (args.bias) {
-    if (whole) {
+    if (inside) {
       const float4_t b = *reinterpret_cast<const float4_t*>(args.bias + n);
 #pragma unroll
       for (int t = 0; t < 4; ++t) y[t] = y[t] + b[t];
@@ -100,19 +101,21 @@ __device__ __forceinline__ void finish4(const Mx4Args& args, int m, int n, float
     o[0] = h0;
     if (n + 2 < N) o[1] = h1;  // N is even
   } else {
+    const bool run = inside && (sizeof(T) == 4 || (N & 1) == 0);
     const int64_t at = static_cast<int64_t>(m) * N + n;
     T* o = static_cast<T*>(args.out) + at;
     if constexpr (EPI == FF_EPI_RESIDUAL) {
       const T* r = static_cast<const T*>(args.residual) + at;
-      if (whole) {
-        const vec4_t<T> x = *reinterpret_cast<const vec4_t<T>*>(r);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) y[t] = y[t] + static_cast<float>(x[t]);
+      vec4_t<T> x = {};
+      if (run) {
+        __builtin_memcpy(&x, r, sizeof(x));
       } else {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
-          if (n + t < N) y[t] = y[t] + static_cast<float>(r[t]);
+          if (n + t < N) x[t] = r[t];
       }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) y[t] = y[t] + static_cast<float>(x[t]);
     }
     if constexpr (EPI == FF_EPI_GELU_F16) {
 #pragma unroll
@@ -121,8 +124,8 @@ __device__ __forceinline__ void finish4(const Mx4Args& args, int m, int n, float
     vec4_t<T> h;
 #pragma unroll
     for (int t = 0; t < 4; ++t) h[t] = static_cast<T>(y[t]);
-    if (whole) {
-      *reinterpret_cast<vec4_t<T>*>(o) = h;
+    if (run) {
+      __builtin_memcpy(o, &h, sizeof(h));
     } else {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -500,9 +503,45 @@ static int launch_ring(const Mx4Args& a, hipStream_t st) {
   return check_launch("gemm_mx4");
 }
 
+// The tile shape without a chosen one: the lowest estimated time. The estimate (us) is fixed + the larger (a 4-norm) of what
+// one tile takes after another, rounds (first + unit u), and what a CU takes for its tiles, each + unit u of throughput, with
+// u units of K, plus the outputs' share. Fitted to the times of 300 products (1 .. 33 000 rows, 32 .. 9000 columns, K 128 ..
+// 5120); on 200 others its pick is 1.4 % slower than the fastest shape on average and 16 % at worst, where the 64 x 64
+// tiles alone are 9 % and 130 %, the 256 x 128 tiles alone 80 % slower on average.
+struct Mx4Cost {
+  int bm, bn, resident;  // tile, workgroups a CU holds
+  bool whole;            // rounds count whole (few tiles a CU) or as a fraction
+  double fixed, first, unit, tile, tile_unit, out;
+};
+constexpr Mx4Cost MX4_COSTS[5] = {
+    {32, 32, 4, false, 3.158, 0.607, 0.0353, 0.144, 0.0972, 1.149},
+    {64, 64, 3, true, 2.968, 0.504, 0.1246, 0.0, 0.1097, 0.586},
+    {128, 128, 3, true, 3.740, 0.528, 0.0971, 0.0, 0.2919, 0.376},
+    {256, 128, 2, false, 3.725, 1.567, 0.1800, 0.674, 0.4621, 0.365},
+    {256, 256, 1, false, 1.317, 4.798, 0.2753, 3.826, 0.6012, 0.389},
+};
+static int pick_variant(int M, int N, int K) {
+  const double u = K / 128;
+  int best = 1;
+  double least = 0.0;
+  for (int v = 0; v < 5; ++v) {
+    const Mx4Cost& c = MX4_COSTS[v];
+    const double tiles = static_cast<double>((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+    double rounds = tiles / (256.0 * c.resident);
+    rounds = c.whole ? std::ceil(rounds) : std::max(1.0, rounds);
+    const double one = rounds * (c.first + c.unit * u), all = std::ceil(tiles / 256.0) * (c.tile + c.tile_unit * u);
+    const double t = c.fixed + std::sqrt(std::sqrt(one * one * one * one + all * all * all * all)) + c.out * 1e-6 * M * N;
+    if (v == 0 || t < least) {
+      least = t;
+      best = v + 1;
+    }
+  }
+  return best;
+}
+
 template <int EPI, typename T>
 static int launch_mx4(const Mx4Args& a, int variant, hipStream_t st) {
-  switch (variant ? variant : (a.M > 256 ? 4 : 1)) {
+  switch (variant ? variant : pick_variant(a.M, a.N, a.K)) {
     case 2: return launch_ring<EPI, T, 64, 64, 2, 2, 2, 3, 3>(a, st);
     case 3: return launch_ring<EPI, T, 128, 128, 2, 2, 1, 3, 3>(a, st);
     case 4: return launch_ring<EPI, T, 256, 128, 2, 2, 1, 3, 2>(a, st);

@@ -171,9 +171,9 @@ def random_mx4(rng, T, C, lo, hi):
     return OX.pack(rng.integers(0, 16, (T, C)).astype(np.uint8), rng.integers(lo, hi, (T, C // 32)).astype(np.uint8))
 
 
-def run_gemm(dev, a, w, bias, kind, epi, variant, residual=None, M=None, N=None):
+def run_gemm(dev, a, w, bias, kind, epi, variant, residual=None):
     """The product into memory between guard rows."""
-    M, N = M or a[0].shape[0], N or w[0].shape[0]
+    M, N = a[0].shape[0], w[0].shape[0]
     cols = N // 2 if epi == OG.EPI_SWIGLU else N
     pad = 64
     buf = torch.full((M * cols + 2 * pad,), 7.0, dtype=TYPES[kind], device=dev)
@@ -243,26 +243,41 @@ def test_gemm_mx4_epilogues(dev, rng, M, N, K, epi, kind, variant):
 
 
 @pytest.mark.parametrize("variant", VARIANTS)
-def test_gemm_mx4_wide_exponents_and_blocks_that_are_not_numbers(dev, rng, variant):
+@pytest.mark.parametrize("M", [70, 64, 20])
+def test_gemm_mx4_wide_exponents_and_blocks_that_are_not_numbers(dev, rng, M, variant):
     """Exponents over 2^+-30, every block with its own: a row with a block of exponent 255 is not a number in all of its
     products, and no other row is; residual in place."""
-    M, N, K = 70, 90, 512
+    N, K = 90, 640
     a, w = random_mx4(rng, M, K, 97, 158), random_mx4(rng, N, K, 97, 158)
     y, size = OX.gemm_mx4(a, w)
     got = run_gemm(dev, a, w, None, "fp32", OG.EPI_BIAS_F16, variant)
     assert (np.abs(got - y) <= sum_error(K, size)).all()
     ac, ae = OX.unpack(*a)
     wc, we = OX.unpack(*w)
-    ae[69, 15], we[31, 3] = 255, 255
+    ae[M - 1, 19], we[31, 3] = 255, 255
     got = run_gemm(dev, OX.pack(ac, ae), OX.pack(wc, we), None, "fp32", OG.EPI_BIAS_F16, variant)
     want = y.copy()
-    want[69], want[:, 31] = np.nan, np.nan
+    want[M - 1], want[:, 31] = np.nan, np.nan
     assert np.array_equal(np.isnan(got), np.isnan(want))
     out, x = typed(rng.standard_normal((M, N)), "bf16", dev)
     kern().gemm_mx4(*(gpu(t, dev) for t in (*a, *w)), None, out, OG.EPI_RESIDUAL, variant)
     want, got = y + x, out.double().cpu().numpy()
     e = sum_error(K, size) + 2.0**-23 * np.abs(want)
     assert (np.abs(got - want) <= e + HALF["bf16"] * (np.abs(want) + e)).all()
+
+
+@pytest.mark.parametrize("variant", [0, 1, 2])
+@pytest.mark.parametrize(("M", "N", "K"), [(16, 70001, 384), (64, 66000, 128), (33, 5001, 1152), (1, 40000, 640),
+                                           (32, 33, 3840)])
+def test_gemm_mx4_few_rows_exact(dev, rng, M, N, K, variant):
+    """Up to 64 rows and many columns, odd unit counts, rows that start off a 4-byte boundary; exact as above."""
+    a, w = random_mx4(rng, M, K, 126, 128), random_mx4(rng, N, K, 126, 128)
+    bias = rng.integers(-8, 8, N).astype(np.float32)
+    got = run_gemm(dev, a, w, bias, "fp32", OG.EPI_BIAS_F16, variant)
+    av, wv = (torch.from_numpy(OX.values(*t).astype(np.float32)) for t in (a, w))
+    want = (av @ wv.T).double().numpy() + bias  # float32 holds every partial sum, so torch's order does not matter
+    bad = np.argwhere(got != want)
+    assert bad.size == 0, f"{len(bad)} differ, first {bad[:4].tolist()}: {got[tuple(bad[0])]} vs {want[tuple(bad[0])]}"
 
 
 def test_gemm_mx4_repeats_bit_for_bit(dev, rng):

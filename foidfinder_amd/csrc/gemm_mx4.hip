@@ -589,6 +589,12 @@ extern "C" int ff_gemm_mx4(const uint8_t* A, const uint32_t* a_scale, const uint
   if (low(A) || low(W) || low(out) || low(bias) || (epi == FF_EPI_RESIDUAL && low(residual)) || (low(a_scale) & 3) ||
       (low(w_scale) & 3))
     return fail(FF_EINVAL, "gemm_mx4: misaligned pointer");
+  if (epi == FF_EPI_RESIDUAL && residual != out) {  // elements are read and written by different workgroups, in no order
+    const uintptr_t r = reinterpret_cast<uintptr_t>(residual), o = reinterpret_cast<uintptr_t>(out);
+    const uintptr_t apart = r < o ? o - r : r - o;
+    if (apart < static_cast<uintptr_t>(M) * static_cast<uintptr_t>(N) * 2)
+      return fail(FF_EINVAL, "gemm_mx4: residual overlaps out in part");
+  }
   const Mx4Args a{A, a_scale, W, w_scale, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), bias, residual,
                   out};
   const hipStream_t st = as_stream(stream);

@@ -211,7 +211,7 @@ extern "C" int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, c
     return fail(FF_EINVAL, "qk_norm_rope: need 0 < heads, kv_heads <= 65535");
   if (T < 0 || T >= (int64_t(1) << 31) || T * (heads + kv_heads) >= (int64_t(1) << 31))
     return fail(FF_EINVAL, "qk_norm_rope: need 0 <= T and T * (heads + kv_heads) < 2^31");
-  if (rope_len <= 0 || rope_len > 0x7fffffff) return fail(FF_EINVAL, "qk_norm_rope: need 0 < rope_len < 2^31");
+  if (rope_len <= 0 || rope_len >= (1 << 30)) return fail(FF_EINVAL, "qk_norm_rope: need 0 < rope_len < 2^30");
   if (norm != FF_NORM_NONE && norm != FF_NORM_RMS && norm != FF_NORM_LAYER)
     return fail(FF_EINVAL, "qk_norm_rope: unknown norm");
   const bool normed = norm != FF_NORM_NONE, centred = norm == FF_NORM_LAYER;
@@ -242,6 +242,8 @@ extern "C" int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, c
   };
   if (overlaps(qo_token, qo_head, heads) || overlaps(ko_token, ko_head, kv_heads))
     return fail(FF_EINVAL, "qk_norm_rope: the rows of an output overlap");
+  if (q_out == k_out || q_out == k || k_out == q)
+    return fail(FF_EINVAL, "qk_norm_rope: q_out and k_out must be two, each apart from the other's input");
   const QkArgs a{{q, k}, {q_out, k_out}, {q_token, k_token}, {q_head, k_head}, {qo_token, ko_token}, {qo_head, ko_head},
                  {q_gamma, k_gamma}, {q_beta, k_beta}, rope_cos, rope_sin, positions, pos64, static_cast<int>(T),
                  {static_cast<int>(heads), static_cast<int>(kv_heads)}, static_cast<int>(D), static_cast<int>(R),

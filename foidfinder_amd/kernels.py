@@ -519,6 +519,7 @@ def quant_mx4(x: torch.Tensor, out: torch.Tensor, scale: torch.Tensor, rotate: b
 
 def dequant_mx4(codes: torch.Tensor, scale: torch.Tensor, out: torch.Tensor) -> None:
     """The values of MX4 codes into out [T, C], fp16, bf16 or fp32 (ff_dequant_mx4)."""
+    _no_grad(out)
     dev = _on_gpu(codes, scale, out)
     T, C = _mx4(codes, scale, "the")
     if out.dtype not in _DTYPES or out.shape != (T, C):
@@ -529,9 +530,9 @@ def dequant_mx4(codes: torch.Tensor, scale: torch.Tensor, out: torch.Tensor) -> 
 def gemm_mx4(A: torch.Tensor, a_scale: torch.Tensor, W: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None,
              out: torch.Tensor, epi: int, stages: int = 0, residual: torch.Tensor | None = None) -> None:
     """MX4 A [M, K] x MX4 W [N, K] + bias fp32 [N] (or None) -> epilogue into out: EPI_BIAS_F16 (out fp16, bf16 or fp32),
-    EPI_GELU_F16, EPI_SWIGLU (out [M, N / 2]) or EPI_RESIDUAL (out = y + residual of out's type; None: out itself).
-    `stages` selects the tile variant (0 = by the sizes) (ff_gemm_mx4)."""
-    _no_grad(bias, residual)
+    EPI_GELU_F16, EPI_SWIGLU (out [M, N / 2]) or EPI_RESIDUAL (out = y + residual of out's type, which is out itself (None)
+    or memory apart from it). `stages` selects the tile variant (0 = by the sizes) (ff_gemm_mx4)."""
+    _no_grad(bias, out, residual)
     dev = _on_gpu(A, a_scale, W, w_scale, bias, out, residual)
     M, K = _mx4(A, a_scale, "A's")
     N, KW = _mx4(W, w_scale, "W's")
@@ -560,7 +561,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: t
     [T, 3 C] row, say: `qkv.view(T, 3, heads, D)[:, 0]`) -> q_out, k_out of the same shapes; an output may be its input
     itself and shares no other memory with q or k. gamma (with a norm) and beta (NORM_LAYER) fp32 [D]; tables fp32 [L, R / 2];
     positions int32 or int64 [T], or None: t % L. `pairs`: columns (2 i, 2 i + 1) turn together, else (i, i + R / 2)."""
-    _no_grad(q, k, q_gamma, k_gamma, q_beta, k_beta, rope_cos, rope_sin)
+    _no_grad(q, k, q_out, k_out, q_gamma, k_gamma, q_beta, k_beta, rope_cos, rope_sin)
     dev = _on_gpu(q_gamma, k_gamma, q_beta, k_beta, rope_cos, rope_sin, positions)
     _require(q.dim() == 3 and k.dim() == 3, "q and k must be [T, heads, D]")
     (T, H, D), (TK, KV, DK), dt = q.shape, k.shape, q.dtype

@@ -84,11 +84,11 @@ int ff_gemm_s8_variants(void);
  * codes uint8 [T, C/2]: the even column in the low half of a byte. scale uint32 [C/128, T]: byte i of word [b, t] is the
  * exponent (bias 127) of columns 128 b + 32 i .. + 31 of row t; 255 stands for a block that is not a number.
  *
- * ff_quant_mx4: x fp16 or bf16 (dtype) [T, C], rows x_stride elements apart (>= C, % 8 == 0), C % 128 == 0, C <= 6144 ->
- * out, scale. First the norm (FF_NORM_*) over the first c_real columns (fp32 gamma/beta [C], zero past c_real; columns past
- * it count as zeros), then with rotate = 1 the block-diagonal 128-point Walsh-Hadamard rotation, then per 32 columns
- * e = floor(log2(max |v|)) - 2 (at least -127) and code = v / 2^e to the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (ties to the
- * even code, saturating). A block with an infinite or undefined value gets the exponent 255. */
+ * ff_quant_mx4: x fp16 or bf16 (dtype) [T, C] (from a multiple of 16 bytes), rows x_stride elements apart (>= C, % 8 == 0),
+ * C % 128 == 0, C <= 6144 -> out, scale. First the norm (FF_NORM_*) over the first c_real columns (fp32 gamma/beta [C], zero
+ * past c_real; columns past it count as zeros), then with rotate = 1 the block-diagonal 128-point Walsh-Hadamard rotation,
+ * then per 32 columns e = floor(log2(max |v|)) - 2 (at least -127) and code = v / 2^e to the nearest of 0, 1/2, 1, 3/2, 2, 3,
+ * 4, 6 (ties to the even code, saturating). A block with an infinite or undefined value gets the exponent 255. */
 int ff_quant_mx4(const void* x, int dtype, int64_t T, int64_t C, int64_t x_stride, int rotate, int norm, int64_t c_real,
                  const float* gamma, const float* beta, float eps, uint8_t* out, uint32_t* scale, void* stream);
 
@@ -96,9 +96,10 @@ int ff_quant_mx4(const void* x, int dtype, int64_t T, int64_t C, int64_t x_strid
 int ff_dequant_mx4(const uint8_t* codes, const uint32_t* scale, int64_t T, int64_t C, void* out, int dtype, void* stream);
 
 /* MX4 product with fp32 sums and a fused epilogue: y[m, n] = sum_k A[m, k] W[n, k] + bias[n] (bias fp32 [N] or NULL), then
- * FF_EPI_BIAS_F16 (out = y, in fp16, bf16 or fp32), FF_EPI_RESIDUAL (out = y + residual; residual may be out),
- * FF_EPI_GELU_F16 or FF_EPI_SWIGLU (out [M, N/2], N even). A MX4 [M, K], W MX4 [N, K], K % 128 == 0, K <= 2^22, any
- * M, any N <= 2^21. `variant` selects the tile shape (1 .. ff_gemm_mx4_variants()), 0 = by the sizes. */
+ * FF_EPI_BIAS_F16 (out = y, in fp16, bf16 or fp32), FF_EPI_RESIDUAL (out = y + residual, which is out itself or memory
+ * apart from it), FF_EPI_GELU_F16 or FF_EPI_SWIGLU (columns are (gate j, value j) pairs, out [M, N/2], N even). A MX4 [M, K],
+ * W MX4 [N, K], K % 128 == 0, K <= 2^22, any M, any N <= 2^21; pointers are multiples of 16 bytes (the scales' of 4).
+ * `variant` selects the tile shape (1 .. ff_gemm_mx4_variants()), 0 = by the sizes. */
 int ff_gemm_mx4(const uint8_t* A, const uint32_t* a_scale, const uint8_t* W, const uint32_t* w_scale, int64_t M, int64_t N,
                 int64_t K, const float* bias, const void* residual, void* out, int dtype, int epi, int variant,
                 void* stream);
@@ -106,11 +107,12 @@ int ff_gemm_mx4_variants(void);
 
 /* The norm of each head's query and key, then their rotation by position, then q x q_scale, in one pass and one rounding.
  * q fp16 or bf16 [T, heads, D] and k [T, kv_heads, D] by strides in elements (token, head; columns contiguous), so views of
- * packed rows are taken as they are; q_out and k_out the same shapes by their own strides, each either its input itself
- * (the same pointer and strides) or memory apart from q and k. D % 8 == 0, D <= 256. Norm (FF_NORM_*) over the D columns
- * with fp32 gamma/beta [D]. Rotation of the first R columns (R % 8 == 0) by row p of rope_cos/rope_sin fp32
- * [rope_len, R/2]: pairs = 1 turns columns (2 i, 2 i + 1), pairs = 0 columns (i, i + R/2); p = positions[t] (int32, or
- * int64 with pos64; a token whose position is outside the table becomes not a number), or t % rope_len without. */
+ * packed rows are taken as they are (pointers and strides multiples of 8 bytes); q_out and k_out the same shapes by their own
+ * strides, each either its input itself (the same pointer and strides) or memory apart from q and k. D % 8 == 0, D <= 256.
+ * Norm (FF_NORM_*) over the D columns with fp32 gamma/beta [D]. Rotation of the first R columns (R % 8 == 0) by row p of
+ * rope_cos/rope_sin fp32 [rope_len, R/2], rope_len < 2^30: pairs = 1 turns columns (2 i, 2 i + 1), pairs = 0 columns
+ * (i, i + R/2); p = positions[t] (int32, or int64 with pos64; a token whose position is outside the table becomes not a
+ * number), or t % rope_len without. */
 int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
                     void* q_out, int64_t qo_token, int64_t qo_head, void* k_out, int64_t ko_token, int64_t ko_head,
                     int dtype, int64_t T, int64_t heads, int64_t kv_heads, int64_t D, int norm, const float* q_gamma,

@@ -46,7 +46,8 @@ def fma32(a: np.ndarray, b: np.ndarray, c: np.ndarray) -> np.ndarray:
 
     The midpoint test runs on the float64 bits: in float32's normal range a float32 midpoint has exactly bit 28 set
     among the 29 low fraction bits that float32 drops. Only such elements, and those outside the normal range
-    (subnormal, overflowing, non-finite), take the TwoSum path."""
+    (subnormal, overflowing), take the TwoSum path; an infinite or undefined s (only from such an operand: float64 holds
+    every product and sum of finite ones) is the result."""
     a, b, c = np.broadcast_arrays(np.asarray(a, F32), np.asarray(b, F32), np.asarray(c, F32))
     p = a.astype(np.float64) * b.astype(np.float64)
     c64 = c.astype(np.float64)
@@ -54,6 +55,7 @@ def fma32(a: np.ndarray, b: np.ndarray, c: np.ndarray) -> np.ndarray:
     r = s.astype(F32)
     mag = np.abs(s)
     cand = ((s.view(np.int64) & ((1 << 29) - 1)) == (1 << 28)) | ~(mag >= 2.0**-125) | (mag >= 2.0**127)
+    cand &= np.isfinite(s)
     if not cand.any():
         return r
     idx = np.nonzero(cand)

@@ -12,6 +12,7 @@ import torch
 from foidfinder_amd import kernels as K
 from oracle import mx4 as OX
 from oracle import qk_norm as OQ
+from oracle.gemm import fma32
 
 FF_OK, FF_EINVAL = 0, 1
 ALL_VALUES = [s * g for g in OX.GRID for s in (1, -1)]
@@ -61,6 +62,24 @@ def test_pack_puts_even_columns_low_and_four_exponents_in_a_word():
     assert scale[1, 0] == 104 | 105 << 8 | 106 << 16 | 107 << 24
     back = OX.unpack(codes, scale)
     assert np.array_equal(back[0], code) and back[1][0].tolist() == list(range(100, 108))
+
+
+def test_fused_multiply_add_of_infinities_in_the_oracle():
+    inf, nan = np.float32(np.inf), np.float32(np.nan)
+    with np.errstate(invalid="ignore"):
+        got = fma32(np.array([inf, 2, inf, nan, 3e38, 1], np.float32), np.array([inf, 3, 0, 1, 10, 1], np.float32),
+                    np.array([1, -inf, 1, 1, 0, inf], np.float32))
+    assert np.array_equal(got, np.array([inf, -inf, nan, nan, inf, inf], np.float32), equal_nan=True)
+
+
+def test_norm_of_a_row_with_an_infinity():
+    """RMS: 1 / sqrt(inf) = 0, so finite columns become zeros and the infinite one undefined; the next row is as without."""
+    x = np.ones((2, 256), np.float32)
+    x[0, 3] = np.inf
+    with np.errstate(invalid="ignore"):
+        v = OX.norm_rows(x, OX.RMS, 256, np.ones(256, np.float32), None, 1e-6)
+    assert np.isnan(v[0, 3]) and not v[0, :3].any() and not v[0, 4:].any()
+    assert np.array_equal(v[1], OX.norm_rows(x[1:], OX.RMS, 256, np.ones(256, np.float32), None, 1e-6)[0])
 
 
 @pytest.mark.parametrize("norm", [OX.RMS, OX.LAYER])
@@ -176,13 +195,14 @@ def test_gemm_mx4_rejects_bad_arguments():
                      (dict(Kd=(1 << 22) + 128), "not supported"), (dict(epi=1), "null"), (dict(A=None), "null"),
                      (dict(Ws=None), "null"), (dict(out=None), "null"), (dict(A=264), "misaligned"),
                      (dict(bias=260), "misaligned"), (dict(out=264), "misaligned"), (dict(As=258), "misaligned"),
-                     (dict(epi=1, res=264), "misaligned")):
+                     (dict(epi=1, res=264), "misaligned"), (dict(epi=1, res=272), "overlaps"),
+                     (dict(epi=1, out=496), "null"), (dict(epi=1, res=256, out=496), "overlaps")):
         status, msg = call(**kw)
         assert status == FF_EINVAL and what in msg, (kw, msg)
 
 
 def test_qk_norm_rope_rejects_bad_arguments():
-    def call(q=256, k=256, qo=256, ko=256, st=((1024, 64),) * 4, dtype=0, T=4, H=16, KV=16, D=64, norm=1, g=256, b=None,
+    def call(q=256, k=65536, qo=256, ko=65536, st=((1024, 64),) * 4, dtype=0, T=4, H=16, KV=16, D=64, norm=1, g=256, b=None,
              eps=1e-6, cos=256, L=8, R=64, pairs=1, pos=None, pos64=0):
         return err(K.lib().ff_qk_norm_rope(q, *st[0], k, *st[1], qo, *st[2], ko, *st[3], dtype, T, H, KV, D, norm, g, g, b,
                                            b, eps, cos, cos, L, R, pairs, pos, pos64, 1.0, None))
@@ -192,6 +212,8 @@ def test_qk_norm_rope_rejects_bad_arguments():
     for kw, what in ((dict(dtype=2), "fp16 or bf16"), (dict(D=60), "heads must"), (dict(D=264), "heads must"),
                      (dict(R=0), "rotated"), (dict(R=60), "rotated"), (dict(R=72), "rotated"), (dict(H=0), "heads"),
                      (dict(KV=65536), "heads"), (dict(T=-1), "T"), (dict(T=1 << 27), "2^31"), (dict(L=0), "rope_len"),
+                     (dict(L=1 << 30), "rope_len"), (dict(ko=256), "two"),
+                     (dict(q=512, qo=512, k=256, ko=512), "two"), (dict(k=512, qo=512), "two"), (dict(q=65536), "two"),
                      (dict(norm=3), "norm"), (dict(norm=0), "gamma"), (dict(g=None), "gamma"), (dict(b=256), "beta"),
                      (dict(norm=2), "beta"), (dict(eps=0.0), "eps"), (dict(q=None), "null"), (dict(ko=None), "null"),
                      (dict(cos=None), "null"), (dict(q=260), "misaligned"), (dict(cos=264), "misaligned"),
@@ -225,6 +247,11 @@ def test_python_layer_refuses_wrong_tensors(monkeypatch):
         K.quant_mx4(x.clone().requires_grad_(), *mx(3, 256))
     with torch.no_grad():
         K.quant_mx4(x.clone().requires_grad_(), *mx(3, 256))
+    followed = torch.zeros(3, 256).requires_grad_()
+    for call in (lambda: K.dequant_mx4(*mx(3, 256), followed),
+                 lambda: K.gemm_mx4(*mx(3, 128), *mx(256, 128), None, followed, K.EPI_BIAS_F16)):
+        with pytest.raises(RuntimeError, match="backward"):
+            call()
     a, w, o = mx(3, 256), mx(6, 256), torch.zeros(3, 6)
     K.gemm_mx4(*a, *w, None, o, K.EPI_BIAS_F16)
     for call in (lambda: K.gemm_mx4(*a, *mx(6, 128), None, o, K.EPI_BIAS_F16),

@@ -125,6 +125,21 @@ def test_quant_mx4_special_rows(dev, rotate):
     assert_same_mx4(*run_quant(dev, x16, "fp16", rotate, OX.NONE))
 
 
+@pytest.mark.parametrize("norm", [OX.RMS, OX.LAYER])
+@pytest.mark.parametrize(("T", "C"), [(6, 640), (6, 1024), (4100, 640), (4100, 768)])
+def test_quant_mx4_norm_special_rows(dev, rng, T, C, norm):
+    """A row that holds a NaN has no codes (every exponent 255), one with an infinity those of the formula; the rows beside
+    them, some in the same wave, are as without them. Rows of zeros and of one value."""
+    x = activations(rng, T, C)
+    x[0, 3], x[2, C - 1], x[3] = np.inf, np.nan, 0
+    x[4] = 0.5
+    g, b = np.ones(C, np.float32), np.linspace(-1, 1, C).astype(np.float32)
+    got, want = run_quant(dev, x, "bf16", True, norm, C, g, b if norm == OX.LAYER else None)
+    assert_same_mx4(got, want)
+    e = OX.unpack(*(t.cpu().numpy() for t in got))[1]
+    assert (e[2] == 255).all() and (e[[1, 3, 4, 5]] != 255).all()
+
+
 @pytest.mark.parametrize("norm", [OX.NONE, OX.LAYER])
 def test_quant_mx4_strided_rows(dev, rng, norm):
     x = rng.standard_normal((6, 1040)).astype(np.float32)
@@ -294,6 +309,62 @@ def test_gemm_mx4_no_rows(dev):
     K.gemm_mx4(*e, *w, None, torch.empty(0, 8, device=dev), K.EPI_BIAS_F16)
     K.quant_mx4(torch.empty(0, 128, dtype=torch.half, device=dev), *e)
     K.dequant_mx4(*e, torch.empty(0, 128, device=dev))
+    q, ko = (torch.empty(0, n, 64, dtype=torch.half, device=dev) for n in (4, 2))
+    t = torch.ones(3, 32, device=dev)
+    K.qk_norm_rope(q, ko, q, ko, K.NORM_NONE, None, None, None, None, t, t)
+    K.qk_norm_rope(q, ko, q, ko, K.NORM_NONE, None, None, None, None, t, t, torch.empty(0, dtype=torch.int32, device=dev))
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+def test_gemm_mx4_offsets_past_32_bits(dev, rng, variant):
+    """An output of 2.3 G elements (4.6 GB): rows whose offsets pass 2^31 elements, the sums exact as above and rounded
+    once to bf16."""
+    K = kern()
+    M, N, Kd = 70001, 32770, 128
+    w = random_mx4(rng, N, Kd, 126, 128)
+    few = random_mx4(rng, 5, Kd, 126, 128)
+    rows = np.array([0, 65536, 65537, 70000, 33000])
+    codes = torch.zeros(M, Kd // 2, dtype=torch.uint8, device=dev)
+    scale = torch.zeros(1, M, dtype=torch.int32, device=dev)
+    codes[rows] = gpu(few[0], dev)
+    scale[:, rows] = gpu(few[1], dev)
+    out = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
+    K.gemm_mx4(codes, scale, *(gpu(t, dev) for t in w), None, out, K.EPI_BIAS_F16, variant)
+    want = torch.from_numpy(OX.gemm_mx4(few, w)[0]).to(torch.bfloat16)
+    assert torch.equal(out[rows].cpu(), want)
+    assert not out[1].any() and not out[69999].any()
+
+
+@pytest.mark.parametrize("norm", [OX.NONE, OX.RMS])
+def test_quant_mx4_offsets_past_32_bits(dev, rng, norm):
+    """2.2 G elements: the last rows start past 2^31 elements of x and 2^30 bytes of codes."""
+    K = kern()
+    T, C = 360_000, 6144
+    x = torch.zeros(T, C, dtype=torch.half, device=dev)
+    last, back = typed(activations(rng, 3, C), "fp16", dev)
+    x[-3:] = last
+    codes = torch.empty(T, C // 2, dtype=torch.uint8, device=dev)
+    scale = torch.empty(C // 128, T, dtype=torch.int32, device=dev)
+    g = np.ones(C, np.float32) if norm else None
+    K.quant_mx4(x, codes, scale, True, norm, None if g is None else gpu(g, dev))
+    assert_same_mx4((codes[-3:], scale[:, -3:]), OX.quant_mx4(back, True, norm, 0, g))
+    assert not scale[:, :-3].any() and not (codes[:-3] & 0x77).any()  # zeros: the lowest exponent, either sign
+    x.fill_(7.0)
+    K.dequant_mx4(codes, scale, x)
+    want = OX.values(codes[-3:].cpu().numpy(), scale[:, -3:].cpu().numpy())
+    assert np.array_equal(x[-3:].double().cpu().numpy(), want) and not x[:-3].any()
+
+
+def test_mx4_ops_refuse_tensors_that_autograd_follows(dev):
+    """Through the dispatcher as well, where no autograd kernel stands before the op."""
+    K = kern()
+    x = torch.zeros(2, 128, dtype=torch.half, device=dev, requires_grad=True)
+    codes, scale, _ = empty_mx4(2, 128, dev)
+    for op in (K.quant_mx4, K.kernels().quant_mx4):
+        with pytest.raises(RuntimeError, match="backward"):
+            op(x, codes, scale)
+        with torch.no_grad():
+            op(x, codes, scale)
 
 
 # ---- head norm and rotation ----
@@ -403,6 +474,29 @@ def test_qk_norm_rope_norms_of_zero_and_large_heads(dev):
     K.qk_norm_rope(x, x, o, o2, OQ.RMS, g, g, None, None, cos, sin)
     assert not o[0].any() and torch.equal(o, o2)
     assert torch.equal(o[1], x[1].sign())
+
+
+@pytest.mark.parametrize("norm", [OQ.NONE, OQ.RMS, OQ.LAYER])
+def test_qk_norm_rope_keeps_values_that_are_not_finite_to_their_head(dev, rng, norm):
+    """Columns past the rotated ones and heads beside the fault are as without it; the fault's head shows it."""
+    K = kern()
+    x, _ = typed(rng.standard_normal((5, 3, 80)), "bf16", dev)
+    cos, sin = (gpu(t, dev) for t in tables(rng, 5, 32))
+    g = torch.ones(80, device=dev) if norm else None
+    b = torch.zeros(80, device=dev) if norm == OQ.LAYER else None
+    outs = []
+    for fault in (False, True):
+        y = x.clone()
+        if fault:
+            y[1, 2, 7], y[3, 0, 79] = float("nan"), float("inf")
+        o, o2 = torch.empty_like(y), torch.empty_like(y)
+        K.qk_norm_rope(y, y, o, o2, norm, g, g, b, b, cos, sin)
+        assert torch.equal(o.view(torch.int16), o2.view(torch.int16))
+        outs.append(o)
+    bad = torch.zeros(5, 3, dtype=torch.bool, device=dev)
+    bad[1, 2] = bad[3, 0] = True
+    assert torch.equal(outs[0][~bad], outs[1][~bad])
+    assert outs[1][1, 2].isnan().any() and not outs[1][3, 0].isfinite().all()
 
 
 # ---- together ----

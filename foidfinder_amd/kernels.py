@@ -109,15 +109,15 @@ def _on_gpu(*ts: torch.Tensor | None) -> int:
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.get_device()  # -1 on the CPU
+        if d < 0:
             raise RuntimeError("foidfinder_rocm ops take GPU tensors")
         if not t.is_contiguous():
             raise RuntimeError("foidfinder_rocm ops take contiguous tensors")
-        d = t.get_device()
-        if dev < 0:
+        if d != dev:
+            if dev >= 0:
+                raise RuntimeError("all tensors must be on one device")
             dev = d
-        elif d != dev:
-            raise RuntimeError("all tensors must be on one device")
     return dev
 
 
@@ -477,9 +477,10 @@ _HALVES = (torch.float16, torch.bfloat16)
 
 def _mx4(codes: torch.Tensor, scale: torch.Tensor, name: str) -> tuple[int, int]:
     """Rows and columns of an MX4 tensor: codes uint8 [T, C / 2], scale int32 [C / 128, T]."""
-    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.size(1) % 64 != 0:
+    shape = codes.shape
+    if codes.dtype != torch.uint8 or len(shape) != 2 or shape[1] % 64 != 0:
         raise RuntimeError(f"{name} codes must be uint8 [T, C / 2] with C a multiple of 128")
-    T, C = codes.size(0), codes.size(1) * 2
+    T, C = shape[0], shape[1] * 2
     if scale.dtype != torch.int32 or scale.shape != (C // 128, T):
         raise RuntimeError(f"{name} scale must be int32 {(C // 128, T)}")
     return T, C

@@ -51,6 +51,13 @@ __device__ __forceinline__ void buf_store_u16(uint16_t v, void* base, int nbytes
   __builtin_amdgcn_raw_buffer_store_b16(v, r, voff, 0, 0);
 }
 
+// A store that does not stay in L2 ahead of other lines: the outputs are larger than what the tiles read again (32800 x 5632 x
+// 1024 SwiGLU 141 -> 134 us, 5184 x 4736 26.3 -> 25.8; what reads the output next is no slower).
+__device__ __forceinline__ void buf_stream_i4(int4_t v, void* base, int nbytes, uint32_t voff) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(base, 0, nbytes, RSRC_WORD3);
+  __builtin_amdgcn_raw_buffer_store_b128(v, r, voff, 0, 2);
+}
+
 // One lane's run (16, 4 or 2 bytes) through a descriptor.
 template <typename R>
 __device__ __forceinline__ R buf_load_run(const void* base, int nbytes, uint32_t voff) {
@@ -64,7 +71,7 @@ __device__ __forceinline__ R buf_load_run(const void* base, int nbytes, uint32_t
 template <typename R>
 __device__ __forceinline__ void buf_store_run(R v, void* base, int nbytes, uint32_t voff) {
   if constexpr (sizeof(R) == 16)
-    buf_store_h8(__builtin_bit_cast(half8_t, v), base, nbytes, voff);
+    buf_stream_i4(__builtin_bit_cast(int4_t, v), base, nbytes, voff);
   else if constexpr (sizeof(R) == 4)
     buf_store_u32(__builtin_bit_cast(uint32_t, v), base, nbytes, voff);
   else
@@ -504,10 +511,10 @@ static int launch_ring(const Mx4Args& a, hipStream_t st) {
 }
 
 // The tile shape without a chosen one: the lowest estimated time. The estimate (us) is fixed + the larger (a 4-norm) of what
-// one tile takes after another, rounds (first + unit u), and what a CU takes for its tiles, each + unit u of throughput, with
-// u units of K, plus the outputs' share. Fitted to the times of 300 products (1 .. 33 000 rows, 32 .. 9000 columns, K 128 ..
-// 5120); on 200 others its pick is 1.4 % slower than the fastest shape on average and 16 % at worst, where the 64 x 64
-// tiles alone are 9 % and 130 %, the 256 x 128 tiles alone 80 % slower on average.
+// one tile takes after another, rounds (first + unit u), and what a CU takes for its tiles, each tile + tile_unit u, with u
+// units of K, plus the outputs' share. Fitted to the times of 300 products (1 .. 33 000 rows, 32 .. 9000 columns, K 128 ..
+// 5120); on 200 others its pick is 1.5 % slower than the fastest shape on average and 19 % at worst, where the 64 x 64
+// tiles alone are 10 % slower on average, the 256 x 128 tiles alone 77 %.
 struct Mx4Cost {
   int bm, bn, resident;  // tile, workgroups a CU holds
   bool whole;            // rounds count whole (few tiles a CU) or as a fraction

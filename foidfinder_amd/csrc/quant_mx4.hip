@@ -283,7 +283,8 @@ __device__ __forceinline__ float e8m0(uint32_t e) {
   return __builtin_bit_cast(float, e == 255 ? 0x7fc00000u : (e == 0 ? 0x00400000u : e << 23));
 }
 
-// The values of the codes: each thread 8 columns of a row.
+// The values of the codes: each thread 8 columns of a row, in stores that stream past L2 (32 800 x 1024 with the quantization
+// before it 43.9 -> 41.2 us; the codes' own stores do not: 4 bytes a lane run slower so). Bound by its bytes: 85 MB in 15 us.
 template <typename T>
 __global__ __launch_bounds__(256) void dequant_mx4_kernel(const uint8_t* __restrict__ codes,
                                                           const uint32_t* __restrict__ scale, int64_t rows, int C,
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(256) void dequant_mx4_kernel(const uint8_t* __restr
       const float mag = __builtin_bit_cast(float, m << 22) * 0x1p126f;
       o[e] = static_cast<T>((s ? -mag : mag) * f);
     }
-    *reinterpret_cast<vec8_t<T>*>(out + 8 * i) = o;
+    __builtin_nontemporal_store(o, reinterpret_cast<vec8_t<T>*>(out + 8 * i));
     row += row_step;
     c += step;
     if (c >= per) {

@@ -91,7 +91,7 @@ def _run(name: str, dev: int, *args) -> None:
     made of a few us of host work in all, so nothing is switched or built that is not needed: the device is entered only
     if it is not the current one already, and the stream comes as its raw handle."""
     fn = getattr(lib(), name)
-    if torch.cuda.current_device() == dev:
+    if torch._C._cuda_getDevice() == dev:  # a tensor on a GPU is there, so the runtime is up
         _check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
         return
     with torch.cuda.device(dev):
@@ -564,17 +564,21 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: t
     positions int32 or int64 [T], or None: t % L. `pairs`: columns (2 i, 2 i + 1) turn together, else (i, i + R / 2)."""
     _no_grad(q, k, q_out, k_out, q_gamma, k_gamma, q_beta, k_beta, rope_cos, rope_sin)
     dev = _on_gpu(q_gamma, k_gamma, q_beta, k_beta, rope_cos, rope_sin, positions)
-    _require(q.dim() == 3 and k.dim() == 3, "q and k must be [T, heads, D]")
-    (T, H, D), (TK, KV, DK), dt = q.shape, k.shape, q.dtype
-    _require(TK == T and DK == D, "q and k must share T and D")
+    shape, k_shape, dt = q.shape, k.shape, q.dtype
+    if len(shape) != 3 or len(k_shape) != 3:
+        raise RuntimeError("q and k must be [T, heads, D]")
+    (T, H, D), (TK, KV, DK) = shape, k_shape
+    if TK != T or DK != D:
+        raise RuntimeError("q and k must share T and D")
     if not (dt in _HALVES and k.dtype == q_out.dtype == k_out.dtype == dt):
         raise RuntimeError("q, k, q_out and k_out must be fp16 or bf16, of one type")
-    if q_out.shape != q.shape or k_out.shape != k.shape:
+    if q_out.shape != shape or k_out.shape != k_shape:
         raise RuntimeError("q_out and k_out must have the shapes of q and k")
     if not (q.get_device() == k.get_device() == q_out.get_device() == k_out.get_device() == dev):
         raise RuntimeError("all tensors must be on one device")
     (qt, qh, q1), (kt, kh, k1), (ot, oh, o1), (pt, ph, p1) = q.stride(), k.stride(), q_out.stride(), k_out.stride()
-    _require(q1 == k1 == o1 == p1 == 1, "q, k, q_out and k_out must have contiguous columns")
+    if not q1 == k1 == o1 == p1 == 1:
+        raise RuntimeError("q, k, q_out and k_out must have contiguous columns")
     if T <= 1:  # a dimension of one has no stride
         qt = kt = ot = pt = 0
     if H == 1:
@@ -584,17 +588,16 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: t
     qp, kp, op, pp = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
     if (qp == op and (qt, qh) != (ot, oh)) or (kp == pp and (kt, kh) != (pt, ph)):
         raise RuntimeError("an output in its input's place must have its strides")
-    if not (rope_cos.dtype == rope_sin.dtype == torch.float32 and rope_cos.dim() == 2 and rope_cos.shape == rope_sin.shape):
+    table = rope_cos.shape
+    if not (rope_cos.dtype == rope_sin.dtype == torch.float32 and len(table) == 2 and rope_sin.shape == table):
         raise RuntimeError("RoPE tables must be fp32 [L, R / 2]")
-    for t in (q_gamma, k_gamma, q_beta, k_beta):
-        if t is not None:
-            _float(D, t)
+    _float(D, *[t for t in (q_gamma, k_gamma, q_beta, k_beta) if t is not None])
     pos64 = False
     if positions is not None:
         pos64 = positions.dtype == torch.int64
         if not (pos64 or positions.dtype == torch.int32) or positions.shape != (T,):
             raise RuntimeError(f"positions must be int32 or int64 [{T}]")
-    L, half = rope_cos.shape
+    L, half = table
     _run("ff_qk_norm_rope", dev, qp, qt, qh, kp, kt, kh, op, ot, oh, pp, pt, ph, _DTYPES[dt], T, H, KV, D, norm,
          _ptr(q_gamma), _ptr(k_gamma), _ptr(q_beta), _ptr(k_beta), eps, rope_cos.data_ptr(), rope_sin.data_ptr(), L,
          2 * half, pairs, _ptr(positions), pos64, q_scale)

@@ -512,10 +512,12 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, OCC) void gemm_mx4_ring_ker
     store_tile<EPI, T, NI, MI, false>(acc, m0 + wm * WM, n0 + wn * WN, lane, args, smem + wave * STAGE);
 }
 
+constexpr int64_t MAX_THREADS = 0xffffffffll;  // of a launch
+
 template <int EPI, typename T, int BM, int BN, int WAVES_M, int WAVES_N, int U, int S, int OCC>
 static int launch_ring(const Mx4Args& a, hipStream_t st) {
   const int64_t tiles = static_cast<int64_t>((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
-  if (tiles > 0x7fffffff) return fail(FF_EINVAL, "gemm_mx4: too many tiles");
+  if (tiles > MAX_THREADS / (64 * WAVES_M * WAVES_N)) return fail(FF_EINVAL, "gemm_mx4: too many tiles for this variant");
   gemm_mx4_ring_kernel<EPI, T, BM, BN, WAVES_M, WAVES_N, U, S, OCC>
       <<<dim3(static_cast<unsigned>(tiles)), 64 * WAVES_M * WAVES_N, 0, st>>>(a);
   return check_launch("gemm_mx4");
@@ -540,8 +542,8 @@ constexpr Mx4Cost MX4_COSTS[5] = {
 };
 static int pick_variant(int M, int N, int K) {
   const double u = K / 128;
-  int best = 1;
-  double least = 0.0;
+  int best = 5;
+  double least = HUGE_VAL;
   for (int v = 0; v < 5; ++v) {
     const Mx4Cost& c = MX4_COSTS[v];
     const double tiles = static_cast<double>((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
@@ -549,7 +551,8 @@ static int pick_variant(int M, int N, int K) {
     rounds = c.whole ? std::ceil(rounds) : std::max(1.0, rounds);
     const double one = rounds * (c.first + c.unit * u), all = std::ceil(tiles / 256.0) * (c.tile + c.tile_unit * u);
     const double t = c.fixed + std::sqrt(std::sqrt(one * one * one * one + all * all * all * all)) + c.out * 1e-6 * M * N;
-    if (v == 0 || t < least) {
+    const bool fits = tiles * (v == 4 ? 512 : 256) <= static_cast<double>(MAX_THREADS);
+    if (fits && t < least) {
       least = t;
       best = v + 1;
     }
@@ -567,7 +570,7 @@ static int launch_mx4(const Mx4Args& a, int variant, hipStream_t st) {
     default: break;
   }
   const int64_t blocks = static_cast<int64_t>((a.M + 31) / 32) * ((a.N + 31) / 32);
-  if (blocks > 0x7fffffff) return fail(FF_EINVAL, "gemm_mx4: too many tiles");
+  if (blocks > MAX_THREADS / 256) return fail(FF_EINVAL, "gemm_mx4: too many tiles for this variant");
   gemm_mx4_split_kernel<EPI, T><<<dim3(static_cast<unsigned>(blocks)), 256, 0, st>>>(a);
   return check_launch("gemm_mx4");
 }

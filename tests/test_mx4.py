@@ -196,6 +196,9 @@ def test_gemm_mx4_rejects_bad_arguments():
                      (dict(Ws=None), "null"), (dict(out=None), "null"), (dict(A=264), "misaligned"),
                      (dict(bias=260), "misaligned"), (dict(out=264), "misaligned"), (dict(As=258), "misaligned"),
                      (dict(epi=1, res=264), "misaligned"), (dict(epi=1, res=272), "overlaps"),
+                     (dict(M=1 << 29, N=64, variant=1), "too many tiles"),
+                     (dict(M=0x7fffff00, N=128, variant=2), "too many tiles"),
+                     (dict(M=1 << 29, N=2048, variant=5), "too many tiles"),
                      (dict(epi=1, out=496), "null"), (dict(epi=1, res=256, out=496), "overlaps")):
         status, msg = call(**kw)
         assert status == FF_EINVAL and what in msg, (kw, msg)

@@ -6,14 +6,16 @@
 // (2 i, 2 i + 1) or halves (i, i + R / 2); q is then multiplied by q_scale. All of it in fp32 with one rounding at the store.
 //
 // HBM-bound: 4 bytes a column (read and written once). A lane holds 8 columns of a head in two pieces of 4 that rotate in
-// the lane: neighbour pairs lie in 8 columns in a row, halves in columns 4 c .. and R / 2 + 4 c .., so either way there is no
-// exchange between lanes but the sums' (DPP), and lane c takes the table entries 4 c .. 4 c + 3. A group of 8, 16 or 32 lanes
-// holds a head; it keeps its head and strides over the tokens, so gamma and beta stay in registers and nothing is divided in
-// the loop. The next token's columns and entries load under this one's arithmetic, its position one token earlier still. Stores
-// stream past L2 (53.5 -> 50.7 us), loads do not (50.0, but the products before and after them then run 5 % slower).
+// the lane: neighbour pairs lie in 8 columns in a row, halves in columns 4 c .. and R / 2 + 4 c .., so the arithmetic has no
+// exchange between lanes but the sums' (DPP), and lane c takes the table entries 4 c .. 4 c + 3. Halves still move 16 bytes a lane
+// where that is aligned: two lanes load two pieces in a row each and swap one (32 800 tokens x 32 heads of 64, RMS: 54 us,
+// 65.6 in 8-byte accesses). A group of 8, 16 or 32 lanes holds a head; it keeps its head and strides over the tokens, so gamma and beta
+// stay in registers and nothing is divided in the loop. The next token's columns and entries load under this one's arithmetic,
+// its position one token earlier still. Stores stream past L2 (53.5 -> 50.7 us), loads do not (50.0, but the products before
+// and after them then run 5 % slower).
 //
-// Measured: 32 800 tokens x (16 + 16) x 64 fp16 LayerNorm 50.7 us, 5.3 TB/s read and written; 9001 x (32 + 8) x 128 bf16 RMS
-// 40.2, 4.7 TB/s (halves: 8-byte accesses); one token 9.1, the host's share of a call.
+// Measured: 32 800 tokens x (16 + 16) x 64 fp16 LayerNorm, pairs, 50.7 us, 5.3 TB/s read and written; 9001 x (32 + 8) x 128 bf16
+// RMS, halves, 37.5, 5.0 TB/s; one token 8.8, the host's share of a call.
 #include <algorithm>
 
 #include "common.h"
@@ -45,6 +47,13 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+typedef int int2_t __attribute__((ext_vector_type(2)));
+
+template <int CTRL>
+__device__ __forceinline__ int dpp_i32(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
+}
+
 template <typename T, int LANES, bool PAIRS, int NORM>
 __global__ __launch_bounds__(256) void qk_norm_kernel(const QkArgs a) {
   constexpr int GROUPS = 256 / LANES;
@@ -55,11 +64,19 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(const QkArgs a) {
   int t = id / chunks;
   const int head = id - t * chunks, which = head >= a.heads[0], h = which ? head - a.heads[0] : head;
   if (t >= stride || t >= a.tokens) return;  // the groups left over
-  // the lane's pieces: turned ones below R, plain ones from there on; lanes past the head load its first columns as zeros
-  const bool in = 8 * c < a.D, turned = 8 * c < a.R;
-  const int pa = !in ? 0 : PAIRS || !turned ? 8 * c : 4 * c;
-  const int pb = !in ? 4 : PAIRS || !turned ? 8 * c + 4 : half + 4 * c;
-  const bool whole = PAIRS && a.wide;  // both pieces in one aligned 16-byte access
+  // The lane's pieces: turned ones below R, plain ones from there on; lanes past the head load its first columns as zeros.
+  // Both in one aligned 16-byte access where that is allowed (a.wide): halves are then loaded as pieces of two lanes, columns
+  // 4 c .. 4 c + 7 by the even one, R / 2 + 4 c .. by the odd one (plain columns 8 c .. by each), and one piece of each is swapped.
+  const bool in = 8 * c < a.D, turned = 8 * c < a.R, whole = a.wide, odd = c & 1, cross = !PAIRS && whole;
+  int at = 8 * c, pa = 8 * c, pb = 8 * c + 4;  // column of the access, of either piece
+  if (!in) {
+    at = 0, pa = 0, pb = 4;
+  } else if (!PAIRS && turned) {
+    pa = 4 * c, pb = half + 4 * c;
+    at = whole && odd ? pb - 4 : pa;
+  } else if (cross) {
+    pa = odd ? 8 * c - 4 : 8 * c, pb = pa + 8;
+  }
   float g[8], b[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -68,8 +85,8 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(const QkArgs a) {
     if constexpr (NORM == FF_NORM_LAYER) b[e] = a.beta[which][col];
   }
   const float q = a.scale[which], inv_d = 1.f / static_cast<float>(a.D);
-  const T* x = static_cast<const T*>(a.x[which]) + h * a.xh[which] + t * a.xt[which] + pa;
-  T* out = static_cast<T*>(a.out[which]) + h * a.oh[which] + t * a.ot[which] + pa;
+  const T* x = static_cast<const T*>(a.x[which]) + h * a.xh[which] + t * a.xt[which] + at;
+  T* out = static_cast<T*>(a.out[which]) + h * a.oh[which] + t * a.ot[which] + at;
   const int64_t xstep = stride * a.xt[which], ostep = stride * a.ot[which];
   const int apart = pb - pa;
   const float* cos = a.cos + (turned ? 4 * c : 0);
@@ -87,26 +104,30 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(const QkArgs a) {
   const int wrap = stride % a.L;  // the step of t mod L
   const int last = a.tokens - 1;
   int row = a.pos ? position(t) : t % a.L, after = a.pos ? position(min(t + stride, last)) : 0;
-  vec4_t<T> nx[2];
+  int4_t nx;
   float4_t nc, ns;
   auto load = [&]() __attribute__((always_inline)) {
     if (whole) {
-      const vec8_t<T> w = *reinterpret_cast<const vec8_t<T>*>(x);
-      nx[0] = vec4_t<T>{w[0], w[1], w[2], w[3]};
-      nx[1] = vec4_t<T>{w[4], w[5], w[6], w[7]};
+      nx = *reinterpret_cast<const int4_t*>(x);
     } else {
-      nx[0] = *reinterpret_cast<const vec4_t<T>*>(x);
-      nx[1] = *reinterpret_cast<const vec4_t<T>*>(x + apart);
+      const int2_t lo = *reinterpret_cast<const int2_t*>(x), hi = *reinterpret_cast<const int2_t*>(x + apart);
+      nx = int4_t{lo[0], lo[1], hi[0], hi[1]};
     }
     const int64_t entry = static_cast<int64_t>(max(row, 0)) * half;
     nc = *reinterpret_cast<const float4_t*>(cos + entry);
     ns = *reinterpret_cast<const float4_t*>(sin + entry);
   };
+  // The even lane's second piece for the odd lane's first; its own inverse.
+  auto swap = [&](int4_t w) __attribute__((always_inline)) {
+    const int r0 = dpp_i32<DPP_XOR1>(odd ? w[0] : w[2]), r1 = dpp_i32<DPP_XOR1>(odd ? w[1] : w[3]);
+    return int4_t{odd ? r0 : w[0], odd ? r1 : w[1], odd ? w[2] : r0, odd ? w[3] : r1};
+  };
   load();
   for (;;) {
+    const vec8_t<T> xs = __builtin_bit_cast(vec8_t<T>, cross ? swap(nx) : nx);
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = in ? static_cast<float>(nx[e >> 2][e & 3]) : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = in ? static_cast<float>(xs[e]) : 0.f;
     const float4_t co = nc, si = ns;
     const float f = row >= 0 ? q : __builtin_nanf("");  // no such row in the table
     const bool more = t < a.tokens - stride;
@@ -148,15 +169,17 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(const QkArgs a) {
         x1 = y1;
       }
     }
-    if (in) {
-      vec8_t<T> w;
+    vec8_t<T> y;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = static_cast<T>(v[e] * f);
+    for (int e = 0; e < 8; ++e) y[e] = static_cast<T>(v[e] * f);
+    int4_t w = __builtin_bit_cast(int4_t, y);
+    if (cross) w = swap(w);
+    if (in) {
       if (whole) {
-        __builtin_nontemporal_store(w, reinterpret_cast<vec8_t<T>*>(out));
+        __builtin_nontemporal_store(w, reinterpret_cast<int4_t*>(out));
       } else {
-        __builtin_nontemporal_store(vec4_t<T>{w[0], w[1], w[2], w[3]}, reinterpret_cast<vec4_t<T>*>(out));
-        __builtin_nontemporal_store(vec4_t<T>{w[4], w[5], w[6], w[7]}, reinterpret_cast<vec4_t<T>*>(out + apart));
+        __builtin_nontemporal_store(int2_t{w[0], w[1]}, reinterpret_cast<int2_t*>(out));
+        __builtin_nontemporal_store(int2_t{w[2], w[3]}, reinterpret_cast<int2_t*>(out + apart));
       }
     }
     if (!more) break;
@@ -248,10 +271,14 @@ extern "C" int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, c
     return fail(FF_EINVAL, "qk_norm_rope: the rows of an output overlap");
   if (q_out == k_out || q_out == k || k_out == q)
     return fail(FF_EINVAL, "qk_norm_rope: q_out and k_out must be two, each apart from the other's input");
+  // 16-byte accesses: halves need pairs of lanes that swap pieces, which pays where columns fill three quarters of a head's
+  // lanes (32 800 tokens x 32 heads of 48 47.4 us, 55.3 without; 16 400 x 24 of 96 37.0 and 42.4, of 80 29.0 and 28.2)
+  const int64_t lanes = D <= 64 ? 8 : D <= 128 ? 16 : 32;
+  const bool wide = (low & 15) == 0 && (pairs || (D % 16 == 0 && R % 16 == 0 && D >= 6 * lanes));
   const QkArgs a{{q, k}, {q_out, k_out}, {q_token, k_token}, {q_head, k_head}, {qo_token, ko_token}, {qo_head, ko_head},
                  {q_gamma, k_gamma}, {q_beta, k_beta}, rope_cos, rope_sin, positions, pos64, static_cast<int>(T),
                  {static_cast<int>(heads), static_cast<int>(kv_heads)}, static_cast<int>(D), static_cast<int>(R),
-                 static_cast<int>(rope_len), norm, (low & 15) == 0, eps, {q_scale, 1.f}};
+                 static_cast<int>(rope_len), norm, wide, eps, {q_scale, 1.f}};
   if (dtype == FF_F16)
     launch_qk_shape<half_t>(a, pairs != 0, as_stream(stream));
   else

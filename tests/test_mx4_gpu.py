@@ -395,7 +395,8 @@ def check_qk(got, x, norm, gamma, beta, cos, sin, pos, pairs, scale, kind):
 @pytest.mark.parametrize(("T", "H", "KV", "D", "R", "L"), [
     (1, 1, 1, 8, 8, 1), (1, 32, 8, 128, 128, 50), (5, 3, 1, 64, 64, 2), (33, 16, 16, 64, 64, 33), (7, 4, 2, 80, 80, 9),
     (6, 5, 5, 96, 24, 6), (9, 2, 2, 256, 256, 11), (4, 8, 4, 256, 72, 7), (130, 6, 2, 128, 64, 17), (3, 2, 1, 40, 16, 5),
-    (1027, 3, 3, 64, 48, 1025), (2, 70, 30, 128, 128, 3)])
+    (1027, 3, 3, 64, 48, 1025), (2, 70, 30, 128, 128, 3), (5, 3, 2, 96, 32, 4), (9, 2, 1, 48, 16, 9), (6, 3, 2, 192, 176, 5),
+    (3, 2, 2, 240, 240, 3)])
 def test_qk_norm_rope(dev, rng, T, H, KV, D, R, L, pairs, norm, kind):
     """Packed rows: q and k are views of [T, H + 2 KV, D], and the packed outputs' value columns stay as they were."""
     K = kern()
@@ -443,6 +444,28 @@ def test_qk_norm_rope_positions_and_layouts(dev, rng, pairs, int_type):
     got = ko.double().cpu().numpy()
     check_qk(got[:, 1 : T + 1].transpose(1, 0, 2), xk, OQ.RMS, g[1], None, cos, sin, pos, pairs, 1.0, "fp16")
     assert (got[:, 0] == 7).all() and (got[:, T + 1 :] == 7).all()
+
+
+@pytest.mark.parametrize("pairs", [True, False])
+@pytest.mark.parametrize(("D", "R"), [(64, 64), (128, 96), (256, 16), (48, 32)])
+def test_qk_norm_rope_is_the_same_at_any_alignment(dev, rng, D, R, pairs):
+    """Rows from multiples of 16 bytes and of 8 only take different accesses and the same arithmetic."""
+    K = kern()
+    T, H = 37, 5
+    x, _ = typed(rng.standard_normal((T, H, D)), "bf16", dev)
+    cos, sin = (gpu(t, dev) for t in tables(rng, T, R))
+    g = gpu((1 + 0.1 * rng.standard_normal(D)).astype(np.float32), dev)
+    outs = []
+    for shift in (0, 4):
+        rows = torch.full((T, H * D + 8), 7.0, dtype=torch.bfloat16, device=dev)
+        y = rows[:, shift : shift + H * D].unflatten(1, (H, D))
+        o = torch.full_like(rows, 7.0)
+        y.copy_(x)
+        K.qk_norm_rope(y, x, o[:, shift : shift + H * D].unflatten(1, (H, D)), torch.empty_like(x), OQ.RMS, g, g, None, None,
+                       cos, sin, None, pairs)
+        assert (o[:, :shift] == 7).all() and (o[:, shift + H * D :] == 7).all()
+        outs.append(o[:, shift : shift + H * D].clone())
+    assert torch.equal(*outs)
 
 
 def test_qk_norm_rope_offsets_past_32_bits(dev, rng):

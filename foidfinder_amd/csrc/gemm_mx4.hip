@@ -13,14 +13,16 @@
 // consecutive columns n: column pairs (SwiGLU) are in-lane and stores are whole runs.
 //
 // Five tile shapes, by an estimate of their times (pick_variant). 32 x 32 blocks with K over the four waves and fragments
-// straight from memory serve few rows and few columns: one row x 2304 x 768 takes 3.9 us. 64 x 64 tiles serve what leaves CUs
-// idle otherwise: 1025 x 1024 x 2816 with a residual 7.6 us, bound by the 22 units that follow each other; 16 x 98 782 x 1152 14 us, 4.8 TB/s, the weights' bytes. 128 x 128, 256 x 128 and 256 x 256 tiles
-// read each operand less often: 5184 x 4736 x 1024 GELU 25 us (2.0 PFLOP/s, the stores of 49 MB take half), 32 800 x 5632 x 1024
-// SwiGLU 131 us (2.9 PFLOP/s), 32 768 x 4096 x 4096 282 us (3.9 PFLOP/s). The instruction alone reaches 6.1 PFLOP/s on random
-// codes (the card's power). At K = 1024 the products take 82 of 131 us, the ring's loads add 23 and the epilogue 25; every
-// part left out gives about its own share, as a limit on power does. Measured and not kept: W as a stream past persistent waves
-// for few rows (16.8 us against 14), workgroups whose ring runs on across tiles (132-134 us against
-// 132-136, spills with a residual, slower for few tiles), slots of two units for the large tiles, loads spread between the products.
+// straight from memory serve few rows and few columns: one row x 2304 x 768 takes 3.9 us. 64 x 64 tiles serve what leaves
+// CUs idle otherwise: 1025 x 1024 x 2816 with a residual 7.6 us (272 tiles, 22 units each: neither more slots nor K on two
+// groups of waves is faster); 16 x 98 782 x 1152 14 us, 4.8 TB/s, the weights' bytes. 128 x 128, 256 x 128 and 256 x 256
+// tiles read each operand less often: 5184 x 4736 x 1024 GELU 25-26 us (1.9-2.0 PFLOP/s with 49 MB of stores), 32 800 x
+// 5632 x 1024 SwiGLU 131-137 us (2.8-2.9 PFLOP/s), 32 768 x 4096 x 4096 282 us (3.9 PFLOP/s). The instruction alone reaches
+// 6.1 PFLOP/s on random codes (the card's power). At K = 1024 the products take 82 of 131 us, the ring's loads add 23 and
+// the epilogue 25; every part left out gives about its own share, as a limit on power does. Measured and not kept: W as a
+// stream past persistent waves for few rows (16.8 us against 14), workgroups whose ring runs on across tiles (132-134 us
+// against 132-136, spills with a residual, slower for few tiles), slots of two units for the large tiles, loads spread
+// between the products.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -17,6 +17,7 @@ from functools import cache
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "libfoidfinder_rocm.so"
 ENV = "FOIDFINDER_ROCM_KERNELS"  # path to a prebuilt library (the reference's $FOIDFINDER_KERNELS)
@@ -487,11 +488,16 @@ def _mx4(codes: torch.Tensor, scale: torch.Tensor, name: str) -> tuple[int, int]
 
 
 def _no_grad(*ts: torch.Tensor | None) -> None:
-    """Refuses tensors that autograd would follow: these ops write into given tensors and have no backward."""
+    """Refuses tensors that autograd would follow, backward or forward: these ops write into given tensors and have no
+    derivative. (Forward mode does not end with torch.no_grad().)"""
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
                 raise RuntimeError("this op has no backward: call it under torch.no_grad() or detach its tensors")
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("this op has no derivative in forward mode: give it tensors without a tangent")
 
 
 def quant_mx4(x: torch.Tensor, out: torch.Tensor, scale: torch.Tensor, rotate: bool = True, norm: int = NORM_NONE,

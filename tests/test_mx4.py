@@ -290,3 +290,33 @@ def test_op_schemas():
     assert "Tensor(a!) out, int epi, int stages=0, Tensor? residual=None" in str(ops.gemm_mx4.default._schema)
     assert "Tensor(a!) q_out, Tensor(b!) k_out, int norm" in str(ops.qk_norm_rope.default._schema)
     assert "Tensor(a!) out" in str(ops.dequant_mx4.default._schema)
+
+
+def test_tensors_with_a_tangent_are_refused(monkeypatch):
+    """A forward-mode dual needs no grad, also under no_grad; the ops would lose its tangent. Inside a level, tensors without
+    a tangent are taken."""
+    from torch.autograd import forward_ad
+
+    monkeypatch.setattr(K, "_on_gpu", lambda *ts: -1)
+    monkeypatch.setattr(K, "_run", lambda *a: None)
+
+    def mx(T, C):
+        return torch.zeros(T, C // 2, dtype=torch.uint8), torch.zeros(C // 128, T, dtype=torch.int32)
+
+    def calls(x, y, q):
+        t = torch.zeros(3, 32)
+        return (lambda: K.quant_mx4(x, *mx(3, 256)), lambda: K.dequant_mx4(*mx(3, 256), x),
+                lambda: K.gemm_mx4(*mx(3, 128), *mx(256, 128), None, x, K.EPI_BIAS_F16),
+                lambda: K.gemm_mx4(*mx(3, 128), *mx(256, 128), y, torch.zeros(3, 256), K.EPI_BIAS_F16),
+                lambda: K.qk_norm_rope(q, q, q.clone(), q.clone(), K.NORM_NONE, None, None, None, None, t, t))
+
+    plain = torch.zeros(3, 256, dtype=torch.half), torch.zeros(256), torch.zeros(3, 4, 64, dtype=torch.half)
+    with forward_ad.dual_level():
+        duals = [forward_ad.make_dual(t, torch.ones_like(t)) for t in plain]
+        for call in calls(*duals):
+            with pytest.raises(RuntimeError, match="forward mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward mode"):
+                call()
+        for call in calls(*plain):
+            call()

@@ -622,3 +622,18 @@ def test_ops_on_two_streams_at_once(dev, rng):
     torch.cuda.synchronize()
     for (_, _, out), ref in zip(jobs, want):
         assert torch.equal(out, ref)
+
+
+def test_mx4_ops_refuse_tensors_with_a_tangent(dev):
+    """Through the dispatcher as well."""
+    from torch.autograd import forward_ad
+
+    K = kern()
+    x = torch.zeros(2, 128, dtype=torch.half, device=dev)
+    codes, scale, _ = empty_mx4(2, 128, dev)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for op in (K.quant_mx4, K.kernels().quant_mx4):
+            with pytest.raises(RuntimeError, match="forward mode"):
+                op(dual, codes, scale)
+            op(x, codes, scale)

@@ -33,6 +33,18 @@ int64_t resident_blocks(const void* kernel, int block, size_t smem);
 
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
+// Bytes that an operand covers: n[0] x n[1] runs of `len` bytes, pitch[0] and pitch[1] (>= 0) bytes apart; a dimension of one
+// run has no pitch.
+struct Extent {
+  uintptr_t at;
+  int64_t n[2], pitch[2], len;
+};
+inline Extent range(const void* p, int64_t bytes) { return {reinterpret_cast<uintptr_t>(p), {1, 1}, {0, 0}, bytes}; }
+// Whether two operands share no byte, as far as their pitches show it: exact for ranges, and for runs whose pitches are equal
+// where both have several; runs at different pitches count as apart if their whole extents are, or if they keep to columns of
+// their own within a common pitch.
+bool apart(const Extent& a, const Extent& b);
+
 // ---- device helpers ----
 
 // Workgroups are dispatched round-robin over the 8 XCDs (block b runs on XCD b % 8), each with its own L2. This

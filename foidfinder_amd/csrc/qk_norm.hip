@@ -271,6 +271,27 @@ extern "C" int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, c
     return fail(FF_EINVAL, "qk_norm_rope: the rows of an output overlap");
   if (q_out == k_out || q_out == k || k_out == q)
     return fail(FF_EINVAL, "qk_norm_rope: q_out and k_out must be two, each apart from the other's input");
+  // Rows are read and written by different workgroups, in no order: an output is its input itself or shares no byte with what
+  // is read or with the other output.
+  auto rows = [&](const void* p, int64_t token, int64_t head, int64_t n) {
+    return Extent{reinterpret_cast<uintptr_t>(p), {T, n}, {2 * token, 2 * head}, 2 * D};
+  };
+  const Extent in[2] = {rows(q, q_token, q_head, heads), rows(k, k_token, k_head, kv_heads)};
+  const Extent to[2] = {rows(q_out, qo_token, qo_head, heads), rows(k_out, ko_token, ko_head, kv_heads)};
+  auto in_place = [](const Extent& a, const Extent& b) {
+    return a.at == b.at && (a.n[0] <= 1 || a.pitch[0] == b.pitch[0]) && (a.n[1] <= 1 || a.pitch[1] == b.pitch[1]);
+  };
+  const Extent read[7] = {range(rope_cos, rope_len * R * 2), range(rope_sin, rope_len * R * 2), range(q_gamma, 4 * D),
+                          range(k_gamma, 4 * D), range(q_beta, 4 * D), range(k_beta, 4 * D),
+                          range(positions, T * (pos64 ? 8 : 4))};
+  bool clear = apart(to[0], to[1]);
+  for (int i = 0; i < 2; ++i) {
+    clear = clear && (in_place(to[i], in[i]) || apart(to[i], in[i])) && apart(to[i], in[1 - i]);
+    for (const Extent& e : read) clear = clear && (e.at == 0 || apart(to[i], e));
+  }
+  if (!clear)
+    return fail(FF_EINVAL, "qk_norm_rope: an output overlaps the other one or what is read (its own input, with its strides, "
+                           "may be in its place)");
   // 16-byte accesses: halves need pairs of lanes that swap pieces, which pays where columns fill three quarters of a head's
   // lanes (32 800 tokens x 32 heads of 48 47.4 us, 55.3 without; 16 400 x 24 of 96 37.0 and 42.4, of 80 29.0 and 28.2)
   const int64_t lanes = D <= 64 ? 8 : D <= 128 ? 16 : 32;

@@ -566,7 +566,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: t
     """Norm of each head's query and key and their rotation by position in one pass (include/foidfinder_rocm.h,
     ff_qk_norm_rope): q fp16 or bf16 [T, heads, D], k [T, kv_heads, D], views with any token and head strides (of a packed
     [T, 3 C] row, say: `qkv.view(T, 3, heads, D)[:, 0]`) -> q_out, k_out of the same shapes; an output may be its input
-    itself and shares no other memory with q or k. gamma (with a norm) and beta (NORM_LAYER) fp32 [D]; tables fp32 [L, R / 2];
+    itself and shares no other memory with what is read or with the other (refused). gamma (with a norm) and beta (NORM_LAYER) fp32 [D]; tables fp32 [L, R / 2];
     positions int32 or int64 [T], or None: t % L. `pairs`: columns (2 i, 2 i + 1) turn together, else (i, i + R / 2)."""
     _no_grad(q, k, q_out, k_out, q_gamma, k_gamma, q_beta, k_beta, rope_cos, rope_sin)
     dev = _on_gpu(q_gamma, k_gamma, q_beta, k_beta, rope_cos, rope_sin, positions)

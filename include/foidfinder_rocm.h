@@ -108,7 +108,9 @@ int ff_gemm_mx4_variants(void);
 /* The norm of each head's query and key, then their rotation by position, then q x q_scale, in one pass and one rounding.
  * q fp16 or bf16 [T, heads, D] and k [T, kv_heads, D] by strides in elements (token, head; columns contiguous), so views of
  * packed rows are taken as they are (pointers and strides multiples of 8 bytes); q_out and k_out the same shapes by their own
- * strides, each either its input itself (the same pointer and strides) or memory apart from q and k. D % 8 == 0, D <= 256.
+ * strides, each either its input itself (the same pointer and strides) or memory apart from all that is read and from the other.
+ * Other calls are refused; where an output lies between rows of another operand, the two must have one token or head stride in
+ * common. D % 8 == 0, D <= 256.
  * Norm (FF_NORM_*) over the D columns with fp32 gamma/beta [D]. Rotation of the first R columns (R % 8 == 0) by row p of
  * rope_cos/rope_sin fp32 [rope_len, R/2], rope_len < 2^30: pairs = 1 turns columns (2 i, 2 i + 1), pairs = 0 columns
  * (i, i + R/2); p = positions[t] (int32, or int64 with pos64; a token whose position is outside the table becomes not a

@@ -3,6 +3,7 @@ come before any HIP call)."""
 
 from __future__ import annotations
 
+import ctypes
 from fractions import Fraction
 
 import numpy as np
@@ -320,3 +321,70 @@ def test_tensors_with_a_tangent_are_refused(monkeypatch):
                 call()
         for call in calls(*plain):
             call()
+
+
+class Extent(ctypes.Structure):
+    """ff::Extent of csrc/common.h."""
+
+    _fields_ = [("at", ctypes.c_uint64), ("n", ctypes.c_int64 * 2), ("pitch", ctypes.c_int64 * 2), ("len", ctypes.c_int64)]
+
+    def bytes(self):
+        return {self.at + i * self.pitch[0] + j * self.pitch[1] + b for i in range(self.n[0]) for j in range(self.n[1])
+                for b in range(self.len)}
+
+
+def test_operands_that_share_bytes_by_brute_force():
+    """Never apart where a byte is shared; always apart where none is, if the pitches are equal or one operand is a range."""
+    fn = K.lib()["_ZN2ff5apartERKNS_6ExtentES2_"]
+    fn.argtypes, fn.restype = [ctypes.POINTER(Extent)] * 2, ctypes.c_bool
+    rng = np.random.default_rng(11)
+    seen = set()
+    for _ in range(6000):
+        kind = rng.integers(4)
+        n = [[int(v) for v in rng.integers(1, 5, 2)] for _ in range(2)]
+        pitch = [[int(v) for v in rng.integers(0, 40, 2)] for _ in range(2)]
+        if kind == 0:
+            pitch[1] = pitch[0]
+        elif kind == 1:
+            n[1] = [1, 1]
+        elif kind == 2:  # one token pitch, heads of their own
+            pitch[1][0] = pitch[0][0] = int(rng.integers(20, 90))
+        a, b = (Extent(int(rng.integers(100, 180)), (ctypes.c_int64 * 2)(*n[i]), (ctypes.c_int64 * 2)(*pitch[i]),
+                       int(rng.integers(1, 9))) for i in range(2))
+        got, want = fn(a, b), not (a.bytes() & b.bytes())
+        assert got == fn(b, a)
+        if kind < 2:
+            assert got == want, (kind, n, pitch, a.at, b.at, a.len, b.len)
+        else:
+            assert want or not got, (kind, n, pitch, a.at, b.at, a.len, b.len)
+        seen.add((kind, got, want))
+    assert {(k, v, v) for k in range(4) for v in (True, False)} <= seen
+    far = 1 << 40  # offsets past 32 bits: the same rows a gigabyte on, then 4 bytes into the last of them
+    a = Extent(far, (ctypes.c_int64 * 2)(5, 1), (ctypes.c_int64 * 2)(1 << 31, 0), 128)
+    for off, want in ((128, True), ((4 << 31) + 128, True), ((4 << 31) + 124, False), (-128, True), (-124, False),
+                      (5 << 31, True), ((4 << 31) - 128, True)):
+        assert fn(a, Extent(far + off, (ctypes.c_int64 * 2)(5, 1), (ctypes.c_int64 * 2)(1 << 31, 0), 128)) == want, off
+
+
+def test_qk_norm_rope_refuses_outputs_that_share_memory():
+    """Different workgroups read and write the rows: any byte in common but an output in its input's own place is a race."""
+    big = 1 << 30
+
+    def call(q=big, k=2 * big, qo=3 * big, ko=4 * big, st=((1024, 64),) * 4, T=4, H=16, KV=16, D=64, cos=5 * big,
+             sin=6 * big, g=7 * big, pos=None, pos64=0):
+        return err(K.lib().ff_qk_norm_rope(q, *st[0], k, *st[1], qo, *st[2], ko, *st[3], 0, T, H, KV, D, 1, g, g, None, None,
+                                           1e-6, cos, sin, 8, 64, 1, pos, pos64, 1.0, None))
+
+    packed = ((3072, 64),) * 4  # q, k and v of [T, 3, 16, 64]
+    last = 2 * (3 * 1024 + 15 * 64 + 63)  # the last value of a [4, 16, 64] operand
+    for kw in (dict(qo=big + 128), dict(qo=big - 128), dict(qo=big + 2048),  # a head or a token further in q
+               dict(k=big + 2048, qo=big + 128, st=packed),  # q_out ends one head into k
+               dict(k=big + 2048, qo=big, ko=big + 2048 + 6144, st=packed),  # k_out one token past k
+               dict(ko=3 * big + 128), dict(qo=4 * big + last - 6),  # the outputs share heads, or the last values
+               dict(qo=big, k=big + 128, st=((1024, 64), (1024, 64), (1024, 64), (1024, 64)), KV=1),  # k is q's second head
+               dict(qo=big, st=((1024, 64), (1024, 64), (2048, 64), (1024, 64))),  # in place with other strides
+               dict(ko=2 * big, st=((1024, 64), (0, 64), (1024, 64), (1024, 64))),  # in place of one row for every token
+               dict(cos=3 * big + 1024), dict(sin=4 * big - 16), dict(g=3 * big + 2 * 3840), dict(pos=4 * big + last - 6),
+               dict(pos=4 * big - 24, pos64=1)):
+        status, msg = call(**kw)
+        assert status == FF_EINVAL and "overlap" in msg, (kw, msg)

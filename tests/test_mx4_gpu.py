@@ -637,3 +637,36 @@ def test_mx4_ops_refuse_tensors_with_a_tangent(dev):
             with pytest.raises(RuntimeError, match="forward mode"):
                 op(dual, codes, scale)
             op(x, codes, scale)
+
+
+@pytest.mark.parametrize("T", [1, 6])
+@pytest.mark.parametrize("layout", ["packed", "by head", "heads first", "heads first, by token", "into the values",
+                                    "one row of keys"])
+def test_qk_norm_rope_rows_between_the_other_operands(dev, rng, layout, T):
+    """Layouts in which the operands lie between each other's rows and share nothing: as with operands of their own."""
+    K = kern()
+    H, D = 4, 64
+    cos, sin = (gpu(t, dev) for t in tables(rng, 3, D))
+    gq, gk = (gpu((1 + 0.1 * rng.standard_normal(D)).astype(np.float32), dev) for _ in range(2))
+    if layout == "one row of keys":
+        b, _ = typed(rng.standard_normal((T, H + 1, D)), "fp16", dev)
+        q, k = b[:, :H], b[:, H:]
+        qo, ko = q, k
+    elif layout in ("packed", "into the values"):
+        b, _ = typed(rng.standard_normal((T, 4, H, D)), "fp16", dev)
+        q, k = b[:, 0], b[:, 1]
+        qo, ko = (q, k) if layout == "packed" else (b[:, 2], b[:, 3])
+    elif layout == "by head":
+        b, _ = typed(rng.standard_normal((T, H, 4, D)), "fp16", dev)
+        q, k, qo, ko = (b[:, :, i] for i in range(4))
+    elif layout == "heads first":
+        b, _ = typed(rng.standard_normal((4, H, T, D)), "fp16", dev)
+        q, k, qo, ko = (b[i].transpose(0, 1) for i in range(4))
+    else:
+        b, _ = typed(rng.standard_normal((H, T, 4, D)), "fp16", dev)
+        q, k, qo, ko = (b[:, :, i].transpose(0, 1) for i in range(4))
+    want = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty_like(k, memory_format=torch.contiguous_format)
+    args = (OQ.RMS, gq, gk, None, None, cos, sin)
+    K.qk_norm_rope(q.clone(), k.clone(), *want, *args)
+    K.qk_norm_rope(q, k, qo, ko, *args)
+    assert torch.equal(qo, want[0]) and torch.equal(ko, want[1])

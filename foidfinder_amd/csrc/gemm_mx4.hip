@@ -513,12 +513,9 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, OCC) void gemm_mx4_ring_ker
     store_tile<EPI, T, NI, MI, false>(acc, m0 + wm * WM, n0 + wn * WN, lane, args, smem + wave * STAGE);
 }
 
-constexpr int64_t MAX_THREADS = 0xffffffffll;  // of a launch
-
 template <int EPI, typename T, int BM, int BN, int WAVES_M, int WAVES_N, int U, int S, int OCC>
 static int launch_ring(const Mx4Args& a, hipStream_t st) {
   const int64_t tiles = static_cast<int64_t>((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
-  if (tiles > MAX_THREADS / (64 * WAVES_M * WAVES_N)) return fail(FF_EINVAL, "gemm_mx4: too many tiles for this variant");
   gemm_mx4_ring_kernel<EPI, T, BM, BN, WAVES_M, WAVES_N, U, S, OCC>
       <<<dim3(static_cast<unsigned>(tiles)), 64 * WAVES_M * WAVES_N, 0, st>>>(a);
   return check_launch("gemm_mx4");
@@ -530,30 +527,35 @@ static int launch_ring(const Mx4Args& a, hipStream_t st) {
 // 5120); on 200 others its pick is 1.5 % slower than the fastest shape on average and 19 % at worst, where the 64 x 64
 // tiles alone are 10 % slower on average, the 256 x 128 tiles alone 77 %.
 struct Mx4Cost {
-  int bm, bn, resident;  // tile, workgroups a CU holds
-  bool whole;            // rounds count whole (few tiles a CU) or as a fraction
+  int bm, bn, threads, resident;  // tile, threads of a workgroup, workgroups a CU holds
+  bool whole;                     // rounds count whole (few tiles a CU) or as a fraction
   double fixed, first, unit, tile, tile_unit, out;
 };
 constexpr Mx4Cost MX4_COSTS[5] = {
-    {32, 32, 4, false, 3.158, 0.607, 0.0353, 0.144, 0.0972, 1.149},
-    {64, 64, 3, true, 2.968, 0.504, 0.1246, 0.0, 0.1097, 0.586},
-    {128, 128, 3, true, 3.740, 0.528, 0.0971, 0.0, 0.2919, 0.376},
-    {256, 128, 2, false, 3.725, 1.567, 0.1800, 0.674, 0.4621, 0.365},
-    {256, 256, 1, false, 1.317, 4.798, 0.2753, 3.826, 0.6012, 0.389},
+    {32, 32, 256, 4, false, 3.158, 0.607, 0.0353, 0.144, 0.0972, 1.149},
+    {64, 64, 256, 3, true, 2.968, 0.504, 0.1246, 0.0, 0.1097, 0.586},
+    {128, 128, 256, 3, true, 3.740, 0.528, 0.0971, 0.0, 0.2919, 0.376},
+    {256, 128, 256, 2, false, 3.725, 1.567, 0.1800, 0.674, 0.4621, 0.365},
+    {256, 256, 512, 1, false, 1.317, 4.798, 0.2753, 3.826, 0.6012, 0.389},
 };
+static int64_t tiles_of(const Mx4Cost& c, int M, int N) {
+  return static_cast<int64_t>((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+}
+static bool launchable(const Mx4Cost& c, int M, int N) {  // a launch has fewer than 2^32 threads
+  return tiles_of(c, M, N) <= 0xffffffffll / c.threads;
+}
 static int pick_variant(int M, int N, int K) {
   const double u = K / 128;
   int best = 5;
   double least = HUGE_VAL;
   for (int v = 0; v < 5; ++v) {
     const Mx4Cost& c = MX4_COSTS[v];
-    const double tiles = static_cast<double>((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+    const double tiles = static_cast<double>(tiles_of(c, M, N));
     double rounds = tiles / (256.0 * c.resident);
     rounds = c.whole ? std::ceil(rounds) : std::max(1.0, rounds);
     const double one = rounds * (c.first + c.unit * u), all = std::ceil(tiles / 256.0) * (c.tile + c.tile_unit * u);
     const double t = c.fixed + std::sqrt(std::sqrt(one * one * one * one + all * all * all * all)) + c.out * 1e-6 * M * N;
-    const bool fits = tiles * (v == 4 ? 512 : 256) <= static_cast<double>(MAX_THREADS);
-    if (fits && t < least) {
+    if (launchable(c, M, N) && t < least) {
       least = t;
       best = v + 1;
     }
@@ -563,7 +565,7 @@ static int pick_variant(int M, int N, int K) {
 
 template <int EPI, typename T>
 static int launch_mx4(const Mx4Args& a, int variant, hipStream_t st) {
-  switch (variant ? variant : pick_variant(a.M, a.N, a.K)) {
+  switch (variant) {
     case 2: return launch_ring<EPI, T, 64, 64, 2, 2, 2, 3, 3>(a, st);
     case 3: return launch_ring<EPI, T, 128, 128, 2, 2, 1, 3, 3>(a, st);
     case 4: return launch_ring<EPI, T, 256, 128, 2, 2, 1, 3, 2>(a, st);
@@ -571,7 +573,6 @@ static int launch_mx4(const Mx4Args& a, int variant, hipStream_t st) {
     default: break;
   }
   const int64_t blocks = static_cast<int64_t>((a.M + 31) / 32) * ((a.N + 31) / 32);
-  if (blocks > MAX_THREADS / 256) return fail(FF_EINVAL, "gemm_mx4: too many tiles for this variant");
   gemm_mx4_split_kernel<EPI, T><<<dim3(static_cast<unsigned>(blocks)), 256, 0, st>>>(a);
   return check_launch("gemm_mx4");
 }
@@ -611,12 +612,16 @@ extern "C" int ff_gemm_mx4(const uint8_t* A, const uint32_t* a_scale, const uint
   if (low(A) || low(W) || low(out) || low(bias) || (epi == FF_EPI_RESIDUAL && low(residual)) || (low(a_scale) & 3) ||
       (low(w_scale) & 3))
     return fail(FF_EINVAL, "gemm_mx4: misaligned pointer");
-  if (epi == FF_EPI_RESIDUAL && residual != out) {  // elements are read and written by different workgroups, in no order
-    const uintptr_t r = reinterpret_cast<uintptr_t>(residual), o = reinterpret_cast<uintptr_t>(out);
-    const uintptr_t apart = r < o ? o - r : r - o;
-    if (apart < static_cast<uintptr_t>(M) * static_cast<uintptr_t>(N) * 2)
-      return fail(FF_EINVAL, "gemm_mx4: residual overlaps out in part");
-  }
+  const Extent to = range(out, M * (epi == FF_EPI_SWIGLU ? N / 2 : N) * (dtype == FF_F32 ? 4 : 2));
+  // elements are read and written by different workgroups, in no order
+  if (epi == FF_EPI_RESIDUAL && residual != out && !apart(to, range(residual, to.len)))
+    return fail(FF_EINVAL, "gemm_mx4: residual overlaps out in part");
+  if (variant == 0) variant = pick_variant(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
+  if (!launchable(MX4_COSTS[variant - 1], static_cast<int>(M), static_cast<int>(N)))
+    return fail(FF_EINVAL, "gemm_mx4: too many tiles for this variant");
+  for (const Extent& e : {range(A, M * (K / 2)), range(a_scale, M * (K / 32)), range(W, N * (K / 2)),
+                          range(w_scale, N * (K / 32)), range(bias, 4 * N)})
+    if (e.at != 0 && !apart(to, e)) return fail(FF_EINVAL, "gemm_mx4: out overlaps an operand");
   const Mx4Args a{A, a_scale, W, w_scale, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), bias, residual,
                   out};
   const hipStream_t st = as_stream(stream);

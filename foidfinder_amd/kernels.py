@@ -538,7 +538,7 @@ def gemm_mx4(A: torch.Tensor, a_scale: torch.Tensor, W: torch.Tensor, w_scale: t
              out: torch.Tensor, epi: int, stages: int = 0, residual: torch.Tensor | None = None) -> None:
     """MX4 A [M, K] x MX4 W [N, K] + bias fp32 [N] (or None) -> epilogue into out: EPI_BIAS_F16 (out fp16, bf16 or fp32),
     EPI_GELU_F16, EPI_SWIGLU (out [M, N / 2]) or EPI_RESIDUAL (out = y + residual of out's type, which is out itself (None)
-    or memory apart from it). `stages` selects the tile variant (0 = by the sizes) (ff_gemm_mx4)."""
+    or memory apart from it). out shares no memory with the other operands (refused). `stages` selects the tile variant (0 = by the sizes) (ff_gemm_mx4)."""
     _no_grad(bias, out, residual)
     dev = _on_gpu(A, a_scale, W, w_scale, bias, out, residual)
     M, K = _mx4(A, a_scale, "A's")

@@ -98,7 +98,8 @@ int ff_dequant_mx4(const uint8_t* codes, const uint32_t* scale, int64_t T, int64
 /* MX4 product with fp32 sums and a fused epilogue: y[m, n] = sum_k A[m, k] W[n, k] + bias[n] (bias fp32 [N] or NULL), then
  * FF_EPI_BIAS_F16 (out = y, in fp16, bf16 or fp32), FF_EPI_RESIDUAL (out = y + residual, which is out itself or memory
  * apart from it), FF_EPI_GELU_F16 or FF_EPI_SWIGLU (columns are (gate j, value j) pairs, out [M, N/2], N even). A MX4 [M, K],
- * W MX4 [N, K], K % 128 == 0, K <= 2^22, any M, any N <= 2^21; pointers are multiples of 16 bytes (the scales' of 4).
+ * W MX4 [N, K], K % 128 == 0, K <= 2^22, any M < 2^31 - 255, any N <= 2^21; pointers are multiples of 16 bytes (the scales'
+ * of 4); out shares no memory with A, W, their scales or the bias.
  * `variant` selects the tile shape (1 .. ff_gemm_mx4_variants()), 0 = by the sizes. */
 int ff_gemm_mx4(const uint8_t* A, const uint32_t* a_scale, const uint8_t* W, const uint32_t* w_scale, int64_t M, int64_t N,
                 int64_t K, const float* bias, const void* residual, void* out, int dtype, int epi, int variant,

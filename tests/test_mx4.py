@@ -388,3 +388,19 @@ def test_qk_norm_rope_refuses_outputs_that_share_memory():
                dict(pos=4 * big - 24, pos64=1)):
         status, msg = call(**kw)
         assert status == FF_EINVAL and "overlap" in msg, (kw, msg)
+
+
+def test_gemm_mx4_refuses_an_out_that_shares_memory():
+    big = 1 << 30
+
+    def call(A=big, As=2 * big, W=3 * big, Ws=4 * big, bias=5 * big, res=None, out=6 * big, dtype=0, epi=4):
+        return err(K.lib().ff_gemm_mx4(A, As, W, Ws, 100, 64, 256, bias, res, out, dtype, epi, 0, None))
+
+    # out 100 x 64 fp16 12 800 bytes (fp32 25 600, SwiGLU 6 400), A 12 800, its scale 800, W 8 192, its scale 512, bias 256
+    for kw in (dict(out=big), dict(out=big + 12784), dict(out=big - 12784), dict(out=2 * big - 12800 + 16),
+               dict(As=6 * big + 12796), dict(out=3 * big + 8176), dict(out=3 * big - 12784), dict(out=4 * big + 496),
+               dict(bias=6 * big + 12784), dict(bias=6 * big + 25584, dtype=2), dict(out=5 * big + 240, dtype=2),
+               dict(out=big - 6384, epi=3), dict(epi=1, res=6 * big, out=6 * big, W=6 * big + 12784),
+               dict(epi=1, res=6 * big + 12784), dict(epi=1, res=6 * big - 12784)):
+        status, msg = call(**kw)
+        assert status == FF_EINVAL and "overlap" in msg, (kw, msg)

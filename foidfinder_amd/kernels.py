@@ -506,7 +506,8 @@ def quant_mx4(x: torch.Tensor, out: torch.Tensor, scale: torch.Tensor, rotate: b
     """x fp16 or bf16 [T, C] (C % 128 == 0; any row stride from C up that is a multiple of 8) -> MX4: out uint8 [T, C / 2],
     scale int32 [C / 128, T] (include/foidfinder_rocm.h, ff_quant_mx4). First the norm over the first c_real columns
     (default: all) with gamma, and beta for NORM_LAYER, fp32 [C] with zeros past c_real (`pad_norm` builds them); then with
-    `rotate` the rotation by blockdiag(H128). Weights are prepared by the same call: rows [N, K], no norm."""
+    `rotate` the rotation by blockdiag(H128). Weights are prepared by the same call: rows [N, K], no norm. The outputs share no memory
+    with each other or with what is read (refused)."""
     _no_grad(x, gamma, beta)
     dev = _on_gpu(out, scale, gamma, beta)
     T, C = _mx4(out, scale, "out")
@@ -525,7 +526,7 @@ def quant_mx4(x: torch.Tensor, out: torch.Tensor, scale: torch.Tensor, rotate: b
 
 
 def dequant_mx4(codes: torch.Tensor, scale: torch.Tensor, out: torch.Tensor) -> None:
-    """The values of MX4 codes into out [T, C], fp16, bf16 or fp32 (ff_dequant_mx4)."""
+    """The values of MX4 codes into out [T, C], fp16, bf16 or fp32, in memory of its own (ff_dequant_mx4)."""
     _no_grad(out)
     dev = _on_gpu(codes, scale, out)
     T, C = _mx4(codes, scale, "the")

@@ -88,11 +88,12 @@ int ff_gemm_s8_variants(void);
  * C % 128 == 0, C <= 6144 -> out, scale. First the norm (FF_NORM_*) over the first c_real columns (fp32 gamma/beta [C], zero
  * past c_real; columns past it count as zeros), then with rotate = 1 the block-diagonal 128-point Walsh-Hadamard rotation,
  * then per 32 columns e = floor(log2(max |v|)) - 2 (at least -127) and code = v / 2^e to the nearest of 0, 1/2, 1, 3/2, 2, 3,
- * 4, 6 (ties to the even code, saturating). A block with an infinite or undefined value gets the exponent 255. */
+ * 4, 6 (ties to the even code, saturating). A block with an infinite or undefined value gets the exponent 255.
+ * out and scale share no memory with each other or with what is read. */
 int ff_quant_mx4(const void* x, int dtype, int64_t T, int64_t C, int64_t x_stride, int rotate, int norm, int64_t c_real,
                  const float* gamma, const float* beta, float eps, uint8_t* out, uint32_t* scale, void* stream);
 
-/* The values of MX4 codes, code * 2^e, as fp16, bf16 or fp32 [T, C] (C % 128 == 0). */
+/* The values of MX4 codes, code * 2^e, as fp16, bf16 or fp32 [T, C] (C % 128 == 0), in memory of their own. */
 int ff_dequant_mx4(const uint8_t* codes, const uint32_t* scale, int64_t T, int64_t C, void* out, int dtype, void* stream);
 
 /* MX4 product with fp32 sums and a fused epilogue: y[m, n] = sum_k A[m, k] W[n, k] + bias[n] (bias fp32 [N] or NULL), then

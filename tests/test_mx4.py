@@ -404,3 +404,26 @@ def test_gemm_mx4_refuses_an_out_that_shares_memory():
                dict(epi=1, res=6 * big + 12784), dict(epi=1, res=6 * big - 12784)):
         status, msg = call(**kw)
         assert status == FF_EINVAL and "overlap" in msg, (kw, msg)
+
+
+def test_quant_and_dequant_mx4_refuse_outputs_that_share_memory():
+    big = 1 << 30
+
+    def quant(x=big, xs=256, g=2 * big, b=3 * big, out=4 * big, s=5 * big):
+        return err(K.lib().ff_quant_mx4(x, 0, 100, 256, xs, 1, 2, 256, g, b, 1e-6, out, s, None))
+
+    # x 100 rows of 512 bytes, gamma and beta 1024 bytes, codes 12 800, scale 800; the codes do not fit between two rows of x
+    for kw in (dict(out=big), dict(out=big - 12796), dict(out=big + 51196), dict(s=big + 51196), dict(s=big - 796),
+               dict(s=4 * big + 12796), dict(out=5 * big + 796), dict(g=4 * big + 12784), dict(b=4 * big - 1008),
+               dict(g=5 * big + 784), dict(b=5 * big - 1008), dict(x=4 * big - 512, xs=512), dict(s=big + 512, xs=512),
+               dict(s=big + 512 - 4, xs=1 << 20), dict(s=big + (99 << 21) - 796, xs=1 << 20)):
+        status, msg = quant(**kw)
+        assert status == FF_EINVAL and "overlap" in msg, (kw, msg)
+
+    def dequant(c=big, s=2 * big, out=3 * big, dtype=0):
+        return err(K.lib().ff_dequant_mx4(c, s, 100, 256, out, dtype, None))
+
+    for kw in (dict(out=big), dict(out=big + 12784), dict(out=big - 51184), dict(out=2 * big + 784),
+               dict(s=3 * big + 51196), dict(s=3 * big + 102396, dtype=2), dict(c=3 * big + 102396, dtype=2)):
+        status, msg = dequant(**kw)
+        assert status == FF_EINVAL and "overlap" in msg, (kw, msg)

@@ -670,3 +670,18 @@ def test_qk_norm_rope_rows_between_the_other_operands(dev, rng, layout, T):
     K.qk_norm_rope(q.clone(), k.clone(), *want, *args)
     K.qk_norm_rope(q, k, qo, ko, *args)
     assert torch.equal(qo, want[0]) and torch.equal(ko, want[1])
+
+
+def test_quant_mx4_outputs_between_the_rows_of_x(dev, rng):
+    """Outputs in the memory that the rows of x leave free are taken."""
+    K = kern()
+    T, C = 5, 128
+    x, back = typed(rng.standard_normal((T, C)), "fp16", dev)
+    rows = torch.full((T, 512), 7.0, dtype=torch.half, device=dev)
+    rows[:, :C] = x
+    bytes_ = rows.view(torch.uint8)
+    codes = bytes_[1, 2 * C : 2 * C + T * C // 2].view(T, C // 2)
+    scale = bytes_[3, 2 * C : 2 * C + 4 * T].view(torch.int32).view(1, T)
+    K.quant_mx4(rows[:, :C], codes, scale)
+    assert_same_mx4((codes, scale), OX.quant_mx4(back))
+    assert torch.equal(rows[:, :C], x)

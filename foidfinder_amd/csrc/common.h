@@ -44,6 +44,11 @@ inline Extent range(const void* p, int64_t bytes) { return {reinterpret_cast<uin
 // where both have several; runs at different pitches count as apart if their whole extents are, or if they keep to columns of
 // their own within a common pitch.
 bool apart(const Extent& a, const Extent& b);
+// The same, for the case that is nearly always met first: extents that do not meet at all.
+inline bool clear_of(const Extent& a, const Extent& b) {
+  const auto end = [](const Extent& e) { return e.at + (e.n[0] - 1) * e.pitch[0] + (e.n[1] - 1) * e.pitch[1] + e.len; };
+  return end(a) <= b.at || end(b) <= a.at || apart(a, b);
+}
 
 // ---- device helpers ----
 

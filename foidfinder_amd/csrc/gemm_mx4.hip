@@ -614,14 +614,14 @@ extern "C" int ff_gemm_mx4(const uint8_t* A, const uint32_t* a_scale, const uint
     return fail(FF_EINVAL, "gemm_mx4: misaligned pointer");
   const Extent to = range(out, M * (epi == FF_EPI_SWIGLU ? N / 2 : N) * (dtype == FF_F32 ? 4 : 2));
   // elements are read and written by different workgroups, in no order
-  if (epi == FF_EPI_RESIDUAL && residual != out && !apart(to, range(residual, to.len)))
+  if (epi == FF_EPI_RESIDUAL && residual != out && !clear_of(to, range(residual, to.len)))
     return fail(FF_EINVAL, "gemm_mx4: residual overlaps out in part");
   if (variant == 0) variant = pick_variant(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
   if (!launchable(MX4_COSTS[variant - 1], static_cast<int>(M), static_cast<int>(N)))
     return fail(FF_EINVAL, "gemm_mx4: too many tiles for this variant");
   for (const Extent& e : {range(A, M * (K / 2)), range(a_scale, M * (K / 32)), range(W, N * (K / 2)),
                           range(w_scale, N * (K / 32)), range(bias, 4 * N)})
-    if (e.at != 0 && !apart(to, e)) return fail(FF_EINVAL, "gemm_mx4: out overlaps an operand");
+    if (e.at != 0 && !clear_of(to, e)) return fail(FF_EINVAL, "gemm_mx4: out overlaps an operand");
   const Mx4Args a{A, a_scale, W, w_scale, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), bias, residual,
                   out};
   const hipStream_t st = as_stream(stream);

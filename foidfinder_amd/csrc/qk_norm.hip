@@ -284,10 +284,10 @@ extern "C" int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, c
   const Extent read[7] = {range(rope_cos, rope_len * R * 2), range(rope_sin, rope_len * R * 2), range(q_gamma, 4 * D),
                           range(k_gamma, 4 * D), range(q_beta, 4 * D), range(k_beta, 4 * D),
                           range(positions, T * (pos64 ? 8 : 4))};
-  bool clear = apart(to[0], to[1]);
+  bool clear = clear_of(to[0], to[1]);
   for (int i = 0; i < 2; ++i) {
-    clear = clear && (in_place(to[i], in[i]) || apart(to[i], in[i])) && apart(to[i], in[1 - i]);
-    for (const Extent& e : read) clear = clear && (e.at == 0 || apart(to[i], e));
+    clear = clear && (in_place(to[i], in[i]) || clear_of(to[i], in[i])) && clear_of(to[i], in[1 - i]);
+    for (const Extent& e : read) clear = clear && (e.at == 0 || clear_of(to[i], e));
   }
   if (!clear)
     return fail(FF_EINVAL, "qk_norm_rope: an output overlaps the other one or what is read (its own input, with its strides, "

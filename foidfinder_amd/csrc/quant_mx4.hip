@@ -393,10 +393,10 @@ extern "C" int ff_quant_mx4(const void* x, int dtype, int64_t T, int64_t C, int6
     return fail(FF_EINVAL, "quant_mx4: misaligned pointer");
   // rows are read by workgroups that run while others write theirs
   const Extent codes = range(out, T * (C / 2)), words = range(scale, T * (C / 32));
-  bool clear = apart(codes, words);
+  bool clear = clear_of(codes, words);
   for (const Extent& e : {Extent{reinterpret_cast<uintptr_t>(x), {T, 1}, {2 * x_stride, 0}, 2 * C}, range(gamma, 4 * C),
                           range(beta, 4 * C)})
-    clear = clear && (e.at == 0 || (apart(codes, e) && apart(words, e)));
+    clear = clear && (e.at == 0 || (clear_of(codes, e) && clear_of(words, e)));
   if (!clear) return fail(FF_EINVAL, "quant_mx4: an output overlaps the other one or what is read");
   const hipStream_t st = as_stream(stream);
   const int Ci = static_cast<int>(C), cr = static_cast<int>(c_real);
@@ -420,7 +420,7 @@ extern "C" int ff_dequant_mx4(const uint8_t* codes, const uint32_t* scale, int64
   if (!aligned(codes, 4) || !aligned(scale, 4) || !aligned(out, 16))
     return fail(FF_EINVAL, "dequant_mx4: misaligned pointer");
   const Extent to = range(out, T * C * (dtype == FF_F32 ? 4 : 2));
-  if (!apart(to, range(codes, T * (C / 2))) || !apart(to, range(scale, T * (C / 32))))
+  if (!clear_of(to, range(codes, T * (C / 2))) || !clear_of(to, range(scale, T * (C / 32))))
     return fail(FF_EINVAL, "dequant_mx4: out overlaps the codes or their scale");
   const hipStream_t st = as_stream(stream);
   const int Ci = static_cast<int>(C);

@@ -155,7 +155,10 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(const QkArgs a) {
       float sq = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) sq = __builtin_fmaf(v[e], v[e], sq);
-      const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(group_sum<LANES>(sq), inv_d, a.eps));  // about 1 ulp
+      // about 1 ulp; v_rsq_f32 takes a subnormal number for zero, and only a subnormal eps leaves one
+      const float ms = __builtin_fmaf(group_sum<LANES>(sq), inv_d, a.eps);
+      float r = __builtin_amdgcn_rsqf(ms);
+      if (a.eps < 0x1p-126f) r = ms < 0x1p-126f ? __builtin_amdgcn_rsqf(ms * 0x1p24f) * 0x1p12f : r;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         v[e] = NORM == FF_NORM_LAYER ? __builtin_fmaf(v[e] * r, g[e], b[e]) : v[e] * r * g[e];

@@ -685,3 +685,23 @@ def test_quant_mx4_outputs_between_the_rows_of_x(dev, rng):
     K.quant_mx4(rows[:, :C], codes, scale)
     assert_same_mx4((codes, scale), OX.quant_mx4(back))
     assert torch.equal(rows[:, :C], x)
+
+
+@pytest.mark.parametrize("norm", [OQ.RMS, OQ.LAYER])
+@pytest.mark.parametrize("eps", [2.0**-149, 2.0**-130, 2.0**-126])
+def test_qk_norm_rope_with_an_eps_that_is_subnormal(dev, norm, eps):
+    """Heads of zeros become beta, heads of +-2^-66 (their mean square, 2^-132, is exact in fp32 and so is its sum with each
+    eps: 2^-132 + 2^-149 has 18 bits) and of +-1 are normed: a root of about an ulp, two products and the output's half
+    step."""
+    K = kern()
+    x = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device=dev)
+    x[1, :, ::2], x[1, :, 1::2] = 2.0**-66, -(2.0**-66)
+    x[2, :, ::2], x[2, :, 1::2] = 1.0, -1.0
+    one, beta = torch.ones(64, device=dev), torch.full((64,), 0.25, device=dev) if norm == OQ.LAYER else None
+    cos, sin = torch.ones(3, 32, device=dev), torch.zeros(3, 32, device=dev)
+    o, o2 = torch.empty_like(x), torch.empty_like(x)
+    K.qk_norm_rope(x, x, o, o2, norm, one, one, beta, beta, cos, sin, None, True, eps)
+    v = x.double()
+    want = v / torch.sqrt(v.square().mean(-1, keepdim=True) + eps) + (0.25 if norm == OQ.LAYER else 0.0)
+    assert torch.equal(o, o2) and torch.equal(o[0].double(), want[0])
+    assert ((o.double() - want).abs() <= (2.0**-8 + 2.0**-20) * want.abs()).all()

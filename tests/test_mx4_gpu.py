@@ -705,3 +705,247 @@ def test_qk_norm_rope_with_an_eps_that_is_subnormal(dev, norm, eps):
     want = v / torch.sqrt(v.square().mean(-1, keepdim=True) + eps) + (0.25 if norm == OQ.LAYER else 0.0)
     assert torch.equal(o, o2) and torch.equal(o[0].double(), want[0])
     assert ((o.double() - want).abs() <= (2.0**-8 + 2.0**-20) * want.abs()).all()
+
+
+# ---- many rows a workgroup, every instantiation, the ends of the exponent range ----
+
+
+def qk64(x, norm, gamma, beta, cos, sin, pos, pairs, scale):
+    """oracle.qk_norm in torch float64 on the GPU: the result and the size of its terms."""
+    x = x.double()
+    if norm == OQ.LAYER:
+        x = x - x.mean(-1, keepdim=True)
+    if norm != OQ.NONE:
+        x = x / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-6) * gamma.double()
+    if norm == OQ.LAYER:
+        x = x + beta.double()
+    L, half = cos.shape
+    ok = (pos >= 0) & (pos < L)
+    c, s = (t.double()[torch.where(ok, pos, 0)][:, None] for t in (cos, sin))
+    i = torch.arange(half, device=x.device)
+    first, second = (2 * i, 2 * i + 1) if pairs else (i, i + half)
+    a, b = x[..., first], x[..., second]
+    y, size = x.clone(), x.abs()
+    y[..., first], y[..., second] = a * c - b * s, a * s + b * c
+    size[..., first], size[..., second] = (a * c).abs() + (b * s).abs(), (a * s).abs() + (b * c).abs()
+    return torch.where(ok[:, None, None], y * scale, torch.nan), size * abs(scale)
+
+
+@pytest.mark.parametrize("norm", [OQ.NONE, OQ.RMS, OQ.LAYER])
+@pytest.mark.parametrize("pairs", [True, False])
+@pytest.mark.parametrize("form", ["rows in order", "int32, in place, 8-byte rows", "int64, in place"])
+@pytest.mark.parametrize(("T", "H", "KV", "D", "R", "L"), [
+    (20011, 8, 2, 64, 64, 1025), (20011, 8, 2, 64, 48, 1), (30011, 5, 2, 48, 32, 13), (9001, 32, 8, 128, 128, 700),
+    (12007, 7, 7, 96, 96, 5000), (9001, 4, 2, 256, 256, 4099)])
+def test_qk_norm_rope_many_tokens_a_group(dev, rng, T, H, KV, D, R, L, form, pairs, norm):
+    """Three to eleven times as many heads as the resident groups of lanes, so that each group walks over several tokens;
+    every token against float64, with check_qk's tolerance. Positions repeat, lie in no order and past both ends."""
+    K = kern()
+    kind, shift = ("fp16", 0) if form == "rows in order" else ("bf16", 4 if "8-byte" in form else 0)
+    g = torch.Generator(device=dev).manual_seed(int(rng.integers(1 << 30)))
+    wide = H + 2 * KV
+    rows = torch.full((T, wide * D + 8), 7.0, dtype=TYPES[kind], device=dev)
+    x = rows[:, shift : shift + wide * D].unflatten(1, (wide, D))
+    x.copy_(2 * torch.randn(T, wide, D, device=dev, generator=g) + 0.3)
+    q, k = x[:, :H], x[:, H : H + KV]
+    gamma = [1 + 0.1 * torch.randn(D, device=dev, generator=g) if norm else None for _ in range(2)]
+    beta = [0.1 * torch.randn(D, device=dev, generator=g) if norm == OQ.LAYER else None for _ in range(2)]
+    cos, sin = (gpu(t, dev) for t in tables(rng, L, R))
+    pos, given = torch.arange(T, device=dev) % L, None
+    if form != "rows in order":
+        pos = torch.randint(-(L // 8 + 1), L + L // 8 + 1, (T,), device=dev, generator=g)
+        given = pos.to(torch.int32 if "int32" in form else torch.int64)
+    want = [qk64(t, norm, gamma[i], beta[i], cos, sin, pos, pairs, s) for i, (t, s) in enumerate(((q, 0.37), (k, 1.0)))]
+    rest = x[:, H + KV :].clone()
+    out = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k)] if given is None else [q, k]
+    K.qk_norm_rope(q, k, *out, norm, *gamma, *beta, cos, sin, given, pairs, 1e-6, 0.37)
+    for o, (w, size), s in zip(out, want, (0.37, 1.0)):
+        o = o.double()
+        assert torch.equal(o.isnan(), w.isnan())
+        e = 2.0**-17 * (size + (s if norm == OQ.LAYER else 0))
+        bad = ((o - w).abs() > e + HALF[kind] * (w.abs() + e) + TINY[kind]).nonzero()
+        assert len(bad) == 0, f"{len(bad)} off, first {bad[:4].tolist()}: {o[tuple(bad[0])]} vs {w[tuple(bad[0])]}"
+    assert torch.equal(x[:, H + KV :], rest)
+    assert (rows[:, :shift] == 7).all() and (rows[:, shift + wide * D :] == 7).all()
+
+
+def norm_weights(rng, C, c_real, norm):
+    g, b = np.zeros(C, np.float32), np.zeros(C, np.float32)
+    g[:c_real] = 1 + 0.1 * rng.standard_normal(c_real)
+    b[:c_real] = 0.1 * rng.standard_normal(c_real)
+    return g, b if norm == OX.LAYER else None
+
+
+def quant_rows(dev, x, norm, c_real, g, b, rotate=True):
+    T, C = x.shape
+    codes, scale, check = empty_mx4(T, C, dev)
+    kern().quant_mx4(x, codes, scale, rotate, norm, *(None if p is None else gpu(p, dev) for p in (g, b)), c_real)
+    assert check(), "wrote outside its outputs"
+    return codes, scale
+
+
+def compare_rows(codes, scale, x, pick, norm, c_real, g, b, rotate=True):
+    pick = torch.as_tensor(np.unique(pick), device=x.device)
+    assert_same_mx4((codes[pick], scale[:, pick]), OX.quant_mx4(x[pick].float().cpu().numpy(), rotate, norm, c_real, g, b))
+
+
+@pytest.mark.parametrize("norm", [OX.RMS, OX.LAYER])
+@pytest.mark.parametrize("padding", [0, 37, 133])
+@pytest.mark.parametrize(("T", "C"), [
+    *((4100, c) for c in (128, 384, 640, 896, 1152, 1408, 256, 768, 1280)),  # one and two lane groups a row
+    *((6, c) for c in (384, 512, 1024, 1280, 2048, 2560, 2816, 3584, 4096, 4608, 4992, 5632, 6144))])
+def test_quant_mx4_norm_every_width(dev, rng, T, C, padding, norm):
+    """Each number of lane groups and blocks that the dispatch knows, the row full, padded inside its last block and by more
+    than a block, with values in the padding that are not finite."""
+    c_real = max(C - padding, 1)
+    kind = "bf16" if (C // 128 + padding) % 2 else "fp16"
+    x = activations(rng, T, C)
+    x[:, c_real:] = rng.choice(np.array([np.inf, -np.inf, np.nan, 5.0], np.float32), (T, C - c_real))
+    g, b = norm_weights(rng, C, c_real, norm)
+    t = gpu(x, dev).to(TYPES[kind])
+    codes, scale = quant_rows(dev, t, norm, c_real, g, b)
+    pick = np.concatenate([np.arange(min(T, 40)), np.arange(max(T - 40, 0), T), rng.integers(0, T, 60)])
+    compare_rows(codes, scale, t, pick, norm, c_real, g, b)
+
+
+@pytest.mark.parametrize("norm", [OX.NONE, OX.RMS, OX.LAYER])
+@pytest.mark.parametrize(("T", "C", "c_real"), [(100_003, 128, 120), (100_003, 640, 640), (60_001, 768, 700),
+                                                (40_003, 512, 512), (40_003, 1024, 1000), (12_007, 2816, 2730),
+                                                (9_001, 6144, 6144)])
+def test_quant_mx4_more_rows_than_are_resident(dev, rng, T, C, c_real, norm):
+    """Each wave walks over several rows: rows of every walk against the oracle, and all of them against calls of 4100 rows,
+    in which a wave has one or two."""
+    gen = torch.Generator(device=dev).manual_seed(int(rng.integers(1 << 30)))
+    c_real = c_real if norm else C
+    x = torch.randn(T, C, device=dev, generator=gen)
+    x[:, :: 100] *= 20
+    x[:, c_real:] = torch.inf
+    x = x.half()
+    g, b = norm_weights(rng, C, c_real, norm) if norm else (None, None)
+    codes, scale = quant_rows(dev, x, norm, c_real, g, b)
+    compare_rows(codes, scale, x, np.concatenate([rng.integers(0, T, 120), np.arange(T - 20, T)]), norm, c_real, g, b)
+    for at in range(0, T, 4100):
+        at = min(at, T - 4100)
+        part = quant_rows(dev, x[at : at + 4100], norm, c_real, g, b)
+        assert torch.equal(part[0], codes[at : at + 4100]) and torch.equal(part[1], scale[:, at : at + 4100])
+    out = torch.empty(T, C, dtype=torch.bfloat16, device=dev)
+    kern().dequant_mx4(codes, scale, out)
+    pick = torch.as_tensor(rng.integers(0, T, 200), device=dev)
+    assert np.array_equal(out[pick].double().cpu().numpy(), OX.values(codes[pick].cpu().numpy(), scale[:, pick].cpu().numpy()))
+    for at in range(0, T, 512):
+        at = min(at, T - 512)
+        part = torch.empty(512, C, dtype=torch.bfloat16, device=dev)
+        kern().dequant_mx4(codes[at : at + 512], scale[:, at : at + 512].contiguous(), part)
+        assert torch.equal(part, out[at : at + 512])
+
+
+@pytest.mark.parametrize("rotate", [True, False])
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+def test_quant_mx4_subnormal_values(dev, rng, kind, rotate):
+    """Blocks whose largest value is subnormal, in the input's type and in fp32 (bf16: the exponent stops at -127 and the codes
+    are what is left), up to ordinary ones."""
+    e = np.arange(-24, -8) if kind == "fp16" else np.arange(-134, -118)
+    x = (rng.standard_normal((len(e), 256)) * np.exp2(e)[:, None]).astype(np.float32)
+    got, want = run_quant(dev, x, kind, rotate, OX.NONE)
+    assert_same_mx4(got, want)
+    code, ex = OX.unpack(*want)
+    assert kind == "fp16" or ((ex[7] == 0).all() and (code[7] & 7).any())  # 2^-127: subnormal, and codes that are not zero
+
+
+@pytest.mark.parametrize("variant", VARIANTS[1:])
+@pytest.mark.parametrize(("ea", "ew"), [
+    ([254], [0]), ([0], [254]), ([1], [253]), ([0], [127]), ([127], [0]), ([1], [106]), ([60], [47]), ([254], [114]),
+    ([184], [184]), ([254, 0, 254, 0, 10, 240, 100, 100], [0, 254, 0, 254, 244, 14, 154, 154])])
+def test_gemm_mx4_ends_of_the_exponents(dev, rng, ea, ew, variant):
+    """The two exponents of a product add up to one power of two over the row, ea + ew - 254 = p: every partial sum is a
+    multiple of 2^(p - 2) below 36 x 256 x 2^p < 2^(p + 14), so 16 bits hold it, in the range of fp32 (subnormal numbers
+    included) for p - 2 >= -149 and p + 14 <= 128: equal to the exact sum."""
+    M, N, K = 70, 90, 256
+    assert all(-147 <= a + b - 254 <= 114 and a + b == ea[0] + ew[0] for a, b in zip(ea, ew))
+    codes = [rng.integers(0, 16, (n, K)).astype(np.uint8) for n in (M, N)]
+    a, w = (OX.pack(c, np.tile(np.array(e * 8, np.uint8)[:8], (len(c), 1))) for c, e in zip(codes, (ea, ew)))
+    got = run_gemm(dev, a, w, None, "fp32", OG.EPI_BIAS_F16, variant)
+    want, _ = OX.gemm_mx4(a, w)
+    assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("variant", VARIANTS[1:])
+def test_gemm_mx4_sums_past_both_ends(dev, rng, variant):
+    """Below half the smallest number: zero, with the bias left to the summation's rounding. One product past the largest:
+    infinite, with its sign, in its own element only (the others are the bias: adding zeros is exact)."""
+    M, N, K = 40, 36, 384
+    codes = [rng.integers(0, 16, (n, K)).astype(np.uint8) for n in (M, N)]
+    low = [OX.pack(c, np.full((len(c), K // 32), 40, np.uint8)) for c in codes]  # 36 x 384 x 2^-174
+    bias = rng.standard_normal(N).astype(np.float32)
+    got = run_gemm(dev, *low, bias, "fp32", OG.EPI_BIAS_F16, variant)
+    assert (np.abs(got - bias) <= sum_error(K, np.abs(bias) + 36 * K * 2.0**-174)).all()
+    assert not run_gemm(dev, *low, None, "fp32", OG.EPI_BIAS_F16, variant).any()
+    one = [np.zeros((n, K), np.uint8) for n in (M, N)]
+    one[0][7, 200], one[1][5, 200], one[1][6, 200] = 7, 7, 15  # 6 x 6 and 6 x -6
+    high = [OX.pack(c, np.full((len(c), K // 32), 190, np.uint8)) for c in one]  # 36 x 2^126
+    got = run_gemm(dev, *high, bias, "fp32", OG.EPI_BIAS_F16, variant)
+    want = np.broadcast_to(bias.astype(np.float64), (M, N)).copy()
+    want[7, 5], want[7, 6] = np.inf, -np.inf
+    assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize(("M", "N"), [(1025, 1030), (300, 768), (513, 771)])
+def test_gemm_mx4_residual_in_place_is_the_same(dev, rng, M, N, kind, variant):
+    """The residual as out itself, over several tiles in both directions, whole and ragged: bit for bit as from memory of its
+    own."""
+    K = kern()
+    a, w = ([gpu(t, dev) for t in random_mx4(rng, n, 384, 118, 126)] for n in (M, N))
+    bias = gpu(rng.standard_normal(N).astype(np.float32), dev)
+    x, _ = typed(rng.standard_normal((M, N)), kind, dev)
+    out = torch.empty_like(x)
+    K.gemm_mx4(*a, *w, bias, out, K.EPI_RESIDUAL, variant, x)
+    K.gemm_mx4(*a, *w, bias, x, K.EPI_RESIDUAL, variant)
+    assert torch.equal(out, x)
+
+
+def test_every_op_on_two_streams_at_once(dev, rng):
+    """Quantization with a norm, its values, the product and the head norm in flight on two streams, each round into outputs
+    of its own: all of them as alone."""
+    K = kern()
+    cos, sin = (gpu(t, dev) for t in tables(rng, 65, 64))
+    one = torch.ones(64, device=dev)
+    jobs = []
+    for T, C, N, norm in ((1300, 1024, 1280, OX.LAYER), (4100, 640, 512, OX.RMS)):
+        x, _ = typed(activations(rng, T, C), "fp16", dev)
+        g, b = norm_weights(rng, C, C, norm)
+        w = [gpu(t, dev) for t in random_mx4(rng, N, C, 118, 124)]
+        jobs.append((x, norm, gpu(g, dev), None if b is None else gpu(b, dev), w))
+
+    def outputs(job):
+        (T, C), N = job[0].shape, job[4][0].shape[0]
+        return (torch.zeros(T, C // 2, dtype=torch.uint8, device=dev), torch.zeros(C // 128, T, dtype=torch.int32, device=dev),
+                torch.zeros(T, C, dtype=torch.half, device=dev), torch.zeros(T, N, dtype=torch.half, device=dev),
+                torch.zeros(T, N // 128, 64, dtype=torch.half, device=dev),
+                torch.zeros(T, N // 128, 64, dtype=torch.half, device=dev))
+
+    def launch(job, to):
+        x, norm, g, b, w = job
+        K.quant_mx4(x, to[0], to[1], True, norm, g, b)
+        K.dequant_mx4(to[0], to[1], to[2])
+        K.gemm_mx4(to[0], to[1], *w, None, to[3], K.EPI_BIAS_F16)
+        heads = to[3].view(len(x), 2, -1, 64)
+        K.qk_norm_rope(heads[:, 0], heads[:, 1], to[4], to[5], K.NORM_RMS, one, one, None, None, cos, sin)
+
+    want = []
+    for job in jobs:
+        want.append(outputs(job))
+        launch(job, want[-1])
+    rounds = [[outputs(job) for job in jobs] for _ in range(6)]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for to in rounds:
+        for job, t, s in zip(jobs, to, streams):
+            with torch.cuda.stream(s):
+                launch(job, t)
+    torch.cuda.synchronize()
+    for i, to in enumerate(rounds):
+        for t, ref in zip(to, want):
+            for n, (a, b) in enumerate(zip(t, ref)):
+                assert torch.equal(a, b), f"round {i}, output {n}"

@@ -375,11 +375,11 @@ def test_qk_norm_rope_refuses_outputs_that_share_memory():
         return err(K.lib().ff_qk_norm_rope(q, *st[0], k, *st[1], qo, *st[2], ko, *st[3], 0, T, H, KV, D, 1, g, g, None, None,
                                            1e-6, cos, sin, 8, 64, 1, pos, pos64, 1.0, None))
 
-    packed = ((3072, 64),) * 4  # q, k and v of [T, 3, 16, 64]
-    last = 2 * (3 * 1024 + 15 * 64 + 63)  # the last value of a [4, 16, 64] operand
+    packed = ((2560, 64),) * 4  # q, k and v of [T, 16 + 16 + 8, 64]
+    last = 2 * (4 * 1024 - 1)  # the last value of a [4, 16, 64] operand
     for kw in (dict(qo=big + 128), dict(qo=big - 128), dict(qo=big + 2048),  # a head or a token further in q
                dict(k=big + 2048, qo=big + 128, st=packed),  # q_out ends one head into k
-               dict(k=big + 2048, qo=big, ko=big + 2048 + 6144, st=packed),  # k_out one token past k
+               dict(k=big + 2048, qo=big, ko=big + 2048 + 5120, st=packed),  # k_out one token past k
                dict(ko=3 * big + 128), dict(qo=4 * big + last - 6),  # the outputs share heads, or the last values
                dict(qo=big, k=big + 128, st=((1024, 64), (1024, 64), (1024, 64), (1024, 64)), KV=1),  # k is q's second head
                dict(qo=big, st=((1024, 64), (1024, 64), (2048, 64), (1024, 64))),  # in place with other strides

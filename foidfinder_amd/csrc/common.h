@@ -77,8 +77,7 @@ __device__ __forceinline__ float swz_xor16(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F));
 }
 
-// Eight consecutive 16-bit values from 16 aligned bytes, and one value of either type to and from fp32 (to nearest, ties to
-// even).
+// Eight or four values of a type, as one load or store takes them.
 template <typename T>
 using vec8_t = T __attribute__((ext_vector_type(8)));
 template <typename T>

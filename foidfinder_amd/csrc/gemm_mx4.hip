@@ -17,11 +17,12 @@
 // CUs idle otherwise: 1025 x 1024 x 2816 with a residual 7.6 us (272 tiles, 22 units each: neither more slots nor K on two
 // groups of waves is faster); 16 x 98 782 x 1152 14 us, 4.8 TB/s, the weights' bytes. 128 x 128, 256 x 128 and 256 x 256
 // tiles read each operand less often: 5184 x 4736 x 1024 GELU 25-26 us (1.9-2.0 PFLOP/s with 49 MB of stores), 32 800 x
-// 5632 x 1024 SwiGLU 131-137 us (2.8-2.9 PFLOP/s), 32 768 x 4096 x 4096 282 us (3.9 PFLOP/s). The instruction alone reaches
-// 6.1 PFLOP/s on random codes (the card's power). At K = 1024 the products take 82 of 131 us, the ring's loads add 23 and
-// the epilogue 25; every part left out gives about its own share, as a limit on power does. Measured and not kept: W as a
-// stream past persistent waves for few rows (16.8 us against 14), workgroups whose ring runs on across tiles (132-134 us
-// against 132-136, spills with a residual, slower for few tiles), slots of two units for the large tiles, loads spread
+// 5632 x 1024 SwiGLU 131-140 us (2.7-2.9 PFLOP/s), 32 768 x 4096 x 4096 282 us (3.9 PFLOP/s). The instruction alone reaches
+// 6.1 PFLOP/s on random codes (8.5 on zeros: power). At K = 1024 the products take 82 of 131 us, the ring's loads add 23 and
+// the epilogue 25: a tile's parts run in turn, the MFMAs busy 35 % of the time, at a clock that falls with their share (1.93
+// GHz; 1.66 at the 53 % of 32 768 x 4096 x 4096). Measured and not kept: W as a stream past persistent waves for few rows (16.8
+// us against 14), workgroups whose ring runs on across tiles (132-134 us against 132-136, spills with a residual, slower for
+// few tiles; their epilogue still stood between two tiles' products), slots of two units for the large tiles, loads spread
 // between the products.
 #include <algorithm>
 #include <cmath>
@@ -524,8 +525,8 @@ static int launch_ring(const Mx4Args& a, hipStream_t st) {
 // The tile shape without a chosen one: the lowest estimated time. The estimate (us) is fixed + the larger (a 4-norm) of what
 // one tile takes after another, rounds (first + unit u), and what a CU takes for its tiles, each tile + tile_unit u, with u
 // units of K, plus the outputs' share. Fitted to the times of 300 products (1 .. 33 000 rows, 32 .. 9000 columns, K 128 ..
-// 5120); on 200 others its pick is 1.5 % slower than the fastest shape on average and 19 % at worst, where the 64 x 64
-// tiles alone are 10 % slower on average, the 256 x 128 tiles alone 77 %.
+// 5120); on 196 others its pick is 1.4 % slower than the fastest shape on average and 12 % at worst, where the 64 x 64
+// tiles alone are 9 % slower on average, the 256 x 128 tiles alone 74 %.
 struct Mx4Cost {
   int bm, bn, threads, resident;  // tile, threads of a workgroup, workgroups a CU holds
   bool whole;                     // rounds count whole (few tiles a CU) or as a fraction

@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256) void quant_mx4_kernel(const T* __restrict__ x,
 }
 
 // a / n for a whole number n > 0, inv = 1 / n rounded: the quotient corrected by its exact remainder is the rounded one
-// (Markstein), in three operations instead of a division's ten.
+// (Markstein; quotients of normal size), in three operations instead of a division's ten.
 __device__ __forceinline__ float divide_by(float a, float n, float inv) {
   const float q = a * inv;
   const float c = __builtin_fmaf(__builtin_fmaf(-q, n, a), inv, q);
@@ -145,8 +145,10 @@ __device__ __forceinline__ float plus(const uint32_t (&w)[4], float s) {
 // columns of bf16: 31 us, held 46; 2816 columns: 32.6, held 33.5). gamma and beta (zeros without one) sit in LDS for the
 // workgroup's rows, zero past c_real; the first rows load ahead of them. The arithmetic bounds it: 386 vector operations a
 // row of 1024 (16 columns a lane at 14 each, 7 of them butterflies; the rest for sums, root, exponents and addresses) keep
-// the SIMDs 75 % busy, 27.5 us at 32 800 rows where the rows' bytes take 16. At 2816 columns its 106 registers leave four
-// waves a SIMD, so 5125 rows are a round and a quarter: 18 us.
+// the SIMDs 75 % busy, 27.5 us at 32 800 rows where the rows' bytes take 16. At 2816 columns (5125 rows: 18 us) its 106
+// registers leave four waves a SIMD, so 5125 rows are a round and a quarter; and the padding's masks, which the compiler forms
+// ahead of the row loop, spill 74 scalar registers into lanes of vector ones: 1297 vector operations a row with what stands
+// before the loop, where columns and sums need about 770.
 template <typename T, int NI, int G>
 __global__ __launch_bounds__(256) void quant_mx4_norm_kernel(const T* __restrict__ x, int64_t x_stride, int64_t rows, int C,
                                                              int c_real, const float* __restrict__ gamma,

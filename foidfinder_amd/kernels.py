@@ -593,7 +593,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: t
     if KV == 1:
         kh = ph = 0
     qp, kp, op, pp = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
-    if (qp == op and (qt, qh) != (ot, oh)) or (kp == pp and (kt, kh) != (pt, ph)):
+    if T and ((qp == op and (qt, qh) != (ot, oh)) or (kp == pp and (kt, kh) != (pt, ph))):
         raise RuntimeError("an output in its input's place must have its strides")
     table = rope_cos.shape
     if not (rope_cos.dtype == rope_sin.dtype == torch.float32 and len(table) == 2 and rope_sin.shape == table):

@@ -427,3 +427,15 @@ def test_quant_and_dequant_mx4_refuse_outputs_that_share_memory():
                dict(s=3 * big + 51196), dict(s=3 * big + 102396, dtype=2), dict(c=3 * big + 102396, dtype=2)):
         status, msg = dequant(**kw)
         assert status == FF_EINVAL and "overlap" in msg, (kw, msg)
+
+
+def test_no_tokens_in_any_layout(monkeypatch):
+    """Empty tensors have one address, none: that is not an output in its input's place with other strides."""
+    monkeypatch.setattr(K, "_on_gpu", lambda *ts: -1)
+    ran = []
+    monkeypatch.setattr(K, "_run", lambda *a: ran.append(a))
+    b, t = torch.zeros(0, 4, 3, 64, dtype=torch.half), torch.zeros(3, 32)
+    o = torch.zeros(0, 4, 64, dtype=torch.half)
+    K.qk_norm_rope(b[:, :, 0], b[:, :, 1], o, o.clone(), K.NORM_NONE, None, None, None, None, t, t)
+    K.qk_norm_rope(o, o, b[:, :, 0], b[:, :, 1], K.NORM_NONE, None, None, None, None, t, t)
+    assert len(ran) == 2

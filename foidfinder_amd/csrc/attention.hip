@@ -41,7 +41,7 @@
 // rescales every block; here every product and sum is fp32).
 #include <type_traits>
 
-#include "common.h"
+#include "attention_common.h"
 
 namespace ff {
 
@@ -66,15 +66,6 @@ static_assert((WAVES - 1) * MERGE_WORDS * 64 * 4 <= 2 * STAGES * TILE * 2, "merg
 // flipping the upper half of the row for rows 2, 3 (mod 4) keeps those 4 rows on distinct banks.
 __device__ __forceinline__ int k_slot(int r, int c) { return c ^ ((r >> 1) & 7); }
 __device__ __forceinline__ int v_slot(int r, int c) { return c ^ ((r & 2) << 1); }
-
-// ds_read_b64_tr_b16 as inline asm. The compiler's wait-insertion pass treats the builtin as possibly reading LDS
-// that in-flight buffer->LDS loads are writing and drains them all (s_waitcnt vmcnt(0)) before it, which would
-// serialize the LDS ring; this form is invisible to that pass. Ordering: "memory" keeps it after the barrier that
-// publishes the tile; the caller waits for the data (s_waitcnt lgkmcnt(0) tied to the result registers).
-template <int OFF>
-__device__ __forceinline__ void tr_read(half4_t& v, uint32_t lds_addr) {
-  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(v) : "v"(lds_addr), "n"(OFF) : "memory");
-}
 
 // One workgroup's work, the queries from q_first. SPLIT = 0: wave w owns queries q_first + 32w .. +31 over both
 // key halves of every tile.

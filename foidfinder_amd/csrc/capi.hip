@@ -86,6 +86,6 @@ bool apart(const Extent& a, const Extent& b) {
 
 }  // namespace ff
 
-extern "C" int ff_abi_version(void) { return 4; }
+extern "C" int ff_abi_version(void) { return 5; }
 
 extern "C" const char* ff_last_error(void) { return ff::g_error.c_str(); }

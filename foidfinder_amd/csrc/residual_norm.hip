@@ -1,0 +1,311 @@
+// A block's output into the residual stream, between the block's post-norm and the next block's pre-norm, in one pass:
+//   x_out = x + scale gate N_post(y),   h = N_pre(x_out),
+// N being RMSNorm v / sqrt(mean(v^2) + eps) gamma, LayerNorm (v - mean) / sqrt(var + eps) gamma + beta, or nothing; gate is a
+// row for each run of tokens (one: a layer scale; one a sequence; one a token), or 1. All of it in fp32; x_out and h are rounded
+// once each, h from the unrounded x_out.
+//
+// HBM-bound: 8 bytes a column (x, y read, x_out, h written). LANES lanes hold a row, 16 bytes a lane and chunk; a group of lanes
+// keeps to its columns and strides over the rows, so that gammas, betas and a single gate row stay in registers (they are 2 to
+// 5 times a row's own bytes). The next row loads under this one's arithmetic. Sums: within a wave by DPP; a row of several
+// waves leaves each wave's sum and squares about its own mean in LDS and every wave joins them (counts and means known, no
+// cancellation), one barrier a norm.
+#include <algorithm>
+
+#include "common.h"
+
+namespace ff {
+
+struct ResidualArgs {
+  const void *x, *y, *gate;
+  void *x_out, *h;
+  int64_t xs, ys, os, hs;  // row strides in elements
+  const float *post_g, *post_b, *pre_g, *pre_b;
+  int rows, width, per_gate, post, pre, gate_f32;  // per_gate: rows that share a gate row
+  float scale, eps;
+};
+
+// Sum over groups of LANES <= 64 lanes, in each of them.
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v = v + dpp<DPP_XOR1>(v);
+  v = v + dpp<DPP_XOR3>(v);
+  v = v + dpp<DPP_XOR7>(v);
+  v = v + dpp<DPP_XOR15>(v);
+  if constexpr (LANES > 16) v = v + swz_xor16(v);
+  if constexpr (LANES > 32) v = v + xor_shuffle(v, 32);
+  return v;
+}
+
+// 1 / sqrt(v), about 1 ulp; v_rsq_f32 takes a subnormal number for zero.
+__device__ __forceinline__ float inv_root(float v) {
+  return v < 0x1p-126f ? __builtin_amdgcn_rsqf(v * 0x1p24f) * 0x1p12f : __builtin_amdgcn_rsqf(v);
+}
+
+template <typename T, int LANES, int CHUNKS>
+__global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kernel(const ResidualArgs a) {
+  constexpr int THREADS = LANES <= 64 ? 256 : LANES, GROUPS = THREADS / LANES, WIDTH = LANES < 64 ? LANES : 64;
+  constexpr int WPR = LANES / WIDTH;  // waves a row
+  constexpr bool KEEP = CHUNKS <= 2;  // the parameters stay in registers
+  typedef vec8_t<T> T8;
+  __shared__ float2 joint[2][THREADS / 64];
+  const int lane = threadIdx.x % LANES, wave = threadIdx.x / 64;
+  const int step = static_cast<int>(gridDim.x) * GROUPS;
+  int row = static_cast<int>(blockIdx.x) * GROUPS + threadIdx.x / LANES;
+  if (row >= a.rows) return;  // (a row of several waves is its block's only one)
+  int col[CHUNKS];
+  bool in[CHUNKS];
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    in[i] = 8 * (i * LANES + lane) < a.width;
+    col[i] = in[i] ? 8 * (i * LANES + lane) : 0;  // lanes past the row load its first columns and hold zeros
+  }
+  const float inv_n = 1.f / static_cast<float>(a.width);
+
+  auto param = [&](const float* p, int i, int e) __attribute__((always_inline)) { return p ? p[col[i] + e] : 0.f; };
+  float post_g[CHUNKS][8], post_b[CHUNKS][8], pre_g[CHUNKS][8], pre_b[CHUNKS][8], factor[CHUNKS][8];
+  auto gate_at = [&](int64_t r, int i, float (&f)[8]) __attribute__((always_inline)) {
+    if (a.gate_f32) {
+      const float* g = static_cast<const float*>(a.gate) + r * a.width + col[i];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = g[e];
+    } else {
+      const T8 g = *reinterpret_cast<const T8*>(static_cast<const T*>(a.gate) + r * a.width + col[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = static_cast<float>(g[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= a.scale;
+  };
+  const bool gate_moves = a.gate && a.per_gate < a.rows;
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) factor[i][e] = a.scale;
+    if (a.gate && !gate_moves) gate_at(0, i, factor[i]);
+    if constexpr (KEEP)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        post_g[i][e] = param(a.post_g, i, e), post_b[i][e] = param(a.post_b, i, e);
+        pre_g[i][e] = param(a.pre_g, i, e), pre_b[i][e] = param(a.pre_b, i, e);
+      }
+  }
+
+  int turn = 0;
+  // The norm of v in its place.
+  auto norm = [&](float (&v)[CHUNKS][8], int kind, const float* g, const float* b, float (&kg)[CHUNKS][8],
+                  float (&kb)[CHUNKS][8]) __attribute__((always_inline)) {
+    const bool centred = kind == FF_NORM_LAYER;
+    float mean = 0.f;
+    if (centred) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = s + v[i][e];
+      mean = lanes_sum<WIDTH>(s);  // the wave's sum
+    }
+    float own = inv_n;  // 1 / columns of the wave
+    int columns = 0;
+    if constexpr (WPR > 1) {
+#pragma unroll
+      for (int i = 0; i < CHUNKS; ++i)
+        columns += min(max(a.width - 8 * (i * LANES + wave * 64), 0), 512);
+      own = columns ? 1.f / static_cast<float>(columns) : 0.f;
+    }
+    const float about = centred ? mean * own : 0.f;
+    float sq = 0.f;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = in[i] ? v[i][e] - about : 0.f;
+        sq = __builtin_fmaf(d, d, sq);
+      }
+    sq = lanes_sum<WIDTH>(sq);
+    float centre = about;
+    if constexpr (WPR > 1) {
+      if (threadIdx.x % 64 == 0) joint[turn][wave] = float2{mean, sq};
+      __syncthreads();
+      float all = 0.f, squares = 0.f;
+      if (centred) {
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) all = all + joint[turn][w].x;
+        centre = all * inv_n;
+      }
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) {
+        const float2 j = joint[turn][w];
+        squares = squares + j.y;
+        if (centred) {
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < CHUNKS; ++i) n += min(max(a.width - 8 * (i * LANES + w * 64), 0), 512);
+          const float d = n ? j.x * (1.f / static_cast<float>(n)) - centre : 0.f;
+          squares = __builtin_fmaf(static_cast<float>(n) * d, d, squares);
+        }
+      }
+      sq = squares;
+      turn ^= 1;  // the next norm writes the other one: its barrier lies between the reads here and the next write
+    }
+    const float r = inv_root(__builtin_fmaf(sq, inv_n, a.eps));
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float gamma = KEEP ? kg[i][e] : g[col[i] + e];
+        if (centred)
+          v[i][e] = __builtin_fmaf((v[i][e] - centre) * r, gamma, KEEP ? kb[i][e] : b[col[i] + e]);
+        else
+          v[i][e] = v[i][e] * r * gamma;
+      }
+  };
+
+  const T *x = static_cast<const T*>(a.x), *y = static_cast<const T*>(a.y);
+  T *xo = static_cast<T*>(a.x_out), *ho = static_cast<T*>(a.h);
+  T8 nx[CHUNKS], ny[CHUNKS];
+  auto load = [&](int r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      nx[i] = *reinterpret_cast<const T8*>(x + r * a.xs + col[i]);
+      ny[i] = *reinterpret_cast<const T8*>(y + r * a.ys + col[i]);
+    }
+  };
+  load(row);
+  for (;;) {
+    float v[CHUNKS][8], s[CHUNKS][8];
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[i][e] = in[i] ? static_cast<float>(ny[i][e]) : 0.f;
+        s[i][e] = in[i] ? static_cast<float>(nx[i][e]) : 0.f;
+      }
+    if (gate_moves)
+#pragma unroll
+      for (int i = 0; i < CHUNKS; ++i) gate_at(row / a.per_gate, i, factor[i]);
+    const int at = row;
+    const bool more = row < a.rows - step;
+    if (more) {
+      row += step;
+      load(row);
+    }
+    if (a.post != FF_NORM_NONE) norm(v, a.post, a.post_g, a.post_b, post_g, post_b);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      T8 w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s[i][e] = in[i] ? __builtin_fmaf(v[i][e], factor[i][e], s[i][e]) : 0.f;
+        w[e] = static_cast<T>(s[i][e]);
+      }
+      if (in[i])
+        __builtin_nontemporal_store(__builtin_bit_cast(int4_t, w), reinterpret_cast<int4_t*>(xo + at * a.os + col[i]));
+    }
+    if (a.pre != FF_NORM_NONE) {
+      norm(s, a.pre, a.pre_g, a.pre_b, pre_g, pre_b);
+#pragma unroll
+      for (int i = 0; i < CHUNKS; ++i) {
+        T8 w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = static_cast<T>(s[i][e]);
+        if (in[i])
+          __builtin_nontemporal_store(__builtin_bit_cast(int4_t, w), reinterpret_cast<int4_t*>(ho + at * a.hs + col[i]));
+      }
+    }
+    if (!more) break;
+  }
+}
+
+template <typename T, int LANES, int CHUNKS>
+static void launch_residual(const ResidualArgs& a, hipStream_t st) {
+  constexpr int THREADS = LANES <= 64 ? 256 : LANES, GROUPS = THREADS / LANES;
+  int64_t cap = resident_blocks(reinterpret_cast<const void*>(&residual_norm_kernel<T, LANES, CHUNKS>), THREADS, 0);
+  if (cap <= 0) cap = 512;
+  const int64_t blocks = std::min<int64_t>((a.rows + GROUPS - 1) / GROUPS, cap);
+  residual_norm_kernel<T, LANES, CHUNKS><<<dim3(static_cast<unsigned>(blocks)), THREADS, 0, st>>>(a);
+}
+
+template <typename T>
+static void launch_residual_width(const ResidualArgs& a, hipStream_t st) {
+  if (a.width <= 128)
+    launch_residual<T, 16, 1>(a, st);
+  else if (a.width <= 256)
+    launch_residual<T, 16, 2>(a, st);
+  else if (a.width <= 512)
+    launch_residual<T, 32, 2>(a, st);
+  else if (a.width <= 1024)
+    launch_residual<T, 64, 2>(a, st);
+  else if (a.width <= 2048)
+    launch_residual<T, 128, 2>(a, st);
+  else if (a.width <= 4096)
+    launch_residual<T, 256, 2>(a, st);
+  else if (a.width <= 8192)
+    launch_residual<T, 512, 2>(a, st);
+  else
+    launch_residual<T, 512, 4>(a, st);
+}
+
+}  // namespace ff
+
+using namespace ff;
+
+extern "C" int ff_residual_norm(const void* x, int64_t x_row, const void* y, int64_t y_row, void* x_out, int64_t xo_row,
+                                void* h, int64_t h_row, int dtype, int64_t T, int64_t C, int post, const float* post_gamma,
+                                const float* post_beta, int pre, const float* pre_gamma, const float* pre_beta,
+                                const void* gate, int64_t gate_rows, int gate_dtype, float scale, float eps, void* stream) {
+  clear_error();
+  if (dtype != FF_F16 && dtype != FF_BF16) return fail(FF_EINVAL, "residual_norm: x, y and the outputs must be fp16 or bf16");
+  if (C <= 0 || C % 8 != 0 || C > 16384)
+    return fail(FF_EINVAL, "residual_norm: rows must be a multiple of 8 columns, at most 16384");
+  if (T < 0 || T >= (int64_t(1) << 31)) return fail(FF_EINVAL, "residual_norm: need 0 <= T < 2^31");
+  for (int n : {post, pre})
+    if (n != FF_NORM_NONE && n != FF_NORM_RMS && n != FF_NORM_LAYER) return fail(FF_EINVAL, "residual_norm: unknown norm");
+  if ((post_gamma != nullptr) != (post != FF_NORM_NONE) || (pre_gamma != nullptr) != (pre != FF_NORM_NONE))
+    return fail(FF_EINVAL, "residual_norm: a gamma goes with its norm");
+  if ((post_beta != nullptr) != (post == FF_NORM_LAYER) || (pre_beta != nullptr) != (pre == FF_NORM_LAYER))
+    return fail(FF_EINVAL, "residual_norm: a beta goes with its LayerNorm");
+  if ((post != FF_NORM_NONE || pre != FF_NORM_NONE) && !(eps > 0.f)) return fail(FF_EINVAL, "residual_norm: eps must be > 0");
+  if (gate && gate_dtype != dtype && gate_dtype != FF_F32)
+    return fail(FF_EINVAL, "residual_norm: gate must be fp32 or of x's type");
+  if (gate && (gate_rows <= 0 || T % gate_rows != 0))
+    return fail(FF_EINVAL, "residual_norm: T must be a multiple of the gate's rows");
+  if (T == 0) return FF_OK;
+  if (!x || !y || !x_out) return fail(FF_EINVAL, "residual_norm: null pointer");
+  if ((h != nullptr) != (pre != FF_NORM_NONE)) return fail(FF_EINVAL, "residual_norm: h goes with a pre-norm");
+  if (T == 1) x_row = y_row = xo_row = h_row = C;  // a single row's stride says nothing
+  if (!h) h_row = C;
+  uint64_t low = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(x_out) |
+                 reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(gate);
+  for (int64_t s : {x_row, y_row, xo_row, h_row}) {
+    if (s < 0) return fail(FF_EINVAL, "residual_norm: strides must not be negative");
+    low |= static_cast<uint64_t>(s) * 2;
+  }
+  if ((low & 15) || ((reinterpret_cast<uintptr_t>(post_gamma) | reinterpret_cast<uintptr_t>(post_beta) |
+                      reinterpret_cast<uintptr_t>(pre_gamma) | reinterpret_cast<uintptr_t>(pre_beta)) & 15))
+    return fail(FF_EINVAL, "residual_norm: misaligned pointer or stride (multiples of 16 bytes)");
+  if (xo_row < C || h_row < C) return fail(FF_EINVAL, "residual_norm: the rows of an output overlap");
+  // Rows are read and written by different workgroups, in no order: an output is x or y itself or shares no byte with what is
+  // read or with the other output.
+  auto rows = [&](const void* p, int64_t stride) {
+    return Extent{reinterpret_cast<uintptr_t>(p), {T, 1}, {2 * stride, 0}, 2 * C};
+  };
+  const Extent in[2] = {rows(x, x_row), rows(y, y_row)}, to[2] = {rows(x_out, xo_row), rows(h, h_row)};
+  const Extent read[5] = {range(post_gamma, 4 * C), range(post_beta, 4 * C), range(pre_gamma, 4 * C), range(pre_beta, 4 * C),
+                          range(gate, gate_rows * C * (gate_dtype == FF_F32 ? 4 : 2))};
+  bool clear = !h || clear_of(to[0], to[1]);
+  for (int o = 0; o < (h ? 2 : 1); ++o) {
+    for (const Extent& e : in) clear = clear && ((to[o].at == e.at && to[o].pitch[0] == e.pitch[0]) || clear_of(to[o], e));
+    for (const Extent& e : read) clear = clear && (e.at == 0 || clear_of(to[o], e));
+  }
+  if (!clear)
+    return fail(FF_EINVAL, "residual_norm: an output overlaps the other one or what is read (x or y, with its stride, may be in "
+                           "its place)");
+  const ResidualArgs a{x, y, gate, x_out, h, x_row, y_row, xo_row, h_row, post_gamma, post_beta, pre_gamma, pre_beta,
+                       static_cast<int>(T), static_cast<int>(C), gate ? static_cast<int>(T / gate_rows) : 1, post, pre,
+                       gate_dtype == FF_F32, scale, eps};
+  if (dtype == FF_F16)
+    launch_residual_width<half_t>(a, as_stream(stream));
+  else
+    launch_residual_width<bf16_t>(a, as_stream(stream));
+  return check_launch("residual_norm");
+}

@@ -25,7 +25,7 @@ ENV = "FOIDFINDER_ROCM_KERNELS"  # path to a prebuilt library (the reference's $
 # Epilogue codes (include/foidfinder_rocm.h); 0-2 as foidfinder/backends/cuda/engine.py:24.
 EPI_QKV_ROPE, EPI_RESIDUAL, EPI_GELU_F16, EPI_SWIGLU, EPI_BIAS_F16, EPI_I32 = 0, 1, 2, 3, 4, 5
 
-# Norm codes of quant_mx4 and qk_norm_rope (include/foidfinder_rocm.h).
+# Norm codes of quant_mx4, qk_norm_rope and residual_norm (include/foidfinder_rocm.h).
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 
 _vp, _i64, _f32, _int = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_int
@@ -37,6 +37,14 @@ SIGNATURES = {
     "ff_gemm_s8": ([_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _int, _int, _vp, _vp, _i64, _f32, _vp], _int),
     "ff_gemm_s8_variants": ([], _int),
     "ff_attention": ([_vp, _vp, _i64, _i64, _i64, _vp], _int),
+    "ff_cross_attention": ([_vp, _i64, _i64, _i64] * 4 + [_int] + [_i64] * 6 + [_f32, _vp, _vp, _i64, _vp, _i64, _vp],
+                           _int),
+    "ff_cross_attention_work": ([_i64] * 6, _i64),
+    "ff_prefix_attention": ([_vp, _i64, _i64, _i64] + [_vp, _i64, _i64] * 2 + [_vp, _i64, _i64, _i64] * 3 + [_int]
+                            + [_i64] * 7 + [_f32, _vp, _vp, _i64, _vp], _int),
+    "ff_prefix_attention_work": ([_i64] * 7, _i64),
+    "ff_residual_norm": ([_vp, _i64] * 4 + [_int, _i64, _i64] + [_int, _vp, _vp] * 2 + [_vp, _i64, _int, _f32, _f32, _vp],
+                         _int),
     "ff_resample_u8": ([_vp, _i64, _i64, _int, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp],
                        _int),
     "ff_bicubic_taps": ([*[_i64] * 3, _vp, _vp, *[_i64] * 4, _vp, _vp, _i64, _vp], _int),
@@ -60,7 +68,7 @@ SIGNATURES = {
                          _int, _f32, _vp], _int),
     "ff_head": ([_vp, _i64, _vp, _vp, _f32, _vp, _vp, _i64, _i64, _i64, _vp, _vp], _int),
 }
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 
 @cache
@@ -610,6 +618,153 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: t
          2 * half, pairs, _ptr(positions), pos64, q_scale)
 
 
+def _rows4(x: torch.Tensor, name: str) -> tuple:
+    """Address and strides (batch, token, head) of [B, L, heads, D] with contiguous columns; a dimension of one has none."""
+    shape = x.shape
+    if len(shape) != 4:
+        raise RuntimeError(f"{name} must be [B, L, heads, D]")
+    (b, n, h, _), (sb, sn, sh, one) = shape, x.stride()
+    if one != 1 and x.numel():
+        raise RuntimeError(f"{name} must have contiguous columns")
+    return x.data_ptr(), sb if b > 1 else 0, sn if n > 1 else 0, sh if h > 1 else 0
+
+
+def _scratch(work: torch.Tensor | None, dev: int) -> tuple:
+    if work is None:
+        return None, 0
+    if work.dtype != torch.float32 or work.get_device() != dev or not work.is_contiguous():
+        raise RuntimeError("work must be contiguous fp32 on the queries' GPU")
+    return work.data_ptr(), work.numel()
+
+
+def _lens(lens: torch.Tensor | None, B: int, dev: int) -> int | None:
+    if lens is None:
+        return None
+    if lens.dtype != torch.int32 or lens.shape != (B,) or lens.get_device() != dev or not lens.is_contiguous():
+        raise RuntimeError(f"lens must be contiguous int32 {(B,)} on the queries' GPU")
+    return lens.data_ptr()
+
+
+def _attended(q: torch.Tensor, out: torch.Tensor, *kv: torch.Tensor) -> int:
+    """The device of queries, keys, values and the output, which agree in type, head width and the output's shape."""
+    dt, dev, D = q.dtype, q.get_device(), q.size(-1)
+    if dev < 0:
+        raise RuntimeError("foidfinder_rocm ops take GPU tensors")
+    if dt not in _HALVES or out.dtype != dt or out.shape != q.shape:
+        raise RuntimeError("q and out must be fp16 or bf16, of one type and shape")
+    if out.get_device() != dev:
+        raise RuntimeError("all tensors must be on one device")
+    for i, t in enumerate(kv):
+        if t.dtype != dt or t.size(-1) != D or t.shape != kv[i & ~1].shape:
+            raise RuntimeError("keys and values must have q's type and head width, and each other's shape")
+        if t.get_device() != dev:
+            raise RuntimeError("all tensors must be on one device")
+    return dev
+
+
+def cross_attention_work(q: torch.Tensor, k: torch.Tensor) -> int:
+    """fp32 elements of the workspace that cross_attention takes for queries and keys of these shapes (0: none)."""
+    B, L, H, D = q.shape
+    return lib().ff_cross_attention_work(B, L, k.size(1), H, k.size(2), D)
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, scale: float,
+                    lens: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                    work: torch.Tensor | None = None) -> None:
+    """Attention of q [B, L, heads, D] to keys and values [B, S, kv_heads, D] of another length into out, fp16 or bf16 with
+    fp32 sums (include/foidfinder_rocm.h, ff_cross_attention): any batch, token and head strides that are multiples of 16
+    bytes (views of packed rows, [B, heads, L, D] transposed, rows expanded over the batch), D a multiple of 8 up to 128,
+    heads a multiple of kv_heads. Keys j >= lens[b] (int32 [B]) and keys with mask[b, j] False (bool [B, S], contiguous
+    columns) are not read; a query without keys gives zeros. work: fp32 of at least cross_attention_work(q, k) elements; calls
+    that run one after another may share it. out and work share no memory with each other or with what is read (refused)."""
+    _no_grad(q, k, v, out, work)
+    dev = _attended(q, out, k, v)
+    qr, kr, vr, to = _rows4(q, "q"), _rows4(k, "k"), _rows4(v, "v"), _rows4(out, "out")
+    (B, L, H, D), (KB, S, KV, _) = q.shape, k.shape
+    if KB != B:
+        raise RuntimeError("q and k must share the batch")
+    mp, mb = None, 0
+    if mask is not None:
+        if mask.dtype != torch.bool or mask.shape != (B, S) or mask.get_device() != dev:
+            raise RuntimeError(f"mask must be bool {(B, S)} on the queries' GPU")
+        mb, one = mask.stride()
+        if one != 1 and S > 1:
+            raise RuntimeError("mask must have contiguous columns")
+        mp, mb = mask.data_ptr(), mb if B > 1 else 0
+    _run("ff_cross_attention", dev, *qr, *kr, *vr, *to, _DTYPES[q.dtype], B, L, S, H, KV, D, scale, _lens(lens, B, dev), mp,
+         mb, *_scratch(work, dev))
+
+
+def prefix_attention_work(q: torch.Tensor, prefix_k: torch.Tensor, k: torch.Tensor) -> int:
+    """fp32 elements of the workspace that prefix_attention takes for tensors of these shapes."""
+    B, L, H, D = q.shape
+    return lib().ff_prefix_attention_work(B, L, prefix_k.size(0), k.size(1), H, k.size(2), D)
+
+
+def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     out: torch.Tensor, scale: float, lens: torch.Tensor | None = None,
+                     work: torch.Tensor | None = None) -> None:
+    """Attention of a batch that shares a prefix (include/foidfinder_rocm.h, ff_prefix_attention): q [B, L, heads, D] are each
+    sequence's newest L tokens, prefix_k and prefix_v [P, kv_heads, D] the rows that all sequences see, read once for all of them,
+    k and v [B, S, kv_heads, D] each sequence's own behind them, lens[b] of them (int32 [B]; None: S) with the new tokens' own
+    last. Query i sees the prefix and the own keys j < lens[b] - L + 1 + i. Types, strides and work (at least
+    prefix_attention_work(q, prefix_k, k) elements) as in cross_attention."""
+    _no_grad(q, prefix_k, prefix_v, k, v, out, work)
+    dev = _attended(q, out, prefix_k, prefix_v, k, v)
+    qr, kr, vr, to = _rows4(q, "q"), _rows4(k, "k"), _rows4(v, "v"), _rows4(out, "out")
+    (B, L, H, D), (KB, S, KV, _) = q.shape, k.shape
+    if KB != B or len(prefix_k.shape) != 3 or prefix_k.size(1) != KV:
+        raise RuntimeError("q and k must share the batch, and the prefix must be [P, kv_heads, D]")
+    P = prefix_k.size(0)
+    shared = []
+    for t in (prefix_k, prefix_v):
+        st, sh, one = t.stride()
+        if one != 1 and P:
+            raise RuntimeError("the prefix must have contiguous columns")
+        shared += t.data_ptr(), st if P > 1 else 0, sh if KV > 1 else 0
+    _run("ff_prefix_attention", dev, *qr, *shared, *kr, *vr, *to, _DTYPES[q.dtype], B, L, P, S, H, KV, D, scale,
+         _lens(lens, B, dev), *_scratch(work, dev))
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor, x_out: torch.Tensor, h: torch.Tensor | None, post: int,
+                  post_gamma: torch.Tensor | None, post_beta: torch.Tensor | None, pre: int,
+                  pre_gamma: torch.Tensor | None, pre_beta: torch.Tensor | None, gate: torch.Tensor | None = None,
+                  scale: float = 1.0, eps: float = 1e-6) -> None:
+    """A block's output into the residual stream between two norms (include/foidfinder_rocm.h, ff_residual_norm): x_out =
+    x + scale * gate * N_post(y) and h = N_pre(x_out) in one pass, h from the unrounded sum. x, y, x_out, h fp16 or bf16 [T, C]
+    with contiguous rows (any row stride that is a multiple of 8), C a multiple of 8 up to 16384; h only with a pre-norm (None
+    otherwise); gammas and betas fp32 [C] as the norms (NORM_*) need them; gate [G, C] or [C], fp32 or of x's type, token t
+    taking row t / (T / G): one row is a layer scale, one a sequence an adaptive gate. An output may be x or y itself and shares
+    no other memory with what is read or with the other (refused)."""
+    _no_grad(x, y, x_out, h, post_gamma, post_beta, pre_gamma, pre_beta, gate)
+    dev = _on_gpu(post_gamma, post_beta, pre_gamma, pre_beta, gate)
+    shape, dt = x.shape, x.dtype
+    if len(shape) != 2 or dt not in _HALVES:
+        raise RuntimeError("x must be fp16 or bf16 [T, C]")
+    T, C = shape
+    here, rows = x.get_device(), []
+    for t in (x, y, x_out, h):
+        if t is None:
+            rows += None, C
+            continue
+        if t.shape != shape or t.dtype != dt:
+            raise RuntimeError("x, y and the outputs must have one type and shape")
+        if t.get_device() != here or here < 0 or dev not in (-1, here):
+            raise RuntimeError("all tensors must be on one GPU")
+        stride, one = t.stride()
+        if one != 1 and C > 1:
+            raise RuntimeError("x, y and the outputs must have contiguous rows")
+        rows += t.data_ptr(), stride
+    _float(C, *[t for t in (post_gamma, post_beta, pre_gamma, pre_beta) if t is not None])
+    gates, kind = 0, 0
+    if gate is not None:
+        if gate.dtype not in (dt, torch.float32) or gate.dim() not in (1, 2) or gate.size(-1) != C:
+            raise RuntimeError("gate must be fp32 or of x's type, [G, C] or [C]")
+        gates, kind = gate.numel() // C, _DTYPES[gate.dtype]
+    _run("ff_residual_norm", here, *rows, _DTYPES[dt], T, C, post, _ptr(post_gamma), _ptr(post_beta), pre, _ptr(pre_gamma),
+         _ptr(pre_beta), _ptr(gate), gates, kind, scale, eps)
+
+
 # ---- torch.ops.foidfinder_rocm registration (schemas as kernels.cu:268-273, plus eps / the fused norm) ----
 
 _LIB = torch.library.Library("foidfinder_rocm", "DEF")
@@ -655,6 +810,16 @@ _LIB.define("qk_norm_rope(Tensor q, Tensor k, Tensor(a!) q_out, Tensor(b!) k_out
             "Tensor? k_gamma, Tensor? q_beta, Tensor? k_beta, Tensor rope_cos, Tensor rope_sin, Tensor? positions=None, "
             "bool pairs=True, float eps=1e-06, float q_scale=1.0) -> ()")
 for _fn in (quant_mx4, dequant_mx4, gemm_mx4, qk_norm_rope):
+    _LIB.impl(_fn.__name__, _fn, "CUDA")
+# the decoder side: attention to other rows and the residual stream between two norms (no reference counterpart)
+_LIB.define("cross_attention(Tensor q, Tensor k, Tensor v, Tensor(a!) out, float scale, Tensor? lens=None, "
+            "Tensor? mask=None, Tensor(b!)? work=None) -> ()")
+_LIB.define("prefix_attention(Tensor q, Tensor prefix_k, Tensor prefix_v, Tensor k, Tensor v, Tensor(a!) out, float scale, "
+            "Tensor? lens=None, Tensor(b!)? work=None) -> ()")
+_LIB.define("residual_norm(Tensor x, Tensor y, Tensor(a!) x_out, Tensor(b!)? h, int post, Tensor? post_gamma, "
+            "Tensor? post_beta, int pre, Tensor? pre_gamma, Tensor? pre_beta, Tensor? gate=None, float scale=1.0, "
+            "float eps=1e-06) -> ()")
+for _fn in (cross_attention, prefix_attention, residual_norm):
     _LIB.impl(_fn.__name__, _fn, "CUDA")
 _LIB.impl("slot_weights", slot_weights, "CUDA")
 

@@ -29,12 +29,12 @@ extern "C" {
 #define FF_EPI_BIAS_F16 4 /* fp16 out = y */
 #define FF_EPI_I32 5      /* int32 out [M,N] = the raw accumulators (no scale, no bias) */
 
-/* Element types of the MX4 and head-norm entries. */
+/* Element types of the MX4, head-norm, cross-attention and residual-norm entries. */
 #define FF_F16 0
 #define FF_BF16 1
 #define FF_F32 2
 
-/* Norms of ff_quant_mx4 and ff_qk_norm_rope: none; x / sqrt(mean(x^2) + eps) * gamma; (x - mean) / sqrt(var + eps) * gamma
+/* Norms of ff_quant_mx4, ff_qk_norm_rope and ff_residual_norm: none; x / sqrt(mean(x^2) + eps) * gamma; (x - mean) / sqrt(var + eps) * gamma
  * + beta. gamma is given with a norm and only then, beta with FF_NORM_LAYER and only then. */
 #define FF_NORM_NONE 0
 #define FF_NORM_RMS 1
@@ -123,6 +123,44 @@ int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, const void* 
                     const float* k_gamma, const float* q_beta, const float* k_beta, float eps, const float* rope_cos,
                     const float* rope_sin, int64_t rope_len, int64_t R, int pairs, const void* positions, int pos64,
                     float q_scale, void* stream);
+
+/* Attention of queries to keys and values of another length: q, out [B, L, heads, D], k, v [B, S, kv_heads, D], fp16 or bf16, by
+ * strides in elements (batch, token, head; columns contiguous), D % 8 == 0, D <= 128, heads % kv_heads == 0 (query head h reads
+ * key head h / (heads / kv_heads)); strides of q, k, v may be 0 (shared rows). out[b, i, h] = sum_j p_j v[b, j], p the softmax of
+ * scale q.k over the keys j < lens[b] (int32 [B], taken into 0 .. S; NULL: S) whose mask[b * mask_batch + j] is not 0 (bytes; NULL:
+ * all); 0 where there are none. What k and v hold for other keys is not read. q, k, v and their strides are multiples of 16
+ * bytes, out's of 8; tokens of k and v are fewer than 2^24 elements apart. work: at least ff_cross_attention_work fp32 elements
+ * (0 where keys are not cut; NULL then), which calls that run one after another may share. out and work share no memory with
+ * each other or with what is read (refused; where rows of three strides lie between another operand's, so are calls that
+ * would not touch it). */
+int64_t ff_cross_attention_work(int64_t B, int64_t L, int64_t S, int64_t heads, int64_t kv_heads, int64_t D);
+int ff_cross_attention(const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* k, int64_t k_batch,
+                       int64_t k_token, int64_t k_head, const void* v, int64_t v_batch, int64_t v_token, int64_t v_head,
+                       void* out, int64_t o_batch, int64_t o_token, int64_t o_head, int dtype, int64_t B, int64_t L,
+                       int64_t S, int64_t heads, int64_t kv_heads, int64_t D, float scale, const int32_t* lens,
+                       const uint8_t* mask, int64_t mask_batch, float* work, int64_t work_size, void* stream);
+
+/* Attention of a batch whose sequences share a prefix: prefix_k, prefix_v [P, kv_heads, D] are read once for all sequences, and
+ * k, v [B, S, kv_heads, D] are each sequence's own keys behind it, lens[b] of them (int32 [B], taken into 0 .. S; NULL: S), the
+ * last L of them the new tokens' own: query i sees the prefix and the own keys j < lens[b] - L + 1 + i. P and S may be 0. The rest
+ * as in ff_cross_attention. */
+int64_t ff_prefix_attention_work(int64_t B, int64_t L, int64_t P, int64_t S, int64_t heads, int64_t kv_heads, int64_t D);
+int ff_prefix_attention(const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* prefix_k,
+                        int64_t pk_token, int64_t pk_head, const void* prefix_v, int64_t pv_token, int64_t pv_head,
+                        const void* k, int64_t k_batch, int64_t k_token, int64_t k_head, const void* v, int64_t v_batch,
+                        int64_t v_token, int64_t v_head, void* out, int64_t o_batch, int64_t o_token, int64_t o_head,
+                        int dtype, int64_t B, int64_t L, int64_t P, int64_t S, int64_t heads, int64_t kv_heads, int64_t D,
+                        float scale, const int32_t* lens, float* work, int64_t work_size, void* stream);
+
+/* A block's output into the residual stream between two norms: x_out = x + scale * gate * N_post(y), h = N_pre(x_out), each
+ * rounded once, h from the unrounded sum. x, y, x_out, h fp16 or bf16 [T, C] by row strides in elements, C % 8 == 0, C <= 16384;
+ * norms FF_NORM_* with fp32 gamma/beta [C]; h with a pre-norm and only then. gate (or NULL: 1) [gate_rows, C] of x's type or
+ * FF_F32: token t takes row t / (T / gate_rows). Pointers and strides are multiples of 16 bytes. An output is x or y itself (the
+ * same pointer and stride) or shares no memory with what is read or with the other one. */
+int ff_residual_norm(const void* x, int64_t x_row, const void* y, int64_t y_row, void* x_out, int64_t xo_row, void* h,
+                     int64_t h_row, int dtype, int64_t T, int64_t C, int post, const float* post_gamma,
+                     const float* post_beta, int pre, const float* pre_gamma, const float* pre_beta, const void* gate,
+                     int64_t gate_rows, int gate_dtype, float scale, float eps, void* stream);
 
 /* Non-causal flash attention, head_dim 64, over packed qkv rows.
  * qkv fp16 [T, 3*heads*64] (q already rotated and scaled by softmax_scale*log2(e), k rotated) -> out fp16

@@ -33,6 +33,7 @@ constexpr int QW = 32;     // rows of a unit
 constexpr int WAVES = 4;   // waves a workgroup
 constexpr int BKV = 64;    // keys a tile
 constexpr float SUM_LIMIT = 8192.f;  // a lane's sum of p over a half tile above which m is raised (fp16 holds p up to it)
+constexpr float CAP = 12.f;          // exponent of the largest p after m was raised
 constexpr float LOWEST = -3.402823466e38f;
 
 struct KeySource {
@@ -76,62 +77,193 @@ __device__ __forceinline__ float16_t mfma(vec8_t<bf16_t> a, vec8_t<bf16_t> b, fl
 
 // What a workgroup works on; the same in all its lanes.
 struct Piece {
-  int seq;          // -1: the shared prefix, rows of all sequences
-  int head;         // key head
+  int seq;           // -1: the shared prefix, rows of all sequences
+  int head;          // key head
   int row0, row_end;
-  int keys, len;    // keys that some row sees; the sequence's length
-  int t0, t1;       // tiles
+  int keys, len;     // keys that some row sees; the sequence's length
+  int front;         // slices of 32 prefix keys before the sequence's own (streams only)
+  int t0, t1;        // tiles, or slices of 32 keys
   int part;
 };
 
-template <typename T, int DP, int SPLIT>
-__device__ __forceinline__ void cross_block(const CrossArgs& a, const Piece& w, T* smem) {
-  constexpr int CH = DP / 8, TILE = BKV * DP, LPW = CH / 4, KS = DP / 16, DT = DP / 32;
+// Where a lane's row lies, and how many of the sequence's own keys it sees.
+struct Place {
+  int seq, token, head, limit;
+};
+__device__ __forceinline__ Place place_of(const CrossArgs& a, const Piece& w, int row) {
+  const int real = min(row, w.row_end - 1), per = a.tokens * a.group;
+  Place p;
+  p.seq = w.seq < 0 ? real / per : w.seq;
+  const int rest = real - p.seq * per;
+  p.token = rest / a.group;
+  p.head = w.head * a.group + rest - p.token * a.group;
+  p.limit = a.causal && w.seq >= 0 ? min(max(w.len - a.tokens + 1 + p.token, 0), w.keys) : w.keys;
+  return p;
+}
+
+// 32 rows in a wave: q, O, m and the lane's part of l. Lane: row fr = lane % 32, half fh = lane / 32.
+template <typename T, int DP>
+struct Unit {
+  static constexpr int KS = DP / 16, DT = DP / 32;
   typedef vec8_t<T> T8;
   typedef vec4_t<T> T4;
-  const uint32_t smem_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)smem));
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int fr = lane & 31, fh = lane >> 5;
-  const int unit = SPLIT == 2 ? 0 : (SPLIT ? wave >> 1 : wave);
-  const int half_sel = SPLIT ? wave & 1 : 0, parity = SPLIT == 2 ? wave >> 1 : 0;
-  const bool active = w.row0 + unit * QW < w.row_end;  // other waves only load
+  T8 qf[KS];       // column operand of S^T: the row's columns 16 s + 8 fh + 0..7
+  float16_t o[DT]; // O^T: columns 32 dt + 8 (r / 4) + 4 fh + r % 4
+  float m = LOWEST, l = 0.f, c;
+  float16_t xs;    // S^T of 32 keys: 8 (r / 4) + 4 fh + r % 4
+  T8 pf[2];
+  int koff[KS], voff[DT];  // LDS offsets (elements) of the fragments within 32 keys
 
-  // The lane's row: sequence, token, head
-  const int row = w.row0 + unit * QW + fr, real = min(row, w.row_end - 1), per = a.tokens * a.group;
-  const int seq = w.seq < 0 ? real / per : w.seq, rest = real - seq * per, token = rest / a.group;
-  const int head = w.head * a.group + rest - token * a.group;
-  const int limit = a.causal && w.seq >= 0 ? min(max(w.len - a.tokens + 1 + token, 0), w.keys) : w.keys;
-
-  T8 qf[KS];  // column operand of S^T: the lane's row, columns 16 s + 8 fh + 0..7
-  {
-    const T* q = static_cast<const T*>(a.q) + seq * a.qb + token * a.qt + head * a.qh;
+  __device__ __forceinline__ void start(const CrossArgs& a, const Place& p, int lane) {
+    const int fr = lane & 31, fh = lane >> 5;
+    const T* q = static_cast<const T*>(a.q) + p.seq * a.qb + p.token * a.qt + p.head * a.qh;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       qf[s] = T8{};
       if (16 * s + 8 * fh < a.dim) qf[s] = *reinterpret_cast<const T8*>(q + 16 * s + 8 * fh);
     }
-    // consumed here, so that the compiler's wait for these loads stands before the loop and not in it
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+    c = a.c;
+    // K fragment s: row fr, chunk 2 s + fh. V^T fragment (dt, tt), part j: lane l of 16 addresses row 16 tt + 8 j + 4 fh + l / 4,
+    // columns 32 dt + 16 (group) + 4 (l % 4), and receives four keys in a row of column 32 dt + fr: the keys of P^T's slots.
+#pragma unroll
+    for (int s = 0; s < KS; ++s) koff[s] = fr * DP + k_slot<DP>(fr, 2 * s + fh) * 8;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int r = 4 * fh + ((lane & 15) >> 2), col = dt * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+      voff[dt] = r * DP + v_slot<DP>(r, col >> 3) * 8 + (col & 7);
+    }
+  }
+  // q consumed, so that the compiler's wait for its loads stands here, before the loop and after the first keys' loads, not in it.
+  __device__ __forceinline__ void settle() {
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" ::"v"(qf[s]));
   }
+  // S^T of the 32 keys at k (+ ka).
+  __device__ __forceinline__ void score(const T* k, const int (&ka)[KS]) {
+    const float16_t zero = {};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) xs = mfma(*reinterpret_cast<const T8*>(k + ka[s]), qf[s], s == 0 ? zero : xs);
+  }
+  // p of the scores, at most 2^cap each, and the lane's sum of it.
+  __device__ __forceinline__ float weights(float cap) {
+    float e[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float x = __builtin_fmaf(xs[r], c, -m);
+      if (!__builtin_isinf(cap)) x = x > cap ? cap : x;  // not a number stays so
+      e[r] = __builtin_amdgcn_exp2f(x);
+      pf[r >> 3][r & 7] = static_cast<T>(e[r]);
+    }
+#pragma unroll
+    for (int n = 8; n >= 1; n >>= 1)
+#pragma unroll
+      for (int r = 0; r < n; ++r) e[r] = e[r] + e[r + n];
+    return e[0];
+  }
+  // p of the scores; bits: the keys that the lane's row sees.
+  // first: m is not set yet, which the first pass would only find out.
+  __device__ __forceinline__ void weigh(uint32_t bits, int fh, bool first) {
+    if (__any(bits != ~0u)) {
+      bits >>= 4 * fh;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) xs[r] = (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? xs[r] : -__builtin_inff();
+    }
+    float sum = 0.f;
+    if (!first) sum = weights(__builtin_inff());
+    if (first || __any(sum > SUM_LIMIT)) {
+      // m becomes the largest c S of these keys, or just below, and O and l follow. Scores from 2^30 up are too coarse for the
+      // multiply-add: what it leaves of the largest can be of any size then, and is capped.
+      float top = xs[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, xs[r]);
+      top = fmaxf(top, xor_shuffle(top, 32)) * c;
+      const float m_old = m;
+      m = fmaxf(m, top - fabsf(top) * 0x1p-23f);
+      const float corr = __builtin_amdgcn_exp2f(m_old - m);
+      l *= corr;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= corr;
+      sum = weights(CAP);
+    }
+    l += sum;
+  }
+  // O^T += V^T P^T, the 32 values at LDS byte v + OFF (+ va).
+  template <int OFF>
+  __device__ __forceinline__ void mix(uint32_t v, const int (&va)[DT]) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      T4 x[4];  // [2 tt + j]
+      const uint32_t base = v + 2u * static_cast<uint32_t>(va[dt]);
+      tr_read<OFF>(x[0], base);
+      tr_read<OFF + 8 * DP * 2>(x[1], base);
+      tr_read<OFF + 16 * DP * 2>(x[2], base);
+      tr_read<OFF + 24 * DP * 2>(x[3], base);
+      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+        o[dt] = mfma(__builtin_shufflevector(x[2 * tt], x[2 * tt + 1], 0, 1, 2, 3, 4, 5, 6, 7), pf[tt], o[dt]);
+    }
+  }
+};
+
+// Four columns of a row's O to the workspace, or its quotient to out; (m, l) with the first.
+template <typename T>
+__device__ __forceinline__ void store4(const CrossArgs& a, const Piece& w, const Place& p, int row, int col, float4_t o, float m,
+                                       float l) {
+  if (col >= a.dim) return;
+  if (a.work) {
+    const int64_t n = (static_cast<int64_t>(w.part) * a.kv + w.head) * a.rows + row;
+    *reinterpret_cast<float4_t*>(a.work + n * a.dim + col) = o;
+    if (col == 0) {
+      const int64_t parts = a.prefix_splits + a.own_splits;
+      *reinterpret_cast<float2*>(a.work + parts * a.kv * a.rows * a.dim + 2 * n) = float2{m, l};
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // no keys: zeros
+  vec4_t<T> v;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) v[u] = static_cast<T>(o[u] * inv);
+  *reinterpret_cast<vec4_t<T>*>(static_cast<T*>(a.out) + p.seq * a.ob + p.token * a.ot + p.head * a.oh + col) = v;
+}
+
+// Tiles of 64 keys for four waves: a wave a unit (SHARE 1), or two (SHARE 2), each with one half of every tile.
+template <typename T, int DP, int SHARE>
+__device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T* smem) {
+  constexpr int CH = DP / 8, TILE = BKV * DP, LPW = CH / 4, KS = DP / 16, DT = DP / 32;
+  const uint32_t smem_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)smem));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int fr = lane & 31, fh = lane >> 5, unit = wave / SHARE, half_sel = SHARE == 2 ? wave & 1 : 0;
+  const bool active = w.row0 + unit * QW < w.row_end;  // other waves only load
+  const int row = w.row0 + unit * QW + fr;
+  const Place p = place_of(a, w, row);
+  Unit<T, DP> u;
+  u.start(a, p, lane);
 
   const KeySource& src = w.seq < 0 ? a.prefix : a.own;
   const int64_t at = max(w.seq, 0);
   const T* kbase = static_cast<const T*>(src.k) + at * src.kb + w.head * src.kh;
   const T* vbase = static_cast<const T*>(src.v) + at * src.vb + w.head * src.vh;
   const uint8_t* mask = a.mask && w.seq >= 0 ? a.mask + at * a.mask_b : nullptr;
+  const bool guard = mask || src.kt < a.dim || src.vt < a.dim;  // rows left out that the descriptor's range does not leave out
 
   // Tile loads: wave w fills the 1 KB blocks LPW w .. of either tile, lane l the chunk l of a block; it fetches what the swizzle
   // puts there.
   uint32_t voff_k[LPW], voff_v[LPW];
   int lrow[LPW];
 #pragma unroll
-  for (int p = 0; p < LPW; ++p) {
-    const int n = (LPW * wave + p) * 64 + lane, r = n / CH, slot = n % CH;
+  for (int i = 0; i < LPW; ++i) {
+    const int n = (LPW * wave + i) * 64 + lane, r = n / CH, slot = n % CH;
     const int ck = k_slot<DP>(r, slot), cv = v_slot<DP>(r, slot);
-    lrow[p] = r;
-    voff_k[p] = 8 * ck < a.dim ? static_cast<uint32_t>((r * static_cast<int>(src.kt) + ck * 8) * 2) : OOB_OFFSET;
-    voff_v[p] = 8 * cv < a.dim ? static_cast<uint32_t>((r * static_cast<int>(src.vt) + cv * 8) * 2) : OOB_OFFSET;
+    lrow[i] = r;
+    voff_k[i] = 8 * ck < a.dim ? static_cast<uint32_t>((r * static_cast<int>(src.kt) + ck * 8) * 2) : OOB_OFFSET;
+    voff_v[i] = 8 * cv < a.dim ? static_cast<uint32_t>((r * static_cast<int>(src.vt) + cv * 8) * 2) : OOB_OFFSET;
   }
   auto issue = [&](int tile, uint64_t word) __attribute__((always_inline)) {
     const int st = (tile - w.t0) & 1, rows = min(BKV, w.keys - tile * BKV);
@@ -139,11 +271,11 @@ __device__ __forceinline__ void cross_block(const CrossArgs& a, const Piece& w, 
     const int nk = ((rows - 1) * static_cast<int>(src.kt) + a.dim) * 2, nv = ((rows - 1) * static_cast<int>(src.vt) + a.dim) * 2;
     const T *k = kbase + first * src.kt, *v = vbase + first * src.vt;
 #pragma unroll
-    for (int p = 0; p < LPW; ++p) {
-      const bool in = !mask || ((word >> lrow[p]) & 1);
-      buffer_to_lds(k, nk, reinterpret_cast<uint8_t*>(smem + st * TILE + (LPW * wave + p) * 512), in ? voff_k[p] : OOB_OFFSET);
-      buffer_to_lds(v, nv, reinterpret_cast<uint8_t*>(smem + (2 + st) * TILE + (LPW * wave + p) * 512),
-                    in ? voff_v[p] : OOB_OFFSET);
+    for (int i = 0; i < LPW; ++i) {
+      const bool in = !guard || ((word >> lrow[i]) & 1);
+      buffer_to_lds(k, nk, reinterpret_cast<uint8_t*>(smem + st * TILE + (LPW * wave + i) * 512), in ? voff_k[i] : OOB_OFFSET);
+      buffer_to_lds(v, nv, reinterpret_cast<uint8_t*>(smem + (2 + st) * TILE + (LPW * wave + i) * 512),
+                    in ? voff_v[i] : OOB_OFFSET);
     }
   };
   // The keys of a tile that may be seen, as bits.
@@ -156,104 +288,22 @@ __device__ __forceinline__ void cross_block(const CrossArgs& a, const Piece& w, 
     const int n = w.keys - tile * BKV;
     return n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1;
   };
-
-  // LDS read offsets within a tile. K fragment (half, s): row 32 half + fr, chunk 2 s + fh. V^T fragment (dt, half, tt), part j:
-  // lane l of 16 addresses row 32 half + 16 tt + 8 j + 4 fh + l / 4, columns 32 dt + 16 (group) + 4 (l % 4), and receives four
-  // keys in a row of column 32 dt + fr: the keys of P^T's slots.
-  int koff[KS], voff[DT];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) koff[s] = (fr + 32 * half_sel) * DP + k_slot<DP>(fr, 2 * s + fh) * 8;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    const int r = 4 * fh + ((lane & 15) >> 2), col = dt * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    voff[dt] = (r + 32 * half_sel) * DP + v_slot<DP>(r, col >> 3) * 8 + (col & 7);
-  }
-
-  float16_t o[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
-  float m = LOWEST, l_run = 0.f, hs[2] = {0.f, 0.f};
-  float16_t xs;  // S^T of a half: keys 8 (r / 4) + 4 fh + r % 4
-  T8 pf[2];
-  int ka[KS], va[DT];
-
-  auto qk = [&](int half) __attribute__((always_inline)) {
-    const float16_t zero = {};
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const T8 kf = *reinterpret_cast<const T8*>(smem + ka[s] + half * 32 * DP);
-      xs = mfma(kf, qf[s], s == 0 ? zero : xs);
-    }
-  };
-  auto soft = [&](int half) __attribute__((always_inline)) {
-    float e[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(xs[r], a.c, -m));
-      pf[r >> 3][r & 7] = static_cast<T>(e[r]);
-    }
-#pragma unroll
-    for (int n = 8; n >= 1; n >>= 1)
-#pragma unroll
-      for (int r = 0; r < n; ++r) e[r] = e[r] + e[r + n];
-    hs[half] = e[0];
-  };
-  // A half whose p passed the limit: m becomes the largest c S of the half, O and l follow.
-  auto raise = [&](int half) __attribute__((always_inline)) {
-    float top = xs[0];
-#pragma unroll
-    for (int r = 1; r < 16; ++r) top = fmaxf(top, xs[r]);
-    top = fmaxf(top, xor_shuffle(top, 32)) * a.c;
-    const float m_old = m;
-    m = fmaxf(m, top);
-    const float corr = __builtin_amdgcn_exp2f(m_old - m);
-    l_run *= corr;
-    if (half == 1) hs[0] *= corr;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[dt][r] *= corr;
-    soft(half);
-  };
-  auto pv = [&](auto halfc) __attribute__((always_inline)) {
+  auto half_tile = [&](int tile, uint64_t word, const int (&ka)[KS], const int (&va)[DT], auto halfc) __attribute__((always_inline)) {
     constexpr int half = decltype(halfc)::value;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      T4 v[4];  // [2 tt + j]
-      const uint32_t base = smem_lds + 2u * static_cast<uint32_t>(va[dt]);
-      tr_read<(half * 32 + 0) * DP * 2>(v[0], base);
-      tr_read<(half * 32 + 8) * DP * 2>(v[1], base);
-      tr_read<(half * 32 + 16) * DP * 2>(v[2], base);
-      tr_read<(half * 32 + 24) * DP * 2>(v[3], base);
-      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-        o[dt] = mfma(__builtin_shufflevector(v[2 * tt], v[2 * tt + 1], 0, 1, 2, 3, 4, 5, 6, 7), pf[tt], o[dt]);
-    }
-  };
-  auto half_tile = [&](int tile, uint64_t word, auto halfc) __attribute__((always_inline)) {
-    constexpr int half = decltype(halfc)::value;
-    const int h = SPLIT ? half_sel : half;  // of the tile
-    qk(half);
-    const int left = limit - (tile * BKV + 32 * h);
+    const int h = SHARE == 2 ? half_sel : half;  // of the tile (SHARE 2: the offsets point to it)
+    u.score(smem + half * 32 * DP, ka);
+    const int left = p.limit - (tile * BKV + 32 * h);
     uint32_t bits = static_cast<uint32_t>(word >> (32 * h));
     bits &= left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
-    if (__any(bits != ~0u)) {
-      bits >>= 4 * fh;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) xs[r] = (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? xs[r] : -__builtin_inff();
-    }
-    soft(half);
-    if (__any(hs[half] > SUM_LIMIT)) raise(half);
-    pv(halfc);
+    u.weigh(bits, fh, tile == w.t0 && half == 0);
+    u.template mix<half * 32 * DP * 2>(smem_lds, va);
   };
 
   if (w.t0 < w.t1) {
     uint64_t word = valid(w.t0, mask_byte(w.t0)), next = 0;
     uint8_t byte = mask_byte(w.t0 + 1);
     issue(w.t0, word);
+    u.settle();
     for (int tile = w.t0; tile < w.t1; ++tile) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();  // no fence: the wait covers this thread's LDS writes
@@ -263,159 +313,290 @@ __device__ __forceinline__ void cross_block(const CrossArgs& a, const Piece& w, 
         byte = mask_byte(tile + 2);
       }
       const int st = (tile - w.t0) & 1;
-      if (active && (SPLIT != 2 || ((tile - w.t0) & 1) == parity) && word != 0) {
+      if (active && word != 0) {
         // read bases, opaque to the compiler so that the fragment offsets fold into the reads' immediate offsets
+        int ka[KS], va[DT];
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          ka[s] = st * TILE + koff[s];
+          ka[s] = st * TILE + half_sel * 32 * DP + u.koff[s];
           asm volatile("" : "+v"(ka[s]));
         }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          va[dt] = (2 + st) * TILE + voff[dt];
+          va[dt] = (2 + st) * TILE + half_sel * 32 * DP + u.voff[dt];
           asm volatile("" : "+v"(va[dt]));
         }
-        hs[1] = 0.f;
-        half_tile(tile, word, std::integral_constant<int, 0>{});
-        if constexpr (!SPLIT) half_tile(tile, word, std::integral_constant<int, 1>{});
-        l_run += hs[0] + hs[1];
+        half_tile(tile, word, ka, va, std::integral_constant<int, 0>{});
+        if constexpr (SHARE == 1) half_tile(tile, word, ka, va, std::integral_constant<int, 1>{});
       }
       word = next;
     }
   }
 
-  if constexpr (SPLIT) {  // the waves of a unit leave O, m and l in LDS; the first joins them
-    constexpr int SHARE = SPLIT == 2 ? WAVES : 2, WORDS = 16 * DT + 2;
-    static_assert((WAVES - 1) * WORDS * 64 * 4 <= 4 * TILE * 2, "the joint exceeds the ring");
-    const int me = SPLIT == 2 ? wave : half_sel;
-    float* joint = reinterpret_cast<float*>(smem) + unit * (SHARE - 1) * WORDS * 64 + lane;
+  if constexpr (SHARE == 2) {  // the second wave of a unit leaves O, m and l in LDS; the first joins them
+    constexpr int WORDS = 16 * DT + 2;
+    static_assert(2 * WORDS * 64 * 4 <= 4 * TILE * 2, "the joint exceeds the ring");
+    float* joint = reinterpret_cast<float*>(smem) + unit * WORDS * 64 + lane;
     __syncthreads();
-    if (active && me != 0) {
-      float* mine = joint + (me - 1) * WORDS * 64;
+    if (active && half_sel) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mine[(dt * 16 + r) * 64] = o[dt][r];
-      mine[(WORDS - 2) * 64] = m;
-      mine[(WORDS - 1) * 64] = l_run;
+        for (int r = 0; r < 16; ++r) joint[(dt * 16 + r) * 64] = u.o[dt][r];
+      joint[(WORDS - 2) * 64] = u.m;
+      joint[(WORDS - 1) * 64] = u.l;
     }
     __syncthreads();
-    if (!active || me != 0) return;
-    float top = m;
-#pragma unroll
-    for (int k = 0; k < SHARE - 1; ++k) top = fmaxf(top, joint[(k * WORDS + WORDS - 2) * 64]);
-    const float c0 = __builtin_amdgcn_exp2f(m - top);
-    m = top;
-    l_run *= c0;
+    if (!active || half_sel) return;
+    const float top = fmaxf(u.m, joint[(WORDS - 2) * 64]);
+    const float c0 = __builtin_amdgcn_exp2f(u.m - top), c1 = __builtin_amdgcn_exp2f(joint[(WORDS - 2) * 64] - top);
+    u.m = top;
+    u.l = __builtin_fmaf(joint[(WORDS - 1) * 64], c1, u.l * c0);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[dt][r] *= c0;
-#pragma unroll
-    for (int k = 0; k < SHARE - 1; ++k) {
-      const float* theirs = joint + k * WORDS * 64;
-      const float ck = __builtin_amdgcn_exp2f(theirs[(WORDS - 2) * 64] - top);
-      l_run = __builtin_fmaf(theirs[(WORDS - 1) * 64], ck, l_run);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] = __builtin_fmaf(theirs[(dt * 16 + r) * 64], ck, o[dt][r]);
-    }
+      for (int r = 0; r < 16; ++r) u.o[dt][r] = __builtin_fmaf(joint[(dt * 16 + r) * 64], c1, u.o[dt][r] * c0);
   } else {
     if (!active) return;
   }
-
-  const float l = l_run + xor_shuffle(l_run, 32);
+  const float l = u.l + xor_shuffle(u.l, 32);
   if (row >= w.row_end) return;
-  if (a.work) {
-    const int64_t n = (static_cast<int64_t>(w.part) * a.kv + w.head) * a.rows + row;
-    float* to = a.work + n * a.dim;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (dt * 32 + 8 * g + 4 * fh < a.dim)
-          *reinterpret_cast<float4_t*>(to + dt * 32 + 8 * g + 4 * fh) =
-              float4_t{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
-    if (fh == 0) {
-      const int64_t parts = a.prefix_splits + a.own_splits;
-      float* ml = a.work + parts * a.kv * a.rows * a.dim + 2 * n;
-      ml[0] = m;
-      ml[1] = l;
-    }
-    return;
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // no keys: zeros
-  T* to = static_cast<T*>(a.out) + seq * a.ob + token * a.ot + head * a.oh;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      T4 v;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = static_cast<T>(o[dt][4 * g + u] * inv);
-      if (dt * 32 + 8 * g + 4 * fh < a.dim) *reinterpret_cast<T4*>(to + dt * 32 + 8 * g + 4 * fh) = v;
-    }
+    for (int g = 0; g < 4; ++g)
+      store4<T>(a, w, p, row, dt * 32 + 8 * g + 4 * fh,
+                float4_t{u.o[dt][4 * g], u.o[dt][4 * g + 1], u.o[dt][4 * g + 2], u.o[dt][4 * g + 3]}, u.m, l);
 }
 
-// Waves a SIMD: what the LDS ring leaves room for (32, 48 and 64 KB).
+// One unit of rows and WAVES waves, each with slices of 32 keys of its own (slice t0 + wave, + WAVES, ...) in LDS of its own, so no
+// barrier stands between load and use: a wave asks for the next slice's K once it has read this one's, and for its V likewise, and
+// has 64 KB (128 columns; 8 waves) or 128 KB (16) of the CU's reads in flight. The slices are those of the prefix (w.front), then the
+// sequence's own. The waves' O, m and l are joined through LDS, four columns a wave and turn.
+template <typename T, int DP, int NW>
+__device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w, T* smem) {
+  constexpr int CH = DP / 8, SLICE = 32 * DP, LP = CH / 2, DT = DP / 32, WORDS = 16 * DT + 2;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 31, fh = lane >> 5;
+  T* kbuf = smem + wave * 2 * SLICE;
+  const uint32_t vbuf = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)(kbuf + SLICE)));
+  const int row = w.row0 + fr;
+  const Place p = place_of(a, w, row);
+  Unit<T, DP> u;
+  u.start(a, p, lane);
+
+  const int64_t seq = max(w.seq, 0);
+  const uint8_t* mask = a.mask && w.seq >= 0 ? a.mask + seq * a.mask_b : nullptr;
+  // Loads of a slice: 1 KB each, lane l the chunk l.
+  int lrow[LP];
+  uint32_t coff_k[LP], coff_v[LP];
+#pragma unroll
+  for (int i = 0; i < LP; ++i) {
+    const int n = i * 64 + lane, r = n / CH, slot = n % CH, ck = k_slot<DP>(r, slot), cv = v_slot<DP>(r, slot);
+    lrow[i] = r;
+    coff_k[i] = 8 * ck < a.dim ? 16 * ck : OOB_OFFSET;
+    coff_v[i] = 8 * cv < a.dim ? 16 * cv : OOB_OFFSET;
+  }
+  // own: of the sequence (the prefix's otherwise)
+  struct Slice {
+    bool own;
+    int first, rows;
+    uint32_t word;
+  };
+  auto mask_byte = [&](int n) __attribute__((always_inline)) {
+    const int key = (n - w.front) * 32 + fr;
+    return mask && n < w.t1 && key < w.keys ? mask[key] : uint8_t(0);
+  };
+  auto slice = [&](int n, uint8_t byte) __attribute__((always_inline)) {
+    Slice s;
+    s.own = w.seq >= 0 && n >= w.front;
+    s.first = (s.own ? n - w.front : n) * 32;
+    s.rows = min(32, (s.own ? w.keys : a.prefix.keys) - s.first);
+    s.word = s.rows >= 32 ? ~0u : (1u << s.rows) - 1;
+    if (mask) s.word = static_cast<uint32_t>(__ballot(byte != 0));
+    return s;
+  };
+  auto load = [&](const Slice& s, bool values) __attribute__((always_inline)) {
+    const KeySource& src = s.own ? a.own : a.prefix;
+    const int64_t step = values ? src.vt : src.kt, at = s.own ? seq : 0;
+    const T* base = static_cast<const T*>(values ? src.v : src.k) + at * (values ? src.vb : src.kb) +
+                    w.head * (values ? src.vh : src.kh) + s.first * step;
+    const int bytes = ((s.rows - 1) * static_cast<int>(step) + a.dim) * 2;
+#pragma unroll
+    for (int i = 0; i < LP; ++i) {
+      const uint32_t chunk = values ? coff_v[i] : coff_k[i];
+      const bool in = (s.word >> lrow[i]) & 1;
+      buffer_to_lds(base, bytes, reinterpret_cast<uint8_t*>(kbuf + (values ? SLICE : 0) + i * 512),
+                    in ? chunk + static_cast<uint32_t>(lrow[i] * static_cast<int>(step)) * 2 : OOB_OFFSET);
+    }
+  };
+
+  int n = w.t0 + wave;
+  if (n < w.t1) {
+    Slice now = slice(n, mask_byte(n));
+    uint8_t byte = mask_byte(n + NW);
+    load(now, false);
+    load(now, true);
+    u.settle();
+    for (;;) {
+      const bool more = n + NW < w.t1;
+      Slice next = now;
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LP) : "memory");  // all but V
+      u.score(kbuf, u.koff);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) {
+        next = slice(n + NW, byte);
+        byte = mask_byte(n + 2 * NW);
+        load(next, false);
+      }
+      const int left = now.own ? p.limit - now.first : 32;
+      u.weigh(now.word & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1), fh, n == w.t0 + wave);
+      if (more)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LP) : "memory");  // all but the next K
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      u.template mix<0>(vbuf, u.voff);
+      if (!more) break;
+      load(next, true);
+      now = next;
+      n += NW;
+    }
+  }
+
+  __syncthreads();  // the slices' memory becomes the joint's
+  float* joint = reinterpret_cast<float*>(smem) + lane;
+  const float l_own = u.l + xor_shuffle(u.l, 32);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) joint[(wave * WORDS + dt * 16 + r) * 64] = u.o[dt][r];
+  joint[(wave * WORDS + WORDS - 2) * 64] = u.m;
+  joint[(wave * WORDS + WORDS - 1) * 64] = l_own;
+  __syncthreads();
+  if (row >= w.row_end) return;
+  float top = LOWEST;
+#pragma unroll
+  for (int k = 0; k < NW; ++k) top = fmaxf(top, joint[(k * WORDS + WORDS - 2) * 64]);
+  for (int g = wave; g < 4 * DT; g += NW) {  // words 4 g .. 4 g + 3: columns 32 (g / 4) + 8 (g % 4) + 4 fh + 0..3
+    float4_t o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < NW; ++k) {
+      const float* part = joint + k * WORDS * 64;
+      const float f = __builtin_amdgcn_exp2f(part[(WORDS - 2) * 64] - top);
+      l = __builtin_fmaf(part[(WORDS - 1) * 64], f, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(part[(4 * g + e) * 64], f, o[e]);
+    }
+    store4<T>(a, w, p, row, (g >> 2) * 32 + (g & 3) * 8 + 4 * fh, o, top, l);
+  }
+}
+
+// The arguments' cache lines asked for at once, at the start: each costs a trip of its own where it is first used.
+__device__ __forceinline__ void touch(const CrossArgs& a) {
+  asm volatile("" ::"s"(a.qb), "s"(a.own.k), "s"(a.own.vt), "s"(a.prefix.kt), "s"(a.lens), "s"(a.batch), "s"(a.c));
+}
+
+// LDS of streams and of tiles, and of the joints that follow in the same place.
+constexpr int stream_bytes(int dp, int waves) {
+  const int slices = waves * 2 * 32 * dp * 2, joint = waves * (dp / 2 + 2) * 256;
+  return slices > joint ? slices : joint;
+}
+constexpr int tile_bytes(int dp) { return 4 * BKV * dp * 2 > stream_bytes(dp, WAVES) ? 4 * BKV * dp * 2 : stream_bytes(dp, WAVES); }
+
+// Waves a SIMD: what the LDS leaves room for (34, 50 and 66 KB a workgroup).
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * WAVES, DP == 64 ? 4 : DP == 96 ? 3 : 2) void cross_kernel(const CrossArgs a) {
-  __shared__ __attribute__((aligned(1024))) T smem[4 * BKV * DP];  // K slots, then V slots
+  __shared__ __attribute__((aligned(1024))) T smem[tile_bytes(DP) / 2];  // K slots, then V slots
+  touch(a);
   const int per = a.tokens * a.group, prefix_items = a.prefix_splits * a.kv * a.prefix_tiles;
   int item = static_cast<int>(blockIdx.x);
   Piece w;
-  int split, splits;
-  // Row tiles of one run of keys are neighbours, and neighbours share an XCD's L2; the prefix's pieces are spread over the XCDs
-  // by themselves, as they differ from the others in length.
+  int split, splits, tile, x;
+  // Row tiles of one run of keys are neighbours, and neighbours share an XCD's L2 (the prefix's pieces by themselves, as they
+  // differ from the others in length). A run's last tile, where it has fewer rows and takes less time, comes after all whole ones
+  // and fills the end of the grid.
+  auto place = [&](int n, int tiles, int rows) __attribute__((always_inline)) {
+    const int whole = rows / a.block_rows, runs = n / tiles;
+    if (item < runs * whole) {
+      item = xcd_remap(item, runs * whole);
+      x = item / whole, tile = item - x * whole;
+    } else {
+      x = xcd_remap(item - runs * whole, runs), tile = whole;
+    }
+  };
   if (item < prefix_items) {
-    item = xcd_remap(item, prefix_items);
-    const int x = item / a.prefix_tiles;
+    place(prefix_items, a.prefix_tiles, a.rows);
     split = x % a.prefix_splits, splits = a.prefix_splits;
     w.seq = -1, w.head = x / a.prefix_splits, w.part = split;
-    w.row0 = (item - x * a.prefix_tiles) * a.block_rows, w.row_end = a.rows;
+    w.row0 = tile * a.block_rows, w.row_end = a.rows;
     w.len = w.keys = a.prefix.keys;
   } else {
-    item = xcd_remap(item - prefix_items, static_cast<int>(gridDim.x) - prefix_items);
-    const int x = item / a.own_tiles, y = x / a.own_splits;
+    item -= prefix_items;
+    place(static_cast<int>(gridDim.x) - prefix_items, a.own_tiles, per);
+    const int y = x / a.own_splits;
     split = x - y * a.own_splits, splits = a.own_splits;
     w.seq = y / a.kv, w.head = y - w.seq * a.kv, w.part = a.prefix_splits + split;
-    w.row0 = w.seq * per + (item - x * a.own_tiles) * a.block_rows, w.row_end = (w.seq + 1) * per;
+    w.row0 = w.seq * per + tile * a.block_rows, w.row_end = (w.seq + 1) * per;
     w.len = w.keys = a.lens ? min(max(a.lens[w.seq], 0), a.own.keys) : a.own.keys;
     if (a.causal) {
       const int last = (min(w.row0 + a.block_rows, w.row_end) - 1 - w.seq * per) / a.group;
       w.keys = min(max(w.len - a.tokens + 1 + last, 0), a.own.keys);
     }
   }
-  const int tiles = (w.keys + BKV - 1) / BKV;
-  w.t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / splits);
-  w.t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / splits);
-  const int units = (min(a.block_rows, w.row_end - w.row0) + QW - 1) / QW;
+  const int units = (min(a.block_rows, w.row_end - w.row0) + QW - 1) / QW, step = units == 1 ? 32 : BKV;
+  const int steps = (w.keys + step - 1) / step;
+  w.t0 = static_cast<int>(static_cast<int64_t>(steps) * split / splits);
+  w.t1 = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / splits);
+  w.front = w.seq < 0 ? w.t1 : 0;
   if (units == 1)
-    cross_block<T, DP, 2>(a, w, smem);
+    stream_block<T, DP, WAVES>(a, w, smem);
   else if (units == 2)
-    cross_block<T, DP, 1>(a, w, smem);
+    tile_block<T, DP, 2>(a, w, smem);
   else
-    cross_block<T, DP, 0>(a, w, smem);
+    tile_block<T, DP, 1>(a, w, smem);
 }
 
-// Joins the parts of a row: a thread has 8 columns.
-template <typename T>
+// Up to 32 rows a sequence and key head, and few of these: one workgroup a CU whose waves all read the same rows' keys, the prefix's
+// among them, so that a single launch does where the keys are few enough. Sequences of a head are neighbours: they share the prefix.
+constexpr int stream_waves(int dp) { return 8; }
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * stream_waves(DP), stream_waves(DP) / 4) void stream_kernel(const CrossArgs a) {
+  __shared__ __attribute__((aligned(1024))) T smem[stream_bytes(DP, stream_waves(DP)) / 2];
+  touch(a);
+  const int split = static_cast<int>(blockIdx.z), per = a.tokens * a.group;
+  Piece w;
+  w.seq = static_cast<int>(blockIdx.x), w.head = static_cast<int>(blockIdx.y), w.part = split;
+  w.row0 = w.seq * per, w.row_end = w.row0 + per;
+  w.len = w.keys = a.lens ? min(max(a.lens[w.seq], 0), a.own.keys) : a.own.keys;
+  w.front = (a.prefix.keys + 31) / 32;
+  const int64_t slices = w.front + (w.keys + 31) / 32;
+  w.t0 = static_cast<int>(slices * split / a.own_splits);
+  w.t1 = static_cast<int>(slices * (split + 1) / a.own_splits);
+  stream_block<T, DP, stream_waves(DP)>(a, w, smem);
+}
+
+// Joins the parts of a row: a wave a row, CH lanes for its columns (8 each), 64 / CH lanes for parts, joined at the end.
+template <typename T, int CH>
 __global__ __launch_bounds__(256) void join_kernel(const CrossArgs a) {
-  const int parts = a.prefix_splits + a.own_splits, chunks = a.dim / 8;
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, all = static_cast<int64_t>(a.kv) * a.rows;
-  const int64_t at = n / chunks;
-  const int col = static_cast<int>(n - at * chunks) * 8;
+  constexpr int LANES = 64 / CH;  // parts at a time
+  const int parts = a.prefix_splits + a.own_splits, lane = threadIdx.x & 63, c = lane % CH, first = lane / CH;
+  const int64_t all = static_cast<int64_t>(a.kv) * a.rows, at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (at >= all) return;
-  const float2* ml = reinterpret_cast<const float2*>(a.work + parts * all * a.dim);
+  const float2* ml = reinterpret_cast<const float2*>(a.work + parts * all * a.dim) + at;
   float top = LOWEST;
-  for (int p = 0; p < parts; ++p) top = fmaxf(top, ml[p * all + at].x);
+  for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml[p * all].x);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, xor_shuffle(top, d));
+  const int col = 8 * c < a.dim ? 8 * c : 0;  // lanes past the columns join the first again
+  const float* from = a.work + at * a.dim + col;
+  const int64_t step = all * a.dim;
   float l = 0.f, o[8] = {};
-  for (int p = 0; p < parts; ++p) {
-    const float2 x = ml[p * all + at];
+#pragma unroll 4
+  for (int p = first; p < parts; p += LANES) {
+    const float2 x = ml[p * all];
+    const float4_t u = *reinterpret_cast<const float4_t*>(from + p * step), v = *reinterpret_cast<const float4_t*>(from + p * step + 4);
     const float f = __builtin_amdgcn_exp2f(x.x - top);
-    const float4_t* from = reinterpret_cast<const float4_t*>(a.work + (p * all + at) * a.dim + col);
-    const float4_t u = from[0], v = from[1];
     l = __builtin_fmaf(x.y, f, l);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -423,6 +604,13 @@ __global__ __launch_bounds__(256) void join_kernel(const CrossArgs a) {
       o[e + 4] = __builtin_fmaf(v[e], f, o[e + 4]);
     }
   }
+#pragma unroll
+  for (int d = CH; d < 64; d <<= 1) {
+    l = l + xor_shuffle(l, d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = o[e] + xor_shuffle(o[e], d);
+  }
+  if (first != 0 || 8 * c >= a.dim) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   vec8_t<T> y;
 #pragma unroll
@@ -435,29 +623,35 @@ __global__ __launch_bounds__(256) void join_kernel(const CrossArgs a) {
 }
 
 template <typename T, int DP>
-static void launch_cross(const CrossArgs& a, int64_t blocks, hipStream_t st) {
-  cross_kernel<T, DP><<<dim3(static_cast<unsigned>(blocks)), 64 * WAVES, 0, st>>>(a);
+static void launch_cross(const CrossArgs& a, int64_t blocks, bool stream, hipStream_t st) {
+  if (stream)
+    stream_kernel<T, DP><<<dim3(a.batch, a.kv, a.own_splits), 64 * stream_waves(DP), 0, st>>>(a);
+  else
+    cross_kernel<T, DP><<<dim3(static_cast<unsigned>(blocks)), 64 * WAVES, 0, st>>>(a);
   if (!a.work) return;
-  const int64_t threads = static_cast<int64_t>(a.kv) * a.rows * (a.dim / 8);
-  join_kernel<T><<<dim3(static_cast<unsigned>((threads + 255) / 256)), 256, 0, st>>>(a);
+  const int64_t rows = static_cast<int64_t>(a.kv) * a.rows;
+  join_kernel<T, DP == 64 ? 8 : 16><<<dim3(static_cast<unsigned>((rows + 3) / 4)), 256, 0, st>>>(a);
 }
 
 template <typename T>
-static void launch_cross_dim(const CrossArgs& a, int64_t blocks, hipStream_t st) {
+static void launch_cross_dim(const CrossArgs& a, int64_t blocks, bool stream, hipStream_t st) {
   if (a.dim <= 64)
-    launch_cross<T, 64>(a, blocks, st);
+    launch_cross<T, 64>(a, blocks, stream, st);
   else if (a.dim <= 96)
-    launch_cross<T, 96>(a, blocks, st);
+    launch_cross<T, 96>(a, blocks, stream, st);
   else
-    launch_cross<T, 128>(a, blocks, st);
+    launch_cross<T, 128>(a, blocks, stream, st);
 }
 
 // How rows and keys are cut, from the sizes alone (the workspace's size follows from it).
 struct Plan {
+  bool stream;  // stream_kernel
   int64_t block_rows, own_tiles, own_splits, prefix_tiles, prefix_splits, parts, blocks;
 };
 
-constexpr int64_t WANT = 512;  // workgroups that fill the 256 CUs
+constexpr int64_t CUS = 256;
+constexpr int64_t WANT = 2 * CUS;             // workgroups of cross_kernel that fill the chip
+constexpr int64_t ONE_GO = int64_t(1) << 20;  // bytes of keys and values that a workgroup reads before cutting them pays
 
 static int64_t split_keys(int64_t blocks, int64_t keys) {
   const int64_t tiles = (keys + BKV - 1) / BKV;
@@ -465,18 +659,28 @@ static int64_t split_keys(int64_t blocks, int64_t keys) {
 }
 
 // prefix < 0: none
-static Plan plan_of(int64_t batch, int64_t tokens, int64_t keys, int64_t prefix, int64_t kv, int64_t group) {
+static Plan plan_of(int64_t batch, int64_t tokens, int64_t keys, int64_t prefix, int64_t kv, int64_t group, int64_t D) {
   Plan p{};
-  const int64_t per = tokens * group, rows = batch * per, most = prefix >= 0 ? rows : per;
+  const int64_t per = tokens * group, rows = batch * per, runs = batch * kv, all = keys + std::max<int64_t>(prefix, 0);
+  const bool cut = all * D * 4 > ONE_GO;
+  if (per <= QW && runs <= CUS && (prefix <= 0 || batch == 1 || !cut)) {
+    p.stream = true;
+    p.block_rows = QW;
+    p.own_tiles = 1;
+    p.parts = p.own_splits = cut ? std::max<int64_t>(1, std::min(CUS / std::max<int64_t>(runs, 1), all / 512)) : 1;
+    p.blocks = runs * p.own_splits;
+    return p;
+  }
+  const int64_t most = prefix >= 0 ? rows : per;
   p.block_rows = most <= QW ? QW : most <= 2 * QW ? 2 * QW : 4 * QW;
   p.own_tiles = (per + p.block_rows - 1) / p.block_rows;
-  p.own_splits = split_keys(p.own_tiles * batch * kv, keys);
+  p.own_splits = split_keys(p.own_tiles * runs, keys);
   if (prefix >= 0) {
     p.prefix_tiles = (rows + p.block_rows - 1) / p.block_rows;
     p.prefix_splits = split_keys(p.prefix_tiles * kv, prefix);
   }
   p.parts = p.own_splits + p.prefix_splits;
-  p.blocks = p.own_tiles * batch * kv * p.own_splits + p.prefix_tiles * kv * p.prefix_splits;
+  p.blocks = p.own_tiles * runs * p.own_splits + p.prefix_tiles * kv * p.prefix_splits;
   return p;
 }
 
@@ -495,6 +699,12 @@ struct Rows {
   const void* p;
   int64_t n[3], stride[3];
 };
+
+// A dimension of one row has no stride.
+Rows plain(Rows r) {
+  for (int d = 0; d < 3; ++d) r.stride[d] = r.n[d] > 1 ? r.stride[d] : 0;
+  return r;
+}
 
 // Sorts the dimensions that have several rows at a pitch, in bytes, from the smallest up.
 int pitches(const Rows& r, int64_t (&n)[3], int64_t (&pitch)[3]) {
@@ -540,8 +750,9 @@ bool misaligned(const Rows& r, uint64_t bytes) {
 
 bool negative(const Rows& r) { return r.stride[0] < 0 || r.stride[1] < 0 || r.stride[2] < 0; }
 
-// Sizes that both entries share; null if they are taken.
-const char* bad_sizes(int64_t batch, int64_t tokens, int64_t keys, int64_t prefix, int64_t heads, int64_t kv, int64_t D) {
+// Sizes that both entries share: null and the plan if they are taken.
+const char* bad_sizes(int64_t batch, int64_t tokens, int64_t keys, int64_t prefix, int64_t heads, int64_t kv, int64_t D,
+                      Plan& p) {
   if (D <= 0 || D % 8 != 0 || D > 128) return "heads must be a multiple of 8 columns, at most 128";
   if (heads <= 0 || kv <= 0 || heads > 65535 || heads % kv != 0)
     return "need 0 < heads <= 65535, a multiple of kv_heads > 0";
@@ -550,19 +761,20 @@ const char* bad_sizes(int64_t batch, int64_t tokens, int64_t keys, int64_t prefi
   if (keys > 0x7fffff00 || prefix > 0x7fffff00) return "need fewer than 2^31 - 255 keys";
   if (batch != 0 && tokens != 0 && (tokens > 0x7fffffff / batch || batch * tokens > 0x7fffffff / heads))
     return "need batch * tokens * heads < 2^31";
-  const Plan p = plan_of(batch, tokens, keys, prefix, kv, heads / kv);
-  if (p.blocks >= (int64_t(1) << 24) || (p.parts > 1 && batch * tokens * heads * (D / 8) > 0xffffff00LL))
+  p = plan_of(batch, tokens, keys, prefix, kv, heads / kv, D);
+  if (p.blocks >= (int64_t(1) << 24) || (p.parts > 1 && batch * tokens * heads > (1 << 26) - 4))
     return "too many rows for one launch";
   return nullptr;
 }
 
-int attend(const std::string& name, const Rows& q, const Rows& k, const Rows& v, const Rows* pk, const Rows* pv, const Rows& out,
+int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const Rows* pk, const Rows* pv, const Rows& out,
            int dtype, int64_t D, float scale, const int32_t* lens, const uint8_t* mask, int64_t mask_batch, float* work,
            int64_t work_size, void* stream) {
-  auto bad = [&](const char* msg) { return fail(FF_EINVAL, name + ": " + msg); };
+  auto bad = [&](const char* msg) { return fail(FF_EINVAL, std::string(name) + ": " + msg); };
   const int64_t batch = q.n[0], tokens = q.n[1], heads = q.n[2], keys = k.n[1], kv = k.n[2], prefix = pk ? pk->n[1] : -1;
   if (dtype != FF_F16 && dtype != FF_BF16) return bad("q, k, v and out must be fp16 or bf16");
-  if (const char* msg = bad_sizes(batch, tokens, keys, prefix, heads, kv, D)) return bad(msg);
+  Plan p;
+  if (const char* msg = bad_sizes(batch, tokens, keys, prefix, heads, kv, D, p)) return bad(msg);
   if (!(scale > 0.f) || !std::isfinite(scale)) return bad("scale must be finite and > 0");
   if (batch == 0 || tokens == 0) return FF_OK;
   const Rows* given[6] = {&q, &k, &v, pk, pv, &out};
@@ -575,8 +787,7 @@ int attend(const std::string& name, const Rows& q, const Rows& k, const Rows& v,
   }
   for (const Rows* r : {&k, &v, pk, pv})
     if (r && r->n[1] > 1 && r->stride[1] >= (1 << 24)) return bad("tokens of k and v must be fewer than 2^24 elements apart");
-  if (mask_batch < 0) return bad("strides must not be negative");
-  const Plan p = plan_of(batch, tokens, keys, prefix, kv, heads / kv);
+  if (mask_batch < 0) return bad("strides must not be negative");  // a batch of one: index 0 alone
   const int64_t need = work_of(p, batch, tokens, heads, D);
   if (need > 0 && (!work || work_size < need)) return bad("the workspace is too small");
   if ((reinterpret_cast<uintptr_t>(work) & 15) || (reinterpret_cast<uintptr_t>(lens) & 3)) return bad("misaligned pointer");
@@ -611,23 +822,23 @@ int attend(const std::string& name, const Rows& q, const Rows& k, const Rows& v,
   a.prefix_splits = static_cast<int>(p.prefix_splits);
   a.c = scale * 1.4426950408889634f;
   if (dtype == FF_F16)
-    launch_cross_dim<half_t>(a, p.blocks, as_stream(stream));
+    launch_cross_dim<half_t>(a, p.blocks, p.stream, as_stream(stream));
   else
-    launch_cross_dim<bf16_t>(a, p.blocks, as_stream(stream));
-  return check_launch(name.c_str());
+    launch_cross_dim<bf16_t>(a, p.blocks, p.stream, as_stream(stream));
+  return check_launch(name);
 }
 
 }  // namespace
 
 extern "C" int64_t ff_cross_attention_work(int64_t B, int64_t L, int64_t S, int64_t heads, int64_t kv_heads, int64_t D) {
-  if (bad_sizes(B, L, S, -1, heads, kv_heads, D)) return 0;
-  return work_of(plan_of(B, L, S, -1, kv_heads, heads / kv_heads), B, L, heads, D);
+  Plan p;
+  return bad_sizes(B, L, S, -1, heads, kv_heads, D, p) ? 0 : work_of(p, B, L, heads, D);
 }
 
 extern "C" int64_t ff_prefix_attention_work(int64_t B, int64_t L, int64_t P, int64_t S, int64_t heads, int64_t kv_heads,
                                             int64_t D) {
-  if (P < 0 || bad_sizes(B, L, S, P, heads, kv_heads, D)) return 0;
-  return work_of(plan_of(B, L, S, P, kv_heads, heads / kv_heads), B, L, heads, D);
+  Plan p;
+  return P < 0 || bad_sizes(B, L, S, P, heads, kv_heads, D, p) ? 0 : work_of(p, B, L, heads, D);
 }
 
 extern "C" int ff_cross_attention(const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* k,
@@ -637,9 +848,10 @@ extern "C" int ff_cross_attention(const void* q, int64_t q_batch, int64_t q_toke
                                   int64_t kv_heads, int64_t D, float scale, const int32_t* lens, const uint8_t* mask,
                                   int64_t mask_batch, float* work, int64_t work_size, void* stream) {
   clear_error();
-  return attend("cross_attention", {q, {B, L, heads}, {q_batch, q_token, q_head}},
-                {k, {B, S, kv_heads}, {k_batch, k_token, k_head}}, {v, {B, S, kv_heads}, {v_batch, v_token, v_head}}, nullptr,
-                nullptr, {out, {B, L, heads}, {o_batch, o_token, o_head}}, dtype, D, scale, lens, mask, mask_batch, work,
+  return attend("cross_attention", plain({q, {B, L, heads}, {q_batch, q_token, q_head}}),
+                plain({k, {B, S, kv_heads}, {k_batch, k_token, k_head}}),
+                plain({v, {B, S, kv_heads}, {v_batch, v_token, v_head}}), nullptr, nullptr,
+                plain({out, {B, L, heads}, {o_batch, o_token, o_head}}), dtype, D, scale, lens, mask, mask_batch, work,
                 work_size, stream);
 }
 
@@ -652,9 +864,11 @@ extern "C" int ff_prefix_attention(const void* q, int64_t q_batch, int64_t q_tok
                                    const int32_t* lens, float* work, int64_t work_size, void* stream) {
   clear_error();
   if (P < 0) return fail(FF_EINVAL, "prefix_attention: sizes must not be negative, nor reach 2^31");
-  const Rows pk{prefix_k, {1, P, kv_heads}, {0, pk_token, pk_head}}, pv{prefix_v, {1, P, kv_heads}, {0, pv_token, pv_head}};
-  return attend("prefix_attention", {q, {B, L, heads}, {q_batch, q_token, q_head}},
-                {k, {B, S, kv_heads}, {k_batch, k_token, k_head}}, {v, {B, S, kv_heads}, {v_batch, v_token, v_head}}, &pk,
-                &pv, {out, {B, L, heads}, {o_batch, o_token, o_head}}, dtype, D, scale, lens, nullptr, 0, work, work_size,
+  const Rows pk = plain({prefix_k, {1, P, kv_heads}, {0, pk_token, pk_head}});
+  const Rows pv = plain({prefix_v, {1, P, kv_heads}, {0, pv_token, pv_head}});
+  return attend("prefix_attention", plain({q, {B, L, heads}, {q_batch, q_token, q_head}}),
+                plain({k, {B, S, kv_heads}, {k_batch, k_token, k_head}}),
+                plain({v, {B, S, kv_heads}, {v_batch, v_token, v_head}}), &pk, &pv,
+                plain({out, {B, L, heads}, {o_batch, o_token, o_head}}), dtype, D, scale, lens, nullptr, 0, work, work_size,
                 stream);
 }

@@ -10,6 +10,7 @@
 // waves leaves each wave's sum and squares about its own mean in LDS and every wave joins them (counts and means known, no
 // cancellation), one barrier a norm.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -20,7 +21,7 @@ struct ResidualArgs {
   void *x_out, *h;
   int64_t xs, ys, os, hs;  // row strides in elements
   const float *post_g, *post_b, *pre_g, *pre_b;
-  int rows, width, per_gate, post, pre, gate_f32;  // per_gate: rows that share a gate row
+  int rows, width, per_gate, gate_f32;  // per_gate: rows that share a gate row
   float scale, eps;
 };
 
@@ -41,7 +42,7 @@ __device__ __forceinline__ float inv_root(float v) {
   return v < 0x1p-126f ? __builtin_amdgcn_rsqf(v * 0x1p24f) * 0x1p12f : __builtin_amdgcn_rsqf(v);
 }
 
-template <typename T, int LANES, int CHUNKS>
+template <typename T, int LANES, int CHUNKS, int POST, int PRE>
 __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kernel(const ResidualArgs a) {
   constexpr int THREADS = LANES <= 64 ? 256 : LANES, GROUPS = THREADS / LANES, WIDTH = LANES < 64 ? LANES : 64;
   constexpr int WPR = LANES / WIDTH;  // waves a row
@@ -61,8 +62,31 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kerne
   }
   const float inv_n = 1.f / static_cast<float>(a.width);
 
-  auto param = [&](const float* p, int i, int e) __attribute__((always_inline)) { return p ? p[col[i] + e] : 0.f; };
+  // columns of wave w of the row
+  auto columns = [&](int w) __attribute__((always_inline)) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) n += min(max(a.width - 8 * (i * LANES + w * 64), 0), 512);
+    return n;
+  };
+  const int mine = WPR > 1 ? columns(wave) : a.width;
+  const float own = mine ? 1.f / static_cast<float>(mine) : 0.f;
+
   float post_g[CHUNKS][8], post_b[CHUNKS][8], pre_g[CHUNKS][8], pre_b[CHUNKS][8], factor[CHUNKS][8];
+  // The compiler's wait for these loads stands here, before the loop: in it, the same counter holds the next row's loads.
+  auto settle = [](float (&k)[CHUNKS][8]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(k[i][e]));
+  };
+  auto keep = [&](const float* p, float (&k)[CHUNKS][8]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) k[i][e] = p[col[i] + e];
+    settle(k);
+  };
   auto gate_at = [&](int64_t r, int i, float (&f)[8]) __attribute__((always_inline)) {
     if (a.gate_f32) {
       const float* g = static_cast<const float*>(a.gate) + r * a.width + col[i];
@@ -82,69 +106,59 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kerne
 #pragma unroll
     for (int e = 0; e < 8; ++e) factor[i][e] = a.scale;
     if (a.gate && !gate_moves) gate_at(0, i, factor[i]);
-    if constexpr (KEEP)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        post_g[i][e] = param(a.post_g, i, e), post_b[i][e] = param(a.post_b, i, e);
-        pre_g[i][e] = param(a.pre_g, i, e), pre_b[i][e] = param(a.pre_b, i, e);
-      }
   }
+  settle(factor);
+  if constexpr (KEEP && POST != FF_NORM_NONE) keep(a.post_g, post_g);
+  if constexpr (KEEP && POST == FF_NORM_LAYER) keep(a.post_b, post_b);
+  if constexpr (KEEP && PRE != FF_NORM_NONE) keep(a.pre_g, pre_g);
+  if constexpr (KEEP && PRE == FF_NORM_LAYER) keep(a.pre_b, pre_b);
 
-  int turn = 0;
-  // The norm of v in its place.
-  auto norm = [&](float (&v)[CHUNKS][8], int kind, const float* g, const float* b, float (&kg)[CHUNKS][8],
-                  float (&kb)[CHUNKS][8]) __attribute__((always_inline)) {
-    const bool centred = kind == FF_NORM_LAYER;
-    float mean = 0.f;
-    if (centred) {
+  // Sum over the wave's lanes and chunks of f(chunk's values); chunks past the row count for nothing, whatever they hold.
+  auto sum_of = [&](float (&v)[CHUNKS][8], auto f) __attribute__((always_inline)) {
+    float all = 0.f;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < CHUNKS; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s = s + v[i][e];
-      mean = lanes_sum<WIDTH>(s);  // the wave's sum
+      for (int e = 0; e < 8; ++e) s = f(s, v[i][e]);
+      all = all + (in[i] ? s : 0.f);
     }
-    float own = inv_n;  // 1 / columns of the wave
-    int columns = 0;
-    if constexpr (WPR > 1) {
-#pragma unroll
-      for (int i = 0; i < CHUNKS; ++i)
-        columns += min(max(a.width - 8 * (i * LANES + wave * 64), 0), 512);
-      own = columns ? 1.f / static_cast<float>(columns) : 0.f;
+    return lanes_sum<WIDTH>(all);
+  };
+  int turn = 0;
+  // The norm of v in its place.
+  auto norm = [&](float (&v)[CHUNKS][8], auto kind, const float* g, const float* b, float (&kg)[CHUNKS][8],
+                  float (&kb)[CHUNKS][8]) __attribute__((always_inline)) {
+    constexpr bool CENTRED = decltype(kind)::value == FF_NORM_LAYER;
+    float sum = 0.f, centre = 0.f;
+    if constexpr (CENTRED) {
+      sum = sum_of(v, [](float s, float x) { return s + x; });
+      centre = sum * own;
     }
-    const float about = centred ? mean * own : 0.f;
-    float sq = 0.f;
-#pragma unroll
-    for (int i = 0; i < CHUNKS; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float d = in[i] ? v[i][e] - about : 0.f;
-        sq = __builtin_fmaf(d, d, sq);
-      }
-    sq = lanes_sum<WIDTH>(sq);
-    float centre = about;
+    float sq = sum_of(v, [centre](float s, float x) {
+      const float d = CENTRED ? x - centre : x;
+      return __builtin_fmaf(d, d, s);
+    });
     if constexpr (WPR > 1) {
-      if (threadIdx.x % 64 == 0) joint[turn][wave] = float2{mean, sq};
+      if (threadIdx.x % 64 == 0) joint[turn][wave] = float2{sum, sq};
       __syncthreads();
-      float all = 0.f, squares = 0.f;
-      if (centred) {
+      if constexpr (CENTRED) {
+        float all = 0.f;
 #pragma unroll
         for (int w = 0; w < WPR; ++w) all = all + joint[turn][w].x;
         centre = all * inv_n;
       }
+      sq = 0.f;
 #pragma unroll
       for (int w = 0; w < WPR; ++w) {
         const float2 j = joint[turn][w];
-        squares = squares + j.y;
-        if (centred) {
-          int n = 0;
-#pragma unroll
-          for (int i = 0; i < CHUNKS; ++i) n += min(max(a.width - 8 * (i * LANES + w * 64), 0), 512);
-          const float d = n ? j.x * (1.f / static_cast<float>(n)) - centre : 0.f;
-          squares = __builtin_fmaf(static_cast<float>(n) * d, d, squares);
+        sq = sq + j.y;
+        if constexpr (CENTRED) {
+          const int n = columns(w);
+          const float d = n ? j.x * __builtin_amdgcn_rcpf(static_cast<float>(n)) - centre : 0.f;
+          sq = __builtin_fmaf(static_cast<float>(n) * d, d, sq);
         }
       }
-      sq = squares;
       turn ^= 1;  // the next norm writes the other one: its barrier lies between the reads here and the next write
     }
     const float r = inv_root(__builtin_fmaf(sq, inv_n, a.eps));
@@ -153,7 +167,7 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kerne
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float gamma = KEEP ? kg[i][e] : g[col[i] + e];
-        if (centred)
+        if constexpr (CENTRED)
           v[i][e] = __builtin_fmaf((v[i][e] - centre) * r, gamma, KEEP ? kb[i][e] : b[col[i] + e]);
         else
           v[i][e] = v[i][e] * r * gamma;
@@ -177,8 +191,8 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kerne
     for (int i = 0; i < CHUNKS; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        v[i][e] = in[i] ? static_cast<float>(ny[i][e]) : 0.f;
-        s[i][e] = in[i] ? static_cast<float>(nx[i][e]) : 0.f;
+        v[i][e] = static_cast<float>(ny[i][e]);
+        s[i][e] = static_cast<float>(nx[i][e]);
       }
     if (gate_moves)
 #pragma unroll
@@ -189,20 +203,20 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kerne
       row += step;
       load(row);
     }
-    if (a.post != FF_NORM_NONE) norm(v, a.post, a.post_g, a.post_b, post_g, post_b);
+    if constexpr (POST != FF_NORM_NONE) norm(v, std::integral_constant<int, POST>{}, a.post_g, a.post_b, post_g, post_b);
 #pragma unroll
     for (int i = 0; i < CHUNKS; ++i) {
       T8 w;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        s[i][e] = in[i] ? __builtin_fmaf(v[i][e], factor[i][e], s[i][e]) : 0.f;
+        s[i][e] = __builtin_fmaf(v[i][e], factor[i][e], s[i][e]);
         w[e] = static_cast<T>(s[i][e]);
       }
       if (in[i])
         __builtin_nontemporal_store(__builtin_bit_cast(int4_t, w), reinterpret_cast<int4_t*>(xo + at * a.os + col[i]));
     }
-    if (a.pre != FF_NORM_NONE) {
-      norm(s, a.pre, a.pre_g, a.pre_b, pre_g, pre_b);
+    if constexpr (PRE != FF_NORM_NONE) {
+      norm(s, std::integral_constant<int, PRE>{}, a.pre_g, a.pre_b, pre_g, pre_b);
 #pragma unroll
       for (int i = 0; i < CHUNKS; ++i) {
         T8 w;
@@ -216,33 +230,51 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kerne
   }
 }
 
-template <typename T, int LANES, int CHUNKS>
+template <typename T, int LANES, int CHUNKS, int POST, int PRE>
 static void launch_residual(const ResidualArgs& a, hipStream_t st) {
   constexpr int THREADS = LANES <= 64 ? 256 : LANES, GROUPS = THREADS / LANES;
-  int64_t cap = resident_blocks(reinterpret_cast<const void*>(&residual_norm_kernel<T, LANES, CHUNKS>), THREADS, 0);
+  int64_t cap = resident_blocks(reinterpret_cast<const void*>(&residual_norm_kernel<T, LANES, CHUNKS, POST, PRE>), THREADS, 0);
   if (cap <= 0) cap = 512;
   const int64_t blocks = std::min<int64_t>((a.rows + GROUPS - 1) / GROUPS, cap);
-  residual_norm_kernel<T, LANES, CHUNKS><<<dim3(static_cast<unsigned>(blocks)), THREADS, 0, st>>>(a);
+  residual_norm_kernel<T, LANES, CHUNKS, POST, PRE><<<dim3(static_cast<unsigned>(blocks)), THREADS, 0, st>>>(a);
+}
+
+template <typename T, int POST, int PRE>
+static void launch_residual_width(const ResidualArgs& a, hipStream_t st) {
+  if (a.width <= 128)
+    launch_residual<T, 16, 1, POST, PRE>(a, st);
+  else if (a.width <= 256)
+    launch_residual<T, 16, 2, POST, PRE>(a, st);
+  else if (a.width <= 512)
+    launch_residual<T, 32, 2, POST, PRE>(a, st);
+  else if (a.width <= 1024)
+    launch_residual<T, 64, 2, POST, PRE>(a, st);
+  else if (a.width <= 2048)
+    launch_residual<T, 128, 2, POST, PRE>(a, st);
+  else if (a.width <= 4096)
+    launch_residual<T, 256, 2, POST, PRE>(a, st);
+  else if (a.width <= 8192)
+    launch_residual<T, 512, 2, POST, PRE>(a, st);
+  else
+    launch_residual<T, 512, 4, POST, PRE>(a, st);
+}
+
+template <typename T, int POST>
+static void launch_residual_pre(const ResidualArgs& a, int pre, hipStream_t st) {
+  switch (pre) {
+    case FF_NORM_RMS: return launch_residual_width<T, POST, FF_NORM_RMS>(a, st);
+    case FF_NORM_LAYER: return launch_residual_width<T, POST, FF_NORM_LAYER>(a, st);
+    default: return launch_residual_width<T, POST, FF_NORM_NONE>(a, st);
+  }
 }
 
 template <typename T>
-static void launch_residual_width(const ResidualArgs& a, hipStream_t st) {
-  if (a.width <= 128)
-    launch_residual<T, 16, 1>(a, st);
-  else if (a.width <= 256)
-    launch_residual<T, 16, 2>(a, st);
-  else if (a.width <= 512)
-    launch_residual<T, 32, 2>(a, st);
-  else if (a.width <= 1024)
-    launch_residual<T, 64, 2>(a, st);
-  else if (a.width <= 2048)
-    launch_residual<T, 128, 2>(a, st);
-  else if (a.width <= 4096)
-    launch_residual<T, 256, 2>(a, st);
-  else if (a.width <= 8192)
-    launch_residual<T, 512, 2>(a, st);
-  else
-    launch_residual<T, 512, 4>(a, st);
+static void launch_residual_norms(const ResidualArgs& a, int post, int pre, hipStream_t st) {
+  switch (post) {
+    case FF_NORM_RMS: return launch_residual_pre<T, FF_NORM_RMS>(a, pre, st);
+    case FF_NORM_LAYER: return launch_residual_pre<T, FF_NORM_LAYER>(a, pre, st);
+    default: return launch_residual_pre<T, FF_NORM_NONE>(a, pre, st);
+  }
 }
 
 }  // namespace ff
@@ -301,11 +333,11 @@ extern "C" int ff_residual_norm(const void* x, int64_t x_row, const void* y, int
     return fail(FF_EINVAL, "residual_norm: an output overlaps the other one or what is read (x or y, with its stride, may be in "
                            "its place)");
   const ResidualArgs a{x, y, gate, x_out, h, x_row, y_row, xo_row, h_row, post_gamma, post_beta, pre_gamma, pre_beta,
-                       static_cast<int>(T), static_cast<int>(C), gate ? static_cast<int>(T / gate_rows) : 1, post, pre,
-                       gate_dtype == FF_F32, scale, eps};
+                       static_cast<int>(T), static_cast<int>(C), gate ? static_cast<int>(T / gate_rows) : 1, gate_dtype == FF_F32,
+                       scale, eps};
   if (dtype == FF_F16)
-    launch_residual_width<half_t>(a, as_stream(stream));
+    launch_residual_norms<half_t>(a, post, pre, as_stream(stream));
   else
-    launch_residual_width<bf16_t>(a, as_stream(stream));
+    launch_residual_norms<bf16_t>(a, post, pre, as_stream(stream));
   return check_launch("residual_norm");
 }

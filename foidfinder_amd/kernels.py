@@ -618,48 +618,35 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: t
          2 * half, pairs, _ptr(positions), pos64, q_scale)
 
 
-def _rows4(x: torch.Tensor, name: str) -> tuple:
-    """Address and strides (batch, token, head) of [B, L, heads, D] with contiguous columns; a dimension of one has none."""
-    shape = x.shape
-    if len(shape) != 4:
-        raise RuntimeError(f"{name} must be [B, L, heads, D]")
-    (b, n, h, _), (sb, sn, sh, one) = shape, x.stride()
-    if one != 1 and x.numel():
-        raise RuntimeError(f"{name} must have contiguous columns")
-    return x.data_ptr(), sb if b > 1 else 0, sn if n > 1 else 0, sh if h > 1 else 0
-
-
-def _scratch(work: torch.Tensor | None, dev: int) -> tuple:
-    if work is None:
-        return None, 0
-    if work.dtype != torch.float32 or work.get_device() != dev or not work.is_contiguous():
-        raise RuntimeError("work must be contiguous fp32 on the queries' GPU")
-    return work.data_ptr(), work.numel()
-
-
-def _lens(lens: torch.Tensor | None, B: int, dev: int) -> int | None:
-    if lens is None:
-        return None
-    if lens.dtype != torch.int32 or lens.shape != (B,) or lens.get_device() != dev or not lens.is_contiguous():
-        raise RuntimeError(f"lens must be contiguous int32 {(B,)} on the queries' GPU")
-    return lens.data_ptr()
-
-
-def _attended(q: torch.Tensor, out: torch.Tensor, *kv: torch.Tensor) -> int:
-    """The device of queries, keys, values and the output, which agree in type, head width and the output's shape."""
-    dt, dev, D = q.dtype, q.get_device(), q.size(-1)
+def _attended(q: torch.Tensor, out: torch.Tensor, lens: torch.Tensor | None, work: torch.Tensor | None,
+              *kv: torch.Tensor) -> int:
+    """The device of an attention's tensors, which agree in type, device and head width; the last two are keys and values
+    [B, S, kv_heads, D] of q's batch."""
+    shape, dt, dev = q.shape, q.dtype, q.get_device()
     if dev < 0:
         raise RuntimeError("foidfinder_rocm ops take GPU tensors")
-    if dt not in _HALVES or out.dtype != dt or out.shape != q.shape:
-        raise RuntimeError("q and out must be fp16 or bf16, of one type and shape")
-    if out.get_device() != dev:
-        raise RuntimeError("all tensors must be on one device")
-    for i, t in enumerate(kv):
-        if t.dtype != dt or t.size(-1) != D or t.shape != kv[i & ~1].shape:
-            raise RuntimeError("keys and values must have q's type and head width, and each other's shape")
-        if t.get_device() != dev:
-            raise RuntimeError("all tensors must be on one device")
+    if len(shape) != 4 or dt not in _HALVES or out.dtype != dt or out.shape != shape or out.get_device() != dev:
+        raise RuntimeError("q and out must be fp16 or bf16 [B, L, heads, D], of one type and shape on one device")
+    for t in kv:
+        if t.dtype != dt or t.get_device() != dev:
+            raise RuntimeError("keys and values must have q's type and device")
+    B, _, _, D = shape
+    kshape = kv[-2].shape
+    if len(kshape) != 4 or kshape[0] != B or kshape[3] != D or kv[-1].shape != kshape:
+        raise RuntimeError("keys and values must be [B, S, kv_heads, D] with q's B and D, and of one shape")
+    if lens is not None and (lens.dtype != torch.int32 or lens.shape != (B,) or lens.get_device() != dev
+                             or not lens.is_contiguous()):
+        raise RuntimeError(f"lens must be contiguous int32 {(B,)} on the queries' GPU")
+    if work is not None and (work.dtype != torch.float32 or work.get_device() != dev or not work.is_contiguous()):
+        raise RuntimeError("work must be contiguous fp32 on the queries' GPU")
     return dev
+
+
+def _columns(ones: tuple, *ts: torch.Tensor) -> None:
+    """Refuses rows with a column stride other than 1 (no rows, no stride)."""
+    for one, t in zip(ones, ts):
+        if one != 1 and t.numel():
+            raise RuntimeError("q, keys, values and out must have contiguous columns")
 
 
 def cross_attention_work(q: torch.Tensor, k: torch.Tensor) -> int:
@@ -678,11 +665,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
     columns) are not read; a query without keys gives zeros. work: fp32 of at least cross_attention_work(q, k) elements; calls
     that run one after another may share it. out and work share no memory with each other or with what is read (refused)."""
     _no_grad(q, k, v, out, work)
-    dev = _attended(q, out, k, v)
-    qr, kr, vr, to = _rows4(q, "q"), _rows4(k, "k"), _rows4(v, "v"), _rows4(out, "out")
-    (B, L, H, D), (KB, S, KV, _) = q.shape, k.shape
-    if KB != B:
-        raise RuntimeError("q and k must share the batch")
+    dev = _attended(q, out, lens, work, k, v)
+    (qb, qt, qh, q1), (kb, kt, kh, k1), (vb, vt, vh, v1), (ob, ot, oh, o1) = q.stride(), k.stride(), v.stride(), out.stride()
+    if not q1 == k1 == v1 == o1 == 1:
+        _columns((q1, k1, v1, o1), q, k, v, out)
+    (B, L, H, D), (_, S, KV, _) = q.shape, k.shape
     mp, mb = None, 0
     if mask is not None:
         if mask.dtype != torch.bool or mask.shape != (B, S) or mask.get_device() != dev:
@@ -690,9 +677,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
         mb, one = mask.stride()
         if one != 1 and S > 1:
             raise RuntimeError("mask must have contiguous columns")
-        mp, mb = mask.data_ptr(), mb if B > 1 else 0
-    _run("ff_cross_attention", dev, *qr, *kr, *vr, *to, _DTYPES[q.dtype], B, L, S, H, KV, D, scale, _lens(lens, B, dev), mp,
-         mb, *_scratch(work, dev))
+        mp = mask.data_ptr()
+    _run("ff_cross_attention", dev, q.data_ptr(), qb, qt, qh, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh,
+         out.data_ptr(), ob, ot, oh, _DTYPES[q.dtype], B, L, S, H, KV, D, scale, None if lens is None else lens.data_ptr(), mp,
+         mb, None if work is None else work.data_ptr(), 0 if work is None else work.numel())
 
 
 def prefix_attention_work(q: torch.Tensor, prefix_k: torch.Tensor, k: torch.Tensor) -> int:
@@ -710,20 +698,20 @@ def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Te
     last. Query i sees the prefix and the own keys j < lens[b] - L + 1 + i. Types, strides and work (at least
     prefix_attention_work(q, prefix_k, k) elements) as in cross_attention."""
     _no_grad(q, prefix_k, prefix_v, k, v, out, work)
-    dev = _attended(q, out, prefix_k, prefix_v, k, v)
-    qr, kr, vr, to = _rows4(q, "q"), _rows4(k, "k"), _rows4(v, "v"), _rows4(out, "out")
-    (B, L, H, D), (KB, S, KV, _) = q.shape, k.shape
-    if KB != B or len(prefix_k.shape) != 3 or prefix_k.size(1) != KV:
-        raise RuntimeError("q and k must share the batch, and the prefix must be [P, kv_heads, D]")
-    P = prefix_k.size(0)
-    shared = []
-    for t in (prefix_k, prefix_v):
-        st, sh, one = t.stride()
-        if one != 1 and P:
-            raise RuntimeError("the prefix must have contiguous columns")
-        shared += t.data_ptr(), st if P > 1 else 0, sh if KV > 1 else 0
-    _run("ff_prefix_attention", dev, *qr, *shared, *kr, *vr, *to, _DTYPES[q.dtype], B, L, P, S, H, KV, D, scale,
-         _lens(lens, B, dev), *_scratch(work, dev))
+    dev = _attended(q, out, lens, work, prefix_k, prefix_v, k, v)
+    (qb, qt, qh, q1), (kb, kt, kh, k1), (vb, vt, vh, v1), (ob, ot, oh, o1) = q.stride(), k.stride(), v.stride(), out.stride()
+    if not q1 == k1 == v1 == o1 == 1:
+        _columns((q1, k1, v1, o1), q, k, v, out)
+    (B, L, H, D), (_, S, KV, _), pshape = q.shape, k.shape, prefix_k.shape
+    if len(pshape) != 3 or pshape[1] != KV or pshape[2] != D or prefix_v.shape != pshape:
+        raise RuntimeError("prefix_k and prefix_v must be [P, kv_heads, D], of one shape")
+    (pkt, pkh, pk1), (pvt, pvh, pv1) = prefix_k.stride(), prefix_v.stride()
+    if not pk1 == pv1 == 1:
+        _columns((pk1, pv1), prefix_k, prefix_v)
+    _run("ff_prefix_attention", dev, q.data_ptr(), qb, qt, qh, prefix_k.data_ptr(), pkt, pkh, prefix_v.data_ptr(), pvt, pvh,
+         k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, out.data_ptr(), ob, ot, oh, _DTYPES[q.dtype], B, L, pshape[0], S,
+         H, KV, D, scale, None if lens is None else lens.data_ptr(), None if work is None else work.data_ptr(),
+         0 if work is None else work.numel())
 
 
 def residual_norm(x: torch.Tensor, y: torch.Tensor, x_out: torch.Tensor, h: torch.Tensor | None, post: int,
@@ -737,32 +725,40 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, x_out: torch.Tensor, h: torc
     taking row t / (T / G): one row is a layer scale, one a sequence an adaptive gate. An output may be x or y itself and shares
     no other memory with what is read or with the other (refused)."""
     _no_grad(x, y, x_out, h, post_gamma, post_beta, pre_gamma, pre_beta, gate)
-    dev = _on_gpu(post_gamma, post_beta, pre_gamma, pre_beta, gate)
-    shape, dt = x.shape, x.dtype
+    shape, dt, dev = x.shape, x.dtype, x.get_device()
     if len(shape) != 2 or dt not in _HALVES:
         raise RuntimeError("x must be fp16 or bf16 [T, C]")
+    if not (y.shape == x_out.shape == shape and y.dtype == x_out.dtype == dt):
+        raise RuntimeError("x, y and the outputs must have one type and shape")
+    if dev < 0 or y.get_device() != dev or x_out.get_device() != dev:
+        raise RuntimeError("all tensors must be on one GPU")
     T, C = shape
-    here, rows = x.get_device(), []
-    for t in (x, y, x_out, h):
-        if t is None:
-            rows += None, C
+    (xs, x1), (ys, y1), (os, o1) = x.stride(), y.stride(), x_out.stride()
+    hp, hs, h1 = None, C, 1
+    if h is not None:
+        if h.shape != shape or h.dtype != dt or h.get_device() != dev:
+            raise RuntimeError("h must have x's type, shape and device")
+        hp, (hs, h1) = h.data_ptr(), h.stride()
+    if not x1 == y1 == o1 == h1 == 1 and T:
+        raise RuntimeError("x, y and the outputs must have contiguous rows")
+    params = []
+    for p in (post_gamma, post_beta, pre_gamma, pre_beta):
+        if p is None:
+            params.append(None)
             continue
-        if t.shape != shape or t.dtype != dt:
-            raise RuntimeError("x, y and the outputs must have one type and shape")
-        if t.get_device() != here or here < 0 or dev not in (-1, here):
-            raise RuntimeError("all tensors must be on one GPU")
-        stride, one = t.stride()
-        if one != 1 and C > 1:
-            raise RuntimeError("x, y and the outputs must have contiguous rows")
-        rows += t.data_ptr(), stride
-    _float(C, *[t for t in (post_gamma, post_beta, pre_gamma, pre_beta) if t is not None])
-    gates, kind = 0, 0
+        if p.dtype != torch.float32 or p.numel() != C or p.get_device() != dev or not p.is_contiguous():
+            raise RuntimeError(f"gammas and betas must be contiguous fp32 of {C} elements on x's GPU")
+        params.append(p.data_ptr())
+    gp, gates, kind = None, 0, 0
     if gate is not None:
-        if gate.dtype not in (dt, torch.float32) or gate.dim() not in (1, 2) or gate.size(-1) != C:
+        if gate.dtype not in (dt, torch.float32) or gate.dim() not in (1, 2) or gate.size(-1) != C or T and not gate.numel():
             raise RuntimeError("gate must be fp32 or of x's type, [G, C] or [C]")
-        gates, kind = gate.numel() // C, _DTYPES[gate.dtype]
-    _run("ff_residual_norm", here, *rows, _DTYPES[dt], T, C, post, _ptr(post_gamma), _ptr(post_beta), pre, _ptr(pre_gamma),
-         _ptr(pre_beta), _ptr(gate), gates, kind, scale, eps)
+        if gate.get_device() != dev or not gate.is_contiguous():
+            raise RuntimeError("gate must be contiguous on x's GPU")
+        gp, gates, kind = gate.data_ptr(), gate.numel() // C, _DTYPES[gate.dtype]
+    pg, pb, qg, qb = params
+    _run("ff_residual_norm", dev, x.data_ptr(), xs, y.data_ptr(), ys, x_out.data_ptr(), os, hp, hs, _DTYPES[dt], T, C, post, pg,
+         pb, pre, qg, qb, gp, gates, kind, scale, eps)
 
 
 # ---- torch.ops.foidfinder_rocm registration (schemas as kernels.cu:268-273, plus eps / the fused norm) ----

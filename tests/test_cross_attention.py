@@ -133,10 +133,10 @@ def test_attention_workspace_is_checked():
     refused(cross(**one, work=WORK, size=need - 1), "workspace is too small")
     refused(cross(**one, work=None, size=need), "workspace is too small")
     refused(cross(**one, work=WORK + 4, size=need), "misaligned")
-    need = K.lib().ff_prefix_attention_work(2, 1, 200, 50, 4, 2, 64)
+    need = K.lib().ff_prefix_attention_work(2, 40, 200, 50, 4, 2, 64)
     assert need > 0
-    refused(prefix(size=need - 1), "workspace is too small")
-    refused(prefix(work=None), "workspace is too small")
+    refused(prefix(L=40, size=need - 1), "workspace is too small")
+    refused(prefix(L=40, work=None), "workspace is too small")
     for bad in ((2, 1, -1, 50, 4, 2, 64), (2, 1, 9, 50, 4, 3, 64), (2, 1, 9, 50, 4, 2, 300), (-2, 1, 9, 50, 4, 2, 64)):
         assert K.lib().ff_prefix_attention_work(*bad) == 0
 
@@ -153,7 +153,7 @@ def test_attention_overlaps_are_refused():
     refused(cross(**one, work=KEY), "workspace overlaps what is read")
     refused(cross(**one, work=Q), "workspace overlaps what is read")
     refused(prefix(pk=OUT), "out overlaps what is read")
-    refused(prefix(work=PV), "workspace overlaps what is read")
+    refused(prefix(L=40, work=PV), "workspace overlaps what is read")
     # a head-major output laid over a token-major query
     refused(cross(q=OUT, os=(40 * 4 * 64, 64, 40 * 64)), "out overlaps what is read")
 

@@ -156,6 +156,41 @@ def test_cross_attention_rising_and_falling_scores(dev, kind):
         assert_near(out.float().cpu().numpy(), o, bound(kind, 1.0, o, size, load, np.abs(vn).max(), S))
 
 
+@pytest.mark.parametrize("L", [1, 40, 100])
+def test_cross_attention_scores_of_any_size(dev, L):
+    """Scores of 2 10^11, whose spacing in fp32 is far above 1, and their negatives: the largest keys, all alike, share the weight.
+    Equal scores have equal weights, so their mean is off by the roundings of one weight and of the output."""
+    K = kern()
+    for sign in (1.0, -1.0):
+        q = torch.full((1, L, 1, 64), 60000.0, dtype=torch.float16, device=dev)
+        k = torch.full((1, 700, 1, 64), sign * 60000.0, dtype=torch.float16, device=dev)
+        k[:, 1::3] = sign * (30000.0 if sign > 0 else 64000.0)
+        v, vn = make(np.random.default_rng(2), "fp16", dev, 1, 700, 1, 64)
+        out = torch.empty_like(q)
+        K.cross_attention(q, k, v, out, 1.0, None, None, torch.empty(max(1, K.cross_attention_work(q, k)), device=dev))
+        top = vn[0, np.arange(700) % 3 != 1, 0].astype(np.float64)
+        o, size = top.mean(0), np.abs(top).mean(0)
+        err = np.abs(out[0, :, 0].float().cpu().numpy() - o)
+        assert (err <= HALF["fp16"] * (np.abs(o) + 2 * size)).all(), err.max()
+
+
+def test_cross_attention_of_one_key_that_is_not_finite(dev):
+    """The rows behind the last key repeat none of it: an infinite value comes out as such."""
+    q = torch.randn(1, 2, 2, 64, device=dev).half()
+    k, v = torch.randn(1, 1, 2, 64, device=dev).half(), torch.full((1, 1, 2, 64), math.inf, device=dev).half()
+    out = torch.empty_like(q)
+    kern().cross_attention(q, k, v, out, 0.125)
+    assert bool((out == math.inf).all())
+    q = torch.randn(1, 70, 2, 64, device=dev).half()
+    out = torch.empty_like(q)
+    kern().cross_attention(q, k, v, out, 0.125)
+    assert bool((out == math.inf).all())
+    five = torch.randn(1, 1, 2, 64, device=dev).half().expand(1, 5, 2, 64)  # one row five times
+    kern().cross_attention(q, five, five, out, 0.125)
+    # equal weights: off by the roundings of a weight, of their sum and of the output
+    assert bool(((out - five[:, :1]).abs() <= 3 * HALF["fp16"] * five[:, :1].abs() + 2.0**-24).all())
+
+
 def test_cross_attention_cut_keys(dev):
     """Few rows and many keys: the keys are cut, with lengths that leave cuts empty."""
     need = run_cross(dev, "fp16", 1, 1, 9000, 2, 1, 64)

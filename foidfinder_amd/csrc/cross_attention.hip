@@ -50,10 +50,12 @@ struct CrossArgs {
   const int32_t* lens;
   const uint8_t* mask;
   int64_t mask_b;
-  float* work;  // parts' O [part, kv, rows, D], then their (m, l) [part, kv, rows, 2]; null: one part, written to out
+  float* work;    // parts' O [slots, D], then their (m, l) [slots, 2]; a slot for each part and row; null: one part a row
+  int64_t slots;
   int batch, tokens, kv, group, dim, causal;
   int rows;  // batch * tokens * group: of a key head
   int block_rows, own_tiles, own_splits, prefix_tiles, prefix_splits;
+  int tail, tail_splits;  // the last row tiles of the grid, whose keys are cut (no prefix, own_splits 1)
   float c;
 };
 
@@ -83,7 +85,7 @@ struct Piece {
   int keys, len;     // keys that some row sees; the sequence's length
   int front;         // slices of 32 prefix keys before the sequence's own (streams only)
   int t0, t1;        // tiles, or slices of 32 keys
-  int part;
+  int64_t slot;      // of row0 in the workspace; -1: rows go to out
 };
 
 // Where a lane's row lies, and how many of the sequence's own keys it sees.
@@ -104,15 +106,19 @@ __device__ __forceinline__ Place place_of(const CrossArgs& a, const Piece& w, in
 // 32 rows in a wave: q, O, m and the lane's part of l. Lane: row fr = lane % 32, half fh = lane / 32.
 template <typename T, int DP>
 struct Unit {
-  static constexpr int KS = DP / 16, DT = DP / 32;
+  static constexpr int KS = DP / 16, DT = DP / 32, VSTEP = DT == 4 ? 2 : 1;
   typedef vec8_t<T> T8;
   typedef vec4_t<T> T4;
   T8 qf[KS];       // column operand of S^T: the row's columns 16 s + 8 fh + 0..7
   float16_t o[DT]; // O^T: columns 32 dt + 8 (r / 4) + 4 fh + r % 4
   float m = LOWEST, l = 0.f, c;
-  float16_t xs;    // S^T of 32 keys: 8 (r / 4) + 4 fh + r % 4
-  T8 pf[2];
-  int koff[KS], voff[DT];  // LDS offsets (elements) of the fragments within 32 keys
+  // LDS offsets (elements) of the first fragments within 32 keys. The others' follow from the swizzle: an exclusive or with the
+  // fragment's place in the row, or for rows of 96 columns a step, from the second one where the fragment is odd.
+  int koff, koff_odd, voff;
+  static __device__ __forceinline__ int kfrag(int ka, int ka_odd, int s) {
+    return DP == 96 ? (s & 1 ? ka_odd : ka) + (s >> 1) * 32 : ka ^ (16 * s);
+  }
+  static __device__ __forceinline__ int vfrag(int va, int dt) { return DP == 96 ? va + 32 * dt : va ^ (32 * dt); }
 
   __device__ __forceinline__ void start(const CrossArgs& a, const Place& p, int lane) {
     const int fr = lane & 31, fh = lane >> 5;
@@ -129,54 +135,67 @@ struct Unit {
     c = a.c;
     // K fragment s: row fr, chunk 2 s + fh. V^T fragment (dt, tt), part j: lane l of 16 addresses row 16 tt + 8 j + 4 fh + l / 4,
     // columns 32 dt + 16 (group) + 4 (l % 4), and receives four keys in a row of column 32 dt + fr: the keys of P^T's slots.
-#pragma unroll
-    for (int s = 0; s < KS; ++s) koff[s] = fr * DP + k_slot<DP>(fr, 2 * s + fh) * 8;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const int r = 4 * fh + ((lane & 15) >> 2), col = dt * 32 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-      voff[dt] = r * DP + v_slot<DP>(r, col >> 3) * 8 + (col & 7);
-    }
+    koff = fr * DP + k_slot<DP>(fr, fh) * 8;
+    if constexpr (DP == 96) koff_odd = fr * DP + k_slot<DP>(fr, 2 + fh) * 8;
+    const int r = 4 * fh + ((lane & 15) >> 2), col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    voff = r * DP + v_slot<DP>(r, col >> 3) * 8 + (col & 7);
   }
   // q consumed, so that the compiler's wait for its loads stands here, before the loop and after the first keys' loads, not in it.
   __device__ __forceinline__ void settle() {
 #pragma unroll
     for (int s = 0; s < KS; ++s) asm volatile("" ::"v"(qf[s]));
   }
-  // S^T of the 32 keys at k (+ ka).
-  __device__ __forceinline__ void score(const T* k, const int (&ka)[KS]) {
+  // x = S^T of the 32 keys at k (+ ka): keys 8 (r / 4) + 4 fh + r % 4.
+  __device__ __forceinline__ void score(float16_t& x, const T* k, int ka, int ka_odd) {
+    T8 kf[KS];
+    keys(kf, k, ka, ka_odd);
+    score(x, kf);
+  }
+  __device__ __forceinline__ void keys(T8 (&kf)[KS], const T* k, int ka, int ka_odd) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) kf[s] = *reinterpret_cast<const T8*>(k + kfrag(ka, ka_odd, s));
+  }
+  __device__ __forceinline__ void score(float16_t& x, const T8 (&kf)[KS]) {
     const float16_t zero = {};
 #pragma unroll
-    for (int s = 0; s < KS; ++s) xs = mfma(*reinterpret_cast<const T8*>(k + ka[s]), qf[s], s == 0 ? zero : xs);
+    for (int s = 0; s < KS; ++s) x = mfma(kf[s], qf[s], s == 0 ? zero : x);
   }
   // p of the scores, at most 2^cap each, and the lane's sum of it.
-  __device__ __forceinline__ float weights(float cap) {
-    float e[16];
+  __device__ __forceinline__ float weights(const float16_t& xs, T8 (&pf)[2], float cap) {
+    float sum[4];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       float x = __builtin_fmaf(xs[r], c, -m);
       if (!__builtin_isinf(cap)) x = x > cap ? cap : x;  // not a number stays so
-      e[r] = __builtin_amdgcn_exp2f(x);
-      pf[r >> 3][r & 7] = static_cast<T>(e[r]);
+      const float e = __builtin_amdgcn_exp2f(x);
+      pf[r >> 3][r & 7] = static_cast<T>(e);
+      sum[r & 3] = r < 4 ? e : sum[r & 3] + e;
     }
-#pragma unroll
-    for (int n = 8; n >= 1; n >>= 1)
-#pragma unroll
-      for (int r = 0; r < n; ++r) e[r] = e[r] + e[r + n];
-    return e[0];
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
   }
-  // p of the scores; bits: the keys that the lane's row sees.
-  // first: m is not set yet, which the first pass would only find out.
-  __device__ __forceinline__ void weigh(uint32_t bits, int fh, bool first) {
+  // Scores of keys that the lane's row does not see (bits: those that it sees).
+  __device__ __forceinline__ void hide(float16_t& xs, uint32_t bits, int fh) {
     if (__any(bits != ~0u)) {
       bits >>= 4 * fh;
 #pragma unroll
       for (int r = 0; r < 16; ++r) xs[r] = (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? xs[r] : -__builtin_inff();
     }
+  }
+  // p of the scores; bits: the keys that the lane's row sees.
+  // first: m is not set yet, which the first pass would only find out.
+  __device__ __forceinline__ void weigh(float16_t& xs, T8 (&pf)[2], uint32_t bits, int fh, bool first) {
+    hide(xs, bits, fh);
     float sum = 0.f;
-    if (!first) sum = weights(__builtin_inff());
-    if (first || __any(sum > SUM_LIMIT)) {
-      // m becomes the largest c S of these keys, or just below, and O and l follow. Scores from 2^30 up are too coarse for the
-      // multiply-add: what it leaves of the largest can be of any size then, and is capped.
+    if (!first) sum = weights(xs, pf, __builtin_inff());
+    if (first || __any(sum > SUM_LIMIT))
+      raise(xs, pf);
+    else
+      l += sum;
+  }
+  // The keys' p passed the limit, or m is not set: m becomes the largest c S of the keys, or just below, and O and l follow. Scores
+  // from 2^30 up are too coarse for the multiply-add: what it leaves of the largest can be of any size then, and is capped.
+  __device__ __forceinline__ void raise(const float16_t& xs, T8 (&pf)[2]) {
+    {
       float top = xs[0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) top = fmaxf(top, xs[r]);
@@ -189,25 +208,25 @@ struct Unit {
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] *= corr;
-      sum = weights(CAP);
+      l += weights(xs, pf, CAP);
     }
-    l += sum;
   }
   // O^T += V^T P^T, the 32 values at LDS byte v + OFF (+ va).
   template <int OFF>
-  __device__ __forceinline__ void mix(uint32_t v, const int (&va)[DT]) {
+  __device__ __forceinline__ void mix(uint32_t v, int va, const T8 (&pf)[2]) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      T4 x[4];  // [2 tt + j]
-      const uint32_t base = v + 2u * static_cast<uint32_t>(va[dt]);
-      tr_read<OFF>(x[0], base);
-      tr_read<OFF + 8 * DP * 2>(x[1], base);
-      tr_read<OFF + 16 * DP * 2>(x[2], base);
-      tr_read<OFF + 24 * DP * 2>(x[3], base);
-      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+    for (int dt = 0; dt < DT; dt += VSTEP) {
+      T4 x[VSTEP][4];  // [][2 tt + j]
+      const uint32_t at = v + 2u * static_cast<uint32_t>(vfrag(va, dt));
+      if constexpr (VSTEP == 2)
+        tr_read4<OFF, 8 * DP * 2>(x[0], at, x[1], v + 2u * static_cast<uint32_t>(vfrag(va, dt + 1)));
+      else
+        tr_read4<OFF, 8 * DP * 2>(x[0], at);
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
-        o[dt] = mfma(__builtin_shufflevector(x[2 * tt], x[2 * tt + 1], 0, 1, 2, 3, 4, 5, 6, 7), pf[tt], o[dt]);
+#pragma unroll
+        for (int i = 0; i < VSTEP; ++i)
+          o[dt + i] = mfma(__builtin_shufflevector(x[i][2 * tt], x[i][2 * tt + 1], 0, 1, 2, 3, 4, 5, 6, 7), pf[tt], o[dt + i]);
     }
   }
 };
@@ -217,13 +236,10 @@ template <typename T>
 __device__ __forceinline__ void store4(const CrossArgs& a, const Piece& w, const Place& p, int row, int col, float4_t o, float m,
                                        float l) {
   if (col >= a.dim) return;
-  if (a.work) {
-    const int64_t n = (static_cast<int64_t>(w.part) * a.kv + w.head) * a.rows + row;
+  if (w.slot >= 0) {
+    const int64_t n = w.slot + row - w.row0;
     *reinterpret_cast<float4_t*>(a.work + n * a.dim + col) = o;
-    if (col == 0) {
-      const int64_t parts = a.prefix_splits + a.own_splits;
-      *reinterpret_cast<float2*>(a.work + parts * a.kv * a.rows * a.dim + 2 * n) = float2{m, l};
-    }
+    if (col == 0) *reinterpret_cast<float2*>(a.work + a.slots * a.dim + 2 * n) = float2{m, l};
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;  // no keys: zeros
@@ -236,15 +252,19 @@ __device__ __forceinline__ void store4(const CrossArgs& a, const Piece& w, const
 // Tiles of 64 keys for four waves: a wave a unit (SHARE 1), or two (SHARE 2), each with one half of every tile.
 template <typename T, int DP, int SHARE>
 __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T* smem) {
+  typedef vec8_t<T> T8;
   constexpr int CH = DP / 8, TILE = BKV * DP, LPW = CH / 4, KS = DP / 16, DT = DP / 32;
   const uint32_t smem_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)smem));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 31, fh = lane >> 5, unit = wave / SHARE, half_sel = SHARE == 2 ? wave & 1 : 0;
   const bool active = w.row0 + unit * QW < w.row_end;  // other waves only load
-  const int row = w.row0 + unit * QW + fr;
-  const Place p = place_of(a, w, row);
+  int row = w.row0 + unit * QW + fr, limit;
   Unit<T, DP> u;
-  u.start(a, p, lane);
+  {
+    const Place p = place_of(a, w, row);
+    u.start(a, p, lane);
+    limit = p.limit;
+  }
 
   const KeySource& src = w.seq < 0 ? a.prefix : a.own;
   const int64_t at = max(w.seq, 0);
@@ -256,12 +276,10 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
   // Tile loads: wave w fills the 1 KB blocks LPW w .. of either tile, lane l the chunk l of a block; it fetches what the swizzle
   // puts there.
   uint32_t voff_k[LPW], voff_v[LPW];
-  int lrow[LPW];
 #pragma unroll
   for (int i = 0; i < LPW; ++i) {
     const int n = (LPW * wave + i) * 64 + lane, r = n / CH, slot = n % CH;
     const int ck = k_slot<DP>(r, slot), cv = v_slot<DP>(r, slot);
-    lrow[i] = r;
     voff_k[i] = 8 * ck < a.dim ? static_cast<uint32_t>((r * static_cast<int>(src.kt) + ck * 8) * 2) : OOB_OFFSET;
     voff_v[i] = 8 * cv < a.dim ? static_cast<uint32_t>((r * static_cast<int>(src.vt) + cv * 8) * 2) : OOB_OFFSET;
   }
@@ -272,7 +290,7 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
     const T *k = kbase + first * src.kt, *v = vbase + first * src.vt;
 #pragma unroll
     for (int i = 0; i < LPW; ++i) {
-      const bool in = !guard || ((word >> lrow[i]) & 1);
+      const bool in = !guard || ((word >> (((LPW * wave + i) * 64 + lane) / CH)) & 1);
       buffer_to_lds(k, nk, reinterpret_cast<uint8_t*>(smem + st * TILE + (LPW * wave + i) * 512), in ? voff_k[i] : OOB_OFFSET);
       buffer_to_lds(v, nv, reinterpret_cast<uint8_t*>(smem + (2 + st) * TILE + (LPW * wave + i) * 512),
                     in ? voff_v[i] : OOB_OFFSET);
@@ -288,15 +306,35 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
     const int n = w.keys - tile * BKV;
     return n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1;
   };
-  auto half_tile = [&](int tile, uint64_t word, const int (&ka)[KS], const int (&va)[DT], auto halfc) __attribute__((always_inline)) {
-    constexpr int half = decltype(halfc)::value;
-    const int h = SHARE == 2 ? half_sel : half;  // of the tile (SHARE 2: the offsets point to it)
-    u.score(smem + half * 32 * DP, ka);
-    const int left = p.limit - (tile * BKV + 32 * h);
-    uint32_t bits = static_cast<uint32_t>(word >> (32 * h));
-    bits &= left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
-    u.weigh(bits, fh, tile == w.t0 && half == 0);
-    u.template mix<half * 32 * DP * 2>(smem_lds, va);
+  auto bits_of = [&](int tile, uint64_t word, int half) __attribute__((always_inline)) {
+    const int left = limit - (tile * BKV + 32 * half);
+    return static_cast<uint32_t>(word >> (32 * half)) & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1);
+  };
+  auto half_tile = [&](int tile, uint64_t word, int half, int ka, int ka_odd, int va) __attribute__((always_inline)) {
+    float16_t x;
+    vec8_t<T> pf[2];
+    u.score(x, smem, ka, ka_odd);
+    u.weigh(x, pf, bits_of(tile, word, half), fh, tile == w.t0 && half == 0);
+    u.template mix<0>(smem_lds, va, pf);
+  };
+  // Both halves of a tile: either product of one runs under the softmax of the other. Returns the half from which on it is not
+  // done, because p passed the limit (2: it is done): half_tile does these, and raises m.
+  auto whole_tile = [&](int tile, uint64_t word, int ka, int ka_odd, int va) __attribute__((always_inline)) {
+    vec8_t<T> pf[2][2];
+    float16_t x[2];
+    u.score(x[0], smem, ka, ka_odd);
+    u.hide(x[0], bits_of(tile, word, 0), fh);
+    u.score(x[1], smem + 32 * DP, ka, ka_odd);
+    float sum = u.weights(x[0], pf[0], __builtin_inff());
+    if (__any(sum > SUM_LIMIT)) return 0;
+    u.l += sum;
+    u.hide(x[1], bits_of(tile, word, 1), fh);
+    u.template mix<0>(smem_lds, va, pf[0]);
+    sum = u.weights(x[1], pf[1], __builtin_inff());
+    if (__any(sum > SUM_LIMIT)) return 1;
+    u.l += sum;
+    u.template mix<32 * DP * 2>(smem_lds, va, pf[1]);
+    return 2;
   };
 
   if (w.t0 < w.t1) {
@@ -315,19 +353,19 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
       const int st = (tile - w.t0) & 1;
       if (active && word != 0) {
         // read bases, opaque to the compiler so that the fragment offsets fold into the reads' immediate offsets
-        int ka[KS], va[DT];
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          ka[s] = st * TILE + half_sel * 32 * DP + u.koff[s];
-          asm volatile("" : "+v"(ka[s]));
+        int ka = st * TILE + half_sel * 32 * DP + u.koff, ka_odd = 0, va = (2 + st) * TILE + half_sel * 32 * DP + u.voff;
+        asm volatile("" : "+v"(ka), "+v"(va));
+        if constexpr (DP == 96) {
+          ka_odd = st * TILE + half_sel * 32 * DP + u.koff_odd;
+          asm volatile("" : "+v"(ka_odd));
         }
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          va[dt] = (2 + st) * TILE + half_sel * 32 * DP + u.voff[dt];
-          asm volatile("" : "+v"(va[dt]));
+        if constexpr (SHARE == 2) {
+          half_tile(tile, word, half_sel, ka, ka_odd, va);
+        } else {
+#pragma unroll 1
+          for (int half = whole_tile(tile, word, ka, ka_odd, va); half < 2; ++half)
+            half_tile(tile, word, half, ka + half * 32 * DP, ka_odd + half * 32 * DP, va + half * 32 * DP);
         }
-        half_tile(tile, word, ka, va, std::integral_constant<int, 0>{});
-        if constexpr (SHARE == 1) half_tile(tile, word, ka, va, std::integral_constant<int, 1>{});
       }
       word = next;
     }
@@ -361,6 +399,8 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
   }
   const float l = u.l + xor_shuffle(u.l, 32);
   if (row >= w.row_end) return;
+  asm volatile("" : "+v"(row));  // its place is found again here: kept through the loop it would hold registers
+  const Place p = place_of(a, w, row);
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -375,6 +415,7 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
 // sequence's own. The waves' O, m and l are joined through LDS, four columns a wave and turn.
 template <typename T, int DP, int NW>
 __device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w, T* smem) {
+  typedef vec8_t<T> T8;
   constexpr int CH = DP / 8, SLICE = 32 * DP, LP = CH / 2, DT = DP / 32, WORDS = 16 * DT + 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 31, fh = lane >> 5;
   T* kbuf = smem + wave * 2 * SLICE;
@@ -441,7 +482,9 @@ __device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w,
       const bool more = n + NW < w.t1;
       Slice next = now;
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LP) : "memory");  // all but V
-      u.score(kbuf, u.koff);
+      float16_t x;
+      T8 pf[2];
+      u.score(x, kbuf, u.koff, u.koff_odd);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (more) {
         next = slice(n + NW, byte);
@@ -449,12 +492,12 @@ __device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w,
         load(next, false);
       }
       const int left = now.own ? p.limit - now.first : 32;
-      u.weigh(now.word & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1), fh, n == w.t0 + wave);
+      u.weigh(x, pf, now.word & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1), fh, n == w.t0 + wave);
       if (more)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LP) : "memory");  // all but the next K
       else
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      u.template mix<0>(vbuf, u.voff);
+      u.template mix<0>(vbuf, u.voff, pf);
       if (!more) break;
       load(next, true);
       now = next;
@@ -511,32 +554,43 @@ __global__ __launch_bounds__(64 * WAVES, DP == 64 ? 4 : DP == 96 ? 3 : 2) void c
   const int per = a.tokens * a.group, prefix_items = a.prefix_splits * a.kv * a.prefix_tiles;
   int item = static_cast<int>(blockIdx.x);
   Piece w;
-  int split, splits, tile, x;
+  int split = 0, splits = 1, tile, x;
   // Row tiles of one run of keys are neighbours, and neighbours share an XCD's L2 (the prefix's pieces by themselves, as they
   // differ from the others in length). A run's last tile, where it has fewer rows and takes less time, comes after all whole ones
-  // and fills the end of the grid.
-  auto place = [&](int n, int tiles, int rows) __attribute__((always_inline)) {
-    const int whole = rows / a.block_rows, runs = n / tiles;
-    if (item < runs * whole) {
-      item = xcd_remap(item, runs * whole);
-      x = item / whole, tile = item - x * whole;
+  // and fills the end of the grid; before it come the tail's pieces.
+  auto place = [&](int n, int tiles, int rows, int tail, int tail_splits) __attribute__((always_inline)) {
+    const int whole = rows / a.block_rows, runs = n / tiles, all = runs * whole;
+    if (item < all - tail) {
+      item = xcd_remap(item, all - tail);
+    } else if (item < all - tail + tail * tail_splits) {
+      const int cut = xcd_remap(item - (all - tail), tail * tail_splits);
+      split = cut / tail, splits = tail_splits, item = all - tail + cut - split * tail;
     } else {
-      x = xcd_remap(item - runs * whole, runs), tile = whole;
+      x = xcd_remap(item - (all - tail + tail * tail_splits), runs), tile = whole;
+      return;
     }
+    x = item / whole, tile = item - x * whole;
   };
   if (item < prefix_items) {
-    place(prefix_items, a.prefix_tiles, a.rows);
+    place(prefix_items, a.prefix_tiles, a.rows, 0, 1);
     split = x % a.prefix_splits, splits = a.prefix_splits;
-    w.seq = -1, w.head = x / a.prefix_splits, w.part = split;
+    w.seq = -1, w.head = x / a.prefix_splits;
     w.row0 = tile * a.block_rows, w.row_end = a.rows;
+    w.slot = (static_cast<int64_t>(split) * a.kv + w.head) * a.rows + w.row0;
     w.len = w.keys = a.prefix.keys;
   } else {
     item -= prefix_items;
-    place(static_cast<int>(gridDim.x) - prefix_items, a.own_tiles, per);
+    place(a.batch * a.kv * a.own_splits * a.own_tiles, a.own_tiles, per, a.tail, a.tail_splits);
     const int y = x / a.own_splits;
-    split = x - y * a.own_splits, splits = a.own_splits;
-    w.seq = y / a.kv, w.head = y - w.seq * a.kv, w.part = a.prefix_splits + split;
+    w.seq = y / a.kv, w.head = y - w.seq * a.kv;
     w.row0 = w.seq * per + tile * a.block_rows, w.row_end = (w.seq + 1) * per;
+    w.slot = -1;
+    if (splits > 1) {  // of the tail
+      w.slot = (static_cast<int64_t>(split) * a.tail + item - (a.batch * a.kv * (per / a.block_rows) - a.tail)) * a.block_rows;
+    } else if (a.tail == 0 && a.work) {
+      split = x - y * a.own_splits, splits = a.own_splits;
+      w.slot = (static_cast<int64_t>(a.prefix_splits + split) * a.kv + w.head) * a.rows + w.row0;
+    }
     w.len = w.keys = a.lens ? min(max(a.lens[w.seq], 0), a.own.keys) : a.own.keys;
     if (a.causal) {
       const int last = (min(w.row0 + a.block_rows, w.row_end) - 1 - w.seq * per) / a.group;
@@ -556,38 +610,39 @@ __global__ __launch_bounds__(64 * WAVES, DP == 64 ? 4 : DP == 96 ? 3 : 2) void c
     tile_block<T, DP, 1>(a, w, smem);
 }
 
-// Up to 32 rows a sequence and key head, and few of these: one workgroup a CU whose waves all read the same rows' keys, the prefix's
-// among them, so that a single launch does where the keys are few enough. Sequences of a head are neighbours: they share the prefix.
-constexpr int stream_waves(int dp) { return 8; }
-
-template <typename T, int DP>
-__global__ __launch_bounds__(64 * stream_waves(DP), stream_waves(DP) / 4) void stream_kernel(const CrossArgs a) {
-  __shared__ __attribute__((aligned(1024))) T smem[stream_bytes(DP, stream_waves(DP)) / 2];
+// Up to 32 rows a sequence and key head: workgroups of NW waves that all read the same rows' keys, the prefix's among them. Where
+// there are few (NW 8, one a CU), a single launch does as long as the keys are few enough. Sequences of a head are neighbours: they
+// share the prefix.
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : DP == 64 ? 4 : DP == 96 ? 3 : 2) void stream_kernel(const CrossArgs a) {
+  __shared__ __attribute__((aligned(1024))) T smem[stream_bytes(DP, NW) / 2];
   touch(a);
   const int split = static_cast<int>(blockIdx.z), per = a.tokens * a.group;
   Piece w;
-  w.seq = static_cast<int>(blockIdx.x), w.head = static_cast<int>(blockIdx.y), w.part = split;
+  w.seq = static_cast<int>(blockIdx.x), w.head = static_cast<int>(blockIdx.y);
   w.row0 = w.seq * per, w.row_end = w.row0 + per;
+  w.slot = a.work ? (static_cast<int64_t>(split) * a.kv + w.head) * a.rows + w.row0 : -1;
   w.len = w.keys = a.lens ? min(max(a.lens[w.seq], 0), a.own.keys) : a.own.keys;
   w.front = (a.prefix.keys + 31) / 32;
   const int64_t slices = w.front + (w.keys + 31) / 32;
   w.t0 = static_cast<int>(slices * split / a.own_splits);
   w.t1 = static_cast<int>(slices * (split + 1) / a.own_splits);
-  stream_block<T, DP, stream_waves(DP)>(a, w, smem);
+  stream_block<T, DP, NW>(a, w, smem);
 }
 
-// Joins the parts of a row: a wave a row, CH lanes for its columns (8 each), 64 / CH lanes for parts, joined at the end.
-template <typename T, int CH>
+// Joins the parts of a row: CH lanes for its columns (8 each), LANES times over for as many parts at a time, joined at the end.
+template <typename T, int CH, int LANES>
 __global__ __launch_bounds__(256) void join_kernel(const CrossArgs a) {
-  constexpr int LANES = 64 / CH;  // parts at a time
-  const int parts = a.prefix_splits + a.own_splits, lane = threadIdx.x & 63, c = lane % CH, first = lane / CH;
-  const int64_t all = static_cast<int64_t>(a.kv) * a.rows, at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, c = lane % CH, first = lane / CH % LANES, of = lane / (CH * LANES);
+  const int parts = a.tail ? a.tail_splits : a.prefix_splits + a.own_splits;
+  const int64_t all = a.tail ? static_cast<int64_t>(a.tail) * a.block_rows : static_cast<int64_t>(a.kv) * a.rows;
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * (64 / (CH * LANES)) + of;
   if (at >= all) return;
-  const float2* ml = reinterpret_cast<const float2*>(a.work + parts * all * a.dim) + at;
+  const float2* ml = reinterpret_cast<const float2*>(a.work + a.slots * a.dim) + at;
   float top = LOWEST;
-  for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml[p * all].x);
+  for (int p = lane % (CH * LANES); p < parts; p += CH * LANES) top = fmaxf(top, ml[p * all].x);
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, xor_shuffle(top, d));
+  for (int d = 1; d < CH * LANES; d <<= 1) top = fmaxf(top, xor_shuffle(top, d));
   const int col = 8 * c < a.dim ? 8 * c : 0;  // lanes past the columns join the first again
   const float* from = a.work + at * a.dim + col;
   const int64_t step = all * a.dim;
@@ -605,7 +660,7 @@ __global__ __launch_bounds__(256) void join_kernel(const CrossArgs a) {
     }
   }
 #pragma unroll
-  for (int d = CH; d < 64; d <<= 1) {
+  for (int d = CH; d < CH * LANES; d <<= 1) {
     l = l + xor_shuffle(l, d);
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = o[e] + xor_shuffle(o[e], d);
@@ -615,26 +670,47 @@ __global__ __launch_bounds__(256) void join_kernel(const CrossArgs a) {
   vec8_t<T> y;
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = static_cast<T>(o[e] * inv);
-  const int head = static_cast<int>(at / a.rows), row = static_cast<int>(at - static_cast<int64_t>(head) * a.rows);
-  const int per = a.tokens * a.group, seq = row / per, rest = row - seq * per, token = rest / a.group;
+  const int per = a.tokens * a.group;
+  int head, seq, rest;
+  if (a.tail) {
+    const int whole = per / a.block_rows, item = a.batch * a.kv * whole - a.tail + static_cast<int>(at / a.block_rows);
+    const int run = item / whole;
+    seq = run / a.kv, head = run - seq * a.kv;
+    rest = (item - run * whole) * a.block_rows + static_cast<int>(at % a.block_rows);
+  } else {
+    head = static_cast<int>(at / a.rows);
+    const int row = static_cast<int>(at - static_cast<int64_t>(head) * a.rows);
+    seq = row / per, rest = row - seq * per;
+  }
+  const int token = rest / a.group;
   T* to = static_cast<T*>(a.out) + seq * a.ob + token * a.ot + (head * a.group + rest - token * a.group) * a.oh + col;
   *reinterpret_cast<vec4_t<T>*>(to) = vec4_t<T>{y[0], y[1], y[2], y[3]};
   *reinterpret_cast<vec4_t<T>*>(to + 4) = vec4_t<T>{y[4], y[5], y[6], y[7]};
 }
 
 template <typename T, int DP>
-static void launch_cross(const CrossArgs& a, int64_t blocks, bool stream, hipStream_t st) {
-  if (stream)
-    stream_kernel<T, DP><<<dim3(a.batch, a.kv, a.own_splits), 64 * stream_waves(DP), 0, st>>>(a);
+static void launch_cross(const CrossArgs& a, int64_t blocks, int stream, hipStream_t st) {
+  const dim3 runs(a.batch, a.kv, a.own_splits);
+  if (stream == 8)
+    stream_kernel<T, DP, 8><<<runs, 64 * 8, 0, st>>>(a);
+  else if (stream == 4)
+    stream_kernel<T, DP, 4><<<runs, 64 * 4, 0, st>>>(a);
   else
     cross_kernel<T, DP><<<dim3(static_cast<unsigned>(blocks)), 64 * WAVES, 0, st>>>(a);
   if (!a.work) return;
-  const int64_t rows = static_cast<int64_t>(a.kv) * a.rows;
-  join_kernel<T, DP == 64 ? 8 : 16><<<dim3(static_cast<unsigned>((rows + 3) / 4)), 256, 0, st>>>(a);
+  constexpr int CH = DP == 64 ? 8 : 16;
+  const int parts = a.tail ? a.tail_splits : a.prefix_splits + a.own_splits;
+  const int64_t rows = a.slots / parts;
+  // a row's parts in several lanes at once where they are many (24 576 rows of 2 parts, 64 columns: 6.0 us in one, 14.7 in 8; 16
+  // rows of 32: 17 us in one, 4.6 in 8)
+  if (parts > 4)
+    join_kernel<T, CH, 64 / CH><<<dim3(static_cast<unsigned>((rows + 3) / 4)), 256, 0, st>>>(a);
+  else
+    join_kernel<T, CH, 1><<<dim3(static_cast<unsigned>((rows + 4 * (64 / CH) - 1) / (4 * (64 / CH)))), 256, 0, st>>>(a);
 }
 
 template <typename T>
-static void launch_cross_dim(const CrossArgs& a, int64_t blocks, bool stream, hipStream_t st) {
+static void launch_cross_dim(const CrossArgs& a, int64_t blocks, int stream, hipStream_t st) {
   if (a.dim <= 64)
     launch_cross<T, 64>(a, blocks, stream, st);
   else if (a.dim <= 96)
@@ -645,17 +721,41 @@ static void launch_cross_dim(const CrossArgs& a, int64_t blocks, bool stream, hi
 
 // How rows and keys are cut, from the sizes alone (the workspace's size follows from it).
 struct Plan {
-  bool stream;  // stream_kernel
-  int64_t block_rows, own_tiles, own_splits, prefix_tiles, prefix_splits, parts, blocks;
+  int stream;  // waves of stream_kernel's workgroups, 0: cross_kernel
+  int64_t block_rows, own_tiles, own_splits, prefix_tiles, prefix_splits, tail, tail_splits, slots, blocks;
 };
 
 constexpr int64_t CUS = 256;
-constexpr int64_t WANT = 2 * CUS;             // workgroups of cross_kernel that fill the chip
 constexpr int64_t ONE_GO = int64_t(1) << 20;  // bytes of keys and values that a workgroup reads before cutting them pays
 
-static int64_t split_keys(int64_t blocks, int64_t keys) {
-  const int64_t tiles = (keys + BKV - 1) / BKV;
-  return std::max<int64_t>(1, std::min(WANT / std::max<int64_t>(blocks, 1), tiles / 2));
+// Times in us, fitted to launches on this card: a tile of 64 keys takes a workgroup of four units TILE_ALONE at least, and a CU
+// TILE_CU per workgroup in it.
+struct Rates {
+  double alone, cu;
+  int64_t resident;  // workgroups a CU holds
+};
+static Rates rates_of(int64_t D) {
+  if (D <= 64) return {1.0, 0.62, 4};
+  if (D <= 96) return {1.1, 0.87, 3};
+  return {1.2, 1.05, 2};
+}
+
+// Cuts of the keys of `blocks` workgroups that have `tiles` tiles each, beside `others` workgroups (of fewer tiles): the cut that
+// ends first. Each part of a row costs its O, m and l written and read again; a second launch where there would be one part.
+static int64_t split_keys(int64_t blocks, int64_t tiles, int64_t others, int64_t rows, int64_t D, bool joined) {
+  if (blocks <= 0 || tiles <= 1) return 1;
+  const Rates r = rates_of(D);
+  int64_t best = 1;
+  double least = 0;
+  for (int64_t s = 1; s <= std::min<int64_t>(64, (tiles + 1) / 2); ++s) {
+    const double per_cu = static_cast<double>(blocks * s + others) / CUS;
+    const double together = std::min<double>(std::max(per_cu, 1.0), static_cast<double>(r.resident));
+    const double rounds = std::max(1.0, static_cast<double>(blocks * s) / static_cast<double>(CUS * r.resident));
+    const double t = 3.0 + static_cast<double>((tiles + s - 1) / s) * rounds * std::max(r.alone, r.cu * together) +
+                     (s > 1 || joined ? 4.0 + static_cast<double>(s * rows * (D + 2)) * 8.0 / 4.5e6 : 0.0);
+    if (s == 1 || t < least) least = t, best = s;
+  }
+  return best;
 }
 
 // prefix < 0: none
@@ -663,29 +763,42 @@ static Plan plan_of(int64_t batch, int64_t tokens, int64_t keys, int64_t prefix,
   Plan p{};
   const int64_t per = tokens * group, rows = batch * per, runs = batch * kv, all = keys + std::max<int64_t>(prefix, 0);
   const bool cut = all * D * 4 > ONE_GO;
-  if (per <= QW && runs <= CUS && (prefix <= 0 || batch == 1 || !cut)) {
-    p.stream = true;
+  p.own_splits = p.tail_splits = 1;
+  if (per <= QW && (prefix < 0 || prefix == 0 || (runs <= CUS && (batch == 1 || !cut)))) {
+    p.stream = runs <= CUS ? 8 : 4;
     p.block_rows = QW;
     p.own_tiles = 1;
-    p.parts = p.own_splits = cut ? std::max<int64_t>(1, std::min(CUS / std::max<int64_t>(runs, 1), all / 512)) : 1;
+    if (cut) p.own_splits = std::max<int64_t>(1, std::min(CUS / std::max<int64_t>(runs, 1), all / 512));
+    p.slots = p.own_splits > 1 ? p.own_splits * rows * kv : 0;
     p.blocks = runs * p.own_splits;
     return p;
   }
   const int64_t most = prefix >= 0 ? rows : per;
   p.block_rows = most <= QW ? QW : most <= 2 * QW ? 2 * QW : 4 * QW;
   p.own_tiles = (per + p.block_rows - 1) / p.block_rows;
-  p.own_splits = split_keys(p.own_tiles * runs, keys);
+  const int64_t own = p.own_tiles * runs, tiles = (keys + BKV - 1) / BKV;
   if (prefix >= 0) {
     p.prefix_tiles = (rows + p.block_rows - 1) / p.block_rows;
-    p.prefix_splits = split_keys(p.prefix_tiles * kv, prefix);
+    p.own_splits = split_keys(own, tiles, p.prefix_tiles * kv, rows * kv, D, true);
+    p.prefix_splits = split_keys(p.prefix_tiles * kv, (prefix + BKV - 1) / BKV, own * p.own_splits, rows * kv, D, true);
+    p.slots = (p.own_splits + p.prefix_splits) * rows * kv;
+  } else {
+    const Rates r = rates_of(D);
+    const int64_t slots = CUS * r.resident, whole = per / p.block_rows * runs, last = whole % slots;
+    p.own_splits = split_keys(own, tiles, 0, rows * kv, D, false);
+    if (p.own_splits == 1 && whole > slots && last > 0) {
+      // The last round's workgroups, cut so that they fill the chip too, if that saves more than the join costs
+      const int64_t cuts = std::min<int64_t>(slots / last, tiles / 8);
+      const double now = static_cast<double>(tiles) * std::max(r.alone, r.cu * static_cast<double>(last) / CUS);
+      const double then = static_cast<double>(tiles) / static_cast<double>(std::max<int64_t>(cuts, 1)) *
+                              std::max(r.alone, r.cu * static_cast<double>(last * cuts) / CUS) +
+                          5.0 + static_cast<double>(cuts * last * p.block_rows * (D + 2)) * 8.0 / 4.5e6;
+      if (cuts > 1 && then < now) p.tail = last, p.tail_splits = cuts;
+    }
+    p.slots = p.tail ? p.tail_splits * p.tail * p.block_rows : p.own_splits > 1 ? p.own_splits * rows * kv : 0;
   }
-  p.parts = p.own_splits + p.prefix_splits;
-  p.blocks = p.own_tiles * runs * p.own_splits + p.prefix_tiles * kv * p.prefix_splits;
+  p.blocks = own * p.own_splits + p.tail * (p.tail_splits - 1) + p.prefix_tiles * kv * p.prefix_splits;
   return p;
-}
-
-static int64_t work_of(const Plan& p, int64_t batch, int64_t tokens, int64_t heads, int64_t dim) {
-  return p.parts > 1 ? p.parts * batch * tokens * heads * (dim + 2) : 0;
 }
 
 }  // namespace ff
@@ -762,7 +875,7 @@ const char* bad_sizes(int64_t batch, int64_t tokens, int64_t keys, int64_t prefi
   if (batch != 0 && tokens != 0 && (tokens > 0x7fffffff / batch || batch * tokens > 0x7fffffff / heads))
     return "need batch * tokens * heads < 2^31";
   p = plan_of(batch, tokens, keys, prefix, kv, heads / kv, D);
-  if (p.blocks >= (int64_t(1) << 24) || (p.parts > 1 && batch * tokens * heads > (1 << 26) - 4))
+  if (p.blocks >= (int64_t(1) << 24) || (p.slots > 0 && batch * tokens * heads > (1 << 26) - 4))
     return "too many rows for one launch";
   return nullptr;
 }
@@ -788,7 +901,7 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
   for (const Rows* r : {&k, &v, pk, pv})
     if (r && r->n[1] > 1 && r->stride[1] >= (1 << 24)) return bad("tokens of k and v must be fewer than 2^24 elements apart");
   if (mask_batch < 0) return bad("strides must not be negative");  // a batch of one: index 0 alone
-  const int64_t need = work_of(p, batch, tokens, heads, D);
+  const int64_t need = p.slots * (D + 2);
   if (need > 0 && (!work || work_size < need)) return bad("the workspace is too small");
   if ((reinterpret_cast<uintptr_t>(work) & 15) || (reinterpret_cast<uintptr_t>(lens) & 3)) return bad("misaligned pointer");
   if (overlaps_itself(out, D)) return bad("the rows of out overlap");
@@ -813,13 +926,14 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
   };
   a.own = source(k, v);
   if (pk) a.prefix = source(*pk, *pv);
-  a.lens = lens, a.mask = mask, a.mask_b = mask_batch, a.work = need > 0 ? work : nullptr;
+  a.lens = lens, a.mask = mask, a.mask_b = mask_batch, a.work = need > 0 ? work : nullptr, a.slots = p.slots;
   a.batch = static_cast<int>(batch), a.tokens = static_cast<int>(tokens), a.kv = static_cast<int>(kv);
   a.group = static_cast<int>(heads / kv), a.dim = static_cast<int>(D), a.causal = pk != nullptr;
   a.rows = static_cast<int>(batch * tokens) * a.group;
   a.block_rows = static_cast<int>(p.block_rows), a.own_tiles = static_cast<int>(p.own_tiles);
   a.own_splits = static_cast<int>(p.own_splits), a.prefix_tiles = static_cast<int>(p.prefix_tiles);
   a.prefix_splits = static_cast<int>(p.prefix_splits);
+  a.tail = static_cast<int>(p.tail), a.tail_splits = static_cast<int>(p.tail_splits);
   a.c = scale * 1.4426950408889634f;
   if (dtype == FF_F16)
     launch_cross_dim<half_t>(a, p.blocks, p.stream, as_stream(stream));
@@ -832,13 +946,13 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
 
 extern "C" int64_t ff_cross_attention_work(int64_t B, int64_t L, int64_t S, int64_t heads, int64_t kv_heads, int64_t D) {
   Plan p;
-  return bad_sizes(B, L, S, -1, heads, kv_heads, D, p) ? 0 : work_of(p, B, L, heads, D);
+  return bad_sizes(B, L, S, -1, heads, kv_heads, D, p) ? 0 : p.slots * (D + 2);
 }
 
 extern "C" int64_t ff_prefix_attention_work(int64_t B, int64_t L, int64_t P, int64_t S, int64_t heads, int64_t kv_heads,
                                             int64_t D) {
   Plan p;
-  return P < 0 || bad_sizes(B, L, S, P, heads, kv_heads, D, p) ? 0 : work_of(p, B, L, heads, D);
+  return P < 0 || bad_sizes(B, L, S, P, heads, kv_heads, D, p) ? 0 : p.slots * (D + 2);
 }
 
 extern "C" int ff_cross_attention(const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* k,

@@ -701,9 +701,9 @@ static void launch_cross(const CrossArgs& a, int64_t blocks, int stream, hipStre
   constexpr int CH = DP == 64 ? 8 : 16;
   const int parts = a.tail ? a.tail_splits : a.prefix_splits + a.own_splits;
   const int64_t rows = a.slots / parts;
-  // a row's parts in several lanes at once where they are many (24 576 rows of 2 parts, 64 columns: 6.0 us in one, 14.7 in 8; 16
-  // rows of 32: 17 us in one, 4.6 in 8)
-  if (parts > 4)
+  // a row's parts in several lanes at once where rows are few (16 rows of 32 parts, 64 columns: 17 us in one, 4.6 in 8; 24 576
+  // rows of 2 parts: 6.0 in one, 14.7 in 8)
+  if (rows * CH < 65536)
     join_kernel<T, CH, 64 / CH><<<dim3(static_cast<unsigned>((rows + 3) / 4)), 256, 0, st>>>(a);
   else
     join_kernel<T, CH, 1><<<dim3(static_cast<unsigned>((rows + 4 * (64 / CH) - 1) / (4 * (64 / CH)))), 256, 0, st>>>(a);
@@ -726,7 +726,7 @@ struct Plan {
 };
 
 constexpr int64_t CUS = 256;
-constexpr int64_t ONE_GO = int64_t(1) << 20;  // bytes of keys and values that a workgroup reads before cutting them pays
+constexpr int64_t ONE_GO = int64_t(5) << 16;  // bytes of keys and values up to which a workgroup reads them all (its launch alone takes 8.6 us, two 9 and more)
 
 // Times in us, fitted to launches on this card: a tile of 64 keys takes a workgroup of four units TILE_ALONE at least, and a CU
 // TILE_CU per workgroup in it.
@@ -740,18 +740,22 @@ static Rates rates_of(int64_t D) {
   return {1.2, 1.05, 2};
 }
 
-// Cuts of the keys of `blocks` workgroups that have `tiles` tiles each, beside `others` workgroups (of fewer tiles): the cut that
-// ends first. Each part of a row costs its O, m and l written and read again; a second launch where there would be one part.
-static int64_t split_keys(int64_t blocks, int64_t tiles, int64_t others, int64_t rows, int64_t D, bool joined) {
+// Cuts of the keys of `blocks` workgroups that have `tiles` tiles each, beside `others` workgroups of `theirs`: the cut that ends
+// first. The two kinds share the chip by their tiles; a tile of the others counts half where this is the prefix (its rows fill the
+// matrix cores, theirs wait for memory). Each part of a row costs its O, m and l written and read again; a second launch where
+// there would be one part.
+static int64_t split_keys(int64_t blocks, int64_t tiles, int64_t others, int64_t theirs, int64_t rows, int64_t D, bool joined) {
   if (blocks <= 0 || tiles <= 1) return 1;
   const Rates r = rates_of(D);
+  const double mine = static_cast<double>(blocks) * static_cast<double>(tiles);
+  const double share = mine / (mine + 0.5 * static_cast<double>(others) * static_cast<double>(theirs));
+  const double slots = static_cast<double>(CUS * r.resident) * share;
   int64_t best = 1;
   double least = 0;
   for (int64_t s = 1; s <= std::min<int64_t>(64, (tiles + 1) / 2); ++s) {
-    const double per_cu = static_cast<double>(blocks * s + others) / CUS;
-    const double together = std::min<double>(std::max(per_cu, 1.0), static_cast<double>(r.resident));
-    const double rounds = std::max(1.0, static_cast<double>(blocks * s) / static_cast<double>(CUS * r.resident));
-    const double t = 3.0 + static_cast<double>((tiles + s - 1) / s) * rounds * std::max(r.alone, r.cu * together) +
+    const double together = std::min(static_cast<double>(blocks * s + others) / CUS, static_cast<double>(r.resident));
+    const double rounds = std::max(1.0, static_cast<double>(blocks * s) / slots);
+    const double t = static_cast<double>((tiles + s - 1) / s) * rounds * std::max(r.alone, r.cu * together) +
                      (s > 1 || joined ? 4.0 + static_cast<double>(s * rows * (D + 2)) * 8.0 / 4.5e6 : 0.0);
     if (s == 1 || t < least) least = t, best = s;
   }
@@ -768,7 +772,7 @@ static Plan plan_of(int64_t batch, int64_t tokens, int64_t keys, int64_t prefix,
     p.stream = runs <= CUS ? 8 : 4;
     p.block_rows = QW;
     p.own_tiles = 1;
-    if (cut) p.own_splits = std::max<int64_t>(1, std::min(CUS / std::max<int64_t>(runs, 1), all / 512));
+    if (cut) p.own_splits = std::max<int64_t>(1, std::min(CUS / std::max<int64_t>(runs, 1), all / 256));
     p.slots = p.own_splits > 1 ? p.own_splits * rows * kv : 0;
     p.blocks = runs * p.own_splits;
     return p;
@@ -779,13 +783,14 @@ static Plan plan_of(int64_t batch, int64_t tokens, int64_t keys, int64_t prefix,
   const int64_t own = p.own_tiles * runs, tiles = (keys + BKV - 1) / BKV;
   if (prefix >= 0) {
     p.prefix_tiles = (rows + p.block_rows - 1) / p.block_rows;
-    p.own_splits = split_keys(own, tiles, p.prefix_tiles * kv, rows * kv, D, true);
-    p.prefix_splits = split_keys(p.prefix_tiles * kv, (prefix + BKV - 1) / BKV, own * p.own_splits, rows * kv, D, true);
+    const int64_t shared = p.prefix_tiles * kv, front = (prefix + BKV - 1) / BKV;
+    p.own_splits = split_keys(own, tiles, shared, front, rows * kv, D, true);
+    p.prefix_splits = split_keys(shared, front, own, tiles, rows * kv, D, true);
     p.slots = (p.own_splits + p.prefix_splits) * rows * kv;
   } else {
     const Rates r = rates_of(D);
     const int64_t slots = CUS * r.resident, whole = per / p.block_rows * runs, last = whole % slots;
-    p.own_splits = split_keys(own, tiles, 0, rows * kv, D, false);
+    p.own_splits = split_keys(own, tiles, 0, 0, rows * kv, D, false);
     if (p.own_splits == 1 && whole > slots && last > 0) {
       // The last round's workgroups, cut so that they fill the chip too, if that saves more than the join costs
       const int64_t cuts = std::min<int64_t>(slots / last, tiles / 8);

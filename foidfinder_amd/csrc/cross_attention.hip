@@ -33,6 +33,7 @@ constexpr int QW = 32;     // rows of a unit
 constexpr int WAVES = 4;   // waves a workgroup
 constexpr int BKV = 64;    // keys a tile
 constexpr float SUM_LIMIT = 8192.f;  // a lane's sum of p over a half tile above which m is raised (fp16 holds p up to it)
+constexpr float LIFT = 8.f;          // m is that far below the largest score when it is set: p down to 2^-22 of it is a normal fp16 number
 constexpr float CAP = 12.f;          // exponent of the largest p after m was raised
 constexpr float LOWEST = -3.402823466e38f;
 
@@ -75,6 +76,15 @@ __device__ __forceinline__ float16_t mfma(vec8_t<half_t> a, vec8_t<half_t> b, fl
 }
 __device__ __forceinline__ float16_t mfma(vec8_t<bf16_t> a, vec8_t<bf16_t> b, float16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+typedef bf16_t bf16x2_t __attribute__((ext_vector_type(2)));
+// a + b + c in fp32, subnormal a and b included.
+__device__ __forceinline__ float add_pair(half_t a, half_t b, float c) {
+  return __builtin_amdgcn_fdot2(half2_t{a, b}, half2_t{half_t(1.f), half_t(1.f)}, c, false);
+}
+__device__ __forceinline__ float add_pair(bf16_t a, bf16_t b, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{a, b}, bf16x2_t{bf16_t(1.f), bf16_t(1.f)}, c, false);
 }
 
 // What a workgroup works on; the same in all its lanes.
@@ -160,18 +170,19 @@ struct Unit {
 #pragma unroll
     for (int s = 0; s < KS; ++s) x = mfma(kf[s], qf[s], s == 0 ? zero : x);
   }
-  // p of the scores, at most 2^cap each, and the lane's sum of it.
+  // p of the scores, at most 2^cap each, and the lane's sum of it: of the rounded p, which the second product takes, so that a key
+  // with most of the weight is divided by itself.
   __device__ __forceinline__ float weights(const float16_t& xs, T8 (&pf)[2], float cap) {
-    float sum[4];
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       float x = __builtin_fmaf(xs[r], c, -m);
       if (!__builtin_isinf(cap)) x = x > cap ? cap : x;  // not a number stays so
-      const float e = __builtin_amdgcn_exp2f(x);
-      pf[r >> 3][r & 7] = static_cast<T>(e);
-      sum[r & 3] = r < 4 ? e : sum[r & 3] + e;
+      pf[r >> 3][r & 7] = static_cast<T>(__builtin_amdgcn_exp2f(x));
     }
-    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) sum[(r >> 1) & 1] = add_pair(pf[r >> 3][r & 7], pf[r >> 3][(r & 7) + 1], sum[(r >> 1) & 1]);
+    return sum[0] + sum[1];
   }
   // Scores of keys that the lane's row does not see (bits: those that it sees).
   __device__ __forceinline__ void hide(float16_t& xs, uint32_t bits, int fh) {
@@ -201,7 +212,7 @@ struct Unit {
       for (int r = 1; r < 16; ++r) top = fmaxf(top, xs[r]);
       top = fmaxf(top, xor_shuffle(top, 32)) * c;
       const float m_old = m;
-      m = fmaxf(m, top - fabsf(top) * 0x1p-23f);
+      m = fmaxf(m, top - fabsf(top) * 0x1p-23f - LIFT);
       const float corr = __builtin_amdgcn_exp2f(m_old - m);
       l *= corr;
 #pragma unroll

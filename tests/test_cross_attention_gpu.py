@@ -339,3 +339,231 @@ def test_attention_on_streams_and_in_graphs(dev):
         both(outs[2], outs[3], works[1])
         torch.cuda.synchronize()
         assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3]), n
+
+
+def reference64(q, k, v, scale, seen):
+    """The oracle's three values from torch in float64 on the GPU, for shapes that are too large for it: q [B, L, H, D], k, v
+    [B, S, KV, D], seen bool [B, L or 1, S] (every query sees a key)."""
+    B, L, H, D = q.shape
+    G = H // k.size(2)
+    out = [torch.empty(B, L, H, n, dtype=torch.float64, device=q.device) for n in (D, D, 1)]
+    for b in range(B):
+        for h in range(H):
+            qq, kk, vv = q[b, :, h].double(), k[b, :, h // G].double(), v[b, :, h // G].double()
+            hidden = ~seen[b].expand(L, -1)
+            p = torch.softmax((qq @ kk.t().contiguous() * scale).masked_fill(hidden, -math.inf), -1)
+            out[0][b, :, h], out[1][b, :, h] = p @ vv, p @ vv.abs()
+            load = (qq.abs() @ kk.abs().t().contiguous()).masked_fill(hidden, 0.0)
+            out[2][b, :, h] = load.amax(-1, keepdim=True)
+    return tuple(t.cpu().numpy() for t in out)
+
+
+@pytest.mark.parametrize("kind,D,B,H,KV", [("fp16", 64, 9, 16, 16), ("bf16", 128, 2, 32, 1)])
+def test_cross_attention_last_round_cut(dev, kind, D, B, H, KV):
+    """More row tiles than the chip holds at once, some of them in a last round whose keys are cut, and rows behind the whole tiles."""
+    K = kern()
+    L, S = 1029, 2100
+    g = torch.Generator(device=dev).manual_seed(7)
+    rnd = lambda *s: torch.randn(*s, device=dev, generator=g).to(TYPES[kind])  # noqa: E731
+    q, k, v = rnd(B, L, H, D), rnd(B, S, KV, D), rnd(B, S, KV, D)
+    lens = torch.randint(1, S + 1, (B,), device=dev, generator=g).int()
+    lens[-1], lens[0] = 3, S  # the tail's sequences among them
+    mask = torch.rand(B, S, device=dev, generator=g) < 0.7
+    mask[:, 0] = True
+    out, check = guarded(kind, dev, B, L, H, D)
+    need = K.cross_attention_work(q, k)
+    assert 0 < need < B * L * H * (D + 2), "the shape does not cut the last round alone"
+    work = torch.full((need + 64,), math.nan, device=dev)
+    K.cross_attention(q, k, v, out, D**-0.5, lens, mask, work[:need])
+    assert check() and bool(work[need:].isnan().all())
+    seen = (mask & (torch.arange(S, device=dev) < lens[:, None]))[:, None]
+    o, size, load = reference64(q, k, v, D**-0.5, seen)
+    assert_near(out.float().cpu().numpy(), o, bound(kind, D**-0.5, o, size, load, v.float().abs().max().item(), S))
+
+
+@pytest.mark.parametrize("kind,B,L,P,S,H,KV,D", [("bf16", 40, 3, 3000, 200, 8, 2, 128), ("fp16", 12, 30, 2000, 900, 16, 16, 64),
+                                                 ("fp16", 100, 1, 700, 2500, 4, 4, 96), ("bf16", 3, 200, 64, 5000, 2, 1, 64)])
+def test_prefix_attention_of_many_rows_and_cuts(dev, kind, B, L, P, S, H, KV, D):
+    K = kern()
+    g = torch.Generator(device=dev).manual_seed(8)
+    rnd = lambda *s: torch.randn(*s, device=dev, generator=g).to(TYPES[kind])  # noqa: E731
+    q, pk, pv, k, v = rnd(B, L, H, D), rnd(P, KV, D), rnd(P, KV, D), rnd(B, S, KV, D), rnd(B, S, KV, D)
+    lens = torch.randint(L, S + 1, (B,), device=dev, generator=g).int()
+    out, check = guarded(kind, dev, B, L, H, D)
+    need = K.prefix_attention_work(q, pk, k)
+    assert need > 0
+    work = torch.full((need + 64,), math.nan, device=dev)
+    K.prefix_attention(q, pk, pv, k, v, out, D**-0.5, lens, work[:need])
+    assert check() and bool(work[need:].isnan().all())
+    last = lens[:, None, None] - L + 1 + torch.arange(L, device=dev)[None, :, None]
+    seen = torch.cat((torch.ones(B, L, P, dtype=torch.bool, device=dev), torch.arange(S, device=dev) < last), 2)
+    both = [torch.cat((a[None].expand(B, -1, -1, -1), b), 1) for a, b in ((pk, k), (pv, v))]
+    o, size, load = reference64(q, *both, D**-0.5, seen)
+    assert_near(out.float().cpu().numpy(), o, bound(kind, D**-0.5, o, size, load, both[1].float().abs().max().item(), P + S))
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("L,D", [(1, 64), (40, 128), (128, 96)])
+def test_cross_attention_long_tails(dev, kind, L, D):
+    """60 000 keys of 2^-16 of the largest's weight, below fp16's normal numbers: they hold 48 % of the weight."""
+    K = kern()
+    S = 60001
+    q = torch.zeros(1, L, 1, D, dtype=TYPES[kind], device=dev)
+    k, v = torch.zeros(1, S, 1, D, dtype=TYPES[kind], device=dev), torch.ones(1, S, 1, D, dtype=TYPES[kind], device=dev)
+    q[..., 0], k[0, 7, 0, 0], v[0, 7] = 1.0, 16.0, 0.0
+    out = torch.empty_like(q)
+    K.cross_attention(q, k, v, out, math.log(2), None, None, torch.empty(max(1, K.cross_attention_work(q, k)), device=dev))
+    want = 60000 * 2.0**-16 / (1 + 60000 * 2.0**-16)
+    # weights are powers of two but for scale's and c's roundings; 60 000 fp32 sums by 16 and by cuts
+    assert bool(((out.float() - want).abs() <= want * (HALF[kind] + 60000 / 16 * 2.0**-24 + 2.0**-18)).all())
+
+
+def test_attentions_share_a_workspace(dev):
+    """Calls that run one after another in one stream, with one workspace."""
+    K = kern()
+    g = torch.Generator(device=dev).manual_seed(9)
+    rnd = lambda *s: torch.randn(*s, device=dev, generator=g).half()  # noqa: E731
+    q, k, v, pk, pv = rnd(4, 40, 4, 64), rnd(4, 3000, 2, 64), rnd(4, 3000, 2, 64), rnd(900, 2, 64), rnd(900, 2, 64)
+    need = max(K.cross_attention_work(q, k), K.prefix_attention_work(q, pk, k))
+    one = torch.empty(need, device=dev)
+    got = [torch.empty_like(q) for _ in range(4)]
+    for a, b in ((got[0], got[1]), (got[2], got[3])):
+        K.cross_attention(q, k, v, a, 0.125, None, None, one)
+        K.prefix_attention(q, pk, pv, k, v, b, 0.125, None, one)
+    K.cross_attention(q, k, v, got[0], 0.125, None, None, torch.empty(need, device=dev))
+    K.prefix_attention(q, pk, pv, k, v, got[1], 0.125, None, torch.empty(need, device=dev))
+    assert torch.equal(got[0], got[2]) and torch.equal(got[1], got[3])
+
+
+def test_registered_ops_take_the_same_calls(dev):
+    K = kern()
+    ops = K.kernels()
+    q, k = torch.randn(2, 3, 4, 64, device=dev).half(), torch.randn(2, 50, 2, 64, device=dev).half()
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    ops.cross_attention(q, k, k, a, 0.125)
+    K.cross_attention(q, k, k, b, 0.125)
+    assert torch.equal(a, b)
+    ops.prefix_attention(q, k[0], k[1], k, k, a, 0.125)
+    K.prefix_attention(q, k[0], k[1], k, k, b, 0.125)
+    assert torch.equal(a, b)
+    x, g = torch.randn(5, 64, device=dev).half(), torch.ones(64, device=dev)
+    h = [torch.empty_like(x) for _ in range(4)]
+    ops.residual_norm(x, x, h[0], h[1], 1, g, None, 1, g, None)
+    K.residual_norm(x, x, h[2], h[3], 1, g, None, 1, g, None)
+    assert torch.equal(h[0], h[2]) and torch.equal(h[1], h[3])
+
+
+def test_python_refusals_on_the_gpu(dev):
+    K = kern()
+    q, k = torch.randn(2, 3, 4, 64, device=dev).half(), torch.randn(2, 50, 2, 64, device=dev).half()
+    out = torch.empty_like(q)
+    bad = [
+        (dict(k=k.bfloat16()), "type"), (dict(k=k.cpu()), "device"), (dict(k=k[:1]), "B and D"), (dict(v=k[:, :9]), "one shape"),
+        (dict(out=out[:, :2]), "shape"), (dict(out=out.float()), "type"), (dict(q=q[0]), "B, L, heads, D"),
+        (dict(q=q.transpose(2, 3).contiguous().transpose(2, 3)), "contiguous columns"),
+        (dict(lens=torch.ones(2, device=dev)), "int32"), (dict(lens=torch.ones(3, dtype=torch.int32, device=dev)), "int32"),
+        (dict(mask=torch.ones(2, 50, device=dev)), "bool"), (dict(mask=torch.ones(2, 49, dtype=torch.bool, device=dev)), "bool"),
+        (dict(mask=torch.ones(50, 2, dtype=torch.bool, device=dev).t()), "contiguous columns"),
+        (dict(work=torch.ones(9, device=dev).half()), "fp32"), (dict(out=q), "overlaps"), (dict(scale=0.0), "scale"),
+        (dict(q=q.clone().requires_grad_()), "no backward"),
+    ]
+    for change, word in bad:
+        args = dict(q=q.detach(), k=k, v=k, out=out, scale=0.125) | change
+        with pytest.raises(RuntimeError, match=word):
+            K.cross_attention(**args)
+    with pytest.raises(RuntimeError, match=r"\[P, kv_heads, D\]"):
+        K.prefix_attention(q.detach(), k[0, :, :1], k[0, :, :1], k, k, out, 0.125)
+    x = torch.randn(4, 64, device=dev).half()
+    g = torch.ones(64, device=dev)
+    for change, word in [(dict(y=x.float()), "type"), (dict(h=None), "h goes"), (dict(gate=g[:8]), "gate"),
+                         (dict(gate=torch.ones(3, 64, device=dev)), "multiple of the gate"), (dict(post_gamma=g[:32]), "64 elements"),
+                         (dict(gate=torch.ones(0, 64, device=dev)), "gate"), (dict(x=x.t().contiguous().t()), "contiguous rows")]:
+        args = dict(x=x, y=x, x_out=torch.empty_like(x), h=torch.empty_like(x), post=1, post_gamma=g, post_beta=None, pre=1,
+                    pre_gamma=g, pre_beta=None) | change
+        with pytest.raises(RuntimeError, match=word):
+            K.residual_norm(**args)
+
+
+def test_decoder_block_eager_and_captured(dev):
+    """A decoder block over an image's tokens: norms, 4-bit linears, head norms with rotation, attention behind the image's tokens
+    as a shared prefix, cross attention to another image's tokens, each attention held to the oracle on the inputs it got; the
+    captured run replayed over new inputs gives the eager run's bits."""
+    K = kern()
+    B, L, C, H, KV, P, S = 3, 2, 512, 8, 4, 200, 70
+    T, D = B * L, 64
+    g = torch.Generator(device=dev).manual_seed(10)
+    rnd = lambda *s, std=1.0: torch.randn(*s, device=dev, generator=g) * std  # noqa: E731
+    mx = lambda n, c: (torch.empty(n, c // 2, dtype=torch.uint8, device=dev),  # noqa: E731
+                       torch.empty(c // 128, n, dtype=torch.int32, device=dev))
+
+    def linear(n):
+        codes = mx(n, C)
+        K.quant_mx4(rnd(n, C, std=C**-0.5).half(), *codes)
+        return codes, rnd(n, std=0.02)
+
+    wide = (H + 2 * KV) * D
+    w_qkv, w_o, w_q, w_co = linear(wide), linear(C), linear(H * D), linear(C)
+    norms = [(1 + rnd(C, std=0.1), rnd(C, std=0.1)) for _ in range(5)]
+    hg = [1 + rnd(D, std=0.1) for _ in range(2)]
+    gate = rnd(C, std=0.5)
+    ang = torch.arange(400, device=dev)[:, None] * 10000.0 ** (-torch.arange(D // 2, device=dev) / (D // 2))
+    cos, sin = ang.cos().contiguous(), ang.sin().contiguous()
+    x0, y0 = rnd(T, C).half(), rnd(T, C).half()
+    pk, pv = rnd(P, KV, D).half(), rnd(P, KV, D).half()
+    cache_k, cache_v = rnd(B, KV, S, D).half().transpose(1, 2), rnd(B, KV, S, D).half().transpose(1, 2)
+    enc = rnd(B, 150, 2, KV, D).half()
+    mask = torch.rand(B, 150, device=dev, generator=g) < 0.6
+    lens = torch.tensor([70, 2, 33], dtype=torch.int32, device=dev)
+    positions = (P + lens[:, None] - L + torch.arange(L, device=dev)).flatten().int()
+
+    def block(t):
+        """One block into the tensors of t."""
+        K.residual_norm(x0, y0, t["x"], t["h"], K.NORM_RMS, norms[0][0], None, K.NORM_LAYER, *norms[1], gate, 0.5)
+        K.quant_mx4(t["h"], *t["a"])
+        K.gemm_mx4(*t["a"], *w_qkv[0], w_qkv[1], t["qkv"], K.EPI_BIAS_F16)
+        rows = t["qkv"].view(T, H + 2 * KV, D)
+        q, k, v = rows[:, :H], rows[:, H : H + KV], rows[:, H + KV :]
+        K.qk_norm_rope(q, k, q, k, K.NORM_RMS, *hg, None, None, cos, sin, positions)
+        at = torch.arange(B, device=dev)[:, None], (lens[:, None] - L + torch.arange(L, device=dev)).long()
+        t["k"].copy_(cache_k)
+        t["v"].copy_(cache_v)
+        t["k"][at], t["v"][at] = k.view(B, L, KV, D), v.view(B, L, KV, D)  # the new tokens' own rows
+        K.prefix_attention(q.view(B, L, H, D), pk, pv, t["k"], t["v"], t["o"], D**-0.5, lens, t["work"])
+        K.quant_mx4(t["o"].view(T, C), *t["a"])
+        K.gemm_mx4(*t["a"], *w_o[0], w_o[1], t["y"], K.EPI_BIAS_F16)
+        K.residual_norm(t["x"], t["y"], t["x"], t["h"], K.NORM_RMS, norms[2][0], None, K.NORM_RMS, norms[3][0], None)
+        K.quant_mx4(t["h"], *t["a"])
+        K.gemm_mx4(*t["a"], *w_q[0], w_q[1], t["q"], K.EPI_BIAS_F16)
+        K.cross_attention(t["q"].view(B, L, H, D), enc[:, :, 0], enc[:, :, 1], t["c"], D**-0.5, None, mask, t["work"])
+        K.quant_mx4(t["c"].view(T, C), *t["a"])
+        K.gemm_mx4(*t["a"], *w_co[0], w_co[1], t["y"], K.EPI_BIAS_F16)
+        K.residual_norm(t["x"], t["y"], t["x"], None, K.NORM_LAYER, *norms[4], K.NORM_NONE, None, None, gate)
+        return t["x"]
+
+    def tensors():
+        e = lambda *s: torch.empty(*s, dtype=torch.float16, device=dev)  # noqa: E731
+        t = dict(x=e(T, C), h=e(T, C), y=e(T, C), qkv=e(T, wide), q=e(T, H * D), o=e(B, L, H, D), c=e(B, L, H, D),
+                 k=e(B, KV, S, D).transpose(1, 2), v=e(B, KV, S, D).transpose(1, 2), a=mx(T, C))
+        need = max(K.prefix_attention_work(t["o"], pk, t["k"]), K.cross_attention_work(t["o"], enc[:, :, 0]))
+        return t | dict(work=torch.empty(max(need, 1), device=dev))
+
+    a, b = tensors(), tensors()
+    block(a)
+    torch.cuda.synchronize()
+    assert bool(a["x"].isfinite().all())
+    n = lambda t: t.float().cpu().numpy()  # noqa: E731
+    q = n(a["qkv"].view(B, L, H + 2 * KV, D)[:, :, :H])
+    o, size, load = OC.prefix_attention(q, n(pk), n(pv), n(a["k"]), n(a["v"]), D**-0.5, lens.tolist())
+    assert_near(n(a["o"]), o, bound("fp16", D**-0.5, o, size, load, max(np.abs(n(a["v"])).max(), np.abs(n(pv)).max()), P + S))
+    o, size, load = OC.cross_attention(n(a["q"].view(B, L, H, D)), n(enc[:, :, 0]), n(enc[:, :, 1]), D**-0.5, None, mask.cpu().numpy())
+    assert_near(n(a["c"]), o, bound("fp16", D**-0.5, o, size, load, np.abs(n(enc)).max(), 150))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        block(a)
+    for _ in range(3):
+        x0.copy_(rnd(T, C).half())
+        enc.copy_(rnd(*enc.shape).half())
+        graph.replay()
+        block(b)
+        torch.cuda.synchronize()
+        assert torch.equal(a["x"], b["x"])

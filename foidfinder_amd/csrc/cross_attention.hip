@@ -32,8 +32,7 @@ namespace ff {
 constexpr int QW = 32;     // rows of a unit
 constexpr int WAVES = 4;   // waves a workgroup
 constexpr int BKV = 64;    // keys a tile
-constexpr float SUM_LIMIT = 8192.f;  // a lane's sum of p over a half tile above which m is raised (fp16 holds p up to it)
-constexpr float LIFT = 8.f;          // m is that far below the largest score when it is set: p down to 2^-22 of it is a normal fp16 number
+constexpr float SUM_LIMIT = 32768.f;  // a lane's sum of 16 p above which m is raised (fp16 holds p up to it)
 constexpr float CAP = 12.f;          // exponent of the largest p after m was raised
 constexpr float LOWEST = -3.402823466e38f;
 
@@ -212,7 +211,7 @@ struct Unit {
       for (int r = 1; r < 16; ++r) top = fmaxf(top, xs[r]);
       top = fmaxf(top, xor_shuffle(top, 32)) * c;
       const float m_old = m;
-      m = fmaxf(m, top - fabsf(top) * 0x1p-23f - LIFT);
+      m = fmaxf(m, top - fabsf(top) * 0x1p-23f);
       const float corr = __builtin_amdgcn_exp2f(m_old - m);
       l *= corr;
 #pragma unroll

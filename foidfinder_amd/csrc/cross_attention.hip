@@ -7,29 +7,19 @@
 // for the second product, half a step each, which is what the matrix cores take.
 //
 // Rows: the G = heads / kv_heads query heads of a key head read the same keys, so a key head's rows are (sequence, token, head
-// of the group), 32 of them a unit.
-// Tiles (cross_kernel): four waves and up to 128 rows, K and V in tiles of 64 keys through two LDS slots that all waves read. Four
-// units: a wave each. Two: two waves a unit, each over one half of every tile. One is streamed.
-// Streams (stream_kernel; up to 32 rows a sequence and key head): four or eight waves share a unit, each with keys of its own, 32
-// at a time through LDS of its own, without a barrier until the waves' O, m and l are joined.
-// Keys: a workgroup runs over all keys of its rows, or over one of several runs of them where there are few rows, or where a last
-// round of workgroups would leave much of the chip idle (Plan). The runs' O, m and l go to the workspace in fp32 and join_kernel
-// joins them in a fixed order.
+// of the group). A workgroup has four waves and 32, 64 or 128 rows; 32 rows are a unit. Four units: a wave each, over all
+// keys. Two: two waves a unit, each over one half of every 64-key tile. One (single tokens): all four share it, by halves and by
+// tiles of either parity. Waves that share a unit are joined through LDS.
+// Keys: a workgroup runs over all keys of its rows, or, where rows are few, over one of several runs of tiles; the runs' O, m
+// and l then go to the workspace in fp32 and join_kernel joins them in a fixed order.
 // Shared prefix: its keys have no sequence, so the rows of all sequences together read it; the same launch's other workgroups
-// take each sequence's own keys, and join_kernel joins the parts. Streams of one sequence, or of short prefixes, read both.
-// Masks: seen_kernel lists the keys that a sequence's mask leaves, and tiles hold only those; short calls and streams load what a
-// tile's mask leaves and skip tiles that it leaves empty.
+// take each sequence's own keys, and join_kernel joins the parts.
 //
-// Loads go straight into LDS. Rows that no query of the workgroup may see (past the length, or masked) and columns past D are
-// out of the descriptor's range: they read as zeros and cost no traffic, and what the memory there holds never reaches a product.
-// Per wave, S^T = K Q^T by 32x32x16 products leaves a lane with one query and 16 of 32 keys; P^T then is the column operand of
-// O^T = V^T P^T, V read with the transposing ds_read_b64_tr_b16. Both tiles are row-major, their 16-byte chunks XOR-swizzled
-// against bank conflicts (counted: none).
-//
-// What bounds it, measured: long keys, the softmax between the products (at 128 columns, 4 x 1024 queries, 4096 keys, 32 / 8
-// heads: matrix cores busy 48 % of the time, vector units 46 %, both at once 42 %; 870 TF/s bf16 on random values, which cost a
-// fifth more time than zeros; 64 columns 8 x 1024 x 4096 x 16: 810 TF/s, 96 columns 850). Few rows, memory: 64 single tokens
-// against 1025 keys of 16 / 8 heads x 128, lengths 1 .. 1025: 4.4 TB/s of the keys read.
+// K and V stream through two LDS slots of 64 keys (buffer loads straight into LDS). Rows that no query of the workgroup may see
+// (past the length, or masked) and columns past D are loads out of the descriptor's range: they read as zeros and cost no
+// traffic, and what the memory there holds never reaches a product. Per wave, S^T = K Q^T by 32x32x16 products leaves a lane
+// with one query and 16 of 32 keys; P^T then is the column operand of O^T = V^T P^T, V read with the transposing
+// ds_read_b64_tr_b16. Both tiles are row-major, their 16-byte chunks XOR-swizzled against bank conflicts.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -67,7 +57,6 @@ struct CrossArgs {
   int block_rows, own_tiles, own_splits, prefix_tiles, prefix_splits;
   int tail, tail_splits;  // the last row tiles of the grid, whose keys are cut (no prefix, own_splits 1)
   float c;
-  int32_t* seen;  // null, or the keys that the mask leaves: how many [batch], then which [batch, keys]
 };
 
 // Physical 16-byte chunk of chunk c in row r of a tile (its own inverse). K is read 16 rows of a chunk at a time, V 4 rows of
@@ -168,8 +157,14 @@ struct Unit {
   // x = S^T of the 32 keys at k (+ ka): keys 8 (r / 4) + 4 fh + r % 4.
   __device__ __forceinline__ void score(float16_t& x, const T* k, int ka, int ka_odd) {
     T8 kf[KS];
+    keys(kf, k, ka, ka_odd);
+    score(x, kf);
+  }
+  __device__ __forceinline__ void keys(T8 (&kf)[KS], const T* k, int ka, int ka_odd) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) kf[s] = *reinterpret_cast<const T8*>(k + kfrag(ka, ka_odd, s));
+  }
+  __device__ __forceinline__ void score(float16_t& x, const T8 (&kf)[KS]) {
     const float16_t zero = {};
 #pragma unroll
     for (int s = 0; s < KS; ++s) x = mfma(kf[s], qf[s], s == 0 ? zero : x);
@@ -196,7 +191,8 @@ struct Unit {
       for (int r = 0; r < 16; ++r) xs[r] = (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? xs[r] : -__builtin_inff();
     }
   }
-  // p of the scores; bits: the keys that the lane's row sees; first: m is not set yet, which the first pass would only find out.
+  // p of the scores; bits: the keys that the lane's row sees.
+  // first: m is not set yet, which the first pass would only find out.
   __device__ __forceinline__ void weigh(float16_t& xs, T8 (&pf)[2], uint32_t bits, int fh, bool first) {
     hide(xs, bits, fh);
     float sum = 0.f;
@@ -209,19 +205,21 @@ struct Unit {
   // The keys' p passed the limit, or m is not set: m becomes the largest c S of the keys, or just below, and O and l follow. Scores
   // from 2^30 up are too coarse for the multiply-add: what it leaves of the largest can be of any size then, and is capped.
   __device__ __forceinline__ void raise(const float16_t& xs, T8 (&pf)[2]) {
-    float top = xs[0];
+    {
+      float top = xs[0];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) top = fmaxf(top, xs[r]);
-    top = fmaxf(top, xor_shuffle(top, 32)) * c;
-    const float m_old = m;
-    m = fmaxf(m, top - fabsf(top) * 0x1p-23f);
-    const float corr = __builtin_amdgcn_exp2f(m_old - m);
-    l *= corr;
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, xs[r]);
+      top = fmaxf(top, xor_shuffle(top, 32)) * c;
+      const float m_old = m;
+      m = fmaxf(m, top - fabsf(top) * 0x1p-23f);
+      const float corr = __builtin_amdgcn_exp2f(m_old - m);
+      l *= corr;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[dt][r] *= corr;
-    l += weights(xs, pf, CAP);
+        for (int r = 0; r < 16; ++r) o[dt][r] *= corr;
+      l += weights(xs, pf, CAP);
+    }
   }
   // O^T += V^T P^T, the 32 values at LDS byte v + OFF (+ va).
   template <int OFF>
@@ -261,9 +259,8 @@ __device__ __forceinline__ void store4(const CrossArgs& a, const Piece& w, const
   *reinterpret_cast<vec4_t<T>*>(static_cast<T*>(a.out) + p.seq * a.ob + p.token * a.ot + p.head * a.oh + col) = v;
 }
 
-// Tiles of 64 keys for four waves: a wave a unit (SHARE 1), or two (SHARE 2), each with one half of every tile. LIST: tile n holds
-// the keys 64 n .. of a.seen, no masked ones.
-template <typename T, int DP, int SHARE, bool LIST>
+// Tiles of 64 keys for four waves: a wave a unit (SHARE 1), or two (SHARE 2), each with one half of every tile.
+template <typename T, int DP, int SHARE>
 __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T* smem) {
   typedef vec8_t<T> T8;
   constexpr int CH = DP / 8, TILE = BKV * DP, LPW = CH / 4, KS = DP / 16, DT = DP / 32;
@@ -283,8 +280,7 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
   const int64_t at = max(w.seq, 0);
   const T* kbase = static_cast<const T*>(src.k) + at * src.kb + w.head * src.kh;
   const T* vbase = static_cast<const T*>(src.v) + at * src.vb + w.head * src.vh;
-  const uint8_t* mask = !LIST && a.mask && w.seq >= 0 ? a.mask + at * a.mask_b : nullptr;
-  const int32_t* seen = LIST ? a.seen + a.batch + at * a.own.keys : nullptr;  // w.keys of them
+  const uint8_t* mask = a.mask && w.seq >= 0 ? a.mask + at * a.mask_b : nullptr;
   const bool guard = mask || src.kt < a.dim || src.vt < a.dim;  // rows left out that the descriptor's range does not leave out
 
   // Tile loads: wave w fills the 1 KB blocks LPW w .. of either tile, lane l the chunk l of a block; it fetches what the swizzle
@@ -297,31 +293,7 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
     voff_k[i] = 8 * ck < a.dim ? static_cast<uint32_t>((r * static_cast<int>(src.kt) + ck * 8) * 2) : OOB_OFFSET;
     voff_v[i] = 8 * cv < a.dim ? static_cast<uint32_t>((r * static_cast<int>(src.vt) + cv * 8) * 2) : OOB_OFFSET;
   }
-  // Of a list, the key in the place of the row that load i fetches (read a tile ahead).
-  int key[LIST ? LPW : 1];
-  auto lrow = [&](int i) __attribute__((always_inline)) { return ((LPW * wave + i) * 64 + lane) / CH; };
-  auto look_up = [&](int tile) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < LPW; ++i) {
-      const int n = tile * BKV + lrow(i);
-      key[i] = n < w.keys ? seen[n] : -1;
-    }
-  };
   auto issue = [&](int tile, uint64_t word) __attribute__((always_inline)) {
-    if constexpr (LIST) {
-      const int st = (tile - w.t0) & 1, kt = static_cast<int>(src.kt), vt = static_cast<int>(src.vt);
-      const int nk = ((a.own.keys - 1) * kt + a.dim) * 2, nv = ((a.own.keys - 1) * vt + a.dim) * 2;
-#pragma unroll
-      for (int i = 0; i < LPW; ++i) {
-        // by 0 .. 2^31 - 1 bytes on, as key n of a list is n at least: what was out of range stays so
-        const uint32_t ko = voff_k[i] + static_cast<uint32_t>((key[i] - lrow(i)) * kt) * 2;
-        const uint32_t vo = voff_v[i] + static_cast<uint32_t>((key[i] - lrow(i)) * vt) * 2;
-        const bool in = key[i] >= 0;
-        buffer_to_lds(kbase, nk, reinterpret_cast<uint8_t*>(smem + st * TILE + (LPW * wave + i) * 512), in ? ko : OOB_OFFSET);
-        buffer_to_lds(vbase, nv, reinterpret_cast<uint8_t*>(smem + (2 + st) * TILE + (LPW * wave + i) * 512), in ? vo : OOB_OFFSET);
-      }
-      return;
-    }
     const int st = (tile - w.t0) & 1, rows = min(BKV, w.keys - tile * BKV);
     const int64_t first = static_cast<int64_t>(tile) * BKV;
     const int nk = ((rows - 1) * static_cast<int>(src.kt) + a.dim) * 2, nv = ((rows - 1) * static_cast<int>(src.vt) + a.dim) * 2;
@@ -378,9 +350,7 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
   if (w.t0 < w.t1) {
     uint64_t word = valid(w.t0, mask_byte(w.t0)), next = 0;
     uint8_t byte = mask_byte(w.t0 + 1);
-    if constexpr (LIST) look_up(w.t0);
     issue(w.t0, word);
-    if constexpr (LIST) look_up(w.t0 + 1);
     u.settle();
     for (int tile = w.t0; tile < w.t1; ++tile) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -389,7 +359,6 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
         next = valid(tile + 1, byte);
         issue(tile + 1, next);
         byte = mask_byte(tile + 2);
-        if constexpr (LIST) look_up(tile + 2);
       }
       const int st = (tile - w.t0) & 1;
       if (active && word != 0) {
@@ -450,10 +419,10 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
                 float4_t{u.o[dt][4 * g], u.o[dt][4 * g + 1], u.o[dt][4 * g + 2], u.o[dt][4 * g + 3]}, u.m, l);
 }
 
-// One unit of rows and NW waves, each with slices of 32 keys of its own (slice t0 + wave, + NW, ...) in LDS of its own, so no
-// barrier stands between load and use: a wave asks for the next slice's K once it has read this one's, and for its V likewise, so
-// that half a slice or more (8 KB at 128 columns) is on its way to each wave at any time. The slices are those of the prefix
-// (w.front), then the sequence's own. The waves' O, m and l are joined through LDS, four columns a wave and turn.
+// One unit of rows and WAVES waves, each with slices of 32 keys of its own (slice t0 + wave, + WAVES, ...) in LDS of its own, so no
+// barrier stands between load and use: a wave asks for the next slice's K once it has read this one's, and for its V likewise, and
+// has 64 KB (128 columns; 8 waves) or 128 KB (16) of the CU's reads in flight. The slices are those of the prefix (w.front), then the
+// sequence's own. The waves' O, m and l are joined through LDS, four columns a wave and turn.
 template <typename T, int DP, int NW>
 __device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w, T* smem) {
   typedef vec8_t<T> T8;
@@ -588,7 +557,7 @@ constexpr int stream_bytes(int dp, int waves) {
 constexpr int tile_bytes(int dp) { return 4 * BKV * dp * 2 > stream_bytes(dp, WAVES) ? 4 * BKV * dp * 2 : stream_bytes(dp, WAVES); }
 
 // Waves a SIMD: what the LDS leaves room for (34, 50 and 66 KB a workgroup).
-template <typename T, int DP, bool LIST>
+template <typename T, int DP>
 __global__ __launch_bounds__(64 * WAVES, DP == 64 ? 4 : DP == 96 ? 3 : 2) void cross_kernel(const CrossArgs a) {
   __shared__ __attribute__((aligned(1024))) T smem[tile_bytes(DP) / 2];  // K slots, then V slots
   touch(a);
@@ -639,7 +608,6 @@ __global__ __launch_bounds__(64 * WAVES, DP == 64 ? 4 : DP == 96 ? 3 : 2) void c
     }
   }
   const int units = (min(a.block_rows, w.row_end - w.row0) + QW - 1) / QW, step = units == 1 ? 32 : BKV;
-  if (LIST && units > 1) w.keys = a.seen[w.seq];  // streams read the mask itself
   const int steps = (w.keys + step - 1) / step;
   w.t0 = static_cast<int>(static_cast<int64_t>(steps) * split / splits);
   w.t1 = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / splits);
@@ -647,9 +615,9 @@ __global__ __launch_bounds__(64 * WAVES, DP == 64 ? 4 : DP == 96 ? 3 : 2) void c
   if (units == 1)
     stream_block<T, DP, WAVES>(a, w, smem);
   else if (units == 2)
-    tile_block<T, DP, 2, LIST>(a, w, smem);
+    tile_block<T, DP, 2>(a, w, smem);
   else
-    tile_block<T, DP, 1, LIST>(a, w, smem);
+    tile_block<T, DP, 1>(a, w, smem);
 }
 
 // Up to 32 rows a sequence and key head: workgroups of NW waves that all read the same rows' keys, the prefix's among them. Where
@@ -670,46 +638,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : DP == 64 ? 4 : DP == 96 ? 3 
   w.t0 = static_cast<int>(slices * split / a.own_splits);
   w.t1 = static_cast<int>(slices * (split + 1) / a.own_splits);
   stream_block<T, DP, NW>(a, w, smem);
-}
-
-// The keys of a sequence that the mask and the length leave, in order, for tiles that hold no others: 16 keys a thread, their
-// count summed over the workgroup. A workgroup a sequence.
-__global__ __launch_bounds__(1024) void seen_kernel(const CrossArgs a) {
-  __shared__ int counts[16];
-  const int tid = threadIdx.x, lane = tid & 63, seq = blockIdx.x;
-  const int keys = a.lens ? min(max(a.lens[seq], 0), a.own.keys) : a.own.keys;
-  const uint8_t* mask = a.mask + seq * a.mask_b;
-  int32_t* to = a.seen + a.batch + static_cast<int64_t>(seq) * a.own.keys;
-  int base = 0;
-  for (int64_t first = 0; first < keys; first += 16 * 1024) {
-    const int64_t k0 = first + 16 * tid;
-    uint32_t bits = 0;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const uint8_t byte = mask[min(k0 + e, static_cast<int64_t>(keys) - 1)];
-      bits |= byte != 0 && k0 + e < keys ? 1u << e : 0u;
-    }
-    const int mine = __popc(bits);
-    int before = mine;  // in the wave, this thread's with them
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int other = __shfl_up(before, d, 64);
-      before += lane >= d ? other : 0;
-    }
-    __syncthreads();  // the last turn's counts have been read
-    if (lane == 63) counts[tid >> 6] = before;
-    __syncthreads();
-    int at = base + before - mine;
-    for (int w = 0; w < 16; ++w) {
-      const int n = counts[w];
-      at += w < tid >> 6 ? n : 0;
-      base += n;
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (bits >> e & 1) to[at++] = static_cast<int32_t>(k0 + e);
-  }
-  if (tid == 0) a.seen[seq] = base;
 }
 
 // Joins the parts of a row: CH lanes for its columns (8 each), LANES times over for as many parts at a time, joined at the end.
@@ -773,15 +701,12 @@ __global__ __launch_bounds__(256) void join_kernel(const CrossArgs a) {
 template <typename T, int DP>
 static void launch_cross(const CrossArgs& a, int64_t blocks, int stream, hipStream_t st) {
   const dim3 runs(a.batch, a.kv, a.own_splits);
-  if (a.seen) seen_kernel<<<dim3(a.batch), 1024, 0, st>>>(a);
   if (stream == 8)
     stream_kernel<T, DP, 8><<<runs, 64 * 8, 0, st>>>(a);
   else if (stream == 4)
     stream_kernel<T, DP, 4><<<runs, 64 * 4, 0, st>>>(a);
-  else if (a.seen)
-    cross_kernel<T, DP, true><<<dim3(static_cast<unsigned>(blocks)), 64 * WAVES, 0, st>>>(a);
   else
-    cross_kernel<T, DP, false><<<dim3(static_cast<unsigned>(blocks)), 64 * WAVES, 0, st>>>(a);
+    cross_kernel<T, DP><<<dim3(static_cast<unsigned>(blocks)), 64 * WAVES, 0, st>>>(a);
   if (!a.work) return;
   constexpr int CH = DP == 64 ? 8 : 16;
   const int parts = a.tail ? a.tail_splits : a.prefix_splits + a.own_splits;
@@ -808,7 +733,6 @@ static void launch_cross_dim(const CrossArgs& a, int64_t blocks, int stream, hip
 struct Plan {
   int stream;  // waves of stream_kernel's workgroups, 0: cross_kernel
   int64_t block_rows, own_tiles, own_splits, prefix_tiles, prefix_splits, tail, tail_splits, slots, blocks;
-  int64_t listed;  // elements for a list of the keys that a mask leaves, 0 where it does not pay
 };
 
 constexpr int64_t CUS = 256;
@@ -875,12 +799,6 @@ static Plan plan_of(int64_t batch, int64_t tokens, int64_t keys, int64_t prefix,
     p.slots = (p.own_splits + p.prefix_splits) * rows * kv;
   } else {
     const Rates r = rates_of(D);
-    // Keys left by a mask are listed from 30 us of whole tiles on: the list takes 5 us and its tiles' loads 4 % more time, which
-    // pays where enough is masked. Times in us for half the keys masked at random, a third at the end, none: 40 -> 31, 36 -> 34,
-    // 37 -> 40 at 20 us (4 x 512 queries, 2048 keys, 16 heads x 64); 62 -> 38, 46 -> 47, 56 -> 61 at 34 us (2 x 512, 2048, 32 / 8 x
-    // 128); 330 -> 182, 226 -> 228, 289 -> 300 at 275 us (4 x 1024, 4096, 32 / 8 x 128). A workgroup a sequence, so no more of them
-    // than a launch takes.
-    if (static_cast<double>(own * tiles) * r.cu / CUS > 30.0 && batch < (1 << 20)) p.listed = batch * (keys + 1);
     const int64_t slots = CUS * r.resident, whole = per / p.block_rows * runs, last = whole % slots;
     p.own_splits = split_keys(own, tiles, 0, 0, rows * kv, D, false);
     if (p.own_splits == 1 && whole > slots && last > 0) {
@@ -985,8 +903,7 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
   if (dtype != FF_F16 && dtype != FF_BF16) return bad("q, k, v and out must be fp16 or bf16");
   Plan p;
   if (const char* msg = bad_sizes(batch, tokens, keys, prefix, heads, kv, D, p)) return bad(msg);
-  const float c = scale * 1.4426950408889634f;  // log2(e)
-  if (!(scale > 0.f) || !std::isfinite(c)) return bad("scale must be > 0, and finite times log2(e)");
+  if (!(scale > 0.f) || !std::isfinite(scale)) return bad("scale must be finite and > 0");
   if (batch == 0 || tokens == 0) return FF_OK;
   const Rows* given[6] = {&q, &k, &v, pk, pv, &out};
   for (const Rows* r : given) {
@@ -1001,22 +918,18 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
   if (mask_batch < 0) return bad("strides must not be negative");  // a batch of one: index 0 alone
   const int64_t need = p.slots * (D + 2);
   if (need > 0 && (!work || work_size < need)) return bad("the workspace is too small");
-  // where there is room for the list; a sequence's rows by 32-bit offsets
-  const bool listed = mask && p.listed > 0 && work && work_size >= need + p.listed &&
-                      keys * std::max(k.stride[1], v.stride[1]) < (int64_t(1) << 30) - D;
   if ((reinterpret_cast<uintptr_t>(work) & 15) || (reinterpret_cast<uintptr_t>(lens) & 3)) return bad("misaligned pointer");
   if (overlaps_itself(out, D)) return bad("the rows of out overlap");
   // Rows are read and written by different workgroups, in no order.
-  const Extent to = extent_of(out, D), scratch = range(work, (need + (listed ? p.listed : 0)) * 4);
+  const Extent to = extent_of(out, D), scratch = range(work, need * 4);
   const Extent read[7] = {extent_of(q, D), extent_of(k, D), extent_of(v, D), pk ? extent_of(*pk, D) : range(nullptr, 0),
                           pv ? extent_of(*pv, D) : range(nullptr, 0), range(lens, lens ? batch * 4 : 0),
                           Extent{reinterpret_cast<uintptr_t>(mask), {batch, 1}, {mask_batch, 0}, mask ? keys : 0}};
-  const bool used = scratch.len > 0;
-  if (used && !clear_of(to, scratch)) return bad("out overlaps the workspace");
+  if (!clear_of(to, scratch)) return bad("out overlaps the workspace");
   for (const Extent& e : read) {
     if (e.len == 0) continue;
     if (!clear_of(to, e)) return bad("out overlaps what is read");
-    if (used && !clear_of(scratch, e)) return bad("the workspace overlaps what is read");
+    if (need > 0 && !clear_of(scratch, e)) return bad("the workspace overlaps what is read");
   }
   CrossArgs a{};
   a.q = q.p, a.out = const_cast<void*>(out.p);
@@ -1028,8 +941,7 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
   };
   a.own = source(k, v);
   if (pk) a.prefix = source(*pk, *pv);
-  a.lens = lens, a.mask = mask, a.mask_b = mask_batch, a.work = p.slots > 0 ? work : nullptr, a.slots = p.slots;
-  a.seen = listed ? reinterpret_cast<int32_t*>(work + need) : nullptr;
+  a.lens = lens, a.mask = mask, a.mask_b = mask_batch, a.work = need > 0 ? work : nullptr, a.slots = p.slots;
   a.batch = static_cast<int>(batch), a.tokens = static_cast<int>(tokens), a.kv = static_cast<int>(kv);
   a.group = static_cast<int>(heads / kv), a.dim = static_cast<int>(D), a.causal = pk != nullptr;
   a.rows = static_cast<int>(batch * tokens) * a.group;
@@ -1037,7 +949,7 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
   a.own_splits = static_cast<int>(p.own_splits), a.prefix_tiles = static_cast<int>(p.prefix_tiles);
   a.prefix_splits = static_cast<int>(p.prefix_splits);
   a.tail = static_cast<int>(p.tail), a.tail_splits = static_cast<int>(p.tail_splits);
-  a.c = c;
+  a.c = scale * 1.4426950408889634f;
   if (dtype == FF_F16)
     launch_cross_dim<half_t>(a, p.blocks, p.stream, as_stream(stream));
   else
@@ -1049,7 +961,7 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
 
 extern "C" int64_t ff_cross_attention_work(int64_t B, int64_t L, int64_t S, int64_t heads, int64_t kv_heads, int64_t D) {
   Plan p;
-  return bad_sizes(B, L, S, -1, heads, kv_heads, D, p) ? 0 : p.slots > 0 ? p.slots * (D + 2) + p.listed : 0;
+  return bad_sizes(B, L, S, -1, heads, kv_heads, D, p) ? 0 : p.slots * (D + 2);
 }
 
 extern "C" int64_t ff_prefix_attention_work(int64_t B, int64_t L, int64_t P, int64_t S, int64_t heads, int64_t kv_heads,

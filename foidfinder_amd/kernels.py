@@ -649,12 +649,10 @@ def _columns(ones: tuple, *ts: torch.Tensor) -> None:
             raise RuntimeError("q, keys, values and out must have contiguous columns")
 
 
-def cross_attention_work(q: torch.Tensor, k: torch.Tensor, mask: torch.Tensor | None = None) -> int:
-    """fp32 elements of the workspace that cross_attention takes for queries and keys of these shapes (0: none); with a mask,
-    room for the list of the keys that it leaves too, which long calls make."""
-    (B, L, H, D), S = q.shape, k.size(1)
-    need = lib().ff_cross_attention_work(B, L, S, H, k.size(2), D)
-    return need if mask is None else max(need, B * (S + 1))
+def cross_attention_work(q: torch.Tensor, k: torch.Tensor) -> int:
+    """fp32 elements of the workspace that cross_attention takes for queries and keys of these shapes (0: none)."""
+    B, L, H, D = q.shape
+    return lib().ff_cross_attention_work(B, L, k.size(1), H, k.size(2), D)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, scale: float,
@@ -664,8 +662,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
     fp32 sums (include/foidfinder_rocm.h, ff_cross_attention): any batch, token and head strides that are multiples of 16
     bytes (views of packed rows, [B, heads, L, D] transposed, rows expanded over the batch), D a multiple of 8 up to 128,
     heads a multiple of kv_heads. Keys j >= lens[b] (int32 [B]) and keys with mask[b, j] False (bool [B, S], contiguous
-    columns) are not read; a query without keys gives zeros. work: fp32 of at least cross_attention_work(q, k) elements (with a
-    mask, of cross_attention_work(q, k, mask): less is slower); calls that run one after another may share it. out and work share no memory with each other or with what is read (refused)."""
+    columns) are not read; a query without keys gives zeros. work: fp32 of at least cross_attention_work(q, k) elements; calls
+    that run one after another may share it. out and work share no memory with each other or with what is read (refused)."""
     _no_grad(q, k, v, out, work)
     dev = _attended(q, out, lens, work, k, v)
     (qb, qt, qh, q1), (kb, kt, kh, k1), (vb, vt, vh, v1), (ob, ot, oh, o1) = q.stride(), k.stride(), v.stride(), out.stride()

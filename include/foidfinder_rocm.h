@@ -130,11 +130,9 @@ int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, const void* 
  * scale q.k over the keys j < lens[b] (int32 [B], taken into 0 .. S; NULL: S) whose mask[b * mask_batch + j] is not 0 (bytes; NULL:
  * all); 0 where there are none. What k and v hold for other keys is not read. q, k, v and their strides are multiples of 16
  * bytes, out's of 8; tokens of k and v are fewer than 2^24 elements apart. work: at least ff_cross_attention_work fp32 elements
- * (0 where keys are not cut; NULL then), which calls that run one after another may share. Long calls list the keys that a mask
- * leaves in B * (S + 1) further elements: ff_cross_attention_work counts them where keys are cut; where it returns 0, a work of
- * that size is used for them, and without it a mask saves whole tiles of keys alone. out and work share no memory with each other
- * or with what is read (refused; where rows of three strides lie between another operand's, so are calls that would not touch
- * it). */
+ * (0 where keys are not cut; NULL then), which calls that run one after another may share. out and work share no memory with
+ * each other or with what is read (refused; where rows of three strides lie between another operand's, so are calls that
+ * would not touch it). */
 int64_t ff_cross_attention_work(int64_t B, int64_t L, int64_t S, int64_t heads, int64_t kv_heads, int64_t D);
 int ff_cross_attention(const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* k, int64_t k_batch,
                        int64_t k_token, int64_t k_head, const void* v, int64_t v_batch, int64_t v_token, int64_t v_head,

@@ -164,22 +164,6 @@ def residual(x=Q, y=KEY, xo=OUT, h=VAL, xr=64, yr=64, xor=64, hr=64, dtype=0, T=
                                         scale, eps, None))
 
 
-def test_attention_scale_reaches_the_exponent():
-    for call in (cross, prefix):
-        refused(call(scale=2.5e38), "scale")  # finite, 2.5e38 log2(e) is not
-
-
-def test_attention_list_of_kept_keys_is_part_of_the_workspace():
-    """64 x 1000 queries, 1000 keys: nothing is cut, and a workspace of 64 x 1001 elements holds the keys that a mask keeps."""
-    rows = (1000 * 1024, 1024, 64)
-    many = dict(B=64, L=1000, S=1000, H=16, KV=16, qs=rows, ks=rows, vs=rows, os=rows, q=1 << 40, k=2 << 40, v=3 << 40, out=4 << 40)
-    for at in (1 << 40, 2 << 40, 3 << 40):
-        refused(cross(**many, mask=5 << 40, mb=1000, work=at - 64 * 1001 * 4 + 16, size=64 * 1001), "workspace overlaps")
-    refused(cross(**many, mask=5 << 40, mb=1000, work=(5 << 40) + 960, size=64 * 1001), "workspace overlaps")
-    refused(cross(**many, mask=5 << 40, mb=1000, work=(4 << 40) + 16, size=64 * 1001), "out overlaps the workspace")
-    refused(cross(**many, mask=5 << 40, mb=1000, work=(6 << 40) + 4, size=64 * 1001), "misaligned")
-
-
 def test_residual_norm_refusals():
     refused(residual(dtype=2), "fp16 or bf16")
     for c in (0, 60, 16392):

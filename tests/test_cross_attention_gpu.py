@@ -381,108 +381,6 @@ def test_cross_attention_last_round_cut(dev, kind, D, B, H, KV):
     assert_near(out.float().cpu().numpy(), o, bound(kind, D**-0.5, o, size, load, v.float().abs().max().item(), S))
 
 
-def masked_call(dev, q, k, v, lens, mask, kind, junk=math.nan):
-    """One call whose keys a mask lists, over workspace and unseen keys of not-a-number; (out, seen)."""
-    K = kern()
-    B, S, D = k.size(0), k.size(1), k.size(3)
-    seen = mask.expand(B, S) & (torch.arange(S, device=dev) < (lens[:, None] if lens is not None else S))
-    if junk is not None:
-        k[~seen], v[~seen] = junk, junk
-    out, check = guarded(kind, dev, *q.shape)
-    need = K.cross_attention_work(q, k, mask)
-    work = torch.full((need + 64,), math.nan, device=dev)
-    K.cross_attention(q, k, v, out, D**-0.5, lens, mask, work[:need])
-    assert check() and bool(work[need:].isnan().all())
-    return out, seen
-
-
-@pytest.mark.parametrize("with_lens", [False, True])
-@pytest.mark.parametrize("kind,B,L,S,H,KV,D", [
-    ("fp16", 6, 140, 4161, 16, 16, 64),   # rows behind the whole tile that are streamed
-    ("bf16", 8, 55, 5000, 24, 8, 96),     # 165 rows: the rest is two units
-    ("fp16", 9, 61, 1111, 64, 64, 88),    # two units alone
-    ("bf16", 6, 200, 4100, 32, 8, 128), ("fp16", 12, 130, 2500, 16, 16, 40),
-])
-def test_cross_attention_listed_masks(dev, kind, B, L, S, H, KV, D, with_lens):
-    g = torch.Generator(device=dev).manual_seed(11)
-    rnd = lambda *s: torch.randn(*s, device=dev, generator=g).to(TYPES[kind])  # noqa: E731
-    q, kv = rnd(B, L, H, D), rnd(B, S, 2, KV, D)
-    k, v = kv[:, :, 0], kv[:, :, 1]
-    at = torch.arange(S, device=dev)
-    mask = torch.rand(B, S, device=dev, generator=g) < torch.linspace(0.02, 0.98, B, device=dev)[:, None]
-    mask[0] = at == S - 1           # the last alone
-    mask[1] = True
-    mask[2] = (at >= 70) & (at < S - 70)
-    mask[3, 64:] = False            # one whole tile
-    lens = None
-    if with_lens:
-        lens = torch.tensor([S + 9, S - 1, S // 2, 65, *[S - 100] * (B - 4)], dtype=torch.int32, device=dev)
-        mask[:, 0] = True
-    elif B > 5:
-        mask[5] = False             # nothing left
-    out, seen = masked_call(dev, q, k, v, lens, mask, kind)
-    some = seen.any(1)
-    k, v = k.masked_fill(~seen[:, :, None, None], 0), v.masked_fill(~seen[:, :, None, None], 0)
-    o, size, load = reference64(q[some], k[some], v[some], D**-0.5, seen[some][:, None])
-    got = out.float().cpu().numpy()
-    assert_near(got[some.cpu().numpy()], o, bound(kind, D**-0.5, o, size, load, v.float().abs().max().item(), S))
-    assert (got[~some.cpu().numpy()] == 0).all()
-
-
-@pytest.mark.parametrize("apart", [131072, 262144])
-def test_cross_attention_masked_keys_far_apart(dev, apart):
-    """A sequence's rows over one and over two GiB (4100 tokens): by list where 32-bit offsets reach, tile by tile where not."""
-    B, L, S, H, D = 1, 300, 4100, 64, 64
-    g = torch.Generator(device=dev).manual_seed(12)
-    store = torch.empty(S * apart, dtype=torch.float16, device=dev)
-    rows = store.view(B, S, apart)[:, :, apart - 2 * H * D :].view(B, S, 2, H, D)
-    rows.copy_(torch.randn(B, S, 2, H, D, device=dev, generator=g))
-    q = torch.randn(B, L, H, D, device=dev, generator=g).half()
-    k, v = rows[:, :, 0], rows[:, :, 1]
-    mask = torch.rand(B, S, device=dev, generator=g) < 0.4
-    mask[:, -1] = True
-    out, seen = masked_call(dev, q, k, v, None, mask, "fp16")
-    k, v = k.masked_fill(~seen[:, :, None, None], 0), v.masked_fill(~seen[:, :, None, None], 0)
-    o, size, load = reference64(q, k, v, D**-0.5, seen[:, None])
-    assert_near(out.float().cpu().numpy(), o, bound("fp16", D**-0.5, o, size, load, v.float().abs().max().item(), S))
-
-
-def test_cross_attention_listed_masks_captured_and_shared(dev):
-    """One mask row for the batch, keys broadcast over it, captured, and replayed over new masks; calls in turn share the workspace."""
-    K = kern()
-    B, L, S, H, D = 6, 140, 4161, 16, 64
-    g = torch.Generator(device=dev).manual_seed(13)
-    q = torch.randn(B, L, H, D, device=dev, generator=g).half()
-    one = torch.randn(1, S, 2, H, D, device=dev, generator=g).half()
-    k, v = (one[:, :, i].expand(B, -1, -1, -1) for i in range(2))
-    row = torch.rand(1, S, device=dev, generator=g) < 0.5
-    other = torch.rand(B, S, device=dev, generator=g) < 0.3
-    outs = [torch.empty_like(q) for _ in range(4)]
-    work = torch.empty(K.cross_attention_work(q, k, row.expand(B, -1)), device=dev)
-
-    def both(a, b, w):
-        K.cross_attention(q, k, v, a, 0.125, None, row.expand(B, -1), w)
-        K.cross_attention(q, k, v, b, 0.125, None, other, w)
-
-    both(outs[0], outs[1], work)
-    torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        both(outs[0], outs[1], work)
-    for n in range(4):
-        row.copy_(torch.rand(1, S, device=dev, generator=g) < 0.2 * n)  # nothing left in the first
-        other.copy_(torch.rand(B, S, device=dev, generator=g) < 0.9 - 0.2 * n)
-        graph.replay()
-        both(outs[2], outs[3], torch.full_like(work, math.nan))
-        torch.cuda.synchronize()
-        assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3]), n
-        if n == 0:
-            assert not outs[0].any()
-        kept = row[0].nonzero()[:, 0]  # the same keys by themselves: other tiles' sums, the same values
-        K.cross_attention(q, k[:, kept], v[:, kept], outs[2], 0.125, None, None, torch.empty_like(work))
-        assert (outs[2].float() - outs[0].float()).abs().max().item() <= 2.0**-8 * max(1.0, v.abs().max().item()), n
-
-
 @pytest.mark.parametrize("kind,B,L,P,S,H,KV,D", [("bf16", 40, 3, 3000, 200, 8, 2, 128), ("fp16", 12, 30, 2000, 900, 16, 16, 64),
                                                  ("fp16", 100, 1, 700, 2500, 4, 4, 96), ("bf16", 3, 200, 64, 5000, 2, 1, 64)])
 def test_prefix_attention_of_many_rows_and_cuts(dev, kind, B, L, P, S, H, KV, D):

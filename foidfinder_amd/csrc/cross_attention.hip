@@ -7,19 +7,29 @@
 // for the second product, half a step each, which is what the matrix cores take.
 //
 // Rows: the G = heads / kv_heads query heads of a key head read the same keys, so a key head's rows are (sequence, token, head
-// of the group). A workgroup has four waves and 32, 64 or 128 rows; 32 rows are a unit. Four units: a wave each, over all
-// keys. Two: two waves a unit, each over one half of every 64-key tile. One (single tokens): all four share it, by halves and by
-// tiles of either parity. Waves that share a unit are joined through LDS.
-// Keys: a workgroup runs over all keys of its rows, or, where rows are few, over one of several runs of tiles; the runs' O, m
-// and l then go to the workspace in fp32 and join_kernel joins them in a fixed order.
+// of the group), 32 of them a unit.
+// Tiles (cross_kernel): four waves and up to 128 rows, K and V in tiles of 64 keys through two LDS slots that all waves read. Four
+// units: a wave each. Two: two waves a unit, each over one half of every tile. One is streamed.
+// Streams (stream_kernel; up to 32 rows a sequence and key head): four or eight waves share a unit, each with keys of its own, 32
+// at a time through LDS of its own, without a barrier until the waves' O, m and l are joined.
+// Keys: a workgroup runs over all keys of its rows, or over one of several runs of them where there are few rows, or where a last
+// round of workgroups would leave much of the chip idle (Plan). The runs' O, m and l go to the workspace in fp32 and join_kernel
+// joins them in a fixed order.
 // Shared prefix: its keys have no sequence, so the rows of all sequences together read it; the same launch's other workgroups
-// take each sequence's own keys, and join_kernel joins the parts.
+// take each sequence's own keys, and join_kernel joins the parts. Streams of one sequence, or of short prefixes, read both.
+// Masks: a workgroup lists the keys that the mask leaves in LDS, a chunk of the mask at a time, and its tiles hold only those;
+// streams leave out masked keys' loads.
 //
-// K and V stream through two LDS slots of 64 keys (buffer loads straight into LDS). Rows that no query of the workgroup may see
-// (past the length, or masked) and columns past D are loads out of the descriptor's range: they read as zeros and cost no
-// traffic, and what the memory there holds never reaches a product. Per wave, S^T = K Q^T by 32x32x16 products leaves a lane
-// with one query and 16 of 32 keys; P^T then is the column operand of O^T = V^T P^T, V read with the transposing
-// ds_read_b64_tr_b16. Both tiles are row-major, their 16-byte chunks XOR-swizzled against bank conflicts.
+// Loads go straight into LDS. Rows that no query of the workgroup may see (past the length, or masked) and columns past D are
+// out of the descriptor's range: they read as zeros and cost no traffic, and what the memory there holds never reaches a product.
+// Per wave, S^T = K Q^T by 32x32x16 products leaves a lane with one query and 16 of 32 keys; P^T then is the column operand of
+// O^T = V^T P^T, V read with the transposing ds_read_b64_tr_b16. Both tiles are row-major, their 16-byte chunks XOR-swizzled
+// against bank conflicts (counted: none).
+//
+// What bounds it, measured: long keys, the softmax between the products (at 128 columns, 4 x 1024 queries, 4096 keys, 32 / 8
+// heads: matrix cores busy 48 % of the time, vector units 46 %, both at once 42 %; 870 TF/s bf16 on random values, which cost a
+// fifth more time than zeros; 64 columns 8 x 1024 x 4096 x 16: 810 TF/s, 96 columns 850). Few rows, memory: 64 single tokens
+// against 1025 keys of 16 / 8 heads x 128, lengths 1 .. 1025: 4.4 TB/s of the keys read.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -157,14 +167,8 @@ struct Unit {
   // x = S^T of the 32 keys at k (+ ka): keys 8 (r / 4) + 4 fh + r % 4.
   __device__ __forceinline__ void score(float16_t& x, const T* k, int ka, int ka_odd) {
     T8 kf[KS];
-    keys(kf, k, ka, ka_odd);
-    score(x, kf);
-  }
-  __device__ __forceinline__ void keys(T8 (&kf)[KS], const T* k, int ka, int ka_odd) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) kf[s] = *reinterpret_cast<const T8*>(k + kfrag(ka, ka_odd, s));
-  }
-  __device__ __forceinline__ void score(float16_t& x, const T8 (&kf)[KS]) {
     const float16_t zero = {};
 #pragma unroll
     for (int s = 0; s < KS; ++s) x = mfma(kf[s], qf[s], s == 0 ? zero : x);
@@ -191,8 +195,7 @@ struct Unit {
       for (int r = 0; r < 16; ++r) xs[r] = (bits >> (8 * (r >> 2) + (r & 3))) & 1 ? xs[r] : -__builtin_inff();
     }
   }
-  // p of the scores; bits: the keys that the lane's row sees.
-  // first: m is not set yet, which the first pass would only find out.
+  // p of the scores; bits: the keys that the lane's row sees; first: m is not set yet, which the first pass would only find out.
   __device__ __forceinline__ void weigh(float16_t& xs, T8 (&pf)[2], uint32_t bits, int fh, bool first) {
     hide(xs, bits, fh);
     float sum = 0.f;
@@ -205,21 +208,19 @@ struct Unit {
   // The keys' p passed the limit, or m is not set: m becomes the largest c S of the keys, or just below, and O and l follow. Scores
   // from 2^30 up are too coarse for the multiply-add: what it leaves of the largest can be of any size then, and is capped.
   __device__ __forceinline__ void raise(const float16_t& xs, T8 (&pf)[2]) {
-    {
-      float top = xs[0];
+    float top = xs[0];
 #pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, xs[r]);
-      top = fmaxf(top, xor_shuffle(top, 32)) * c;
-      const float m_old = m;
-      m = fmaxf(m, top - fabsf(top) * 0x1p-23f);
-      const float corr = __builtin_amdgcn_exp2f(m_old - m);
-      l *= corr;
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, xs[r]);
+    top = fmaxf(top, xor_shuffle(top, 32)) * c;
+    const float m_old = m;
+    m = fmaxf(m, top - fabsf(top) * 0x1p-23f);
+    const float corr = __builtin_amdgcn_exp2f(m_old - m);
+    l *= corr;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= corr;
-      l += weights(xs, pf, CAP);
-    }
+      for (int r = 0; r < 16; ++r) o[dt][r] *= corr;
+    l += weights(xs, pf, CAP);
   }
   // O^T += V^T P^T, the 32 values at LDS byte v + OFF (+ va).
   template <int OFF>
@@ -259,8 +260,21 @@ __device__ __forceinline__ void store4(const CrossArgs& a, const Piece& w, const
   *reinterpret_cast<vec4_t<T>*>(static_cast<T*>(a.out) + p.seq * a.ob + p.token * a.ot + p.head * a.oh + col) = v;
 }
 
-// Tiles of 64 keys for four waves: a wave a unit (SHARE 1), or two (SHARE 2), each with one half of every tile.
-template <typename T, int DP, int SHARE>
+// LDS of streams and of tiles, and of the joints that follow in the same place.
+constexpr int stream_bytes(int dp, int waves) {
+  const int slices = waves * 2 * 32 * dp * 2, joint = waves * (dp / 2 + 2) * 256;
+  return slices > joint ? slices : joint;
+}
+constexpr int tile_bytes(int dp) { return 4 * BKV * dp * 2 > stream_bytes(dp, WAVES) ? 4 * BKV * dp * 2 : stream_bytes(dp, WAVES); }
+// Keys of a mask that are listed at a time: what the LDS leaves room for beside a CU's workgroups.
+constexpr int list_chunk(int dp) { return dp == 64 ? 1024 : dp == 96 ? 512 : 2048; }
+
+// Tiles of 64 keys for four waves: a wave a unit (SHARE 1), or two (SHARE 2), each with one half of every tile. LIST: tiles hold
+// keys that the mask leaves, and no others. Us for half the keys masked at random, a third at the end, none, where a tile's mask
+// word left out loads and empty tiles, and by list: 15.1 -> 16.1, 14.7 -> 16.1, 14.6 -> 15.7 (2 x 256 queries, 512 keys, 8 heads x
+// 64); 26.8 -> 18.4, 20.5 -> 20.4, 24.3 -> 25.8 (4 x 512, 1024, 16 x 64); 62 -> 36, 46 -> 44, 56 -> 58 (2 x 512, 2048, 32 / 8 x
+// 128); 330 -> 172, 226 -> 217, 289 -> 291 (4 x 1024, 4096, 32 / 8 x 128). A list in memory, by a kernel of its own: 182, 228, 300.
+template <typename T, int DP, int SHARE, bool LIST>
 __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T* smem) {
   typedef vec8_t<T> T8;
   constexpr int CH = DP / 8, TILE = BKV * DP, LPW = CH / 4, KS = DP / 16, DT = DP / 32;
@@ -280,8 +294,7 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
   const int64_t at = max(w.seq, 0);
   const T* kbase = static_cast<const T*>(src.k) + at * src.kb + w.head * src.kh;
   const T* vbase = static_cast<const T*>(src.v) + at * src.vb + w.head * src.vh;
-  const uint8_t* mask = a.mask && w.seq >= 0 ? a.mask + at * a.mask_b : nullptr;
-  const bool guard = mask || src.kt < a.dim || src.vt < a.dim;  // rows left out that the descriptor's range does not leave out
+  const bool guard = src.kt < a.dim || src.vt < a.dim;  // rows left out that the descriptor's range does not leave out
 
   // Tile loads: wave w fills the 1 KB blocks LPW w .. of either tile, lane l the chunk l of a block; it fetches what the swizzle
   // puts there.
@@ -290,9 +303,54 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
   for (int i = 0; i < LPW; ++i) {
     const int n = (LPW * wave + i) * 64 + lane, r = n / CH, slot = n % CH;
     const int ck = k_slot<DP>(r, slot), cv = v_slot<DP>(r, slot);
-    voff_k[i] = 8 * ck < a.dim ? static_cast<uint32_t>((r * static_cast<int>(src.kt) + ck * 8) * 2) : OOB_OFFSET;
-    voff_v[i] = 8 * cv < a.dim ? static_cast<uint32_t>((r * static_cast<int>(src.vt) + cv * 8) * 2) : OOB_OFFSET;
+    const int kr = LIST ? 0 : r * static_cast<int>(src.kt), vr = LIST ? 0 : r * static_cast<int>(src.vt);
+    voff_k[i] = 8 * ck < a.dim ? static_cast<uint32_t>((kr + ck * 8) * 2) : OOB_OFFSET;
+    voff_v[i] = 8 * cv < a.dim ? static_cast<uint32_t>((vr + cv * 8) * 2) : OOB_OFFSET;
   }
+  // The list: keys that the mask leaves, in order; [pos, have) have not been loaded yet.
+  constexpr int CHUNK = list_chunk(DP), EACH = CHUNK / (64 * WAVES);
+  int32_t *list = reinterpret_cast<int32_t*>(smem + tile_bytes(DP) / 2), *counts = list + CHUNK + BKV;
+  const uint8_t* bytes = LIST ? a.mask + at * a.mask_b : nullptr;
+  const int end = LIST ? min(w.t1 * BKV, w.keys) : 0;
+  int pos = 0, have = 0, raw = w.t0 * BKV;
+  // Moves them to the front and lists the next chunks' keys behind them until there are a tile's, or all.
+  auto refill = [&]() __attribute__((always_inline)) {
+    const int tid = threadIdx.x, left = have - pos, carried = tid < left ? list[pos + tid] : 0;
+    __syncthreads();
+    if (tid < left) list[tid] = carried;
+    pos = 0, have = left;
+    while (have < BKV && raw < end) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int n = EACH * tid + e;
+        const uint8_t byte = bytes[raw + min(n, end - raw - 1)];
+        bits |= byte != 0 && n < end - raw ? 1u << e : 0u;
+      }
+      const int mine = __popc(bits);
+      int before = mine;  // in the wave, this thread's with them
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int other = __shfl_up(before, d, 64);
+        before += lane >= d ? other : 0;
+      }
+      if (lane == 63) counts[wave] = before;
+      __syncthreads();
+      int to = have + before - mine, all = 0;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) {
+        const int n = counts[i];
+        to += i < wave ? n : 0;
+        all += n;
+      }
+#pragma unroll
+      for (int e = 0; e < EACH; ++e)
+        if (bits >> e & 1) list[to++] = raw + EACH * tid + e;
+      __syncthreads();
+      have += __builtin_amdgcn_readfirstlane(all);
+      raw = end - raw > CHUNK ? raw + CHUNK : end;
+    }
+  };
   auto issue = [&](int tile, uint64_t word) __attribute__((always_inline)) {
     const int st = (tile - w.t0) & 1, rows = min(BKV, w.keys - tile * BKV);
     const int64_t first = static_cast<int64_t>(tile) * BKV;
@@ -307,16 +365,9 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
     }
   };
   // The keys of a tile that may be seen, as bits.
-  auto mask_byte = [&](int tile) __attribute__((always_inline)) {
-    const int key = tile * BKV + lane;
-    return mask && tile < w.t1 && key < w.keys ? mask[key] : uint8_t(0);
-  };
-  auto valid = [&](int tile, uint8_t byte) __attribute__((always_inline)) {
-    if (mask) return static_cast<uint64_t>(__ballot(byte != 0));
-    const int n = w.keys - tile * BKV;
-    return n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1;
-  };
+  auto valid = [&](int n) __attribute__((always_inline)) { return n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1; };
   auto bits_of = [&](int tile, uint64_t word, int half) __attribute__((always_inline)) {
+    if constexpr (LIST) return static_cast<uint32_t>(word >> (32 * half));
     const int left = limit - (tile * BKV + 32 * half);
     return static_cast<uint32_t>(word >> (32 * half)) & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1);
   };
@@ -347,21 +398,55 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
     return 2;
   };
 
+  // The list's rows: those of the keys up to `usable` lie within 2^31 bytes from that of key `base` on.
+  const int kt = static_cast<int>(src.kt), vt = static_cast<int>(src.vt), reach = ((1 << 30) - 2 * DP) / max(max(kt, vt), 1);
+  int usable = 0, base = 0;
+  // Takes the next tile's keys from the list and loads their rows into a slot: how many.
+  auto issue_listed = [&](int st) __attribute__((always_inline)) {
+    if (usable - pos < BKV) {
+      if (have - pos < BKV && raw < end) refill();
+      if (have == pos) return 0;
+      base = __builtin_amdgcn_readfirstlane(list[pos]), usable = have;
+      if (__builtin_amdgcn_readfirstlane(list[have - 1]) - base > reach)
+        usable = pos + __popcll(__ballot(lane < have - pos && list[min(pos + lane, have - 1)] - base <= reach));
+    }
+    const int n = min(BKV, usable - pos), span = min(reach, w.keys - 1 - base);
+    const int nk = (span * kt + a.dim) * 2, nv = (span * vt + a.dim) * 2;
+    const T *k = kbase + base * src.kt, *v = vbase + base * src.vt;
+    int on[LPW];
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) on[i] = list[pos + min(((LPW * wave + i) * 64 + lane) / CH, n - 1)] - base;
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      const bool in = ((LPW * wave + i) * 64 + lane) / CH < n;
+      const uint32_t ko = voff_k[i] + static_cast<uint32_t>(on[i] * kt) * 2, vo = voff_v[i] + static_cast<uint32_t>(on[i] * vt) * 2;
+      buffer_to_lds(k, nk, reinterpret_cast<uint8_t*>(smem + st * TILE + (LPW * wave + i) * 512), in ? ko : OOB_OFFSET);
+      buffer_to_lds(v, nv, reinterpret_cast<uint8_t*>(smem + (2 + st) * TILE + (LPW * wave + i) * 512), in ? vo : OOB_OFFSET);
+    }
+    pos += n;
+    return n;
+  };
+
   if (w.t0 < w.t1) {
-    uint64_t word = valid(w.t0, mask_byte(w.t0)), next = 0;
-    uint8_t byte = mask_byte(w.t0 + 1);
-    issue(w.t0, word);
+    uint64_t word, next = 0;  // of a list, 0 behind the last tile
+    if constexpr (LIST) {
+      word = valid(issue_listed(0));
+    } else {
+      word = valid(w.keys - w.t0 * BKV);
+      issue(w.t0, word);
+    }
     u.settle();
-    for (int tile = w.t0; tile < w.t1; ++tile) {
+    for (int tile = w.t0; LIST ? word != 0 : tile < w.t1; ++tile) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();  // no fence: the wait covers this thread's LDS writes
-      if (tile + 1 < w.t1) {         // its slot was last read for tile - 1, which every wave has finished
-        next = valid(tile + 1, byte);
+      const int st = (tile - w.t0) & 1;  // the other slot was last read for tile - 1, which every wave has finished
+      if constexpr (LIST) {
+        next = valid(issue_listed(st ^ 1));
+      } else if (tile + 1 < w.t1) {
+        next = valid(w.keys - (tile + 1) * BKV);
         issue(tile + 1, next);
-        byte = mask_byte(tile + 2);
       }
-      const int st = (tile - w.t0) & 1;
-      if (active && word != 0) {
+      if (active) {
         // read bases, opaque to the compiler so that the fragment offsets fold into the reads' immediate offsets
         int ka = st * TILE + half_sel * 32 * DP + u.koff, ka_odd = 0, va = (2 + st) * TILE + half_sel * 32 * DP + u.voff;
         asm volatile("" : "+v"(ka), "+v"(va));
@@ -419,10 +504,10 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
                 float4_t{u.o[dt][4 * g], u.o[dt][4 * g + 1], u.o[dt][4 * g + 2], u.o[dt][4 * g + 3]}, u.m, l);
 }
 
-// One unit of rows and WAVES waves, each with slices of 32 keys of its own (slice t0 + wave, + WAVES, ...) in LDS of its own, so no
-// barrier stands between load and use: a wave asks for the next slice's K once it has read this one's, and for its V likewise, and
-// has 64 KB (128 columns; 8 waves) or 128 KB (16) of the CU's reads in flight. The slices are those of the prefix (w.front), then the
-// sequence's own. The waves' O, m and l are joined through LDS, four columns a wave and turn.
+// One unit of rows and NW waves, each with slices of 32 keys of its own (slice t0 + wave, + NW, ...) in LDS of its own, so no
+// barrier stands between load and use: a wave asks for the next slice's K once it has read this one's, and for its V likewise, so
+// that half a slice or more (8 KB at 128 columns) is on its way to each wave at any time. The slices are those of the prefix
+// (w.front), then the sequence's own. The waves' O, m and l are joined through LDS, four columns a wave and turn.
 template <typename T, int DP, int NW>
 __device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w, T* smem) {
   typedef vec8_t<T> T8;
@@ -549,17 +634,10 @@ __device__ __forceinline__ void touch(const CrossArgs& a) {
   asm volatile("" ::"s"(a.qb), "s"(a.own.k), "s"(a.own.vt), "s"(a.prefix.kt), "s"(a.lens), "s"(a.batch), "s"(a.c));
 }
 
-// LDS of streams and of tiles, and of the joints that follow in the same place.
-constexpr int stream_bytes(int dp, int waves) {
-  const int slices = waves * 2 * 32 * dp * 2, joint = waves * (dp / 2 + 2) * 256;
-  return slices > joint ? slices : joint;
-}
-constexpr int tile_bytes(int dp) { return 4 * BKV * dp * 2 > stream_bytes(dp, WAVES) ? 4 * BKV * dp * 2 : stream_bytes(dp, WAVES); }
-
 // Waves a SIMD: what the LDS leaves room for (34, 50 and 66 KB a workgroup).
-template <typename T, int DP>
+template <typename T, int DP, bool LIST>
 __global__ __launch_bounds__(64 * WAVES, DP == 64 ? 4 : DP == 96 ? 3 : 2) void cross_kernel(const CrossArgs a) {
-  __shared__ __attribute__((aligned(1024))) T smem[tile_bytes(DP) / 2];  // K slots, then V slots
+  __shared__ __attribute__((aligned(1024))) T smem[tile_bytes(DP) / 2 + (LIST ? 2 * (list_chunk(DP) + BKV + WAVES) : 0)];  // K slots, then V slots; list
   touch(a);
   const int per = a.tokens * a.group, prefix_items = a.prefix_splits * a.kv * a.prefix_tiles;
   int item = static_cast<int>(blockIdx.x);
@@ -615,9 +693,9 @@ __global__ __launch_bounds__(64 * WAVES, DP == 64 ? 4 : DP == 96 ? 3 : 2) void c
   if (units == 1)
     stream_block<T, DP, WAVES>(a, w, smem);
   else if (units == 2)
-    tile_block<T, DP, 2>(a, w, smem);
+    tile_block<T, DP, 2, LIST>(a, w, smem);
   else
-    tile_block<T, DP, 1>(a, w, smem);
+    tile_block<T, DP, 1, LIST>(a, w, smem);
 }
 
 // Up to 32 rows a sequence and key head: workgroups of NW waves that all read the same rows' keys, the prefix's among them. Where
@@ -705,8 +783,10 @@ static void launch_cross(const CrossArgs& a, int64_t blocks, int stream, hipStre
     stream_kernel<T, DP, 8><<<runs, 64 * 8, 0, st>>>(a);
   else if (stream == 4)
     stream_kernel<T, DP, 4><<<runs, 64 * 4, 0, st>>>(a);
+  else if (a.mask)
+    cross_kernel<T, DP, true><<<dim3(static_cast<unsigned>(blocks)), 64 * WAVES, 0, st>>>(a);
   else
-    cross_kernel<T, DP><<<dim3(static_cast<unsigned>(blocks)), 64 * WAVES, 0, st>>>(a);
+    cross_kernel<T, DP, false><<<dim3(static_cast<unsigned>(blocks)), 64 * WAVES, 0, st>>>(a);
   if (!a.work) return;
   constexpr int CH = DP == 64 ? 8 : 16;
   const int parts = a.tail ? a.tail_splits : a.prefix_splits + a.own_splits;
@@ -903,7 +983,8 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
   if (dtype != FF_F16 && dtype != FF_BF16) return bad("q, k, v and out must be fp16 or bf16");
   Plan p;
   if (const char* msg = bad_sizes(batch, tokens, keys, prefix, heads, kv, D, p)) return bad(msg);
-  if (!(scale > 0.f) || !std::isfinite(scale)) return bad("scale must be finite and > 0");
+  const float c = scale * 1.4426950408889634f;  // log2(e)
+  if (!(scale > 0.f) || !std::isfinite(c)) return bad("scale must be > 0, and finite times log2(e)");
   if (batch == 0 || tokens == 0) return FF_OK;
   const Rows* given[6] = {&q, &k, &v, pk, pv, &out};
   for (const Rows* r : given) {
@@ -925,11 +1006,12 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
   const Extent read[7] = {extent_of(q, D), extent_of(k, D), extent_of(v, D), pk ? extent_of(*pk, D) : range(nullptr, 0),
                           pv ? extent_of(*pv, D) : range(nullptr, 0), range(lens, lens ? batch * 4 : 0),
                           Extent{reinterpret_cast<uintptr_t>(mask), {batch, 1}, {mask_batch, 0}, mask ? keys : 0}};
-  if (!clear_of(to, scratch)) return bad("out overlaps the workspace");
+  const bool used = scratch.len > 0;
+  if (used && !clear_of(to, scratch)) return bad("out overlaps the workspace");
   for (const Extent& e : read) {
     if (e.len == 0) continue;
     if (!clear_of(to, e)) return bad("out overlaps what is read");
-    if (need > 0 && !clear_of(scratch, e)) return bad("the workspace overlaps what is read");
+    if (used && !clear_of(scratch, e)) return bad("the workspace overlaps what is read");
   }
   CrossArgs a{};
   a.q = q.p, a.out = const_cast<void*>(out.p);
@@ -941,7 +1023,7 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
   };
   a.own = source(k, v);
   if (pk) a.prefix = source(*pk, *pv);
-  a.lens = lens, a.mask = mask, a.mask_b = mask_batch, a.work = need > 0 ? work : nullptr, a.slots = p.slots;
+  a.lens = lens, a.mask = mask, a.mask_b = mask_batch, a.work = p.slots > 0 ? work : nullptr, a.slots = p.slots;
   a.batch = static_cast<int>(batch), a.tokens = static_cast<int>(tokens), a.kv = static_cast<int>(kv);
   a.group = static_cast<int>(heads / kv), a.dim = static_cast<int>(D), a.causal = pk != nullptr;
   a.rows = static_cast<int>(batch * tokens) * a.group;
@@ -949,7 +1031,7 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
   a.own_splits = static_cast<int>(p.own_splits), a.prefix_tiles = static_cast<int>(p.prefix_tiles);
   a.prefix_splits = static_cast<int>(p.prefix_splits);
   a.tail = static_cast<int>(p.tail), a.tail_splits = static_cast<int>(p.tail_splits);
-  a.c = scale * 1.4426950408889634f;
+  a.c = c;
   if (dtype == FF_F16)
     launch_cross_dim<half_t>(a, p.blocks, p.stream, as_stream(stream));
   else

@@ -164,6 +164,11 @@ def residual(x=Q, y=KEY, xo=OUT, h=VAL, xr=64, yr=64, xor=64, hr=64, dtype=0, T=
                                         scale, eps, None))
 
 
+def test_attention_scale_reaches_the_exponent():
+    for call in (cross, prefix):
+        refused(call(scale=2.5e38), "scale")  # finite, 2.5e38 log2(e) is not
+
+
 def test_residual_norm_refusals():
     refused(residual(dtype=2), "fp16 or bf16")
     for c in (0, 60, 16392):

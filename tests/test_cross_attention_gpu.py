@@ -381,6 +381,119 @@ def test_cross_attention_last_round_cut(dev, kind, D, B, H, KV):
     assert_near(out.float().cpu().numpy(), o, bound(kind, D**-0.5, o, size, load, v.float().abs().max().item(), S))
 
 
+def masked_call(dev, q, k, v, lens, mask, kind):
+    """One call with not-a-number in the keys that are not seen, against float64 on the GPU."""
+    K = kern()
+    B, S, D = k.size(0), k.size(1), k.size(3)
+    seen = mask.expand(B, S) & (torch.arange(S, device=dev) < (lens[:, None] if lens is not None else S))
+    k[~seen], v[~seen] = math.nan, math.nan
+    out, check = guarded(kind, dev, *q.shape)
+    need = K.cross_attention_work(q, k)
+    work = torch.full((need + 64,), math.nan, device=dev)
+    K.cross_attention(q, k, v, out, D**-0.5, lens, mask, work[:need])
+    assert check() and bool(work[need:].isnan().all())
+    some = seen.any(1)
+    k, v = k[some].masked_fill(~seen[some][:, :, None, None], 0), v[some].masked_fill(~seen[some][:, :, None, None], 0)
+    o, size, load = reference64(q[some], k, v, D**-0.5, seen[some][:, None])
+    got, some = out.float().cpu().numpy(), some.cpu().numpy()
+    assert_near(got[some], o, bound(kind, D**-0.5, o, size, load, v.abs().max().item(), S))
+    assert (got[~some] == 0).all()
+
+
+@pytest.mark.parametrize("with_lens", [False, True])
+@pytest.mark.parametrize("kind,B,L,S,H,KV,D", [
+    ("fp16", 6, 140, 4161, 16, 16, 64),   # rows behind the whole tile that are streamed
+    ("bf16", 8, 55, 5000, 24, 8, 96),     # 165 rows: the rest is two units
+    ("fp16", 9, 61, 1111, 64, 64, 88),    # two units alone
+    ("bf16", 6, 200, 4100, 32, 8, 128), ("fp16", 12, 130, 2500, 16, 16, 40),
+    ("bf16", 6, 70, 6000, 1, 1, 128),     # few rows: keys cut, some runs of them without any left
+])
+def test_cross_attention_of_listed_keys(dev, kind, B, L, S, H, KV, D, with_lens):
+    g = torch.Generator(device=dev).manual_seed(11)
+    rnd = lambda *s: torch.randn(*s, device=dev, generator=g).to(TYPES[kind])  # noqa: E731
+    q, kv = rnd(B, L, H, D), rnd(B, S, 2, KV, D)
+    at = torch.arange(S, device=dev)
+    mask = torch.rand(B, S, device=dev, generator=g) < torch.linspace(0.02, 0.98, B, device=dev)[:, None]
+    mask[0] = at == S - 1           # the last alone
+    mask[1] = True
+    mask[2] = (at >= 70) & (at < S - 70)
+    mask[3, 64:] = False            # one whole tile
+    lens = None
+    if with_lens:
+        lens = torch.tensor([S + 9, S - 1, S // 2, 65, *[S - 100] * (B - 4)], dtype=torch.int32, device=dev)
+        mask[:, 0] = True
+    else:
+        mask[5] = False             # nothing left
+    masked_call(dev, q, kv[:, :, 0], kv[:, :, 1], lens, mask, kind)
+
+
+@pytest.mark.parametrize("dim,chunk", [(64, 1024), (96, 512), (128, 2048)])
+@pytest.mark.parametrize("tokens", [40, 100])
+def test_cross_attention_keys_left_over_chunks_of_the_mask(dev, dim, chunk, tokens):
+    """Keys that earlier chunks leave for a later one's first tile: none, fewer than a tile, one, more; in every second chunk."""
+    left = [0, 1, 63, 64, 65, 127, 128, chunk - 1, chunk]
+    S, B = 5 * chunk + 3, len(left)
+    g = torch.Generator(device=dev).manual_seed(14)
+    rnd = lambda *s: torch.randn(*s, device=dev, generator=g).half()  # noqa: E731
+    q, k, v = rnd(B, tokens, 1, dim), rnd(B, S, 1, dim), rnd(B, S, 1, dim)
+    mask = torch.zeros(B, S, dtype=torch.bool, device=dev)
+    for b, n in enumerate(left):
+        for c in (0, 2, 3):
+            mask[b, c * chunk + torch.randperm(chunk, device=dev, generator=g)[:n]] = True
+        mask[b, S - 1 - b % 3] = True
+    masked_call(dev, q, k, v, None, mask, "fp16")
+
+
+@pytest.mark.parametrize("apart,S", [(131072, 4100), (1 << 22, 600), ((1 << 24) - 8, 200)])
+def test_cross_attention_masked_keys_far_apart(dev, apart, S):
+    """Up to 32 MiB between a sequence's rows: 64 keys of a list, or fewer, span more than 32-bit offsets reach."""
+    L, H, D = 70, 4, 64
+    g = torch.Generator(device=dev).manual_seed(12)
+    store = torch.empty(S * apart, dtype=torch.float16, device=dev)
+    rows = store.view(1, S, apart)[:, :, apart - 2 * H * D :].view(1, S, 2, H, D)
+    rows.copy_(torch.randn(1, S, 2, H, D, device=dev, generator=g))
+    q = torch.randn(1, L, H, D, device=dev, generator=g).half()
+    for kept in (0.05, 0.6):
+        mask = torch.rand(1, S, device=dev, generator=g) < kept
+        mask[:, -1] = True
+        rows.copy_(torch.randn(1, S, 2, H, D, device=dev, generator=g))
+        masked_call(dev, q, rows[:, :, 0], rows[:, :, 1], None, mask, "fp16")
+
+
+def test_cross_attention_masks_captured_and_shared(dev):
+    """One mask row for the batch, keys broadcast over it, captured, and replayed over new masks."""
+    K = kern()
+    B, L, S, H, D = 8, 524, 4161, 16, 64
+    g = torch.Generator(device=dev).manual_seed(13)
+    q = torch.randn(B, L, H, D, device=dev, generator=g).half()
+    one = torch.randn(1, S, 2, H, D, device=dev, generator=g).half()
+    k, v = (one[:, :, i].expand(B, -1, -1, -1) for i in range(2))
+    row = torch.rand(1, S, device=dev, generator=g) < 0.5
+    other = torch.rand(B, S, device=dev, generator=g) < 0.3
+    outs = [torch.empty_like(q) for _ in range(4)]
+    work = torch.empty(max(1, K.cross_attention_work(q, k)), device=dev)
+
+    def both(a, b, w):
+        K.cross_attention(q, k, v, a, 0.125, None, row.expand(B, -1), w)
+        K.cross_attention(q, k, v, b, 0.125, None, other, w)
+
+    both(outs[0], outs[1], work)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both(outs[0], outs[1], work)
+    for n in range(4):
+        row.copy_(torch.rand(1, S, device=dev, generator=g) < 0.2 * n)  # nothing left in the first
+        other.copy_(torch.rand(B, S, device=dev, generator=g) < 0.9 - 0.2 * n)
+        graph.replay()
+        both(outs[2], outs[3], torch.full_like(work, math.nan))
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3]), n
+        kept = row[0].nonzero()[:, 0]  # the same keys by themselves: the same tiles, for whole tiles of rows
+        K.cross_attention(q, k[:, kept], v[:, kept], outs[2], 0.125)
+        assert torch.equal(outs[2][:, :512], outs[0][:, :512]) and (n > 0) == bool(outs[0].any()), n
+
+
 @pytest.mark.parametrize("kind,B,L,P,S,H,KV,D", [("bf16", 40, 3, 3000, 200, 8, 2, 128), ("fp16", 12, 30, 2000, 900, 16, 16, 64),
                                                  ("fp16", 100, 1, 700, 2500, 4, 4, 96), ("bf16", 3, 200, 64, 5000, 2, 1, 64)])
 def test_prefix_attention_of_many_rows_and_cuts(dev, kind, B, L, P, S, H, KV, D):

@@ -819,35 +819,37 @@ struct Plan {
 constexpr int64_t CUS = 256;
 constexpr int64_t ONE_GO = int64_t(5) << 16;  // bytes of keys and values up to which a workgroup reads them all (its launch alone takes 8.6 us, two 9 and more)
 
-// Times in us, fitted to launches on this card: a tile of 64 keys takes a workgroup of four units TILE_ALONE at least, and a CU
-// TILE_CU per workgroup in it.
+// Times in us on this card: a tile of 64 keys takes a workgroup of four units `alone` at least, and a CU `cu` for each workgroup in
+// it.
 struct Rates {
   double alone, cu;
   int64_t resident;  // workgroups a CU holds
 };
 static Rates rates_of(int64_t D) {
-  if (D <= 64) return {1.0, 0.62, 4};
-  if (D <= 96) return {1.1, 0.87, 3};
-  return {1.2, 1.05, 2};
+  if (D <= 64) return {1.0, 0.55, 4};
+  if (D <= 96) return {1.1, 0.80, 3};
+  return {1.2, 0.95, 2};
 }
 
 // Cuts of the keys of `blocks` workgroups that have `tiles` tiles each, beside `others` workgroups of `theirs`: the cut that ends
-// first. The two kinds share the chip by their tiles; a tile of the others counts half where this is the prefix (its rows fill the
-// matrix cores, theirs wait for memory). Each part of a row costs its O, m and l written and read again; a second launch where
-// there would be one part.
+// first. A CU's load is taken halfway between the mean and the fullest CU's, and rounds halfway between their number and the next
+// whole one; the two kinds share the chip by their tiles. Parts of a row are written and read again, half of it within the caches,
+// and joined by a second launch. Two workgroups a CU are not cut (640 of 66 tiles: 124 us, in two 118, in four 127; 720 of 32: 65,
+// 78, 91). Over 32 shapes, timed with 1 .. 48 cuts (1 to 128 sequences of 1 to 1025 tokens, 512 to 16384 keys, 9 of them with a
+// prefix), its choice takes 2 % more than the fastest cut on average and 14 % at worst.
 static int64_t split_keys(int64_t blocks, int64_t tiles, int64_t others, int64_t theirs, int64_t rows, int64_t D, bool joined) {
-  if (blocks <= 0 || tiles <= 1) return 1;
+  if (blocks <= 0 || tiles <= 1 || (!joined && blocks >= 2 * CUS)) return 1;
   const Rates r = rates_of(D);
   const double mine = static_cast<double>(blocks) * static_cast<double>(tiles);
-  const double share = mine / (mine + 0.5 * static_cast<double>(others) * static_cast<double>(theirs));
+  const double share = mine / (mine + static_cast<double>(others) * static_cast<double>(theirs));
   const double slots = static_cast<double>(CUS * r.resident) * share;
   int64_t best = 1;
   double least = 0;
   for (int64_t s = 1; s <= std::min<int64_t>(64, (tiles + 1) / 2); ++s) {
-    const double together = std::min(static_cast<double>(blocks * s + others) / CUS, static_cast<double>(r.resident));
-    const double rounds = std::max(1.0, static_cast<double>(blocks * s) / slots);
-    const double t = static_cast<double>((tiles + s - 1) / s) * rounds * std::max(r.alone, r.cu * together) +
-                     (s > 1 || joined ? 4.0 + static_cast<double>(s * rows * (D + 2)) * 8.0 / 4.5e6 : 0.0);
+    const double all = static_cast<double>(blocks * s), rounds = std::max(1.0, all / slots);
+    const double together = std::min(0.5 * (all / CUS + std::ceil(all / CUS)), static_cast<double>(r.resident));
+    const double t = static_cast<double>((tiles + s - 1) / s) * 0.5 * (rounds + std::ceil(rounds)) * std::max(r.alone, r.cu * together) +
+                     (s > 1 || joined ? 6.0 + static_cast<double>(s * rows * (D + 2)) * 8.0 / 9e6 : 0.0);
     if (s == 1 || t < least) least = t, best = s;
   }
   return best;

@@ -26,10 +26,10 @@
 // O^T = V^T P^T, V read with the transposing ds_read_b64_tr_b16. Both tiles are row-major, their 16-byte chunks XOR-swizzled
 // against bank conflicts (counted: none).
 //
-// What bounds it, measured: long keys, the softmax between the products (at 128 columns, 4 x 1024 queries, 4096 keys, 32 / 8
-// heads: matrix cores busy 48 % of the time, vector units 46 %, both at once 42 %; 870 TF/s bf16 on random values, which cost a
-// fifth more time than zeros; 64 columns 8 x 1024 x 4096 x 16: 810 TF/s, 96 columns 850). Few rows, memory: 64 single tokens
-// against 1025 keys of 16 / 8 heads x 128, lengths 1 .. 1025: 4.4 TB/s of the keys read.
+// What bounds it, measured: with long keys the softmax between the products (8 x 1025 queries, 5184 keys, 16 heads x 64, fp16, in
+// 219 us or 795 TF/s: matrix cores busy 40 % of the cycles, vector units 63 %, both at once 22 %, at 1.9 GHz) and the card's power
+// (random values take a fifth more time than zeros); at 96 columns 850, at 128 870 TF/s. With few rows memory: 64 single tokens
+// against up to 1025 keys of 8 heads x 128 in 45 us, 4.5 TB/s of the keys read.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -637,16 +637,18 @@ __device__ __forceinline__ void touch(const CrossArgs& a) {
 // Waves a SIMD: what the LDS leaves room for (34, 50 and 66 KB a workgroup).
 template <typename T, int DP, bool LIST>
 __global__ __launch_bounds__(64 * WAVES, DP == 64 ? 4 : DP == 96 ? 3 : 2) void cross_kernel(const CrossArgs a) {
-  __shared__ __attribute__((aligned(1024))) T smem[tile_bytes(DP) / 2 + (LIST ? 2 * (list_chunk(DP) + BKV + WAVES) : 0)];  // K slots, then V slots; list
+  // K slots, then V slots; the list and its counts
+  __shared__ __attribute__((aligned(1024))) T smem[tile_bytes(DP) / 2 + (LIST ? 2 * (list_chunk(DP) + BKV + WAVES) : 0)];
   touch(a);
   const int per = a.tokens * a.group, prefix_items = a.prefix_splits * a.kv * a.prefix_tiles;
   int item = static_cast<int>(blockIdx.x);
   Piece w;
   int split = 0, splits = 1, tile, x;
   // Row tiles of one run of keys are neighbours, and neighbours share an XCD's L2 (the prefix's pieces by themselves, as they
-  // differ from the others in length). Runs are counted by sequences first, so that every XCD has long and short ones: 8 x 1024 queries of
-  // 16 heads x 64 to 4096 / 8 .. 4096 keys 146 -> 123 us, 4 x 1000 of 32 / 8 x 128 265 -> 192. A run's last tile, where it has fewer rows and takes less time, comes after all whole ones
-  // and fills the end of the grid; before it come the tail's pieces.
+  // differ from the others in length). Runs are counted by sequences first, so that every XCD has long and short ones: 8 x 1024
+  // queries of 16 heads x 64 to 4096 / 8 .. 4096 keys 146 -> 123 us, 4 x 1000 of 32 / 8 x 128 265 -> 192. A run's last tile, where
+  // it has fewer rows and takes less time, comes after all whole ones and fills the end of the grid; before it come the tail's
+  // pieces.
   auto place = [&](int n, int tiles, int rows, int tail, int tail_splits) __attribute__((always_inline)) {
     const int whole = rows / a.block_rows, runs = n / tiles, all = runs * whole;
     if (item < all - tail) {
@@ -739,7 +741,8 @@ __global__ __launch_bounds__(256) void join_kernel(const CrossArgs a) {
 #pragma unroll 4
   for (int p = first; p < parts; p += LANES) {
     const float2 x = ml[p * all];
-    const float4_t u = *reinterpret_cast<const float4_t*>(from + p * step), v = *reinterpret_cast<const float4_t*>(from + p * step + 4);
+    const float4_t u = *reinterpret_cast<const float4_t*>(from + p * step);
+    const float4_t v = *reinterpret_cast<const float4_t*>(from + p * step + 4);
     const float f = __builtin_amdgcn_exp2f(x.x - top);
     l = __builtin_fmaf(x.y, f, l);
 #pragma unroll
@@ -817,7 +820,8 @@ struct Plan {
 };
 
 constexpr int64_t CUS = 256;
-constexpr int64_t ONE_GO = int64_t(5) << 16;  // bytes of keys and values up to which a workgroup reads them all (its launch alone takes 8.6 us, two 9 and more)
+// Bytes of keys and values up to which one workgroup reads a sequence's and head's: 8.6 us, where two launches take 9 and more.
+constexpr int64_t ONE_GO = int64_t(5) << 16;
 
 // Times in us on this card: a tile of 64 keys takes a workgroup of four units `alone` at least, and a CU `cu` for each workgroup in
 // it.
@@ -848,7 +852,8 @@ static int64_t split_keys(int64_t blocks, int64_t tiles, int64_t others, int64_t
   for (int64_t s = 1; s <= std::min<int64_t>(64, (tiles + 1) / 2); ++s) {
     const double all = static_cast<double>(blocks * s), rounds = std::max(1.0, all / slots);
     const double together = std::min(0.5 * (all / CUS + std::ceil(all / CUS)), static_cast<double>(r.resident));
-    const double t = static_cast<double>((tiles + s - 1) / s) * 0.5 * (rounds + std::ceil(rounds)) * std::max(r.alone, r.cu * together) +
+    const double turns = static_cast<double>((tiles + s - 1) / s) * 0.5 * (rounds + std::ceil(rounds));
+    const double t = turns * std::max(r.alone, r.cu * together) +
                      (s > 1 || joined ? 6.0 + static_cast<double>(s * rows * (D + 2)) * 8.0 / 9e6 : 0.0);
     if (s == 1 || t < least) least = t, best = s;
   }

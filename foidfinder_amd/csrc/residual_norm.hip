@@ -9,6 +9,9 @@
 // 5 times a row's own bytes). The next row loads under this one's arithmetic. Sums: within a wave by DPP; a row of several
 // waves leaves each wave's sum and squares about its own mean in LDS and every wave joins them (counts and means known, no
 // cancellation), one barrier a norm.
+// Measured: 32 800 x 1024 fp16 with two LayerNorms and a gate row 51.5 us (5.2 TB/s), 9001 x 4096 bf16 with two RMS norms 55.7
+// (5.3); a copy of 1 GiB reaches 5.07, of 256 MB 5.42. With the norms chosen by branches in the row loop, whose parameters' loads
+// it then waited for: 71. A single row: 2.5 us.
 #include <algorithm>
 #include <type_traits>
 

@@ -684,7 +684,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
 
 
 def prefix_attention_work(q: torch.Tensor, prefix_k: torch.Tensor, k: torch.Tensor) -> int:
-    """fp32 elements of the workspace that prefix_attention takes for tensors of these shapes."""
+    """fp32 elements of the workspace that prefix_attention takes for tensors of these shapes (0: none)."""
     B, L, H, D = q.shape
     return lib().ff_prefix_attention_work(B, L, prefix_k.size(0), k.size(1), H, k.size(2), D)
 

@@ -16,7 +16,7 @@
 // round of workgroups would leave much of the chip idle (Plan). The runs' O, m and l go to the workspace in fp32 and join_kernel
 // joins them in a fixed order.
 // Shared prefix: its keys have no sequence, so the rows of all sequences together read it; the same launch's other workgroups
-// take each sequence's own keys, and join_kernel joins the parts. Streams of one sequence, or of short prefixes, read both.
+// take each sequence's own keys, and join_kernel joins the parts. Streams of one sequence, or behind a short prefix, read both.
 // Masks: a workgroup lists the keys that the mask leaves in LDS, a chunk of the mask at a time, and its tiles hold only those;
 // streams leave out masked keys' loads.
 //
@@ -822,6 +822,10 @@ struct Plan {
 constexpr int64_t CUS = 256;
 // Bytes of keys and values up to which one workgroup reads a sequence's and head's: 8.6 us, where two launches take 9 and more.
 constexpr int64_t ONE_GO = int64_t(5) << 16;
+// Bytes of a prefix that a CU's streams may read, once for each of theirs, in place of pieces of its own and a join: 12.6 -> 6.5 us
+// at 32 KB (64 x 4 tokens, 64 + 64 keys, 8 heads x 64), 22.6 -> 18.9 at 250 (300 x 1, 100 + 50, 16 / 4 x 128), 17.4 -> 16.1 at 500
+// (64 x 1, 500 + 100, 32 / 8 x 128), 19.0 -> 19.6 at 600, 17.6 -> 22.9 at 1000.
+constexpr double AGAIN = 512 << 10;
 
 // Times in us on this card: a tile of 64 keys takes a workgroup of four units `alone` at least, and a CU `cu` for each workgroup in
 // it.
@@ -866,7 +870,8 @@ static Plan plan_of(int64_t batch, int64_t tokens, int64_t keys, int64_t prefix,
   const int64_t per = tokens * group, rows = batch * per, runs = batch * kv, all = keys + std::max<int64_t>(prefix, 0);
   const bool cut = all * D * 4 > ONE_GO;
   p.own_splits = p.tail_splits = 1;
-  if (per <= QW && (prefix < 0 || prefix == 0 || (runs <= CUS && (batch == 1 || !cut)))) {
+  const double again = static_cast<double>((runs + CUS - 1) / CUS) * static_cast<double>(prefix) * static_cast<double>(D * 4);
+  if (per <= QW && (prefix <= 0 || (runs <= CUS ? batch == 1 || !cut : again <= AGAIN))) {
     p.stream = runs <= CUS ? 8 : 4;
     p.block_rows = QW;
     p.own_tiles = 1;

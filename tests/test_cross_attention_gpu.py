@@ -494,6 +494,23 @@ def test_cross_attention_masks_captured_and_shared(dev):
         assert torch.equal(outs[2][:, :512], outs[0][:, :512]) and (n > 0) == bool(outs[0].any()), n
 
 
+@pytest.mark.parametrize("kind,shape", [
+    ("fp16", (70, 4, 40, 20, 8, 4, 64)), ("bf16", (300, 1, 1, 3, 2, 1, 32)), ("fp16", (40, 3, 700, 33, 8, 8, 64)),
+    ("bf16", (33, 8, 31, 65, 16, 8, 128)), ("fp16", (90, 2, 330, 100, 3, 3, 96)), ("bf16", (520, 1, 64, 0, 1, 1, 48)),
+])
+def test_prefix_attention_of_many_sequences_read_by_each(dev, kind, shape):
+    """More sequences and key heads than CUs behind a short prefix: one launch, no workspace, the prefix read by each."""
+    B, L, _, S = shape[:4]
+    rng = np.random.default_rng(21)
+    lens = rng.integers(0, S + 1, B)  # some shorter than the new tokens: these see the prefix alone
+    lens[:3] = 0, S, S + 7
+    K = kern()
+    q, pk, k = (torch.empty(s, dtype=torch.float16, device=dev) for s in
+                ((B, L, shape[4], shape[6]), (shape[2], shape[5], shape[6]), (B, S, shape[5], shape[6])))
+    assert K.prefix_attention_work(q, pk, k) == 0
+    run_prefix(dev, kind, *shape, lens=lens.tolist(), junk=math.nan)
+
+
 @pytest.mark.parametrize("kind,B,L,P,S,H,KV,D", [("bf16", 40, 3, 3000, 200, 8, 2, 128), ("fp16", 12, 30, 2000, 900, 16, 16, 64),
                                                  ("fp16", 100, 1, 700, 2500, 4, 4, 96), ("bf16", 3, 200, 64, 5000, 2, 1, 64)])
 def test_prefix_attention_of_many_rows_and_cuts(dev, kind, B, L, P, S, H, KV, D):

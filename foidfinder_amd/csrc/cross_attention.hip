@@ -880,11 +880,14 @@ static Plan plan_of(int64_t batch, int64_t tokens, int64_t keys, int64_t prefix,
     p.blocks = runs * p.own_splits;
     return p;
   }
-  const int64_t most = prefix >= 0 ? rows : per;
+  const int64_t most = prefix > 0 ? rows : per;
   p.block_rows = most <= QW ? QW : most <= 2 * QW ? 2 * QW : 4 * QW;
   p.own_tiles = (per + p.block_rows - 1) / p.block_rows;
   const int64_t own = p.own_tiles * runs, tiles = (keys + BKV - 1) / BKV;
-  if (prefix >= 0) {
+  if (prefix == 0) {  // nothing to join: 12.5 -> 7.6 us for 4 x 128 tokens of 16 heads x 64
+    p.own_splits = split_keys(own, tiles, 0, 0, rows * kv, D, false);
+    p.slots = p.own_splits > 1 ? p.own_splits * rows * kv : 0;
+  } else if (prefix > 0) {
     p.prefix_tiles = (rows + p.block_rows - 1) / p.block_rows;
     const int64_t shared = p.prefix_tiles * kv, front = (prefix + BKV - 1) / BKV;
     p.own_splits = split_keys(own, tiles, shared, front, rows * kv, D, true);

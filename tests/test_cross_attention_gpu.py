@@ -511,6 +511,16 @@ def test_prefix_attention_of_many_sequences_read_by_each(dev, kind, shape):
     run_prefix(dev, kind, *shape, lens=lens.tolist(), junk=math.nan)
 
 
+@pytest.mark.parametrize("kind,shape", [
+    ("fp16", (4, 128, 0, 128, 4, 4, 64)), ("bf16", (2, 45, 0, 700, 4, 2, 128)), ("fp16", (1, 40, 0, 3000, 2, 1, 96)),
+    ("bf16", (3, 70, 0, 50, 1, 1, 40)),
+])
+def test_prefix_attention_without_a_prefix(dev, kind, shape):
+    B, S = shape[0], shape[3]
+    run_prefix(dev, kind, *shape)
+    run_prefix(dev, kind, *shape, lens=[S, 0, S // 2, 1][:B], junk=math.inf)
+
+
 @pytest.mark.parametrize("kind,B,L,P,S,H,KV,D", [("bf16", 40, 3, 3000, 200, 8, 2, 128), ("fp16", 12, 30, 2000, 900, 16, 16, 64),
                                                  ("fp16", 100, 1, 700, 2500, 4, 4, 96), ("bf16", 3, 200, 64, 5000, 2, 1, 64)])
 def test_prefix_attention_of_many_rows_and_cuts(dev, kind, B, L, P, S, H, KV, D):

@@ -898,7 +898,8 @@ static Plan plan_of(int64_t batch, int64_t tokens, int64_t keys, int64_t prefix,
     const int64_t slots = CUS * r.resident, whole = per / p.block_rows * runs, last = whole % slots;
     p.own_splits = split_keys(own, tiles, 0, 0, rows * kv, D, false);
     if (p.own_splits == 1 && whole > slots && last > 0) {
-      // The last round's workgroups, cut so that they fill the chip too, if that saves more than the join costs
+      // The last round's workgroups, cut so that they fill the chip too, if that saves more than the join costs: 120 -> 99 us (2 x
+      // 1029 queries, 2100 keys, 32 / 1 heads x 128), 246 -> 231 (9 x 1024, 5184, 16 x 64), 122 -> 122 (9 x 1024, 2100)
       const int64_t cuts = std::min<int64_t>(slots / last, tiles / 8);
       const double now = static_cast<double>(tiles) * std::max(r.alone, r.cu * static_cast<double>(last) / CUS);
       const double then = static_cast<double>(tiles) / static_cast<double>(std::max<int64_t>(cuts, 1)) *

@@ -207,15 +207,17 @@ struct Unit {
   }
   // The keys' p passed the limit, or m is not set: m becomes the largest c S of the keys, or just below, and O and l follow. Scores
   // from 2^30 up are too coarse for the multiply-add: what it leaves of the largest can be of any size then, and is capped.
+  // An infinite c S makes m infinite, and l not a number from then on (m - m): inf - inf, as the row's softmax has it. The joints
+  // of m and l keep it so.
   __device__ __forceinline__ void raise(const float16_t& xs, T8 (&pf)[2]) {
     float top = xs[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, xs[r]);
     top = fmaxf(top, xor_shuffle(top, 32)) * c;
     const float m_old = m;
-    m = fmaxf(m, top - fabsf(top) * 0x1p-23f);
+    m = fmaxf(m, top * (top > 0.f ? 1.f - 0x1p-23f : 1.f + 0x1p-23f));
     const float corr = __builtin_amdgcn_exp2f(m_old - m);
-    l *= corr;
+    l = __builtin_fmaf(l, corr, m - m);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll

@@ -1,0 +1,145 @@
+"""Attention to other rows and behind a prefix for scores and values that are not finite, on the GPU, against float64.
+
+Scores are fp32: one of +inf (an infinite element, or a product past fp32's range) makes its row not a number, as the softmax's
+inf - inf does; -inf has no weight while another seen key has some. The bar for finite rows is `bound` of the operators' own tests,
+for the keys that have a weight.
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+from test_cross_attention_gpu import TYPES, assert_near, bound, guarded, kern, reference64
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+INF = math.inf
+
+# B, L, S, H, KV, D by what computes them
+CROSS = {
+    "streams of eight waves": (2, 3, 700, 4, 2, 64),
+    "streams, keys cut": (2, 2, 6000, 4, 2, 128),
+    "streams of four waves": (140, 2, 200, 4, 2, 96),
+    "two units": (2, 50, 300, 2, 2, 64),
+    "two units of groups": (3, 25, 257, 8, 4, 128),
+    "tiles": (3, 100, 300, 2, 2, 64),
+    "tiles, a streamed rest": (2, 140, 333, 4, 2, 96),
+    "tiles, keys cut": (2, 70, 6000, 1, 1, 128),
+    "tiles, the last round cut": (9, 1029, 2100, 16, 16, 64),
+}
+# B, L, P, S, H, KV, D
+PREFIX = {
+    "streams of both": (1, 4, 300, 40, 8, 4, 64),
+    "streams of many sequences": (70, 4, 40, 20, 8, 4, 64),
+    "streams of own keys": (5, 2, 1025, 70, 4, 2, 128),
+    "two units": (3, 20, 200, 33, 4, 2, 96),
+    "tiles": (2, 130, 64, 200, 2, 1, 64),
+    "no prefix": (2, 140, 0, 170, 2, 2, 64),
+}
+
+
+def random(dev, kind, seed, *shapes):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return [torch.randn(*s, device=dev, generator=g).to(TYPES[kind]) for s in shapes]
+
+
+def call_cross(dev, kind, q, k, v, scale, lens, mask):
+    K = kern()
+    out, check = guarded(kind, dev, *q.shape)
+    need = K.cross_attention_work(q, k)
+    work = torch.full((need + 64,), math.nan, device=dev)
+    K.cross_attention(q, k, v, out, scale, lens, mask, work[:need])
+    assert check() and bool(work[need:].isnan().all())
+    return out
+
+
+def call_prefix(dev, kind, q, pk, pv, k, v, scale, lens):
+    K = kern()
+    out, check = guarded(kind, dev, *q.shape)
+    need = K.prefix_attention_work(q, pk, k)
+    work = torch.full((need + 64,), math.nan, device=dev)
+    K.prefix_attention(q, pk, pv, k, v, out, scale, lens, work[:need])
+    assert check() and bool(work[need:].isnan().all())
+    return out
+
+
+def own_seen(dev, B, L, S, lens):
+    """[B, L, S]: the own keys that a new token sees."""
+    n = (torch.full((B,), S, device=dev) if lens is None else lens.clamp(0, S))[:, None, None]
+    return torch.arange(S, device=dev) < n - L + 1 + torch.arange(L, device=dev)[:, None]
+
+
+def assert_rows(kind, got, q, k, v, scale, weighty, bad):
+    """weighty [B, L or 1, S]: keys with a finite score; bad [B, L or 1]: rows that are not a number; other rows without keys: 0."""
+    B, L = q.shape[:2]
+    weighty, bad = weighty.expand(B, L, -1), bad.expand(B, L)
+    some = weighty.any(-1)
+    got = got.float()
+    assert bool(got[bad].isnan().all()), f"{int((~got[bad].isnan()).sum())} finite values in rows that have none"
+    assert bool((got[~some & ~bad] == 0).all())
+    kept = (weighty & ~bad[..., None]).any(1)[:, :, None, None]  # what no good row needs holds anything
+    k, v = k.masked_fill(~kept, 0), v.masked_fill(~kept, 0)
+    dummy = weighty | ~some[..., None]
+    want = reference64(q.masked_fill(bad[..., None, None], 0), k, v, scale, dummy)
+    rows = (some & ~bad).cpu().numpy()
+    o, size, load = (x[rows] for x in want)
+    if rows.any():
+        tol = bound(kind, scale, o, size, load, v.float().abs().max().item(), k.size(1))
+        assert_near(got.cpu().numpy()[rows], o, tol)
+
+
+@pytest.mark.parametrize("kind,how", [("fp16", "key"), ("bf16", "key"), ("fp16", "query"), ("bf16", "query"), ("bf16", "dot"),
+                                      ("bf16", "scaled")])
+@pytest.mark.parametrize("name", CROSS)
+def test_cross_attention_of_an_infinite_score(dev, kind, how, name):
+    """An infinity in a key (rows with a negative query there give it no weight) or a query; a dot product past fp32's range, or
+    one past it times scale."""
+    B, L, S, H, KV, D = CROSS[name]
+    q, k0, v = random(dev, kind, 31, (B, L, H, D), (B, S, KV, D), (B, S, KV, D))
+    scale = 8.0 if how == "scaled" else D**-0.5
+    if how == "scaled":
+        q *= 2.0**-6
+    turn = (torch.arange(B, device=dev)[:, None] + torch.arange(L, device=dev)) % 3  # 0: infinite scores
+    sign = torch.where(turn == 0, 1.0, -1.0).to(q.dtype)[..., None]
+    g = torch.Generator(device=dev).manual_seed(32)
+    every = torch.ones(B, S, dtype=torch.bool, device=dev)
+    for at in (5, 40, S // 2, S - 1):
+        k = k0.clone()
+        weighty = every.clone()
+        if how == "query":
+            q[..., 0] = torch.where(turn[..., None] == 0, INF, 0.5).to(q.dtype)
+        else:
+            size, far = {"key": (1.0, INF), "dot": (2.0**70, 2.0**70), "scaled": (2.0**63, 2.0**63)}[how]
+            q[..., 0] = sign * size
+            if how != "key":
+                k[..., 0] = 0
+            k[:, at, :, 0] = far
+            weighty[:, at] = False
+        assert_rows(kind, call_cross(dev, kind, q, k, v, scale, None, None), q, k, v, scale, weighty[:, None], turn == 0)
+        mask = torch.rand(B, S, device=dev, generator=g) < 0.6
+        mask[:, at] = True
+        got = call_cross(dev, kind, q, k, v, scale, None, mask)
+        assert_rows(kind, got, q, k, v, scale, (weighty & mask)[:, None], turn == 0)
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("name", PREFIX)
+def test_prefix_attention_of_an_infinite_score(dev, kind, name):
+    B, L, P, S, H, KV, D = PREFIX[name]
+    q, pk0, pv, k0, v = random(dev, kind, 33, (B, L, H, D), (P, KV, D), (P, KV, D), (B, S, KV, D), (B, S, KV, D))
+    turn = (torch.arange(B, device=dev)[:, None] + torch.arange(L, device=dev)) % 3
+    q[..., 0] = torch.where(turn == 0, 1.0, -1.0).to(q.dtype)[..., None]
+    seen = torch.cat((torch.ones(B, L, P, dtype=torch.bool, device=dev), own_seen(dev, B, L, S, None)), 2)
+    vs = torch.cat((pv.expand(B, -1, -1, -1), v), 1)
+    for at in sorted({*([5, P - 1] if P else []), P, P + S - L, P + S - 1}):
+        pk, k = pk0.clone(), k0.clone()
+        (pk[at] if at < P else k[:, at - P])[..., 0] = INF
+        weighty = seen.clone()
+        weighty[:, :, at] = False
+        got = call_prefix(dev, kind, q, pk, pv, k, v, D**-0.5, None)
+        ks = torch.cat((pk.expand(B, -1, -1, -1), k), 1)
+        assert_rows(kind, got, q, ks, vs, D**-0.5, weighty, (turn == 0) & seen[:, :, at])

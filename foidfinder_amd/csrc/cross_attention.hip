@@ -45,6 +45,13 @@ constexpr int BKV = 64;    // keys a tile
 constexpr float SUM_LIMIT = 32768.f;  // a lane's sum of 16 p above which m is raised (fp16 holds p up to it)
 constexpr float CAP = 12.f;          // exponent of the largest p after m was raised
 constexpr float LOWEST = -3.402823466e38f;
+// m of a row, or of a part of it, that saw no key. One that saw keys of -inf alone keeps LOWEST: its sum is 0 too, and its softmax
+// not a number.
+constexpr float NONE = -__builtin_inff();
+// 1 / l, 0 without keys.
+__device__ __forceinline__ float inverse(float m, float l) {
+  return l != 0.f ? 1.f / l : m == NONE ? 0.f : __builtin_nanf("");
+}
 
 struct KeySource {
   const void *k, *v;
@@ -255,7 +262,7 @@ __device__ __forceinline__ void store4(const CrossArgs& a, const Piece& w, const
     if (col == 0) *reinterpret_cast<float2*>(a.work + a.slots * a.dim + 2 * n) = float2{m, l};
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // no keys: zeros
+  const float inv = inverse(m, l);
   vec4_t<T> v;
 #pragma unroll
   for (int u = 0; u < 4; ++u) v[u] = static_cast<T>(o[u] * inv);
@@ -429,10 +436,12 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
     return n;
   };
 
+  bool listed = false;  // any key
   if (w.t0 < w.t1) {
     uint64_t word, next = 0;  // of a list, 0 behind the last tile
     if constexpr (LIST) {
       word = valid(issue_listed(0));
+      listed = word != 0;
     } else {
       word = valid(w.keys - w.t0 * BKV);
       issue(w.t0, word);
@@ -468,6 +477,8 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
     }
   }
 
+  // A row that saw keys saw the first of the first tile, or of the list.
+  if (!(w.t0 < w.t1 && (LIST ? listed : limit > w.t0 * BKV))) u.m = NONE;
   if constexpr (SHARE == 2) {  // the second wave of a unit leaves O, m and l in LDS; the first joins them
     constexpr int WORDS = 16 * DT + 2;
     static_assert(2 * WORDS * 64 * 4 <= 4 * TILE * 2, "the joint exceeds the ring");
@@ -483,9 +494,9 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
     }
     __syncthreads();
     if (!active || half_sel) return;
-    const float top = fmaxf(u.m, joint[(WORDS - 2) * 64]);
-    const float c0 = __builtin_amdgcn_exp2f(u.m - top), c1 = __builtin_amdgcn_exp2f(joint[(WORDS - 2) * 64] - top);
-    u.m = top;
+    const float m1 = joint[(WORDS - 2) * 64], top = fmaxf(fmaxf(u.m, m1), LOWEST);
+    const float c0 = __builtin_amdgcn_exp2f(u.m - top), c1 = __builtin_amdgcn_exp2f(m1 - top);
+    u.m = fmaxf(u.m, m1);
     u.l = __builtin_fmaf(joint[(WORDS - 1) * 64], c1, u.l * c0);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -569,6 +580,7 @@ __device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w,
   };
 
   int n = w.t0 + wave;
+  uint32_t seen = 0;  // of any slice
   if (n < w.t1) {
     Slice now = slice(n, mask_byte(n));
     uint8_t byte = mask_byte(n + NW);
@@ -589,7 +601,9 @@ __device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w,
         load(next, false);
       }
       const int left = now.own ? p.limit - now.first : 32;
-      u.weigh(x, pf, now.word & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1), fh, n == w.t0 + wave);
+      const uint32_t bits = now.word & (left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1);
+      seen |= bits;
+      u.weigh(x, pf, bits, fh, n == w.t0 + wave);
       if (more)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LP) : "memory");  // all but the next K
       else
@@ -609,13 +623,14 @@ __device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w,
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) joint[(wave * WORDS + dt * 16 + r) * 64] = u.o[dt][r];
-  joint[(wave * WORDS + WORDS - 2) * 64] = u.m;
+  joint[(wave * WORDS + WORDS - 2) * 64] = seen ? u.m : NONE;
   joint[(wave * WORDS + WORDS - 1) * 64] = l_own;
   __syncthreads();
   if (row >= w.row_end) return;
-  float top = LOWEST;
+  float m = NONE;
 #pragma unroll
-  for (int k = 0; k < NW; ++k) top = fmaxf(top, joint[(k * WORDS + WORDS - 2) * 64]);
+  for (int k = 0; k < NW; ++k) m = fmaxf(m, joint[(k * WORDS + WORDS - 2) * 64]);
+  const float top = fmaxf(m, LOWEST);
   for (int g = wave; g < 4 * DT; g += NW) {  // words 4 g .. 4 g + 3: columns 32 (g / 4) + 8 (g % 4) + 4 fh + 0..3
     float4_t o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
@@ -627,7 +642,7 @@ __device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w,
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(part[(4 * g + e) * 64], f, o[e]);
     }
-    store4<T>(a, w, p, row, (g >> 2) * 32 + (g & 3) * 8 + 4 * fh, o, top, l);
+    store4<T>(a, w, p, row, (g >> 2) * 32 + (g & 3) * 8 + 4 * fh, o, m, l);
   }
 }
 
@@ -732,10 +747,11 @@ __global__ __launch_bounds__(256) void join_kernel(const CrossArgs a) {
   const int64_t at = (static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)) * (64 / (CH * LANES)) + of;
   if (at >= all) return;
   const float2* ml = reinterpret_cast<const float2*>(a.work + a.slots * a.dim) + at;
-  float top = LOWEST;
-  for (int p = lane % (CH * LANES); p < parts; p += CH * LANES) top = fmaxf(top, ml[p * all].x);
+  float m = NONE;
+  for (int p = lane % (CH * LANES); p < parts; p += CH * LANES) m = fmaxf(m, ml[p * all].x);
 #pragma unroll
-  for (int d = 1; d < CH * LANES; d <<= 1) top = fmaxf(top, xor_shuffle(top, d));
+  for (int d = 1; d < CH * LANES; d <<= 1) m = fmaxf(m, xor_shuffle(m, d));
+  const float top = fmaxf(m, LOWEST);
   const int col = 8 * c < a.dim ? 8 * c : 0;  // lanes past the columns join the first again
   const float* from = a.work + at * a.dim + col;
   const int64_t step = all * a.dim;
@@ -760,7 +776,7 @@ __global__ __launch_bounds__(256) void join_kernel(const CrossArgs a) {
     for (int e = 0; e < 8; ++e) o[e] = o[e] + xor_shuffle(o[e], d);
   }
   if (first != 0 || 8 * c >= a.dim) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = inverse(m, l);
   vec8_t<T> y;
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = static_cast<T>(o[e] * inv);

@@ -143,3 +143,53 @@ def test_prefix_attention_of_an_infinite_score(dev, kind, name):
         got = call_prefix(dev, kind, q, pk, pv, k, v, D**-0.5, None)
         ks = torch.cat((pk.expand(B, -1, -1, -1), k), 1)
         assert_rows(kind, got, q, ks, vs, D**-0.5, weighty, (turn == 0) & seen[:, :, at])
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("name", CROSS)
+def test_cross_attention_of_keys_at_minus_infinity(dev, kind, masked, name):
+    """Seen keys whose scores are all -inf are no missing keys: 0 / 0, not 0. With others behind or before them they weigh nothing."""
+    B, L, S, H, KV, D = CROSS[name]
+    q, k0, v = random(dev, kind, 34, (B, L, H, D), (B, S, KV, D), (B, S, KV, D))
+    q[..., 0] = 1.0
+    g = torch.Generator(device=dev).manual_seed(35)
+    at = torch.arange(S, device=dev)
+    lens = torch.full((B,), S, dtype=torch.int32, device=dev)
+    lens[0], lens[1] = 0, S - 7  # none in the first
+    for gone in (at >= 0, at < S * 7 // 10, at >= 40, at != S - 9):
+        minus = gone.expand(B, -1).clone()
+        if B > 2:
+            minus[2] = False
+        k = k0.clone()
+        k[..., 0].masked_fill_(minus[..., None], -INF)
+        mask, seen = None, at < lens[:, None]
+        if masked:
+            mask = torch.rand(B, S, device=dev, generator=g) < 0.5
+            mask[:, S - 9] = True
+            seen = seen & mask
+        weighty = seen & ~minus
+        bad = seen.any(1) & ~weighty.any(1)
+        got = call_cross(dev, kind, q, k, v, D**-0.5, lens, mask)
+        assert_rows(kind, got, q, k, v, D**-0.5, weighty[:, None], bad[:, None])
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("name", PREFIX)
+def test_prefix_attention_of_keys_at_minus_infinity(dev, kind, name):
+    B, L, P, S, H, KV, D = PREFIX[name]
+    q, pk0, pv, k0, v = random(dev, kind, 36, (B, L, H, D), (P, KV, D), (P, KV, D), (B, S, KV, D), (B, S, KV, D))
+    q[..., 0] = 1.0
+    lens = torch.full((B,), S, dtype=torch.int32, device=dev)
+    lens[0] = L - 1  # its first token sees the prefix alone, or nothing
+    seen = torch.cat((torch.ones(B, L, P, dtype=torch.bool, device=dev), own_seen(dev, B, L, S, lens)), 2)
+    vs = torch.cat((pv.expand(B, -1, -1, -1), v), 1)
+    at = torch.arange(P + S, device=dev)
+    for gone in (at >= 0, at < P, at >= P, at != P + S - L, at >= P + S // 2):
+        pk, k = pk0.clone(), k0.clone()
+        pk[..., 0].masked_fill_(gone[:P, None], -INF)
+        k[..., 0].masked_fill_(gone[P:, None], -INF)
+        weighty = seen & ~gone
+        bad = seen.any(2) & ~weighty.any(2)
+        got = call_prefix(dev, kind, q, pk, pv, k, v, D**-0.5, lens)
+        assert_rows(kind, got, q, torch.cat((pk.expand(B, -1, -1, -1), k), 1), vs, D**-0.5, weighty, bad)

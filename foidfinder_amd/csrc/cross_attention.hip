@@ -4,7 +4,9 @@
 // o = sum_j p_j v_j / sum_j p_j with p_j = 2^(c q.k_j - m), c = scale log2(e), over the keys that a query sees; m is a reference
 // near the largest c q.k_j, raised as larger ones come, and drops out of the quotient. q is used as given: c multiplies the
 // products in fp32 (folded into q it would round q once more). Sums, p's sum, m and O are fp32; p is rounded to the values' type
-// for the second product, half a step each, which is what the matrix cores take.
+// for the second product, half a step each, which is what the matrix cores take. fp16 has 2^-14 as its least normal number, so its p
+// reach 2^LIFT where m is set, and those below 2^-22 of the largest are rounded to steps of 2^-32 of it: n keys lose n 2^-33 of
+// the weight at most.
 //
 // Rows: the G = heads / kv_heads query heads of a key head read the same keys, so a key head's rows are (sequence, token, head
 // of the group), 32 of them a unit.
@@ -44,6 +46,11 @@ constexpr int WAVES = 4;   // waves a workgroup
 constexpr int BKV = 64;    // keys a tile
 constexpr float SUM_LIMIT = 32768.f;  // a lane's sum of 16 p above which m is raised (fp16 holds p up to it)
 constexpr float CAP = 12.f;          // exponent of the largest p after m was raised
+// m below the largest c S, where it is set. SUM_LIMIT is passed by a p of 2^11 at least, so that a raise moves m. Less room above
+// means more raises: us for 0, 6, 8, 10 of it 220, 222, 222, 226 (8 x 1025 queries, 5184 keys, 16 heads x 64), 12.8, 12.8, 13.2, 14.9
+// (2 x 256, 512, 8 x 64). bf16 has the exponents of fp32.
+template <typename T>
+constexpr float LIFT = std::is_same_v<T, half_t> ? 8.f : 0.f;
 constexpr float LOWEST = -3.402823466e38f;
 // m of a row, or of a part of it, that saw no key. One that saw keys of -inf alone keeps LOWEST: its sum is 0 too, and its softmax
 // not a number.
@@ -212,7 +219,7 @@ struct Unit {
     else
       l += sum;
   }
-  // The keys' p passed the limit, or m is not set: m becomes the largest c S of the keys, or just below, and O and l follow. Scores
+  // The keys' p passed the limit, or m is not set: m becomes LIFT less than the largest c S, or just below, and O and l follow. Scores
   // from 2^30 up are too coarse for the multiply-add: what it leaves of the largest can be of any size then, and is capped.
   // An infinite c S makes m infinite, and l not a number from then on (m - m): inf - inf, as the row's softmax has it. The joints
   // of m and l keep it so.
@@ -222,7 +229,7 @@ struct Unit {
     for (int r = 1; r < 16; ++r) top = fmaxf(top, xs[r]);
     top = fmaxf(top, xor_shuffle(top, 32)) * c;
     const float m_old = m;
-    m = fmaxf(m, top * (top > 0.f ? 1.f - 0x1p-23f : 1.f + 0x1p-23f));
+    m = fmaxf(m, top * (top > 0.f ? 1.f - 0x1p-23f : 1.f + 0x1p-23f) - LIFT<T>);
     const float corr = __builtin_amdgcn_exp2f(m_old - m);
     l = __builtin_fmaf(l, corr, m - m);
 #pragma unroll

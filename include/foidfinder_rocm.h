@@ -130,10 +130,11 @@ int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, const void* 
  * scale q.k over the keys j < lens[b] (int32 [B], taken into 0 .. S; NULL: S) whose mask[b * mask_batch + j] is not 0 (bytes; NULL:
  * all); 0 where there are none. What k and v hold for other keys is not read. Scores are fp32: one of +inf, as an infinite element
  * or a product past fp32's range gives it, makes its row not a number, and so do keys of -inf alone; beside others these have no
- * weight. q, k, v and their strides are multiples of 16 bytes, out's of 8; tokens of k and v are fewer than 2^24 elements apart.
- * work: at least ff_cross_attention_work fp32 elements (0 where keys are not cut; NULL then), which calls that run one after
- * another may share. out and work share no memory with each other or with what is read (refused; where rows of three strides
- * lie between another operand's, so are calls that would not touch it). */
+ * weight. p is rounded to the values' type before it multiplies them, half a step each; in fp16 p below 2^-22 of the row's largest
+ * are rounded to steps of 2^-32 of it. q, k, v and their strides are multiples of 16 bytes, out's of 8; tokens of k and v are fewer
+ * than 2^24 elements apart. work: at least ff_cross_attention_work fp32 elements (0 where keys are not cut; NULL then), which calls
+ * that run one after another may share. out and work share no memory with each other or with what is read (refused; where rows of
+ * three strides lie between another operand's, so are calls that would not touch it). */
 int64_t ff_cross_attention_work(int64_t B, int64_t L, int64_t S, int64_t heads, int64_t kv_heads, int64_t D);
 int ff_cross_attention(const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* k, int64_t k_batch,
                        int64_t k_token, int64_t k_head, const void* v, int64_t v_batch, int64_t v_token, int64_t v_head,

@@ -193,3 +193,41 @@ def test_prefix_attention_of_keys_at_minus_infinity(dev, kind, name):
         bad = seen.any(2) & ~weighty.any(2)
         got = call_prefix(dev, kind, q, pk, pv, k, v, D**-0.5, lens)
         assert_rows(kind, got, q, torch.cat((pk.expand(B, -1, -1, -1), k), 1), vs, D**-0.5, weighty, bad)
+
+
+# Weights of a row run from 2^8 of its largest score's down (fp16): half a subnormal step, 2^-25, is 2^-33 of the largest.
+TAIL = 2.0**-33
+
+
+@pytest.mark.parametrize("below", [24.625, 25.5, 28.0])
+@pytest.mark.parametrize("B,L,D", [(300, 1, 64), (600, 40, 128), (520, 128, 96)])
+def test_cross_attention_fp16_tails_below_the_subnormals(dev, below, B, L, D):
+    """60 000 keys of 2^-24.6 to 2^-28 of the largest's weight, below the last step of fp16 or just above it, not cut: they hold up
+    to 0.2 % of the weight. Weights are exact but for scale's and c's roundings (28 2^-23 in the exponent) and the tails'."""
+    S = 60001
+    q = torch.zeros(B, L, 1, D, dtype=torch.float16, device=dev)
+    k, v = torch.zeros(1, S, 1, D, dtype=torch.float16, device=dev), torch.ones(1, S, 1, D, dtype=torch.float16, device=dev)
+    q[..., 0], k[..., 0] = 1.0, -below / 2
+    k[0, 7, 0, 0], v[0, 7] = below / 2, 0.0
+    assert kern().cross_attention_work(q, k.expand(B, -1, -1, -1)) == 0
+    got = call_cross(dev, "fp16", q, k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1), math.log(2), None, None).float()
+    rest = 60000 * 2.0**-below
+    want = rest / (1 + rest)
+    tol = want * (2.0**-11 + 60000 / 16 * 2.0**-24 + 2.0**-17) + 60000 * TAIL + 2.0**-25
+    assert bool(((got - want).abs() <= tol).all()), ((got - want).abs().max().item(), want, tol)
+
+
+@pytest.mark.parametrize("B,L,D", [(300, 1, 64), (600, 40, 128), (520, 128, 96)])
+def test_cross_attention_fp16_tails_of_all_sizes(dev, B, L, D):
+    """Scores from the largest's down to 2^-40 of its weight, in no order."""
+    S = 40001
+    g = torch.Generator(device=dev).manual_seed(37)
+    q = torch.zeros(B, L, 1, D, dtype=torch.float16, device=dev)
+    k, v = torch.zeros(1, S, 1, D, dtype=torch.float16, device=dev), torch.rand(1, S, 1, D, device=dev, generator=g).half()
+    q[..., 0], k[0, :, 0, 0] = 1.0, -torch.linspace(16, 40, S, device=dev)[torch.randperm(S, device=dev, generator=g)].half()
+    k[0, 3, 0, 0], v[0, 3] = 0.0, 0.0
+    got = call_cross(dev, "fp16", q, k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1), math.log(2), None, None)
+    p = torch.exp2(k[0, :, 0, 0].double())
+    want = ((p @ v[0, :, 0].double()) / p.sum()).expand(B, L, 1, D)
+    tol = want * (2 * 2.0**-11 + S / 16 * 2.0**-24 + 2.0**-17) + S * TAIL + 2.0**-25
+    assert bool(((got.double() - want).abs() <= tol).all()), ((got.double() - want).abs() / tol).max().item()

@@ -22,6 +22,9 @@
 // Masks: a workgroup lists the keys that the mask leaves in LDS, a chunk of the mask at a time, and its tiles hold only those;
 // streams leave out masked keys' loads.
 //
+// Causal: a key that only later tokens see is in the tile all the same, with p = 0 for the earlier ones. Where its value is not
+// finite that product would not be 0: such values are found, added to the rows that see them (add_unbounded), and cleared in LDS.
+//
 // Loads go straight into LDS. Rows that no query of the workgroup may see (past the length, or masked) and columns past D are
 // out of the descriptor's range: they read as zeros and cost no traffic, and what the memory there holds never reaches a product.
 // Per wave, S^T = K Q^T by 32x32x16 products leaves a lane with one query and 16 of 32 keys; P^T then is the column operand of
@@ -108,6 +111,41 @@ __device__ __forceinline__ float add_pair(half_t a, half_t b, float c) {
 }
 __device__ __forceinline__ float add_pair(bf16_t a, bf16_t b, float c) {
   return __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{a, b}, bf16x2_t{bf16_t(1.f), bf16_t(1.f)}, c, false);
+}
+
+// Keys that rows see: all up to a length; those of them that a mask leaves; fewer for earlier tokens.
+enum class Keys { ALL, LISTED, CAUSAL };
+
+typedef unsigned short ushort8_t __attribute__((ext_vector_type(8)));
+// Magnitude of an infinity as bits; those above are not numbers.
+template <typename T>
+constexpr unsigned short INFINITE = std::is_same_v<T, half_t> ? 0x7c00 : 0x7f80;
+template <typename T>
+__device__ __forceinline__ bool finite(T v) {
+  return (__builtin_bit_cast(unsigned short, v) & 0x7fff) < INFINITE<T>;
+}
+// Whether N KB of LDS hold finite values alone.
+template <int N, typename T>
+__device__ __forceinline__ bool all_finite(const T* p, int lane) {
+  ushort8_t top = {};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    top = __builtin_elementwise_max(top, *reinterpret_cast<const ushort8_t*>(p + i * 512 + lane * 8) & ushort8_t(0x7fff));
+  int most = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) most = max(most, static_cast<int>(top[e]));
+  return !__any(most >= INFINITE<T>);
+}
+
+// Clears the others, N times 16 bytes of each of `threads` threads.
+template <int N, typename T>
+__device__ __forceinline__ void keep_finite(T* p, int thread, int threads) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    vec8_t<T>& x = *reinterpret_cast<vec8_t<T>*>(p + (i * threads + thread) * 8);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = finite(x[e]) ? x[e] : static_cast<T>(0.f);
+  }
 }
 
 // What a workgroup works on; the same in all its lanes.
@@ -230,7 +268,7 @@ struct Unit {
     top = fmaxf(top, xor_shuffle(top, 32)) * c;
     const float m_old = m;
     m = fmaxf(m, top * (top > 0.f ? 1.f - 0x1p-23f : 1.f + 0x1p-23f) - LIFT<T>);
-    const float corr = __builtin_amdgcn_exp2f(m_old - m);
+    const float corr = m_old == LOWEST ? 1.f : __builtin_amdgcn_exp2f(m_old - m);  // O held nothing, or infinities to be kept
     l = __builtin_fmaf(l, corr, m - m);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -254,6 +292,21 @@ struct Unit {
 #pragma unroll
         for (int i = 0; i < VSTEP; ++i)
           o[dt + i] = mfma(__builtin_shufflevector(x[i][2 * tt], x[i][2 * tt + 1], 0, 1, 2, 3, 4, 5, 6, 7), pf[tt], o[dt + i]);
+    }
+  }
+  // Adds the values that are not finite among those of N keys at `rows` to the rows that see them: the first `left` keys.
+  template <int N>
+  __device__ __forceinline__ void add_unbounded(const T* rows, int left, int fh) {
+#pragma unroll 1
+    for (int j = 0; j < N; ++j) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const T4 x = *reinterpret_cast<const T4*>(rows + j * DP + v_slot<DP>(j, 4 * dt + g) * 8 + 4 * fh);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[dt][4 * g + e] += j < left && !finite(x[e]) ? static_cast<float>(x[e]) : 0.f;
+        }
     }
   }
 };
@@ -285,20 +338,22 @@ constexpr int tile_bytes(int dp) { return 4 * BKV * dp * 2 > stream_bytes(dp, WA
 // Keys of a mask that are listed at a time: what the LDS leaves room for beside a CU's workgroups.
 constexpr int list_chunk(int dp) { return dp == 64 ? 1024 : dp == 96 ? 512 : 2048; }
 
-// Tiles of 64 keys for four waves: a wave a unit (SHARE 1), or two (SHARE 2), each with one half of every tile. LIST: tiles hold
+// Tiles of 64 keys for four waves: a wave a unit (SHARE 1), or two (SHARE 2), each with one half of every tile. LISTED: tiles hold
 // keys that the mask leaves, and no others. Us for half the keys masked at random, a third at the end, none, where a tile's mask
 // word left out loads and empty tiles, and by list: 15.1 -> 16.1, 14.7 -> 16.1, 14.6 -> 15.7 (2 x 256 queries, 512 keys, 8 heads x
 // 64); 26.8 -> 18.4, 20.5 -> 20.4, 24.3 -> 25.8 (4 x 512, 1024, 16 x 64); 62 -> 36, 46 -> 44, 56 -> 58 (2 x 512, 2048, 32 / 8 x
 // 128); 330 -> 172, 226 -> 217, 289 -> 291 (4 x 1024, 4096, 32 / 8 x 128). A list in memory, by a kernel of its own: 182, 228, 300.
-template <typename T, int DP, int SHARE, bool LIST>
+template <typename T, int DP, int SHARE, Keys KEYS>
 __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T* smem) {
   typedef vec8_t<T> T8;
+  constexpr bool LIST = KEYS == Keys::LISTED, CAUSAL = KEYS == Keys::CAUSAL;
   constexpr int CH = DP / 8, TILE = BKV * DP, LPW = CH / 4, KS = DP / 16, DT = DP / 32;
   const uint32_t smem_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)smem));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 31, fh = lane >> 5, unit = wave / SHARE, half_sel = SHARE == 2 ? wave & 1 : 0;
   const bool active = w.row0 + unit * QW < w.row_end;  // other waves only load
   int row = w.row0 + unit * QW + fr, limit;
+  const int lowest = CAUSAL ? place_of(a, w, w.row0).limit : 0;  // of the workgroup's first row
   Unit<T, DP> u;
   {
     const Place p = place_of(a, w, row);
@@ -464,6 +519,15 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
         next = valid(w.keys - (tile + 1) * BKV);
         issue(tile + 1, next);
       }
+      if constexpr (CAUSAL) {
+        T* values = smem + (2 + st) * TILE;
+        if (min((tile + 1) * BKV, w.keys) > lowest && !all_finite<TILE * 2 / 1024>(values, lane)) {  // the same in all waves
+          if (active) u.template add_unbounded<BKV / SHARE>(values + half_sel * 32 * DP, limit - tile * BKV - 32 * half_sel, fh);
+          __syncthreads();
+          keep_finite<LPW>(values, threadIdx.x, 64 * WAVES);
+          __syncthreads();
+        }
+      }
       if (active) {
         // read bases, opaque to the compiler so that the fragment offsets fold into the reads' immediate offsets
         int ka = st * TILE + half_sel * 32 * DP + u.koff, ka_odd = 0, va = (2 + st) * TILE + half_sel * 32 * DP + u.voff;
@@ -528,7 +592,7 @@ __device__ __forceinline__ void tile_block(const CrossArgs& a, const Piece& w, T
 // barrier stands between load and use: a wave asks for the next slice's K once it has read this one's, and for its V likewise, so
 // that half a slice or more (8 KB at 128 columns) is on its way to each wave at any time. The slices are those of the prefix
 // (w.front), then the sequence's own. The waves' O, m and l are joined through LDS, four columns a wave and turn.
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool CAUSAL>
 __device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w, T* smem) {
   typedef vec8_t<T> T8;
   constexpr int CH = DP / 8, SLICE = 32 * DP, LP = CH / 2, DT = DP / 32, WORDS = 16 * DT + 2;
@@ -615,6 +679,11 @@ __device__ __forceinline__ void stream_block(const CrossArgs& a, const Piece& w,
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LP) : "memory");  // all but the next K
       else
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (CAUSAL && __any(bits != now.word) && !all_finite<LP>(kbuf + SLICE, lane)) {
+        u.template add_unbounded<32>(kbuf + SLICE, left, fh);
+        keep_finite<LP>(kbuf + SLICE, lane, 64);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
       u.template mix<0>(vbuf, u.voff, pf);
       if (!more) break;
       load(next, true);
@@ -659,8 +728,9 @@ __device__ __forceinline__ void touch(const CrossArgs& a) {
 }
 
 // Waves a SIMD: what the LDS leaves room for (34, 50 and 66 KB a workgroup).
-template <typename T, int DP, bool LIST>
+template <typename T, int DP, Keys KEYS>
 __global__ __launch_bounds__(64 * WAVES, DP == 64 ? 4 : DP == 96 ? 3 : 2) void cross_kernel(const CrossArgs a) {
+  constexpr bool LIST = KEYS == Keys::LISTED;
   // K slots, then V slots; the list and its counts
   __shared__ __attribute__((aligned(1024))) T smem[tile_bytes(DP) / 2 + (LIST ? 2 * (list_chunk(DP) + BKV + WAVES) : 0)];
   touch(a);
@@ -718,17 +788,17 @@ __global__ __launch_bounds__(64 * WAVES, DP == 64 ? 4 : DP == 96 ? 3 : 2) void c
   w.t1 = static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / splits);
   w.front = w.seq < 0 ? w.t1 : 0;
   if (units == 1)
-    stream_block<T, DP, WAVES>(a, w, smem);
+    stream_block<T, DP, WAVES, KEYS == Keys::CAUSAL>(a, w, smem);
   else if (units == 2)
-    tile_block<T, DP, 2, LIST>(a, w, smem);
+    tile_block<T, DP, 2, KEYS>(a, w, smem);
   else
-    tile_block<T, DP, 1, LIST>(a, w, smem);
+    tile_block<T, DP, 1, KEYS>(a, w, smem);
 }
 
 // Up to 32 rows a sequence and key head: workgroups of NW waves that all read the same rows' keys, the prefix's among them. Where
 // there are few (NW 8, one a CU), a single launch does as long as the keys are few enough. Sequences of a head are neighbours: they
 // share the prefix.
-template <typename T, int DP, int NW>
+template <typename T, int DP, int NW, bool CAUSAL>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : DP == 64 ? 4 : DP == 96 ? 3 : 2) void stream_kernel(const CrossArgs a) {
   __shared__ __attribute__((aligned(1024))) T smem[stream_bytes(DP, NW) / 2];
   touch(a);
@@ -742,7 +812,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : DP == 64 ? 4 : DP == 96 ? 3 
   const int64_t slices = w.front + (w.keys + 31) / 32;
   w.t0 = static_cast<int>(slices * split / a.own_splits);
   w.t1 = static_cast<int>(slices * (split + 1) / a.own_splits);
-  stream_block<T, DP, NW>(a, w, smem);
+  stream_block<T, DP, NW, CAUSAL>(a, w, smem);
 }
 
 // Joins the parts of a row: CH lanes for its columns (8 each), LANES times over for as many parts at a time, joined at the end.
@@ -808,14 +878,17 @@ __global__ __launch_bounds__(256) void join_kernel(const CrossArgs a) {
 template <typename T, int DP>
 static void launch_cross(const CrossArgs& a, int64_t blocks, int stream, hipStream_t st) {
   const dim3 runs(a.batch, a.kv, a.own_splits);
+  const dim3 all(static_cast<unsigned>(blocks));
   if (stream == 8)
-    stream_kernel<T, DP, 8><<<runs, 64 * 8, 0, st>>>(a);
+    a.causal ? stream_kernel<T, DP, 8, true><<<runs, 64 * 8, 0, st>>>(a) : stream_kernel<T, DP, 8, false><<<runs, 64 * 8, 0, st>>>(a);
   else if (stream == 4)
-    stream_kernel<T, DP, 4><<<runs, 64 * 4, 0, st>>>(a);
+    a.causal ? stream_kernel<T, DP, 4, true><<<runs, 64 * 4, 0, st>>>(a) : stream_kernel<T, DP, 4, false><<<runs, 64 * 4, 0, st>>>(a);
   else if (a.mask)
-    cross_kernel<T, DP, true><<<dim3(static_cast<unsigned>(blocks)), 64 * WAVES, 0, st>>>(a);
+    cross_kernel<T, DP, Keys::LISTED><<<all, 64 * WAVES, 0, st>>>(a);
+  else if (a.causal)
+    cross_kernel<T, DP, Keys::CAUSAL><<<all, 64 * WAVES, 0, st>>>(a);
   else
-    cross_kernel<T, DP, false><<<dim3(static_cast<unsigned>(blocks)), 64 * WAVES, 0, st>>>(a);
+    cross_kernel<T, DP, Keys::ALL><<<all, 64 * WAVES, 0, st>>>(a);
   if (!a.work) return;
   constexpr int CH = DP == 64 ? 8 : 16;
   const int parts = a.tail ? a.tail_splits : a.prefix_splits + a.own_splits;
@@ -1067,7 +1140,7 @@ int attend(const char* name, const Rows& q, const Rows& k, const Rows& v, const 
   if (pk) a.prefix = source(*pk, *pv);
   a.lens = lens, a.mask = mask, a.mask_b = mask_batch, a.work = p.slots > 0 ? work : nullptr, a.slots = p.slots;
   a.batch = static_cast<int>(batch), a.tokens = static_cast<int>(tokens), a.kv = static_cast<int>(kv);
-  a.group = static_cast<int>(heads / kv), a.dim = static_cast<int>(D), a.causal = pk != nullptr;
+  a.group = static_cast<int>(heads / kv), a.dim = static_cast<int>(D), a.causal = pk && tokens > 1;  // a single token sees all
   a.rows = static_cast<int>(batch * tokens) * a.group;
   a.block_rows = static_cast<int>(p.block_rows), a.own_tiles = static_cast<int>(p.own_tiles);
   a.own_splits = static_cast<int>(p.own_splits), a.prefix_tiles = static_cast<int>(p.prefix_tiles);

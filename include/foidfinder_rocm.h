@@ -144,8 +144,8 @@ int ff_cross_attention(const void* q, int64_t q_batch, int64_t q_token, int64_t 
 
 /* Attention of a batch whose sequences share a prefix: prefix_k, prefix_v [P, kv_heads, D] are seen by all (a long one is read once
  * for all), and k, v [B, S, kv_heads, D] are each sequence's own keys behind it, lens[b] of them (int32 [B], taken into 0 .. S;
- * NULL: S), the last L of them the new tokens' own: query i sees the prefix and the own keys j < lens[b] - L + 1 + i. P and S may
- * be 0. The rest as in ff_cross_attention. */
+ * NULL: S), the last L of them the new tokens' own: query i sees the prefix and the own keys j < lens[b] - L + 1 + i, and what
+ * later ones hold does not reach it. P and S may be 0. The rest as in ff_cross_attention. */
 int64_t ff_prefix_attention_work(int64_t B, int64_t L, int64_t P, int64_t S, int64_t heads, int64_t kv_heads, int64_t D);
 int ff_prefix_attention(const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* prefix_k,
                         int64_t pk_token, int64_t pk_head, const void* prefix_v, int64_t pv_token, int64_t pv_head,

@@ -231,3 +231,49 @@ def test_cross_attention_fp16_tails_of_all_sizes(dev, B, L, D):
     want = ((p @ v[0, :, 0].double()) / p.sum()).expand(B, L, 1, D)
     tol = want * (2 * 2.0**-11 + S / 16 * 2.0**-24 + 2.0**-17) + S * TAIL + 2.0**-25
     assert bool(((got.double() - want).abs() <= tol).all()), ((got.double() - want).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+@pytest.mark.parametrize("shape", [
+    (1, 4, 300, 40, 8, 4, 64), (70, 4, 40, 20, 8, 4, 96), (5, 6, 1025, 70, 4, 2, 128), (3, 20, 200, 33, 4, 2, 96),
+    (2, 130, 64, 200, 2, 1, 64), (2, 140, 0, 170, 2, 2, 64), (3, 50, 80, 150, 4, 2, 128), (2, 45, 0, 64, 1, 1, 40),
+    (2, 100, 31, 100, 1, 1, 128),
+])
+def test_prefix_attention_of_values_that_earlier_tokens_do_not_see(dev, kind, shape):
+    """Infinities and not-a-numbers in new tokens' values and keys reach the tokens that see them, and no others."""
+    B, L, P, S, H, KV, D = shape
+    q, pk, pv, k, v = random(dev, kind, 38, (B, L, H, D), (P, KV, D), (P, KV, D), (B, S, KV, D), (B, S, KV, D))
+    lens = torch.full((B,), S, dtype=torch.int32, device=dev)
+    lens[0] = max(L - 2, 1) if B > 1 else S  # tokens that see the prefix alone, or nothing
+    for b in range(B):
+        n = int(lens[b])
+        v[b, n - 1, :, 0], v[b, n - 1, :, 1], v[b, n - 1, :, 2] = INF, -INF, math.nan
+        v[b, n - 1, :, D - 1] = INF
+        v[b, n - 2, :, 3], v[b, n - 2, :, 4] = INF, math.nan
+        v[b, max(n - 2 * L // 3, 0), :, 5], v[b, n - 1, :, 5] = INF, -INF  # both: not a number
+        v[b, max(n - L // 2, 0), :, 6] = -INF
+    got = call_prefix(dev, kind, q, pk, pv, k, v, D**-0.5, lens).float()
+    seen = torch.cat((torch.ones(B, L, P, dtype=torch.bool, device=dev), own_seen(dev, B, L, S, lens)), 2)
+    ks, vs = torch.cat((pk.expand(B, -1, -1, -1), k), 1), torch.cat((pv.expand(B, -1, -1, -1), v), 1)
+    # what a row sees that is not finite, by column; every weight is far above 0
+    some = seen.any(-1, keepdim=True)
+    o, size, load = reference64(q, ks, vs.masked_fill(~vs.isfinite(), 0), D**-0.5, seen | ~some)
+    G = H // KV
+    hits = [(seen.float() @ f.float().reshape(B, P + S, KV * D)).view(B, L, KV, D).repeat_interleave(G, 2) > 0
+            for f in (vs == INF, vs == -INF, vs.isnan())]
+    bad = hits[2] | (hits[0] & hits[1])
+    assert bool(got[bad].isnan().all())
+    assert bool((got[hits[0] & ~bad] == INF).all() and (got[hits[1] & ~bad] == -INF).all())
+    plain = ~(bad | hits[0] | hits[1])
+    assert bool((got[plain & ~some[..., None]] == 0).all())
+    at = (plain & some[..., None]).cpu().numpy()
+    tol = bound(kind, D**-0.5, o, size, load, vs[vs.isfinite()].float().abs().max().item(), P + S)
+    assert_near(got.cpu().numpy()[at], o[at], np.broadcast_to(tol, o.shape)[at])
+    # a key that is not a number: the tokens that see it, and no others
+    v = v.masked_fill(~v.isfinite(), 0)
+    for b in range(B):
+        k[b, int(lens[b]) - 1] = math.nan
+    got = call_prefix(dev, kind, q, pk, pv, k, v, D**-0.5, lens).float()
+    last = torch.zeros(B, L, dtype=torch.bool, device=dev)
+    last[:, -1] = True
+    assert bool(got[last].isnan().all() and got[~last].isfinite().all())

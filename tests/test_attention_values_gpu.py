@@ -277,3 +277,28 @@ def test_prefix_attention_of_values_that_earlier_tokens_do_not_see(dev, kind, sh
     last = torch.zeros(B, L, dtype=torch.bool, device=dev)
     last[:, -1] = True
     assert bool(got[last].isnan().all() and got[~last].isfinite().all())
+
+
+@pytest.mark.parametrize("kind,D", [("fp16", 48), ("bf16", 96), ("fp16", 128), ("bf16", 64)])
+@pytest.mark.parametrize("with_lens", [False, True])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("B,L,H,KV", [(280, 1, 4, 1), (70, 5, 24, 4)])
+def test_cross_attention_streams_of_four_waves(dev, kind, D, with_lens, masked, B, L, H, KV):
+    """More sequences and key heads than CUs, up to 32 rows of each: four waves a workgroup, keys uncut."""
+    S = 333
+    q, k, v = random(dev, kind, 39, (B, L, H, D), (B, S, KV, D), (B, S, KV, D))
+    assert B * KV > 256 and kern().cross_attention_work(q, k) == 0
+    g = torch.Generator(device=dev).manual_seed(40)
+    lens = mask = None
+    seen = torch.ones(B, S, dtype=torch.bool, device=dev)
+    if with_lens:
+        lens = torch.randint(0, S + 1, (B,), device=dev, generator=g).int()
+        lens[:6] = torch.tensor([0, 1, 32, 33, S + 5, -3], device=dev)
+        seen = torch.arange(S, device=dev) < lens[:, None]
+    if masked:
+        mask = torch.rand(B, S, device=dev, generator=g) < torch.linspace(0.02, 0.98, B, device=dev)[:, None]
+        mask[3], mask[7], mask[8, :] = False, True, torch.arange(S, device=dev) == S - 1
+        seen = seen & mask
+    k[~seen], v[~seen] = math.nan, math.nan
+    got = call_cross(dev, kind, q, k, v, D**-0.5, lens, mask)
+    assert_rows(kind, got, q, k, v, D**-0.5, seen[:, None], torch.zeros(B, 1, dtype=torch.bool, device=dev))

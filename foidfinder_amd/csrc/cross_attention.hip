@@ -1085,8 +1085,8 @@ const char* bad_sizes(int64_t batch, int64_t tokens, int64_t keys, int64_t prefi
   if (batch != 0 && tokens != 0 && (tokens > 0x7fffffff / batch || batch * tokens > 0x7fffffff / heads))
     return "need batch * tokens * heads < 2^31";
   p = plan_of(batch, tokens, keys, prefix, kv, heads / kv, D);
-  if (p.blocks >= (int64_t(1) << 24) || (p.slots > 0 && batch * tokens * heads > (1 << 26) - 4))
-    return "too many rows for one launch";
+  const int64_t joined = p.tail ? p.tail * p.block_rows : p.slots > 0 ? batch * tokens * heads : 0;
+  if (p.blocks >= (int64_t(1) << 24) || joined > (1 << 26) - 4) return "too many rows for one launch";
   return nullptr;
 }
 

@@ -132,7 +132,8 @@ int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, const void* 
  * or a product past fp32's range gives it, makes its row not a number, and so do keys of -inf alone; beside others these have no
  * weight. p is rounded to the values' type before it multiplies them, half a step each; in fp16 p below 2^-22 of the row's largest
  * are rounded to steps of 2^-32 of it. q, k, v and their strides are multiples of 16 bytes, out's of 8; tokens of k and v are fewer
- * than 2^24 elements apart. work: at least ff_cross_attention_work fp32 elements (0 where keys are not cut; NULL then), which calls
+ * than 2^24 elements apart. B L heads < 2^31, in fewer than 2^24 workgroups of up to 128 rows of a sequence and key head; where the
+ * keys of all rows are cut, B L heads <= 2^26 - 4 (both refused). work: at least ff_cross_attention_work fp32 elements (0 where keys are not cut; NULL then), which calls
  * that run one after another may share. out and work share no memory with each other or with what is read (refused; where rows of
  * three strides lie between another operand's, so are calls that would not touch it). */
 int64_t ff_cross_attention_work(int64_t B, int64_t L, int64_t S, int64_t heads, int64_t kv_heads, int64_t D);

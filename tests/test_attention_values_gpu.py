@@ -302,3 +302,17 @@ def test_cross_attention_streams_of_four_waves(dev, kind, D, with_lens, masked, 
     k[~seen], v[~seen] = math.nan, math.nan
     got = call_cross(dev, kind, q, k, v, D**-0.5, lens, mask)
     assert_rows(kind, got, q, k, v, D**-0.5, seen[:, None], torch.zeros(B, 1, dtype=torch.bool, device=dev))
+
+
+def test_cross_attention_of_more_rows_than_a_join_takes(dev):
+    """67 million rows, of which the last round's are cut and joined: that round's head and sequence, and rows of all others."""
+    B, L, S, H, D = 8, 524544, 2100, 16, 8
+    q, k, v = random(dev, "fp16", 42, (1, L, H, D), (B, S, H, D), (B, S, H, D))
+    out = call_cross(dev, "fp16", q.expand(B, -1, -1, -1), k, v, D**-0.5, None, None)
+    every = torch.ones(1, 1, S, dtype=torch.bool, device=dev)
+    for b, h, rows in [(B - 1, H - 1, slice(L - 40000, L)), (B - 1, H - 1, slice(0, 1000))] + [
+            (b, h, slice(b * 65536 + h * 64, None, 99991)) for b in range(B) for h in range(H)]:
+        args = q[:, rows, h : h + 1], k[b : b + 1, :, h : h + 1], v[b : b + 1, :, h : h + 1]
+        o, size, load = reference64(*args, D**-0.5, every)
+        got = out[b : b + 1, rows, h : h + 1].float().cpu().numpy()
+        assert_near(got, o, bound("fp16", D**-0.5, o, size, load, args[2].float().abs().max().item(), S))

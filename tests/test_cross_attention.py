@@ -218,3 +218,13 @@ def test_python_ops_refuse_what_does_not_fit():
     for name, n in (("cross_attention", 5), ("prefix_attention", 7)):
         with pytest.raises((RuntimeError, NotImplementedError)):  # no CPU kernel is registered
             getattr(K.kernels(), name)(*([q] * (n - 1)), 1.0)
+
+
+def test_cross_attention_of_many_rows_whose_last_round_alone_is_cut():
+    """Only the rows of that round are joined: 2^26 rows in all are no limit there."""
+    size, few = (8, 524544, 2100, 16, 16, 8), (8, 4352, 2100, 16, 16, 8)
+    work = K.lib().ff_cross_attention_work
+    assert 8 * 524544 * 16 > 1 << 26
+    assert work(*size) == work(*few) > 0  # the same rest of 256 whole row tiles
+    refused(cross(B=8, L=524544, S=2100, H=16, KV=16, D=8), "workspace is too small")
+    refused(prefix(B=1 << 22, L=1, P=9000, S=9, H=32, KV=1), "too many rows")  # every row is joined

@@ -45,6 +45,13 @@ __device__ __forceinline__ float inv_root(float v) {
   return v < 0x1p-126f ? __builtin_amdgcn_rsqf(v * 0x1p24f) * 0x1p12f : __builtin_amdgcn_rsqf(v);
 }
 
+// sum / n, rounded once; inv: 1 / n, whose own rounding the quotient would keep. Equal elements, whose sum is exact, then have their
+// own value as mean: what is left of it would be divided by a variance of nothing.
+__device__ __forceinline__ float mean_of(float sum, float n, float inv) {
+  const float q = sum * inv;
+  return __builtin_fmaf(__builtin_fmaf(-q, n, sum), inv, q);
+}
+
 template <typename T, int LANES, int CHUNKS, int POST, int PRE>
 __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kernel(const ResidualArgs a) {
   constexpr int THREADS = LANES <= 64 ? 256 : LANES, GROUPS = THREADS / LANES, WIDTH = LANES < 64 ? LANES : 64;
@@ -73,7 +80,7 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kerne
     return n;
   };
   const int mine = WPR > 1 ? columns(wave) : a.width;
-  const float own = mine ? 1.f / static_cast<float>(mine) : 0.f;
+  const float own_n = static_cast<float>(mine), own = mine ? 1.f / own_n : 0.f;
 
   float post_g[CHUNKS][8], post_b[CHUNKS][8], pre_g[CHUNKS][8], pre_b[CHUNKS][8], factor[CHUNKS][8];
   // The compiler's wait for these loads stands here, before the loop: in it, the same counter holds the next row's loads.
@@ -136,7 +143,7 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kerne
     float sum = 0.f, centre = 0.f;
     if constexpr (CENTRED) {
       sum = sum_of(v, [](float s, float x) { return s + x; });
-      centre = sum * own;
+      centre = mean_of(sum, own_n, own);
     }
     float sq = sum_of(v, [centre](float s, float x) {
       const float d = CENTRED ? x - centre : x;
@@ -149,7 +156,7 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kerne
         float all = 0.f;
 #pragma unroll
         for (int w = 0; w < WPR; ++w) all = all + joint[turn][w].x;
-        centre = all * inv_n;
+        centre = mean_of(all, static_cast<float>(a.width), inv_n);
       }
       sq = 0.f;
 #pragma unroll
@@ -157,9 +164,9 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_norm_kerne
         const float2 j = joint[turn][w];
         sq = sq + j.y;
         if constexpr (CENTRED) {
-          const int n = columns(w);
-          const float d = n ? j.x * __builtin_amdgcn_rcpf(static_cast<float>(n)) - centre : 0.f;
-          sq = __builtin_fmaf(static_cast<float>(n) * d, d, sq);
+          const float n = static_cast<float>(columns(w));  // 0: of no columns, and j.x is 0
+          const float d = __builtin_fmaf(-centre, n, j.x);
+          sq = __builtin_fmaf(n > 0.f ? d * __builtin_amdgcn_rcpf(n) : 0.f, d, sq);
         }
       }
       turn ^= 1;  // the next norm writes the other one: its barrier lies between the reads here and the next write

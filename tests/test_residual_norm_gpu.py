@@ -169,3 +169,21 @@ def test_residual_norm_on_streams_and_in_graphs(dev):
         call(c)
         torch.cuda.synchronize()
         assert torch.equal(a[0], c[0]) and torch.equal(a[1], c[1])
+
+
+@pytest.mark.parametrize("kind,value", [("fp16", 300.0), ("fp16", -60000.0), ("fp16", 0.1), ("bf16", 300.0), ("bf16", 1e30)])
+@pytest.mark.parametrize("C", [8, 72, 200, 1000, 1032, 3000, 5000, 8184])
+def test_residual_norm_of_constant_rows(dev, kind, value, C):
+    """Equal elements have no variance: LayerNorm leaves beta. Their sum has at most 11 + 13 significant bits, as fp32 holds, so that
+    the mean is exact."""
+    K = kern()
+    dt = TYPES[kind]
+    x = torch.full((3, C), value, device=dev).to(dt)
+    zero = torch.zeros_like(x)
+    g = torch.Generator(device=dev).manual_seed(41)
+    gamma, beta = 1 + 0.2 * torch.randn(C, device=dev, generator=g), torch.randn(C, device=dev, generator=g)
+    xo, h = torch.empty_like(x), torch.empty_like(x)
+    K.residual_norm(zero, x, xo, None, K.NORM_LAYER, gamma, beta, K.NORM_NONE, None, None)
+    assert torch.equal(xo, beta.to(dt).expand(3, -1))
+    K.residual_norm(x, zero, xo, h, K.NORM_NONE, None, None, K.NORM_LAYER, gamma, beta)
+    assert torch.equal(xo, x) and torch.equal(h, beta.to(dt).expand(3, -1))

@@ -901,9 +901,9 @@ static void launch_cross(const CrossArgs& a, int64_t blocks, int stream, hipStre
     join_kernel<T, CH, 1><<<dim3(static_cast<unsigned>((rows + 4 * (64 / CH) - 1) / (4 * (64 / CH)))), 256, 0, st>>>(a);
 }
 
-// Kernels of 64, 96 and 128 columns; between them the rest is zeros, which take products and LDS but no memory: 32, 48, 64 columns in
-// 156, 165, 178 us, 72, 80, 88, 96 in 242 to 253, 104 and 128 in 319 and 322 (8 x 1024 queries, 4096 keys, 16 heads, fp16); 32, 64, 72,
-// 96, 128 in 15, 25, 33, 43, 59 (64 single tokens, 1025 keys, 32 / 8 heads).
+// Kernels of 64, 96 and 128 columns; between them the rest is zeros, which take products and LDS but no memory: 32, 48, 64
+// columns in 156, 165, 178 us, 72, 80, 88, 96 in 242 to 253, 104 and 128 in 319 and 322 (8 x 1024 queries, 4096 keys, 16 heads,
+// fp16); 32, 64, 72, 96, 128 in 15, 25, 33, 43, 59 (64 single tokens, 1025 keys, 32 / 8 heads).
 template <typename T>
 static void launch_cross_dim(const CrossArgs& a, int64_t blocks, int stream, hipStream_t st) {
   if (a.dim <= 64)
@@ -943,10 +943,10 @@ static Rates rates_of(int64_t D) {
 // Cuts of the keys of `blocks` workgroups that have `tiles` tiles each, beside `others` workgroups of `theirs`: the cut that ends
 // first. A CU's load is taken halfway between the mean and the fullest CU's, and rounds halfway between their number and the next
 // whole one; the two kinds share the chip by their tiles. Parts of a row are written and read again, half of it within the caches,
-// and joined by a second launch. From two workgroups a CU on keys are not cut: what that loses is small (640 of 66 tiles: 124 us uncut,
-// 118 in two, 127 in four), and a cut may lose more (720 of 32: 65, 78, 91). Over the 32 shapes timed with 1 .. 48 cuts (1 to 128
-// sequences of 1 to 1025 tokens, 512 to 16384 keys, 9 of them with a prefix) its choice takes 2 % more than the fastest cut on average
-// and 14 % at worst.
+// and joined by a second launch. From two workgroups a CU on keys are not cut: what that loses is small (640 of 66 tiles: 124 us
+// uncut, 118 in two, 127 in four), and a cut may lose more (720 of 32: 65, 78, 91). Over the 32 shapes timed with 1 .. 48 cuts (1
+// to 128 sequences of 1 to 1025 tokens, 512 to 16384 keys, 9 of them with a prefix) its choice takes 2 % more than the fastest
+// cut on average and 14 % at worst.
 static int64_t split_keys(int64_t blocks, int64_t tiles, int64_t others, int64_t theirs, int64_t rows, int64_t D, bool joined) {
   if (blocks <= 0 || tiles <= 1 || (!joined && blocks >= 2 * CUS)) return 1;
   const Rates r = rates_of(D);

@@ -662,8 +662,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
     fp32 sums (include/foidfinder_rocm.h, ff_cross_attention): any batch, token and head strides that are multiples of 16
     bytes (views of packed rows, [B, heads, L, D] transposed, rows expanded over the batch), D a multiple of 8 up to 128,
     heads a multiple of kv_heads. Keys j >= lens[b] (int32 [B]) and keys with mask[b, j] False (bool [B, S], contiguous
-    columns) are not read; a query without keys gives zeros. work: fp32 of at least cross_attention_work(q, k) elements; calls
-    that run one after another may share it. out and work share no memory with each other or with what is read (refused)."""
+    columns) are not read; a query without keys gives zeros, one with a score of +inf, or of -inf alone, is not a number.
+    work: fp32 of at least cross_attention_work(q, k) elements; calls that run one after another may share it. out and work
+    share no memory with each other or with what is read (refused)."""
     _no_grad(q, k, v, out, work)
     dev = _attended(q, out, lens, work, k, v)
     (qb, qt, qh, q1), (kb, kt, kh, k1), (vb, vt, vh, v1), (ob, ot, oh, o1) = q.stride(), k.stride(), v.stride(), out.stride()
@@ -695,8 +696,8 @@ def prefix_attention(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Te
     """Attention of a batch that shares a prefix (include/foidfinder_rocm.h, ff_prefix_attention): q [B, L, heads, D] are each
     sequence's newest L tokens, prefix_k and prefix_v [P, kv_heads, D] the rows that all sequences see, read once for all of them,
     k and v [B, S, kv_heads, D] each sequence's own behind them, lens[b] of them (int32 [B]; None: S) with the new tokens' own
-    last. Query i sees the prefix and the own keys j < lens[b] - L + 1 + i. Types, strides and work (at least
-    prefix_attention_work(q, prefix_k, k) elements) as in cross_attention."""
+    last. Query i sees the prefix and the own keys j < lens[b] - L + 1 + i, and nothing of later ones, whatever they hold.
+    Types, strides and work (at least prefix_attention_work(q, prefix_k, k) elements) as in cross_attention."""
     _no_grad(q, prefix_k, prefix_v, k, v, out, work)
     dev = _attended(q, out, lens, work, prefix_k, prefix_v, k, v)
     (qb, qt, qh, q1), (kb, kt, kh, k1), (vb, vt, vh, v1), (ob, ot, oh, o1) = q.stride(), k.stride(), v.stride(), out.stride()

@@ -131,11 +131,12 @@ int ff_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, const void* 
  * all); 0 where there are none. What k and v hold for other keys is not read. Scores are fp32: one of +inf, as an infinite element
  * or a product past fp32's range gives it, makes its row not a number, and so do keys of -inf alone; beside others these have no
  * weight. p is rounded to the values' type before it multiplies them, half a step each; in fp16 p below 2^-22 of the row's largest
- * are rounded to steps of 2^-32 of it. Sums of p v are fp32, p up to 2^15: they may overflow for |v| of 2^113 / S and more. q, k, v and their strides are multiples of 16 bytes, out's of 8; tokens of k and v are fewer
- * than 2^24 elements apart. B L heads < 2^31, in fewer than 2^24 workgroups of up to 128 rows of a sequence and key head; where the
- * keys of all rows are cut, B L heads <= 2^26 - 4 (both refused). work: at least ff_cross_attention_work fp32 elements (0 where keys are not cut; NULL then), which calls
- * that run one after another may share. out and work share no memory with each other or with what is read (refused; where rows of
- * three strides lie between another operand's, so are calls that would not touch it). */
+ * are rounded to steps of 2^-32 of it. Sums of p v are fp32, p up to 2^15: they may overflow for |v| of 2^113 / S and more. q, k,
+ * v and their strides are multiples of 16 bytes, out's of 8; tokens of k and v are fewer than 2^24 elements apart. B L heads <
+ * 2^31, in fewer than 2^24 workgroups of up to 128 rows of a sequence and key head; where the keys of all rows are cut, or joined
+ * to a prefix's, B L heads <= 2^26 - 4 (both refused). work: at least ff_cross_attention_work fp32 elements (0 where keys are not cut; NULL then), which
+ * calls that run one after another may share. out and work share no memory with each other or with what is read (refused; where
+ * rows of three strides lie between another operand's, so are calls that would not touch it). */
 int64_t ff_cross_attention_work(int64_t B, int64_t L, int64_t S, int64_t heads, int64_t kv_heads, int64_t D);
 int ff_cross_attention(const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* k, int64_t k_batch,
                        int64_t k_token, int64_t k_head, const void* v, int64_t v_batch, int64_t v_token, int64_t v_head,
@@ -158,8 +159,9 @@ int ff_prefix_attention(const void* q, int64_t q_batch, int64_t q_token, int64_t
 /* A block's output into the residual stream between two norms: x_out = x + scale * gate * N_post(y), h = N_pre(x_out), each
  * rounded once, h from the unrounded sum. x, y, x_out, h fp16 or bf16 [T, C] by row strides in elements, C % 8 == 0, C <= 16384;
  * norms FF_NORM_* with fp32 gamma/beta [C]; h with a pre-norm and only then. gate (or NULL: 1) [gate_rows, C] of x's type or
- * FF_F32: token t takes row t / (T / gate_rows). Sums of squares are fp32: of values past 2^57 they may overflow. Pointers and strides are multiples of 16 bytes. An output is x or y itself (the
- * same pointer and stride) or shares no memory with what is read or with the other one. */
+ * FF_F32: token t takes row t / (T / gate_rows). Sums of squares are fp32: of values past 2^57 they may overflow. Pointers and
+ * strides are multiples of 16 bytes. An output is x or y itself (the same pointer and stride) or shares no memory with what is
+ * read or with the other one. */
 int ff_residual_norm(const void* x, int64_t x_row, const void* y, int64_t y_row, void* x_out, int64_t xo_row, void* h,
                      int64_t h_row, int dtype, int64_t T, int64_t C, int post, const float* post_gamma,
                      const float* post_beta, int pre, const float* pre_gamma, const float* pre_beta, const void* gate,

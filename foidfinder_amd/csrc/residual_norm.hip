@@ -9,11 +9,11 @@
 // column; past 8192 columns gammas and betas are read for each row, from the caches). The next row loads under this one's
 // arithmetic. Sums: within a wave by DPP; a row of several waves leaves each wave's sum and squares about its own mean in LDS
 // and every wave joins them (counts and means known, no cancellation), one barrier a norm.
-// Measured: 32 800 x 1024 fp16 with two LayerNorms and a gate row 51.5 us (5.2 TB/s), 9001 x 4096 bf16 with two RMS norms 55.7 (5.3); a copy of 1 GiB reaches
-// 5.07, of 256 MB 5.42. Gates of their own for each token, loaded in their row and not before it, 62 (fp16, 10 bytes a column:
-// 5.4) and 74 (fp32, 12: 5.4), with a post-norm or without; for each of 32 sequences 46, as without a gate. 4028 rows of 8192
-// columns 48 us (5.5 TB/s), 4024 of 8200 77 and 2014 of 16 384 61 (4.4). With the norms chosen by branches in the row loop,
-// whose parameters' loads it then waited for: 71. A single row: 2.5 us.
+// Measured: 32 800 x 1024 fp16 with two LayerNorms and a gate row 51.5 us (5.2 TB/s), 9001 x 4096 bf16 with two RMS norms 55.7
+// (5.3); a copy of 1 GiB reaches 5.07, of 256 MB 5.42. Gates of their own for each token, loaded in their row and not before
+// it, 62 (fp16, 10 bytes a column: 5.4) and 74 (fp32, 12: 5.4), with a post-norm or without; for each of 32 sequences 46, as
+// without a gate. 4028 rows of 8192 columns 48 us (5.5 TB/s), 4024 of 8200 77 and 2014 of 16 384 61 (4.4). With the norms
+// chosen by branches in the row loop, whose parameters' loads it then waited for: 71. A single row: 2.5 us.
 #include <algorithm>
 #include <type_traits>
 
